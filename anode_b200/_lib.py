@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("ANODE_B200_LIB") or os.path.join(HERE, "libanode_routines_gpu.so")
 
 u32, f32, c_int = ctypes.c_uint32, ctypes.c_float, ctypes.c_int
-vp, size_t = ctypes.c_void_p, ctypes.c_size_t
+vp, size_t, u64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint64
 
 
 class KernelConfig(ctypes.Structure):
@@ -19,8 +19,16 @@ class KernelConfig(ctypes.Structure):
     _fields_ = [("block_sz", u32), ("max_block_ct", u32)]
 
 
+class Heads(ctypes.Structure):
+    """struct AnodeHeads: heads of a [batch, seq, heads, dim] array, strides in elements."""
+    _fields_ = [("data", vp), ("batch_stride", u64), ("seq_stride", u64), ("head_stride", u64), ("heads", u32)]
+
+
 _D = [u32, u32, u32]          # dim0, dim1, dim2
 _T = [vp, vp]                 # cfg, stream
+_H = ctypes.POINTER(Heads)
+# type, batch, seq, dim, rot, interleaved, amplitude, freq, positions and their strides, norm, epsilon, gammas and their type
+_R = [c_int, u32, u32, u32, u32, c_int, f32, vp, vp, c_int, u64, u64, c_int, f32, vp, vp, c_int]
 
 # name -> (restype, argtypes); order matches include/anode_routines_gpu.h
 SIGNATURES = {
@@ -91,6 +99,16 @@ SIGNATURES = {
     "anode_gpu_sync_batch_norm_host_step_blocks": (u32, _D + [ctypes.c_uint64, vp, u32]),
     "anode_gpu_sync_batch_norm_relu_step_host_3d1_packed_f32":
         (c_int, _D + [ctypes.c_uint64, f32, f32, c_int] + [vp] * 12 + [vp, vp, size_t, u32] + _T),
+    "anode_gpu_rms_norm_add_fwd":
+        (c_int, [c_int, u64, u32, f32, vp, u64, vp, u64, vp, c_int, vp, u64, vp, u64, vp] + _T),
+    "anode_gpu_rms_norm_add_bwd_workspace_bytes": (size_t, [u64, u32]),
+    "anode_gpu_rms_norm_add_bwd":
+        (c_int, [c_int, u64, u32, vp, u64, vp, u64, vp, vp, c_int, vp, u64, vp, u64, vp, vp, size_t] + _T),
+    "anode_gpu_rms_norm_add_quant_fwd":
+        (c_int, [c_int, u64, u32, f32, u32, vp, u64, vp, u64, vp, c_int, vp, u64, vp, u64, u64, vp, u64] + _T),
+    "anode_gpu_rotary_positions_fwd": (c_int, _R + [_H] * 4 + _T),
+    "anode_gpu_rotary_positions_bwd_workspace_bytes": (size_t, [u32] * 5),
+    "anode_gpu_rotary_positions_bwd": (c_int, _R + [_H] * 6 + [vp, vp, vp, size_t] + _T),
     "anode_gpu_batch_norm_fused_plan": (c_int, _D + [c_int, u32, u32, u32, ctypes.POINTER(u32), u32]),
     "anode_gpu_batch_norm_fused_plan_walk":
         (c_int, _D + [c_int, u32, u32, u32, u32, u32, ctypes.POINTER(ctypes.c_uint64)]),
@@ -177,6 +195,8 @@ ERRORS = {
     -5: "ANODE_E_COMM: communicator missing, inconsistent, or NCCL failure",
     -6: "ANODE_E_ALIGN: tensor pointers must be 4-byte aligned",
     -7: "ANODE_E_TOO_LARGE: the problem needs more scratch than the library's built-in array holds",
+    -8: "ANODE_E_TYPE: an element type that the call does not take",
+    -9: "ANODE_E_STRIDE: strides that overlap in an output, or an output in the place of an input with other strides",
 }
 
 

@@ -12,6 +12,7 @@ values the reference accepts (src/ops_gpu.rs:3736 `assert_eq!([0, 1], axes)`).
 """
 import ctypes
 import enum
+import math
 
 import torch
 
@@ -584,6 +585,196 @@ class FusedBatchNormRelu:
         if rc:
             check(rc, "anode_gpu_batch_norm_relu_fused_bwd_3d1_packed_f32")
         return dx
+
+
+# --------------------------------------------------------------------------------------------
+# Normalization over rows and rotary positions: what a transformer's layers have in the place of batch-norm (no counterpart in
+# the reference).  f32, f16 and bf16; rows and heads may lie apart (a slice of a packed projection), only the last dimension is
+# packed.  A call runs on its tensors' device, on that device's current stream unless one is given.
+# --------------------------------------------------------------------------------------------
+
+class RmsNormalizeAddOp:
+    """y = t*r*gamma with t = x + residual (rounded to the tensors' type) and r = (mean(t^2) + epsilon)^-1/2 per row, in one
+    launch.  x, residual, y, total: [*, cols] of one type; gamma: [cols] of any of the three types, None for ones.  total
+    receives t, inv_rms (float32, one per row) receives r: the backward pass takes both (and x for total where there was no
+    residual).  y may be x or residual, total may be either, too, but not y's array."""
+    @staticmethod
+    def apply(epsilon, x, y, gamma=None, residual=None, total=None, inv_rms=None, cfg=None, stream=None):
+        _hint(cfg)
+        rc = native().rms_fwd(epsilon, x, y, gamma, residual, total, inv_rms, stream)
+        if rc:
+            check(rc, "anode_gpu_rms_norm_add_fwd")
+        return y
+
+    @staticmethod
+    def adjoint(dy, total, inv_rms, dx, gamma=None, dtotal=None, dgamma=None, cap=WriteCap.Assign, workspace=None, cfg=None, stream=None):
+        """dx = r*(g - xh*mean(g*xh)) + dtotal with g = dy*gamma, xh = total*r: the gradient of x and of the residual alike;
+        dgamma = sum over rows of dy*xh, in gamma's type, or in its own where gamma is None.  dtotal: the gradient that reaches the sum by other ways.  dx may be
+        dy or dtotal; Accumulate adds into dx (and leaves no room for dtotal).  workspace: a tensor of
+        rms_norm_workspace_bytes, needed for dgamma only; None has one made on the call's stream."""
+        _hint(cfg)
+        rc = native().rms_bwd(dy, total, inv_rms, dx, gamma, dtotal, dgamma, cap is WriteCap.Accumulate, workspace, stream)
+        if rc:
+            check(rc, "anode_gpu_rms_norm_add_bwd")
+        return dx
+
+
+class RmsNormalizeAddQuantOp:
+    """RmsNormalizeAddOp with its output in 8 bits, for a product that takes e4m3 operands: q = e4m3(y/scale), float8_e4m3fn, with
+    scale = max(max |y|, 2^-96)/448 over the row (scale of x.shape[:-1]) or over each 128 columns of it (scale of
+    x.shape[:-1] + (ceil(cols/128),), any strides).  y is not rounded in between."""
+    @staticmethod
+    def apply(epsilon, x, q, scale, gamma=None, residual=None, total=None, cfg=None, stream=None):
+        _hint(cfg)
+        rc = native().rms_quant(epsilon, x, q, scale, gamma, residual, total, stream)
+        if rc:
+            check(rc, "anode_gpu_rms_norm_add_quant_fwd")
+        return q
+
+
+def rms_norm_workspace_bytes(rows, cols):
+    """Bytes that RmsNormalizeAddOp.adjoint needs for dgamma.  Nothing is kept in them from call to call; calls that may overlap on
+    the device, graphs among them, take a workspace each."""
+    return int(_lib.load().anode_gpu_rms_norm_add_bwd_workspace_bytes(rows, cols))
+
+
+class RotaryPositionsOp:
+    """Rotary positions of queries and keys in one launch, after the RMS norm of each head where epsilon is a number (None: no
+    norm): the pair (u, v) of the head becomes amplitude*(u cos a - v sin a, u sin a + v cos a), a = position*freq[i], for the
+    pairs (i, i + rot/2) or, interleaved, (2i, 2i + 1), i < rot/2 = len(freq); elements from rot on pass.  q, k: [tokens,
+    heads, dim] or [batch, seq, heads, dim] at any strides (k None: one array only); positions: int32 or int64, [tokens], [batch, seq] or [seq]; freq: float64
+    (rotary_frequencies).  q_out may be q, k_out may be k."""
+    @staticmethod
+    def apply(positions, freq, q, k, q_out, k_out, interleaved=False, amplitude=1.0, epsilon=None, gamma_q=None, gamma_k=None, cfg=None, stream=None):
+        _hint(cfg)
+        rc = native().rotary_fwd(positions, freq, q, k, q_out, k_out, interleaved, amplitude, epsilon, gamma_q, gamma_k, stream)
+        if rc:
+            check(rc, "anode_gpu_rotary_positions_fwd")
+        return q_out, k_out
+
+    @staticmethod
+    def adjoint(positions, freq, dq_out, dk_out, dq, dk, interleaved=False, amplitude=1.0, epsilon=None, q=None, k=None, gamma_q=None, gamma_k=None,
+                dgamma_q=None, dgamma_k=None, workspace=None, cfg=None, stream=None):
+        """dq, dk from the gradients of q_out, k_out; with a norm also from q and k, the forward pass's inputs, and then the gradients of
+        the norm's weights where they are asked for.  dq may be dq_out, dk may be dk_out.  workspace: a tensor of rotary_workspace_bytes,
+        needed for those only; None has one made on the call's stream."""
+        _hint(cfg)
+        rc = native().rotary_bwd(positions, freq, dq_out, dk_out, dq, dk, interleaved, amplitude, epsilon, q, k, gamma_q, gamma_k, dgamma_q, dgamma_k,
+                                 workspace, stream)
+        if rc:
+            check(rc, "anode_gpu_rotary_positions_bwd")
+        return dq, dk
+
+
+def rotary_workspace_bytes(batch, seq, q_heads, k_heads, dim):
+    """Bytes that RotaryPositionsOp.adjoint needs for the gradients of the norms' weights (see rms_norm_workspace_bytes)."""
+    return int(_lib.load().anode_gpu_rotary_positions_bwd_workspace_bytes(batch, seq, q_heads, k_heads, dim))
+
+
+def rotary_frequencies(rot, base=10000.0, factor=1.0, context=None, slow=1.0, fast=4.0, device="cuda"):
+    """Angles per position, base^(-2i/rot) for i < rot/2, as float64.  For a context stretched by `factor`: all of them divided by it
+    (context None), or, where `context` is the length that the model was trained at, those that turn fewer than `slow`
+    times in it divided, those that turn more than `fast` times kept, and the ones between in proportion."""
+    if rot < 2 or rot % 2:
+        raise ValueError("rot must be even and at least 2")
+    if not (base > 0 and factor > 0) or not 0 <= slow < fast:
+        raise ValueError("base and factor are positive, and 0 <= slow < fast")
+    freq = base ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    if context is None:
+        freq = freq / factor
+    else:
+        keep = ((context * freq / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+        freq = freq * (keep + (1 - keep) / factor)
+    return freq.to(device)
+
+
+class RmsNormAdd:
+    """An RMS-norm layer with the residual's addition that keeps its weights and what its backward pass needs: a training loop makes
+    two calls per step, forward(x, residual) and backward(dy, dtotal); serving calls infer or infer_quant."""
+
+    def __init__(self, cols, epsilon=1e-5, affine=True, dtype=torch.float32, device="cuda"):
+        self.epsilon = float(epsilon)
+        self.gamma = torch.ones(cols, device=device, dtype=dtype) if affine else None
+        self.dgamma = torch.zeros(cols, device=device, dtype=dtype) if affine else None
+        self._saved = None
+
+    def infer(self, x, residual=None, out=None, total=None):
+        """(y, total): the norm of the sum, and the sum, which is x itself without a residual."""
+        y = out if out is not None else torch.empty_like(x)
+        if residual is not None and total is None:
+            total = torch.empty_like(x)
+        RmsNormalizeAddOp.apply(self.epsilon, x, y, self.gamma, residual, total)
+        return y, x if residual is None else total
+
+    def infer_quant(self, x, residual=None, block=128, total=None):
+        """(q, scale, total): infer's output in 8 bits, a scale per `block` = 128 columns or, block=None, per row."""
+        if block not in (None, 128):
+            raise ValueError("block is 128 or None")
+        q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+        groups = x.shape[:-1] if block is None else x.shape[:-1] + (-(-x.shape[-1] // 128),)
+        scale = torch.empty(groups, device=x.device, dtype=torch.float32)
+        if residual is not None and total is None:
+            total = torch.empty_like(x)
+        RmsNormalizeAddQuantOp.apply(self.epsilon, x, q, scale, self.gamma, residual, total)
+        return q, scale, x if residual is None else total
+
+    def forward(self, x, residual=None, out=None, total=None):
+        """infer, keeping the sum and 1/rms for the backward pass.  The sum (x without a residual) has to stay as it is until then."""
+        y = out if out is not None else torch.empty_like(x)
+        if residual is not None and total is None:
+            total = torch.empty_like(x)
+        inv_rms = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+        RmsNormalizeAddOp.apply(self.epsilon, x, y, self.gamma, residual, total, inv_rms)
+        total = x if residual is None else total
+        self._saved = total, inv_rms
+        return y, total
+
+    def backward(self, dy, dtotal=None, out=None):
+        """The gradient of x, which is the residual's, too; that of gamma is left in dgamma."""
+        if self._saved is None:
+            raise RuntimeError("backward before forward")
+        total, inv_rms = self._saved
+        dx = out if out is not None else torch.empty_like(dy)
+        return RmsNormalizeAddOp.adjoint(dy, total, inv_rms, dx, self.gamma, dtotal, self.dgamma)
+
+
+class RotaryPositions:
+    """Rotary positions, with or without a norm of each head before them, as a layer that keeps its frequencies and weights."""
+
+    def __init__(self, dim, rot=None, base=10000.0, interleaved=False, factor=1.0, context=None, slow=1.0, fast=4.0, amplitude=1.0,
+                 norm=False, epsilon=1e-5, dtype=torch.float32, device="cuda"):
+        rot = dim if rot is None else rot
+        if not 2 <= rot <= dim:
+            raise ValueError("rot must be between 2 and dim")
+        self.freq = rotary_frequencies(rot, base, factor, context, slow, fast, device)
+        self.interleaved, self.amplitude = bool(interleaved), float(amplitude)
+        self.epsilon = float(epsilon) if norm else None
+        self.gamma_q, self.gamma_k, self.dgamma_q, self.dgamma_k = \
+            (make(dim, device=device, dtype=dtype) if norm else None for make in (torch.ones, torch.ones, torch.zeros, torch.zeros))
+        self._saved = None
+
+    def infer(self, q, k, positions, q_out=None, k_out=None):
+        q_out = q_out if q_out is not None else torch.empty_like(q)
+        k_out = k_out if k_out is not None or k is None else torch.empty_like(k)
+        return RotaryPositionsOp.apply(positions, self.freq, q, k, q_out, k_out, self.interleaved, self.amplitude, self.epsilon, self.gamma_q,
+                                       self.gamma_k if k is not None else None)
+
+    def forward(self, q, k, positions, q_out=None, k_out=None):
+        """infer, keeping the positions and, with a norm, q and k for the backward pass: they have to stay as they are until then."""
+        out = self.infer(q, k, positions, q_out, k_out)
+        self._saved = (positions, q, k) if self.epsilon is not None else (positions, None, None)
+        return out
+
+    def backward(self, dq_out, dk_out, dq=None, dk=None):
+        """(dq, dk); the gradients of the norm's weights are left in dgamma_q and dgamma_k."""
+        if self._saved is None:
+            raise RuntimeError("backward before forward")
+        positions, q, k = self._saved
+        two = dk_out is not None
+        dq = dq if dq is not None else torch.empty_like(dq_out)
+        dk = dk if dk is not None or not two else torch.empty_like(dk_out)
+        return RotaryPositionsOp.adjoint(positions, self.freq, dq_out, dk_out, dq, dk, self.interleaved, self.amplitude, self.epsilon, q, k, self.gamma_q,
+                                         self.gamma_k if two else None, self.dgamma_q, self.dgamma_k if two else None)
 
 
 class SyncWorkspace(Workspace):

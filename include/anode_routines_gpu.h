@@ -173,6 +173,8 @@ void anode_gpu_positive_clip_flat_map_bwd_f32(
 #define ANODE_E_COMM       -5   /* communicator missing / inconsistent / NCCL failure */
 #define ANODE_E_ALIGN      -6   /* tensor pointers must be 4-byte aligned */
 #define ANODE_E_TOO_LARGE  -7   /* the problem needs more scratch than the library's built-in array holds */
+#define ANODE_E_TYPE       -8   /* an element type that the call does not take */
+#define ANODE_E_STRIDE     -9   /* strides that overlap in an output, or an output in the place of an input with other strides */
 
 /* Bits of the device status word. */
 #define ANODE_ST_WAIT_STATS   1u  /* a wait for a channel's statistics ran out */
@@ -499,6 +501,100 @@ int anode_gpu_sync_batch_norm_add_act_bwd_3d1_packed_f32(
     const float *gamma, const float *beta,
     float *dx, float *dresidual, float *dgamma, float *dbeta,
     struct AnodeSyncComm *comm, void *workspace, size_t workspace_bytes,
+    const struct KernelConfig *cfg, struct CUstream_st *stream);
+
+/* ===================================================================================
+ * 4. Normalization over rows, and rotary positions (new): what a transformer's layers have in the place of
+ *    batch-norm, with the residual's addition and the map after the norm fused as in section 2.
+ *
+ * Conventions that differ from the above: the element type is an argument (ANODE_TYPE_*; f16 and bf16 beside f32), rows
+ * and heads may lie apart (strides in elements; the innermost dimension is packed), and no rows or no tokens are a call
+ * that does nothing (gradients of weights are then zero).  All arithmetic is in f32, angles in f64; every output is
+ * rounded once.  An output may be an input's array (same pointer and strides); other overlaps are not allowed.
+ * Tensors are aligned to their elements; 16-byte aligned ones of such strides are faster.  Nothing synchronises, nothing
+ * is allocated, and no state is kept in a workspace from call to call: it is written before it is read in every call, and
+ * calls that may overlap on the device take one each.
+ * =================================================================================== */
+#define ANODE_TYPE_F32   0
+#define ANODE_TYPE_F16   1
+#define ANODE_TYPE_BF16  2
+
+/* RMS norm with the residual's addition, forward:
+ *   total = round(x + residual)                  (x where residual is NULL; stored where total is not NULL)
+ *   r     = (sum(total^2)/cols + epsilon)^-1/2   per row (stored where inv_rms is not NULL)
+ *   y     = total * r * gamma                    (gamma NULL: 1)
+ * The norm reads the sum as it is stored, so that the backward pass sees the same numbers.  total without residual is
+ * refused (it would be a copy).  Squares are summed in f32: rows with elements beyond 1e19 give y = 0, rows that hold a NaN
+ * or an infinity give NaN where the formula does. */
+int anode_gpu_rms_norm_add_fwd(
+    int type, uint64_t rows, uint32_t cols, float epsilon,
+    const void *x, uint64_t x_stride, const void *residual, uint64_t residual_stride,
+    const void *gamma, int gamma_type,
+    void *y, uint64_t y_stride, void *total, uint64_t total_stride, float *inv_rms,
+    const struct KernelConfig *cfg, struct CUstream_st *stream);
+
+/* Its adjoint, from the stored total (x where there was no residual) and inv_rms:
+ *   g = dy*gamma, xh = total*r:  dx = r*(g - xh*sum(g*xh)/cols) + dtotal,  dgamma = sum over rows of dy*xh
+ * dtotal is the gradient that reaches the sum by other ways (NULL: none); dx is the gradient of x and of the residual alike.
+ * dx may be dy or dtotal (the latter adds into it).  dgamma NULL: not computed; it has gamma's type and needs the workspace
+ * (anode_gpu_rms_norm_add_bwd_workspace_bytes, 16-byte aligned).  Sums are taken in a fixed order: the same call gives the
+ * same bits. */
+size_t anode_gpu_rms_norm_add_bwd_workspace_bytes(uint64_t rows, uint32_t cols);
+int anode_gpu_rms_norm_add_bwd(
+    int type, uint64_t rows, uint32_t cols,
+    const void *dy, uint64_t dy_stride, const void *total, uint64_t total_stride, const float *inv_rms,
+    const void *gamma, int gamma_type, const void *dtotal, uint64_t dtotal_stride,
+    void *dx, uint64_t dx_stride, void *dgamma, void *workspace, size_t workspace_bytes,
+    const struct KernelConfig *cfg, struct CUstream_st *stream);
+
+/* The forward pass with its output in 8 bits, for a product that takes e4m3 operands:
+ *   a = max |y| over the row (block = 0) or over each 128 columns of it (block = 128; the last may be shorter)
+ *   scale = max(a, 2^-96)/448,  q = e4m3(y/scale)   (nearest, ties to even; |q| <= 448)
+ * y itself is not rounded in between.  scale[row*scale_row_stride + group*scale_group_stride]; a scale is never 0, and a
+ * group that holds a NaN has NaN for its scale and its values. */
+int anode_gpu_rms_norm_add_quant_fwd(
+    int type, uint64_t rows, uint32_t cols, float epsilon, uint32_t block,
+    const void *x, uint64_t x_stride, const void *residual, uint64_t residual_stride,
+    const void *gamma, int gamma_type,
+    uint8_t *q, uint64_t q_stride, float *scale, uint64_t scale_row_stride, uint64_t scale_group_stride,
+    void *total, uint64_t total_stride,
+    const struct KernelConfig *cfg, struct CUstream_st *stream);
+
+/* Heads of a [batch, seq, heads, dim] array; strides in elements, dim packed.  [batch, heads, seq, dim] arrays and slices of
+ * a packed projection are such arrays with other strides. */
+struct AnodeHeads {
+  void *data;
+  uint64_t batch_stride, seq_stride, head_stride;
+  uint32_t heads;
+};
+
+/* Rotary positions of queries and keys (k NULL: of one array), after the RMS norm of each head where norm != 0:
+ *   n = x * (sum(x^2)/dim + epsilon)^-1/2 * gamma        (norm = 0: n = x; gamma NULL: 1)
+ *   angle = position * freq[i],  c = amplitude*cos(angle),  s = amplitude*sin(angle),   i < rot/2
+ *   (n[u], n[v]) -> (n[u]*c - n[v]*s, n[u]*s + n[v]*c);   n[rot..dim) passes as it is
+ * (u, v) = (i, i + rot/2), or (2i, 2i + 1) where interleaved != 0.  rot is even, 2 <= rot <= dim <= 1024.  freq: rot/2 doubles on the
+ * device (for long contexts stretched as the caller likes).  Angles are formed and reduced in f64, so that far positions
+ * keep their digits.  positions[b*pos_batch_stride + s*pos_seq_stride]: signed integers of position_bytes (4 or 8) bytes. */
+int anode_gpu_rotary_positions_fwd(
+    int type, uint32_t batch, uint32_t seq, uint32_t dim, uint32_t rot, int interleaved, float amplitude,
+    const double *freq, const void *positions, int position_bytes, uint64_t pos_batch_stride, uint64_t pos_seq_stride,
+    int norm, float epsilon, const void *gamma_q, const void *gamma_k, int gamma_type,
+    const struct AnodeHeads *q, const struct AnodeHeads *k, const struct AnodeHeads *q_out, const struct AnodeHeads *k_out,
+    const struct KernelConfig *cfg, struct CUstream_st *stream);
+
+/* Its adjoint: dn is dout turned back (by -angle, times amplitude);
+ *   norm = 0: dx = dn (q and k are not read and may be NULL)
+ *   else r, xh = x*r, g = dn*gamma:  dx = r*(g - xh*sum(g*xh)/dim),  dgamma = sum over batch, seq and heads of dn*xh
+ * dgamma_q, dgamma_k NULL: not computed; they have gamma's type and need the workspace
+ * (anode_gpu_rotary_positions_bwd_workspace_bytes, 16-byte aligned).  dq may be dq_out.  Fixed order of sums, as above. */
+size_t anode_gpu_rotary_positions_bwd_workspace_bytes(uint32_t batch, uint32_t seq, uint32_t q_heads, uint32_t k_heads, uint32_t dim);
+int anode_gpu_rotary_positions_bwd(
+    int type, uint32_t batch, uint32_t seq, uint32_t dim, uint32_t rot, int interleaved, float amplitude,
+    const double *freq, const void *positions, int position_bytes, uint64_t pos_batch_stride, uint64_t pos_seq_stride,
+    int norm, float epsilon, const void *gamma_q, const void *gamma_k, int gamma_type,
+    const struct AnodeHeads *dq_out, const struct AnodeHeads *dk_out, const struct AnodeHeads *q, const struct AnodeHeads *k,
+    const struct AnodeHeads *dq, const struct AnodeHeads *dk, void *dgamma_q, void *dgamma_k,
+    void *workspace, size_t workspace_bytes,
     const struct KernelConfig *cfg, struct CUstream_st *stream);
 
 #ifdef __cplusplus

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/anode_routines_gpu.h"
 
 namespace anode_b200 {
@@ -24,6 +26,29 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 struct Weights {
   const void *p;
   int type;
+  // N of them from column c on; all at once where they are aligned to 16 bytes
+  template <int N> __device__ __forceinline__ void load(uint32_t c, float *f) const
+  {
+    static_assert(N == 4 || N == 8, "as many as 16 bytes of a type hold");
+    if (!p) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = 1.0f;
+    } else if (type == ANODE_TYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) *reinterpret_cast<float4 *>(f + i) = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + c + i);
+    } else {
+      uint32_t w[N / 2];
+      if constexpr (N == 8) *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + c);
+      else *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + c);
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        if (type == ANODE_TYPE_F16) {
+          const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+          f[2 * i] = v.x; f[2 * i + 1] = v.y;
+        } else { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+      }
+    }
+  }
   __device__ __forceinline__ float at(uint32_t i) const
   {
     if (!p) return 1.0f;
@@ -37,6 +62,53 @@ __device__ __forceinline__ void put_weight(void *p, int type, uint32_t i, float 
   else if (type == ANODE_TYPE_F16) static_cast<__half *>(p)[i] = from_float<__half>(v);
   else static_cast<__nv_bfloat16 *>(p)[i] = from_float<__nv_bfloat16>(v);
 }
+
+// 16 bytes of an array: V elements
+template <typename T> struct Vec {
+  static constexpr int V = 16 / sizeof(T);
+  uint4 bits;
+  __device__ __forceinline__ static Vec load(const T *p) { return Vec{*reinterpret_cast<const uint4 *>(p)}; }
+  __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint4 *>(p) = bits; }
+  __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? bits.x : i == 1 ? bits.y : i == 2 ? bits.z : bits.w; }
+  __device__ __forceinline__ void floats(float *f) const
+  {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = word(i);
+      if constexpr (sizeof(T) == 4) f[i] = __uint_as_float(w);
+      else if constexpr (std::is_same<T, __half>::value) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        f[2 * i] = v.x; f[2 * i + 1] = v.y;
+      } else { f[2 * i] = __uint_as_float(w << 16); f[2 * i + 1] = __uint_as_float(w & 0xffff0000u); }
+    }
+  }
+  __device__ __forceinline__ static Vec of(const float *f)
+  {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+      else if constexpr (std::is_same<T, __half>::value) { const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t *>(&v); }
+      else { const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t *>(&v); }
+    }
+    return Vec{make_uint4(w[0], w[1], w[2], w[3])};
+  }
+  // element by element, those of [first, end); the others are zero, or stay
+  __device__ __forceinline__ static Vec load_some(const T *p, int first, int end)
+  {
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = i >= first && i < end ? to_float(p[i]) : 0.0f;
+    return of(f);
+  }
+  __device__ __forceinline__ void store_some(T *p, int first, int end) const
+  {
+    float f[V];
+    floats(f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (i >= first && i < end) p[i] = from_float<T>(f[i]);
+  }
+};
 
 __device__ __forceinline__ float warp_sum_all(float v)
 {
@@ -54,6 +126,13 @@ __device__ __forceinline__ float block_sum_all(float v, float *buf)
   __syncthreads();
   v = lane < warps ? buf[lane] : 0.0f;
   return warp_sum_all(v);
+}
+// The same of a team: a power of two of a warp's lanes, or a block
+__device__ __forceinline__ float team_sum_all(float v, uint32_t team, float *buf)
+{
+  if (team > 32) return block_sum_all(v, buf);
+  for (uint32_t o = team / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
 inline bool known_type(int t) { return t == ANODE_TYPE_F32 || t == ANODE_TYPE_F16 || t == ANODE_TYPE_BF16; }

@@ -552,10 +552,8 @@ template <typename T, int W, int CH, bool PRE> int launch_grad(const GradArgs &a
 {
   const auto kernel = rms_norm_grad_kernel<T, W, CH, PRE>;
   const size_t shared = a.dgamma ? (size_t)h.teams * a.cols * 4 : 0;
-  if (shared > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return ANODE_E_LAUNCH;
-  }
+  static SharedMemory allowed;
+  if (!allowed.up_to((const void *)kernel, shared)) return ANODE_E_LAUNCH;
   return launch(kernel, dim3(a.parts), kGradThreads, shared, stream, a, h);
 }
 

@@ -7,8 +7,9 @@
 // or 2V elements that pass.  In the half layout an item is two vectors rot/2 apart, so that both elements of a pair are in one lane and the
 // turn needs no exchange; only the norm's sums go across the group.  Lanes keep their items from head to head, and with them the
 // weights and the sums of the weights' gradients.
-// A block has a few tokens of the queries or of the keys at a time: it makes their cosines and sines once, in shared memory, for all of
-// their heads, while the first heads are on their way.
+// A warp takes a token of the queries or of the keys (or as many tokens as fill it, or part of a token's heads where there are few tokens),
+// makes its cosines and sines once, in shared memory of its own, and goes through the heads with the next ones' data on their way by
+// asynchronous copies, each lane into a ring of its own: no warp waits for another, and no lane for what another lane copies.
 #include "bn_host.h"
 #include "rows.cuh"
 
@@ -17,7 +18,7 @@ namespace rows {
 
 constexpr uint32_t kThreads = 256, kMostDim = 1024;
 constexpr uint32_t kMostParts = 148 * 4;      // blocks that have sums of the weights' gradients
-constexpr uint32_t kMostTokens = 64;          // of a block at a time
+constexpr uint32_t kWarps = kThreads / 32;
 
 struct HeadArray {
   void *p;
@@ -28,7 +29,8 @@ struct RotarySide {
   HeadArray in, x, out;                // backward: in = dout, x = the norm's input, out = dx
   Weights gamma;
   uint32_t heads;
-  uint32_t tokens;                     // of a block at a time
+  uint32_t tokens, parts, span;        // a unit of a warp: `tokens` tokens, or one of the `parts` spans of a token's heads
+  uint32_t units;
   uint32_t blocks, want;               // blocks of the grid; whether the weights' gradient is asked for
 };
 struct RotaryArgs {
@@ -38,7 +40,7 @@ struct RotaryArgs {
   const void *positions;
   uint32_t position_bytes;
   uint64_t pos_batch, pos_seq;
-  uint64_t total;                      // tokens
+  uint32_t total;                      // tokens
   uint32_t norm;
   RotarySide side[2];
   float *partial;                      // [blocks, dim] of the gradients of the weights
@@ -53,47 +55,82 @@ template <> struct RawOf<8> { typedef uint2 type; };
 template <> struct RawOf<4> { typedef uint32_t type; };
 template <> struct RawOf<2> { typedef uint16_t type; };
 template <typename T, int V> struct Few {
-  union { typename RawOf<V * sizeof(T)>::type raw; T e[V]; };
+  union { typename RawOf<V * sizeof(T)>::type raw; T e[V]; uint32_t w[(V * sizeof(T) + 3) / 4]; };
   __device__ __forceinline__ Few() {}
   __device__ __forceinline__ void load(const T *p) { raw = *reinterpret_cast<const decltype(raw) *>(p); }
   __device__ __forceinline__ void clear() { raw = decltype(raw){}; }
   __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<decltype(raw) *>(p) = raw; }
   __device__ __forceinline__ void floats(float *f) const
   {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value && V > 1) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = to_float(e[i]);
+      for (int i = 0; i < V / 2; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = to_float(e[i]);
+    }
   }
   __device__ __forceinline__ void of(const float *f)
   {
+    if constexpr (sizeof(T) == 2 && V > 1) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = from_float<T>(f[i]);
+      for (int i = 0; i < V / 2; ++i) {
+        if constexpr (std::is_same<T, __half>::value) { const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t *>(&v); }
+        else { const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t *>(&v); }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = from_float<T>(f[i]);
+    }
   }
 };
 
-__device__ __forceinline__ double position_of(const RotaryArgs &a, uint64_t token)
+template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const void *from)
 {
-  const uint64_t b = a.batch == 1 ? 0 : token / a.seq, i = b * a.pos_batch + (token - b * a.seq) * a.pos_seq;
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+__device__ __forceinline__ double position_of(const RotaryArgs &a, uint32_t token)
+{
+  const uint32_t b = a.batch == 1 ? 0 : token / a.seq;
+  const uint64_t i = b * a.pos_batch + (token - b * a.seq) * a.pos_seq;
   return a.position_bytes == 8 ? (double)static_cast<const long long *>(a.positions)[i] : (double)static_cast<const int *>(a.positions)[i];
 }
 // cos and sin of position*freq, by whole turns in f64: what is left of them is exact, and small
-__device__ __forceinline__ float2 turn_of(double position, double freq, float amplitude)
+__device__ __forceinline__ float2 turn_of(double position, double freq, float amplitude, float way)
 {
   const double turns = position * (freq * 0.15915494309189533577);      // 1/(2 pi)
   float s, c;
   sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-  return make_float2(c * amplitude, s * amplitude);
+  return make_float2(c * amplitude, s * amplitude * way);
 }
 
+// Registers: two or three blocks of a multiprocessor
+constexpr int resident(int floats, bool both) { return floats > 16 ? 1 : both ? 2 : 3; }
+// Heads of a lane's ring, and its bytes: pieces of less than four bytes cannot be copied asynchronously and go through registers
+__host__ __device__ constexpr int ring_depth(int v, int it) { return v == 1 ? 1 : it == 1 ? 4 : 2; }
+__host__ __device__ constexpr size_t ring_bytes(int v, int it, bool both, size_t e) { return v == 1 ? 0 : (size_t)ring_depth(v, it) * kThreads * it * 2 * v * e * (both ? 2 : 1); }
+
 template <typename T, int V, int IT, bool NORM, bool BWD>
-__global__ void __launch_bounds__(kThreads) rotary_heads_kernel(const RotaryArgs a)
+__global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM && BWD)) rotary_heads_kernel(const RotaryArgs a)
 {
-  // [tokens][rot/2] cosines and sines, pair j = item*V + i of a token at (i/2*turned + item)*2 + i%2, so that lanes read 16 bytes side by
-  // side; behind them the sums of the weights' gradients, when the block is done
+  constexpr bool BOTH = NORM && BWD;        // two arrays are read
+  constexpr bool KEEP = V * IT <= 8;        // a lane's cosines and sines stay in its registers from head to head
+  constexpr int DEPTH = ring_depth(V, IT), PIECES = IT * 2 * (BOTH ? 2 : 1);
+  typedef typename RawOf<V * sizeof(T)>::type Raw;
+  // the rings, [depth][piece][thread]; of each warp, [tokens][rot/2] cosines and sines, pair j = item*V + i of a token at
+  // (i/2*turned + item)*2 + i%2, so that lanes read 16 bytes side by side; in their place the warps' sums of the weights' gradients, when the block is done
   extern __shared__ float4 shared[];
-  float2 *table = reinterpret_cast<float2 *>(shared);
   const uint32_t which = blockIdx.x >= a.side[0].blocks, block = which ? blockIdx.x - a.side[0].blocks : blockIdx.x;
   const RotarySide &d = a.side[which];
-  const uint32_t lane = threadIdx.x & (a.lanes - 1), group = threadIdx.x / a.lanes, groups = kThreads / a.lanes, half = a.rot / 2;
+  const uint32_t wlane = threadIdx.x & 31, warp = threadIdx.x >> 5, lane = wlane & (a.lanes - 1), group = wlane / a.lanes, groups = 32 / a.lanes;
+  const uint32_t half = a.rot / 2, heads = d.heads;
+  Raw *ring = reinterpret_cast<Raw *>(shared) + threadIdx.x;
+  float2 *table = reinterpret_cast<float2 *>(reinterpret_cast<char *>(shared) + ring_bytes(V, IT, BOTH, sizeof(T))) + (size_t)warp * d.tokens * half;
   // this lane's items: two vectors, at e0 and e1
   uint32_t e0[IT], e1[IT];
   bool has[IT], second[IT], turns[IT];
@@ -107,8 +144,8 @@ __global__ void __launch_bounds__(kThreads) rotary_heads_kernel(const RotaryArgs
     second[k] = has[k] && e1[k] < a.dim;
   }
   pdl_wait();
-  float g[IT][2 * V], acc[IT][2 * V];
-  if (NORM) {
+  float g[NORM ? IT : 1][2 * V], acc[NORM && BWD ? IT : 1][2 * V];
+  if constexpr (NORM) {
     const bool aligned_gamma = ((uintptr_t)d.gamma.p & 15) == 0;
 #pragma unroll
     for (int k = 0; k < IT; ++k)
@@ -117,7 +154,7 @@ __global__ void __launch_bounds__(kThreads) rotary_heads_kernel(const RotaryArgs
         const bool any = j ? second[k] : has[k];
         const uint32_t e = j ? e1[k] : e0[k];
 #pragma unroll
-        for (int i = 0; i < V; ++i) { g[k][j * V + i] = 0.0f; if (BWD) acc[k][j * V + i] = 0.0f; }
+        for (int i = 0; i < V; ++i) { g[k][j * V + i] = 0.0f; if constexpr (BWD) acc[k][j * V + i] = 0.0f; }
         if (!any) continue;
         if (V > 1 && aligned_gamma) { if constexpr (V > 1) d.gamma.load<V>(e, g[k] + j * V); }
         else {
@@ -126,92 +163,145 @@ __global__ void __launch_bounds__(kThreads) rotary_heads_kernel(const RotaryArgs
         }
       }
   }
-  struct Head { Few<T, V> in[IT][2], x[BWD && NORM ? IT : 1][2]; } now, next;
+  struct Head { Few<T, V> in[IT][2], x[BOTH ? IT : 1][2]; } now, next;
   // (what a lane does not have is never loaded, and counts as zeros)
 #pragma unroll
   for (int k = 0; k < IT; ++k)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      now.in[k][j].clear(); next.in[k][j].clear();
-      if (BWD && NORM) { now.x[k][j].clear(); next.x[k][j].clear(); }
-    }
-  const uint32_t more = groups / d.heads, rest = groups - more * d.heads;
-  for (uint64_t first = (uint64_t)block * d.tokens; first < a.total; first += (uint64_t)d.blocks * d.tokens) {
-    const uint32_t count = (uint32_t)min((uint64_t)d.tokens, a.total - first);       // tokens of this round
-    uint32_t t = group / d.heads, h = group - t * d.heads;
-    auto place = [&](const HeadArray &x, uint32_t t, uint32_t h) {
-      const uint64_t token = first + t, b = a.batch == 1 ? 0 : token / a.seq;
-      return static_cast<T *>(x.p) + b * x.batch + (token - b * a.seq) * x.seq + h * x.head;
-    };
-    auto load = [&](Head &w, uint32_t t, uint32_t h) {
-      const T *in = place(d.in, t, h);
-#pragma unroll
-      for (int k = 0; k < IT; ++k) {
-        if (has[k]) w.in[k][0].load(in + e0[k]);
-        if (second[k]) w.in[k][1].load(in + e1[k]);
-      }
-      if (BWD && NORM) {
-        const T *x = place(d.x, t, h);
-#pragma unroll
-        for (int k = 0; k < IT; ++k) {
-          if (has[k]) w.x[k][0].load(x + e0[k]);
-          if (second[k]) w.x[k][1].load(x + e1[k]);
+      if constexpr (V == 1) {
+        now.in[k][j].clear(); next.in[k][j].clear();
+        if constexpr (BOTH) { now.x[k][j].clear(); next.x[k][j].clear(); }
+      } else if (!(j ? second[k] : has[k])) {
+        for (int i = 0; i < DEPTH; ++i) {
+          ring[(i * PIECES + 2 * k + j) * kThreads] = Raw{};
+          if constexpr (BOTH) ring[(i * PIECES + 2 * IT + 2 * k + j) * kThreads] = Raw{};
         }
       }
-    };
-    if (t < count) load(now, t, h);
-    __syncthreads();                 // (the table of the round before has been read)
-    for (uint32_t i = threadIdx.x; i < count * half; i += kThreads) {
-      const uint32_t token = i / half, j = i - token * half, item = j / V, k = j % V;
-      table[token * half + (V == 1 ? item : (k / 2 * a.turned + item) * 2 + k % 2)] = turn_of(position_of(a, first + token), a.freq[j], a.amplitude);
     }
-    __syncthreads();
-    // all groups of a warp go round as often as its first: the sums need every lane
-    for (uint32_t t0 = (group & ~(32 / a.lanes - 1)) / d.heads, h0 = (group & ~(32 / a.lanes - 1)) - t0 * d.heads; t0 < count;) {
-      const bool live = t < count;
-      uint32_t nt = t + more, nh = h + rest;
-      if (nh >= d.heads) { nh -= d.heads; ++nt; }
-      t0 += more; h0 += rest;
-      if (h0 >= d.heads) { h0 -= d.heads; ++t0; }
-      if (nt < count) load(next, nt, nh);
-      float f[IT][2 * V], x[BWD && NORM ? IT : 1][2 * V], sq = 0.0f, dot = 0.0f, r = 1.0f;
+  // Where this group is: the unit, its head (none: from `end` on), the passes that the unit has left, and addresses
+  struct Place { uint32_t unit, head, end, left; const T *p, *x; };
+  const uint32_t step = d.blocks * kWarps, mine = d.tokens > 1 ? group / heads : 0;      // mine: of the unit's tokens
+  const uint64_t hop = d.in.head * groups, hop_x = BOTH ? d.x.head * groups : 0, hop_out = d.out.head * groups;
+  auto enter = [&](Place &w, const HeadArray &p, const HeadArray *x) {       // the first head of its unit
+    if (w.unit >= d.units) { w.head = w.end = 0; w.left = 1; return; }
+    const uint32_t first = d.parts > 1 ? w.unit / d.parts : w.unit * d.tokens, low = d.parts > 1 ? (w.unit - first * d.parts) * d.span : 0;
+    const uint32_t token = first + mine;
+    w.end = min(heads, low + d.span);
+    w.left = d.tokens > 1 ? 1 : (w.end - low + groups - 1) / groups;
+    w.head = low + group - mine * heads;
+    if (mine >= d.tokens || token >= a.total) w.head = w.end;
+    const uint32_t b = a.batch == 1 ? 0 : token / a.seq, s = token - b * a.seq;
+    w.p = static_cast<const T *>(p.p) + b * p.batch + s * p.seq + w.head * p.head;
+    if (x) w.x = static_cast<const T *>(x->p) + b * x->batch + s * x->seq + w.head * x->head;
+  };
+  uint32_t turn_in = 0;                  // the ring's place that is filled next
+  auto load = [&](const Place &w) {
+    if (w.head < w.end) {
 #pragma unroll
-      for (int k = 0; k < IT; ++k) {
-        now.in[k][0].floats(f[k]);
-        now.in[k][1].floats(f[k] + V);
+      for (int k = 0; k < IT; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (!(j ? second[k] : has[k])) continue;
+          const uint32_t e = j ? e1[k] : e0[k];
+          if constexpr (V == 1) {
+            next.in[k][j].load(w.p + e);
+            if constexpr (BOTH) next.x[k][j].load(w.x + e);
+          } else {
+            copy_async<V * sizeof(T)>(ring + (turn_in * PIECES + 2 * k + j) * kThreads, w.p + e);
+            if constexpr (BOTH) copy_async<V * sizeof(T)>(ring + (turn_in * PIECES + 2 * IT + 2 * k + j) * kThreads, w.x + e);
+          }
+        }
+    }
+    if constexpr (V > 1) {
+      copies_commit();
+      turn_in = turn_in + 1 == DEPTH ? 0 : turn_in + 1;
+    }
+  };
+  auto advance = [&](Place &w, uint64_t hop, uint64_t hop_x, const HeadArray &p, const HeadArray *x) {
+    if (--w.left) { w.head += groups; w.p += hop; if (x) w.x += hop_x; }
+    else { w.unit += step; enter(w, p, x); }
+  };
+  float2 w[KEEP ? IT : 1][V];
+  auto fetch = [&](int k, uint32_t t, float2 *w) {
+    const uint32_t p = lane + k * a.lanes;
+    const float2 *cs = table + t * half;
+    if constexpr (V == 1) w[0] = cs[p];
+    else {
+#pragma unroll
+      for (int i = 0; i < V; i += 2) *reinterpret_cast<float4 *>(w + i) = *reinterpret_cast<const float4 *>(cs + (i / 2 * a.turned + p) * 2);
+    }
+  };
+  Place at, ahead;
+  at.unit = ahead.unit = block * kWarps + warp;
+  enter(at, d.out, nullptr);
+  enter(ahead, d.in, BOTH ? &d.x : nullptr);
+  uint32_t turn_out = 0;
+#pragma unroll
+  for (int i = 0; i < (V == 1 ? 1 : DEPTH - 1); ++i) {
+    load(ahead);
+    advance(ahead, hop, hop_x, d.in, BOTH ? &d.x : nullptr);
+  }
+  for (; at.unit < d.units;) {
+    // the unit's cosines and sines
+    const uint32_t first = d.parts > 1 ? at.unit / d.parts : at.unit * d.tokens, count = min(d.tokens, a.total - first) * half;
+    __syncwarp();
+    for (uint32_t i = wlane; i < count; i += 32) {
+      const uint32_t t = d.tokens > 1 ? i / half : 0, j = i - t * half, item = j / V, k = j % V;
+      table[t * half + (V == 1 ? item : (k / 2 * a.turned + item) * 2 + k % 2)] = turn_of(position_of(a, first + t), a.freq[j], a.amplitude, a.way);
+    }
+    __syncwarp();
+    if (KEEP && at.head < at.end) {
+#pragma unroll
+      for (int k = 0; k < IT; ++k) if (turns[k]) fetch(k, mine, w[KEEP ? k : 0]);
+    }
+    // heads of this unit, as many at a time as the warp has groups
+    for (const uint32_t unit = at.unit; at.unit == unit;) {
+      const bool live = at.head < at.end;
+      if constexpr (V == 1) now = next;
+      load(ahead);
+      advance(ahead, hop, hop_x, d.in, BOTH ? &d.x : nullptr);
+      if constexpr (V > 1) {
+        copies_wait<DEPTH - 1>();
+#pragma unroll
+        for (int k = 0; k < IT; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            now.in[k][j].raw = ring[(turn_out * PIECES + 2 * k + j) * kThreads];
+            if constexpr (BOTH) now.x[k][j].raw = ring[(turn_out * PIECES + 2 * IT + 2 * k + j) * kThreads];
+          }
+        turn_out = turn_out + 1 == DEPTH ? 0 : turn_out + 1;
       }
-      const float2 *cs = table + t * half;
+      float f[IT][2 * V], sq = 0.0f;
+#pragma unroll
+      for (int k = 0; k < IT; ++k) { now.in[k][0].floats(f[k]); now.in[k][1].floats(f[k] + V); }
       auto turn = [&](int k) {
         if (!live || !turns[k]) return;
-        const uint32_t p = lane + k * a.lanes;
-        float2 w[V];
-        if constexpr (V == 1) w[0] = cs[p];
-        else {
-#pragma unroll
-          for (int i = 0; i < V; i += 2) *reinterpret_cast<float4 *>(w + i) = *reinterpret_cast<const float4 *>(cs + (i / 2 * a.turned + p) * 2);
-        }
+        float2 own[V];
+        if constexpr (!KEEP) fetch(k, mine, own);
+        const float2 *cs = KEEP ? w[KEEP ? k : 0] : own;
         if (a.interleaved) {
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float u = f[k][2 * i], v = f[k][2 * i + 1], s = a.way * w[i].y;
-            f[k][2 * i] = u * w[i].x - v * s; f[k][2 * i + 1] = u * s + v * w[i].x;
+            const float u = f[k][2 * i], v = f[k][2 * i + 1];
+            f[k][2 * i] = u * cs[i].x - v * cs[i].y; f[k][2 * i + 1] = u * cs[i].y + v * cs[i].x;
           }
         } else {
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float u = f[k][i], v = f[k][V + i], s = a.way * w[i].y;
-            f[k][i] = u * w[i].x - v * s; f[k][V + i] = u * s + v * w[i].x;
+            const float u = f[k][i], v = f[k][V + i];
+            f[k][i] = u * cs[i].x - v * cs[i].y; f[k][V + i] = u * cs[i].y + v * cs[i].x;
           }
         }
       };
-      if (!BWD) {
-        if (NORM) {
+      if constexpr (!BWD) {
+        if constexpr (NORM) {
 #pragma unroll
           for (int k = 0; k < IT; ++k)
 #pragma unroll
             for (int i = 0; i < 2 * V; ++i) sq = fmaf(f[k][i], f[k][i], sq);
           for (uint32_t o = a.lanes / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-          r = rsqrtf(sq * a.inv_dim + a.epsilon);
+          const float r = rsqrtf(sq * a.inv_dim + a.epsilon);
 #pragma unroll
           for (int k = 0; k < IT; ++k)
 #pragma unroll
@@ -222,57 +312,63 @@ __global__ void __launch_bounds__(kThreads) rotary_heads_kernel(const RotaryArgs
       } else {
 #pragma unroll
         for (int k = 0; k < IT; ++k) turn(k);
-        if (NORM) {
+        float x[IT][2 * V], dot = 0.0f;
 #pragma unroll
-          for (int k = 0; k < IT; ++k) {
-            now.x[k][0].floats(x[k]);
-            now.x[k][1].floats(x[k] + V);
+        for (int k = 0; k < IT; ++k) {
+          now.x[k][0].floats(x[k]);
+          now.x[k][1].floats(x[k] + V);
 #pragma unroll
-            for (int i = 0; i < 2 * V; ++i) { sq = fmaf(x[k][i], x[k][i], sq); dot = fmaf(f[k][i] * g[k][i], x[k][i], dot); }
-          }
-          for (uint32_t o = a.lanes / 2; o > 0; o >>= 1) {
-            sq += __shfl_xor_sync(0xffffffffu, sq, o);
-            dot += __shfl_xor_sync(0xffffffffu, dot, o);
-          }
-          r = rsqrtf(sq * a.inv_dim + a.epsilon);
-          const float c = dot * r * r * a.inv_dim;
+          for (int i = 0; i < 2 * V; ++i) { sq = fmaf(x[k][i], x[k][i], sq); dot = fmaf(f[k][i] * g[k][i], x[k][i], dot); }
+        }
+        for (uint32_t o = a.lanes / 2; o > 0; o >>= 1) {
+          sq += __shfl_xor_sync(0xffffffffu, sq, o);
+          dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        }
+        const float r = rsqrtf(sq * a.inv_dim + a.epsilon), c = dot * r * r * r * a.inv_dim;
+        if (live) {
 #pragma unroll
           for (int k = 0; k < IT; ++k)
 #pragma unroll
             for (int i = 0; i < 2 * V; ++i) {
-              if (live) acc[k][i] = fmaf(f[k][i], x[k][i] * r, acc[k][i]);
-              f[k][i] = f[k][i] * (g[k][i] * r) - x[k][i] * (c * r);
+              acc[k][i] = fmaf(f[k][i], x[k][i] * r, acc[k][i]);
+              f[k][i] = f[k][i] * (g[k][i] * r) - x[k][i] * c;
             }
         }
       }
       if (live) {
-        T *out = place(d.out, t, h);
+        T *out = const_cast<T *>(at.p);
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
-          Few<T, V> w;
-          if (has[k]) { w.of(f[k]); w.store(out + e0[k]); }
-          if (second[k]) { w.of(f[k] + V); w.store(out + e1[k]); }
+          Few<T, V> o;
+          if (has[k]) { o.of(f[k]); o.store(out + e0[k]); }
+          if (second[k]) { o.of(f[k] + V); o.store(out + e1[k]); }
         }
       }
-      now = next; t = nt; h = nh;
+      advance(at, hop_out, 0, d.out, nullptr);
     }
   }
-  if (!BWD || !NORM || !d.want) return;
-  // the groups' sums in turn, in the order of the groups
-  float *sums = reinterpret_cast<float *>(shared);
-  for (uint32_t i = 0; i < groups; ++i) {
+  if constexpr (BWD && NORM) {
+    if (!d.want) return;
+    // the groups' sums join within the warp, the warps' in shared memory
+    float *sums = reinterpret_cast<float *>(shared);
+    if constexpr (V > 1) copies_wait<0>();
     __syncthreads();
-    if (group != i) continue;
 #pragma unroll
     for (int k = 0; k < IT; ++k)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (has[k]) sums[e0[k] + j] = acc[k][j] + (i ? sums[e0[k] + j] : 0.0f);
-        if (second[k]) sums[e1[k] + j] = acc[k][V + j] + (i ? sums[e1[k] + j] : 0.0f);
+      for (int j = 0; j < 2 * V; ++j) {
+        for (uint32_t o = a.lanes; o < 32; o *= 2) acc[k][j] += __shfl_xor_sync(0xffffffffu, acc[k][j], o);
+        const bool any = j < V ? has[k] : second[k];
+        if (group == 0 && any) sums[(size_t)warp * a.dim + (j < V ? e0[k] + j : e1[k] + j - V)] = acc[k][j];
       }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.dim; i += kThreads) {
+      float sum = 0.0f;
+#pragma unroll
+      for (uint32_t n = 0; n < kWarps; ++n) sum += sums[(size_t)n * a.dim + i];
+      a.partial[(uint64_t)blockIdx.x * a.dim + i] = sum;
+    }
   }
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < a.dim; i += kThreads) a.partial[(uint64_t)blockIdx.x * a.dim + i] = sums[i];
 }
 
 // The blocks' sums: a lane has an element of one of the two gradients, a warp every 32nd block
@@ -321,6 +417,17 @@ inline bool same_place(const AnodeHeads *o, const AnodeHeads *i, uint32_t batch,
 }
 
 #define TRY(call) do { const int rc_ = (call); if (rc_) return rc_; } while (0)
+
+template <typename T, int V, int IT, bool NORM, bool BWD>
+int launch_rotary(const RotaryArgs &a, uint32_t blocks, size_t tables, size_t sums, cudaStream_t stream)
+{
+  const auto kernel = rotary_heads_kernel<T, V, IT, NORM, BWD>;
+  size_t shared = ring_bytes(V, IT, NORM && BWD, sizeof(T)) + tables;
+  if (shared < sums) shared = sums;
+  static SharedMemory allowed;
+  if (!allowed.up_to((const void *)kernel, shared)) return ANODE_E_LAUNCH;
+  return launch(kernel, dim3(blocks), kThreads, shared, stream, a);
+}
 
 struct RotaryCall {
   int type, gamma_type, position_bytes;
@@ -373,7 +480,8 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
       put(d.x, c.x[k]);
     }
   }
-  a.total = (uint64_t)a.batch * a.seq;
+  if ((uint64_t)a.batch * a.seq >> 31) return ANODE_E_DIMS;
+  a.total = a.batch * a.seq;
   a.partial = static_cast<float *>(c.workspace);
   if (wants && (!c.workspace || !aligned_to(c.workspace, 16) ||
                 c.workspace_bytes < anode_gpu_rotary_positions_bwd_workspace_bytes(a.batch, a.seq, a.side[0].heads, a.side[1].heads, a.dim)))
@@ -395,35 +503,48 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
   a.items = a.turned + (a.dim - a.rot + 2 * v - 1) / (2 * v);
   a.lanes = 1;
   while (a.lanes < 32 && a.lanes < a.items) a.lanes *= 2;
-  const uint32_t each = (a.items + a.lanes - 1) / a.lanes, groups = kThreads / a.lanes;
-  uint32_t blocks = 0, most = 0;
+  const uint32_t each = (a.items + a.lanes - 1) / a.lanes, groups = 32 / a.lanes;
+  // blocks that the device holds; both arrays' warps work side by side, as many on either as its share of the heads asks for
+  const uint32_t room = sm_count() * (c.bwd && a.norm ? 2 : 3);
+  uint32_t blocks = 0, most = 1, units[2] = {0, 0}, passes[2];
+  double cost[2] = {0.0, 0.0};
   for (int k = 0; k < 1 + two; ++k) {
     RotarySide &d = a.side[k];
-    // about four heads to a group, fewer where that leaves SMs without a block
-    uint64_t tokens = (4 * groups + d.heads - 1) / d.heads, fit = 32768 / (4 * a.rot);
-    if (tokens > fit) tokens = fit;
-    if (tokens > kMostTokens) tokens = kMostTokens;
-    const uint64_t spread = (a.total + sm_count() - 1) / sm_count();
-    if (tokens > spread) tokens = spread;
-    if (tokens < 1) tokens = 1;
-    d.tokens = (uint32_t)tokens;
-    const uint64_t need = (a.total + d.tokens - 1) / d.tokens, limit = wants ? kMostParts / 2 : 1u << 29;
-    d.blocks = (uint32_t)(need < limit ? need : limit);
-    blocks += d.blocks;
+    // a warp has tokens that fill it, or a token's heads
+    d.tokens = d.heads < groups ? groups / d.heads : 1;
+    while (d.tokens > 1 && d.tokens * a.rot / 2 > 512) --d.tokens;
+    units[k] = (a.total - 1) / d.tokens + 1;
+    passes[k] = (d.heads + groups - 1) / groups;
     if (d.tokens > most) most = d.tokens;
   }
-  size_t shared = (size_t)most * a.rot / 2 * 8;
-  if (wants && shared < a.dim * 4) shared = a.dim * 4;
+  for (int k = 0; k < 1 + two; ++k) {
+    RotarySide &d = a.side[k];
+    // or, where that leaves warps of the device idle, a span of them
+    d.parts = room * kWarps / ((uint64_t)units[0] + units[1]);
+    if (d.parts > passes[k]) d.parts = passes[k];
+    if (d.parts < 1 || d.tokens > 1) d.parts = 1;
+    d.span = (passes[k] + d.parts - 1) / d.parts * groups;
+    d.parts = (d.heads + d.span - 1) / d.span;
+    d.units = units[k] * d.parts;
+    cost[k] = (double)units[k] * (passes[k] + 1.5 * d.parts);        // (the cosines and sines cost a unit about one and a half passes)
+  }
+  for (int k = 0; k < 1 + two; ++k) {
+    RotarySide &d = a.side[k];
+    const uint32_t need = (d.units - 1) / kWarps + 1, share = (uint32_t)(room * cost[k] / (cost[0] + cost[1]));
+    d.blocks = need < share ? need : share ? share : 1;
+    blocks += d.blocks;
+  }
+  const size_t tables = (size_t)kWarps * most * a.rot / 2 * 8, sums = wants ? (size_t)kWarps * a.dim * 4 : 0;
   TRY(by_type(c.type, [&](auto t) {
     using T = decltype(t);
-    auto go = [&](auto kernel) { return launch(kernel, dim3(blocks), kThreads, shared, stream, a); };
     auto with = [&](auto norm, auto bwd) {
       constexpr bool N = decltype(norm)::value, B = decltype(bwd)::value;
       if constexpr (sizeof(T) == 2)
-        if (v == 8) return each == 1 ? go(rotary_heads_kernel<T, 8, 1, N, B>) : go(rotary_heads_kernel<T, 8, 2, N, B>);
-      if (v == 4) return each == 1 ? go(rotary_heads_kernel<T, 4, 1, N, B>) : each == 2 ? go(rotary_heads_kernel<T, 4, 2, N, B>) : go(rotary_heads_kernel<T, 4, 4, N, B>);
-      return each == 1 ? go(rotary_heads_kernel<T, 1, 1, N, B>) : each == 2 ? go(rotary_heads_kernel<T, 1, 2, N, B>)
-           : each <= 4 ? go(rotary_heads_kernel<T, 1, 4, N, B>) : go(rotary_heads_kernel<T, 1, 16, N, B>);
+        if (v == 8) return each == 1 ? launch_rotary<T, 8, 1, N, B>(a, blocks, tables, sums, stream) : launch_rotary<T, 8, 2, N, B>(a, blocks, tables, sums, stream);
+      if (v == 4) return each == 1 ? launch_rotary<T, 4, 1, N, B>(a, blocks, tables, sums, stream)
+                       : each == 2 ? launch_rotary<T, 4, 2, N, B>(a, blocks, tables, sums, stream) : launch_rotary<T, 4, 4, N, B>(a, blocks, tables, sums, stream);
+      return each == 1 ? launch_rotary<T, 1, 1, N, B>(a, blocks, tables, sums, stream) : each == 2 ? launch_rotary<T, 1, 2, N, B>(a, blocks, tables, sums, stream)
+           : each <= 4 ? launch_rotary<T, 1, 4, N, B>(a, blocks, tables, sums, stream) : launch_rotary<T, 1, 16, N, B>(a, blocks, tables, sums, stream);
     };
     const std::true_type yes;
     const std::false_type no;

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/anode_routines_gpu.h"
@@ -144,6 +145,29 @@ template <typename F> inline int by_type(int type, F f)
 {
   return type == ANODE_TYPE_F32 ? f(float()) : type == ANODE_TYPE_F16 ? f(__half()) : f(__nv_bfloat16());
 }
+
+// A kernel's leave to use more dynamic shared memory than 48 KB, asked for once per device and for all that a block may have
+class SharedMemory {
+ public:
+  bool up_to(const void *kernel, size_t bytes)
+  {
+    if (bytes <= 48 * 1024) return true;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (done_.load(std::memory_order_relaxed) >> dev & 1) return true;
+    cudaFuncAttributes f;
+    if (cudaFuncGetAttributes(&f, kernel) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)f.sharedSizeBytes) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return false;
+    }
+    done_.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return true;
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
 
 // A launch that may overlap the tail of the kernel before it on the stream: every kernel here waits for that one's results
 // before it touches memory.

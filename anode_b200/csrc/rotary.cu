@@ -3,13 +3,15 @@
 //   n = x*r*gamma, r = (mean(x^2) + epsilon)^-1/2 over the head;   angle = position*freq[i]
 //   (n[u], n[v]) -> A*(n[u] cos - n[v] sin, n[u] sin + n[v] cos);   backward: the same with -sin, then the norm's adjoint
 //
-// A head is read once and written once.  It belongs to a group of lanes of a warp; a lane has ITEMS of 2V elements each: V pairs,
-// or 2V elements that pass.  In the half layout an item is two vectors rot/2 apart, so that both elements of a pair are in one lane and the
-// turn needs no exchange; only the norm's sums go across the group.  Lanes keep their items from head to head, and with them the
-// weights and the sums of the weights' gradients.
-// A warp takes a token of the queries or of the keys (or as many tokens as fill it, or part of a token's heads where there are few tokens),
-// makes its cosines and sines once, in shared memory of its own, and goes through the heads with the next ones' data on their way by
-// asynchronous copies, each lane into a ring of its own: no warp waits for another, and no lane for what another lane copies.
+// A head is read once and written once.  It belongs to a group of lanes of a warp, and a warp takes a token of the queries or of the keys (or
+// as many tokens as fill it, or part of a token's heads where there are few tokens), makes its cosines and sines once, in shared memory of its
+// own, and goes through the heads with the next ones' data on their way by asynchronous copies: no warp waits for another.
+//
+// rotary_heads_kernel: the pairs' places divide by 16 (or 8) bytes.  A lane has ITEMS of 2V elements each: V pairs, or 2V elements that pass.
+// In the half layout an item is two vectors rot/2 apart, so that both elements of a pair are in one lane and the turn needs no exchange;
+// only the norm's sums go across the group.  What a lane computes with is what it copied itself.  Lanes keep their items from head to head,
+// and with them the weights and the sums of the weights' gradients.
+// rotary_pairs_kernel: pairs anywhere.  Heads are copied as they lie, a lane has single pairs of them and puts the results in their place.
 #include "bn_host.h"
 #include "rows.cuh"
 
@@ -17,8 +19,8 @@ namespace anode_b200 {
 namespace rows {
 
 constexpr uint32_t kThreads = 256, kMostDim = 1024;
-constexpr uint32_t kMostParts = 148 * 4;      // blocks that have sums of the weights' gradients
 constexpr uint32_t kWarps = kThreads / 32;
+constexpr uint32_t kMostParts = 148 * 4;      // blocks that have sums of the weights' gradients
 
 struct HeadArray {
   void *p;
@@ -46,44 +48,58 @@ struct RotaryArgs {
   float *partial;                      // [blocks, dim] of the gradients of the weights
   uint32_t lanes, items, turned;       // lanes of a head's group; items of a head, and those of them that turn
   float way;                           // 1 forward, -1 back
+  uint32_t copy, slot;                 // of rotary_pairs_kernel: bytes of a copy, bytes of a head's place in shared memory
 };
 
 // V elements, moved at once
 template <int BYTES> struct RawOf;
 template <> struct RawOf<16> { typedef uint4 type; };
 template <> struct RawOf<8> { typedef uint2 type; };
-template <> struct RawOf<4> { typedef uint32_t type; };
-template <> struct RawOf<2> { typedef uint16_t type; };
 template <typename T, int V> struct Few {
-  union { typename RawOf<V * sizeof(T)>::type raw; T e[V]; uint32_t w[(V * sizeof(T) + 3) / 4]; };
+  typedef typename RawOf<V * sizeof(T)>::type Raw;
+  union { Raw raw; uint32_t w[V * sizeof(T) / 4]; };
   __device__ __forceinline__ Few() {}
-  __device__ __forceinline__ void load(const T *p) { raw = *reinterpret_cast<const decltype(raw) *>(p); }
-  __device__ __forceinline__ void clear() { raw = decltype(raw){}; }
-  __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<decltype(raw) *>(p) = raw; }
-  __device__ __forceinline__ void floats(float *f) const
+  // elements 2m and 2m + 1
+  __device__ __forceinline__ float2 two(int m) const
   {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value && V > 1) {
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = to_float(e[i]);
-    }
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * m]), __uint_as_float(w[2 * m + 1]));
+    else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w[m]));
+    else return make_float2(__uint_as_float(w[m] << 16), __uint_as_float(w[m] & 0xffff0000u));
   }
-  __device__ __forceinline__ void of(const float *f)
+  __device__ __forceinline__ void put(int m, float x, float y)
   {
-    if constexpr (sizeof(T) == 2 && V > 1) {
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) {
-        if constexpr (std::is_same<T, __half>::value) { const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t *>(&v); }
-        else { const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t *>(&v); }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) e[i] = from_float<T>(f[i]);
-    }
+    if constexpr (sizeof(T) == 4) { w[2 * m] = __float_as_uint(x); w[2 * m + 1] = __float_as_uint(y); }
+    else if constexpr (std::is_same<T, __half>::value) { const __half2 v = __floats2half2_rn(x, y); w[m] = *reinterpret_cast<const uint32_t *>(&v); }
+    else { const __nv_bfloat162 v = __floats2bfloat162_rn(x, y); w[m] = *reinterpret_cast<const uint32_t *>(&v); }
   }
 };
+// An item's 2V elements as pairs of floats: f[0..V/2) the first elements of the pairs that turn together, f[V/2..V) the second ones
+template <typename T, int V> __device__ __forceinline__ void spread(const Few<T, V> (&in)[2], bool interleaved, float2 *f)
+{
+  if (interleaved) {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+      const float2 a = in[2 * j / (V / 2)].two(2 * j % (V / 2)), b = in[(2 * j + 1) / (V / 2)].two((2 * j + 1) % (V / 2));
+      f[j] = make_float2(a.x, b.x); f[V / 2 + j] = make_float2(a.y, b.y);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) { f[j] = in[0].two(j); f[V / 2 + j] = in[1].two(j); }
+  }
+}
+template <typename T, int V> __device__ __forceinline__ void gather(Few<T, V> (&out)[2], bool interleaved, const float2 *f)
+{
+  if (interleaved) {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+      out[2 * j / (V / 2)].put(2 * j % (V / 2), f[j].x, f[V / 2 + j].x);
+      out[(2 * j + 1) / (V / 2)].put((2 * j + 1) % (V / 2), f[j].y, f[V / 2 + j].y);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) { out[0].put(j, f[j].x, f[j].y); out[1].put(j, f[V / 2 + j].x, f[V / 2 + j].y); }
+  }
+}
 
 template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const void *from)
 {
@@ -94,43 +110,106 @@ template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const 
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-__device__ __forceinline__ double position_of(const RotaryArgs &a, uint32_t token)
+// The position of a unit's token `lane` (lanes beyond its tokens: 0), as it is asked for a unit ahead
+__device__ __forceinline__ long long position_of(const RotaryArgs &a, uint32_t first, uint32_t tokens, uint32_t lane)
 {
-  const uint32_t b = a.batch == 1 ? 0 : token / a.seq;
+  if (lane >= tokens || first >= a.total || lane >= a.total - first) return 0;
+  const uint32_t token = first + lane, b = a.batch == 1 ? 0 : token / a.seq;
   const uint64_t i = b * a.pos_batch + (token - b * a.seq) * a.pos_seq;
-  return a.position_bytes == 8 ? (double)static_cast<const long long *>(a.positions)[i] : (double)static_cast<const int *>(a.positions)[i];
+  return a.position_bytes == 8 ? static_cast<const long long *>(a.positions)[i] : static_cast<const int *>(a.positions)[i];
 }
-// cos and sin of position*freq, by whole turns in f64: what is left of them is exact, and small
-__device__ __forceinline__ float2 turn_of(double position, double freq, float amplitude, float way)
+// Whole turns per position of each pair, for the block
+__device__ __forceinline__ void make_rates(const RotaryArgs &a, double *rates)
 {
-  const double turns = position * (freq * 0.15915494309189533577);      // 1/(2 pi)
-  float s, c;
-  sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-  return make_float2(c * amplitude, s * amplitude * way);
+  for (uint32_t i = threadIdx.x; i < a.rot / 2; i += kThreads) rates[i] = a.freq[i] * 0.15915494309189533577;      // 1/(2 pi)
+}
+// The cosines and sines of a unit's tokens: put(t, j, (cos, sin)) for each pair j of token t.  Angles are reduced to what is left of
+// whole turns in f64: that is exact, and small.
+template <typename Put> __device__ __forceinline__ void make_table(const RotaryArgs &a, const double *rates, uint32_t tokens, long long position, Put put)
+{
+  const uint32_t half = a.rot / 2, lane = threadIdx.x & 31, count = tokens * half, rounds = (count + 31) / 32;
+  const uint32_t inverse = 0xffffffffu / half + 1;          // i/half = the upper half of i*inverse, for the few hundred i there are (half = 1: 0)
+  const double own = (double)position;
+#pragma unroll 2
+  for (uint32_t n = 0; n < rounds; ++n) {
+    const uint32_t i = n * 32 + lane, t = tokens == 1 ? 0 : half == 1 ? i : __umulhi(i, inverse), j = min(i - t * half, half - 1);
+    const double turns = __shfl_sync(0xffffffffu, own, min(t, 31u)) * rates[j];
+    float s, c;
+    sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+    if (i < count) put(t, j, make_float2(c * a.amplitude, s * a.amplitude * a.way));
+  }
+}
+
+// Where a group of lanes is: the unit, its head (none: from `end` on), the passes that the unit has left, and addresses
+template <typename T> struct Place { uint32_t unit, head, end, left; const T *p, *x; };
+// A group's way through its warp's units: as many heads at a time as the warp has groups
+template <typename T> struct Walk {
+  const RotaryArgs &a;
+  const RotarySide &d;
+  uint32_t group, groups, mine, step;       // mine: of the unit's tokens
+  __device__ __forceinline__ Walk(const RotaryArgs &a, const RotarySide &d, uint32_t group, uint32_t groups)
+      : a(a), d(d), group(group), groups(groups), mine(d.tokens > 1 ? group / d.heads : 0), step(d.blocks * kWarps) {}
+  // the first token of a unit; none, beyond the last one
+  __device__ __forceinline__ uint32_t token(uint32_t unit) const { return unit >= d.units ? a.total : d.parts > 1 ? unit / d.parts : unit * d.tokens; }
+  // the first head of the unit
+  __device__ __forceinline__ void enter(Place<T> &w, const HeadArray &p, const HeadArray *x) const
+  {
+    if (w.unit >= d.units) { w.head = w.end = 0; w.left = 1; return; }
+    const uint32_t first = token(w.unit), low = d.parts > 1 ? (w.unit - first * d.parts) * d.span : 0, token = first + mine;
+    w.end = min(d.heads, low + d.span);
+    w.left = d.tokens > 1 ? 1 : (w.end - low + groups - 1) / groups;
+    w.head = low + group - mine * d.heads;
+    if (mine >= d.tokens || token >= a.total || group >= groups) w.head = w.end = 0;
+    const uint32_t b = a.batch == 1 ? 0 : token / a.seq, s = token - b * a.seq;
+    w.p = static_cast<const T *>(p.p) + b * p.batch + s * p.seq + w.head * p.head;
+    if (x) w.x = static_cast<const T *>(x->p) + b * x->batch + s * x->seq + w.head * x->head;
+  }
+  __device__ __forceinline__ void advance(Place<T> &w, const HeadArray &p, const HeadArray *x) const
+  {
+    if (--w.left) {
+      // (a group beyond the last stays there: its end is 0)
+      w.head += groups; w.p += p.head * groups;
+      if (x) w.x += x->head * groups;
+    } else { w.unit += step; enter(w, p, x); }
+  }
+};
+// The sum over a group of lanes, the same bits in all of them
+__device__ __forceinline__ float group_sum(float v, uint32_t lanes, uint32_t first)
+{
+  if ((lanes & (lanes - 1)) == 0) {
+    for (uint32_t o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
+  float sum = 0.0f;
+  for (uint32_t i = 0; i < lanes; ++i) sum += __shfl_sync(0xffffffffu, v, first + i);
+  return sum;
 }
 
 // Registers: two or three blocks of a multiprocessor
-constexpr int resident(int floats, bool both) { return floats > 16 ? 1 : both ? 2 : 3; }
-// Heads of a lane's ring, and its bytes: pieces of less than four bytes cannot be copied asynchronously and go through registers
-__host__ __device__ constexpr int ring_depth(int v, int it) { return v == 1 ? 1 : it == 1 ? 4 : 2; }
-__host__ __device__ constexpr size_t ring_bytes(int v, int it, bool both, size_t e) { return v == 1 ? 0 : (size_t)ring_depth(v, it) * kThreads * it * 2 * v * e * (both ? 2 : 1); }
+__host__ __device__ constexpr int resident(int floats, bool norm) { return floats > 16 ? 1 : norm ? 2 : 3; }
+// Heads of a lane's ring, and its bytes
+__host__ __device__ constexpr int ring_depth(int it) { return it == 1 ? 4 : 2; }
+__host__ __device__ constexpr size_t ring_bytes(int v, int it, bool both, size_t e) { return (size_t)ring_depth(it) * kThreads * it * 2 * v * e * (both ? 2 : 1); }
 
 template <typename T, int V, int IT, bool NORM, bool BWD>
-__global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM && BWD)) rotary_heads_kernel(const RotaryArgs a)
+__global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_heads_kernel(const RotaryArgs a)
 {
   constexpr bool BOTH = NORM && BWD;        // two arrays are read
-  constexpr bool KEEP = V * IT <= 8;        // a lane's cosines and sines stay in its registers from head to head
-  constexpr int DEPTH = ring_depth(V, IT), PIECES = IT * 2 * (BOTH ? 2 : 1);
-  typedef typename RawOf<V * sizeof(T)>::type Raw;
-  // the rings, [depth][piece][thread]; of each warp, [tokens][rot/2] cosines and sines, pair j = item*V + i of a token at
-  // (i/2*turned + item)*2 + i%2, so that lanes read 16 bytes side by side; in their place the warps' sums of the weights' gradients, when the block is done
+  constexpr bool KEEP = V * IT <= (BOTH ? 4 : 8);       // a lane's cosines and sines stay in its registers from head to head
+  constexpr int DEPTH = ring_depth(IT), PIECES = IT * 2 * (BOTH ? 2 : 1);
+  typedef typename Few<T, V>::Raw Raw;
+  // each pair's turns per position; the rings, [depth][piece][thread]; of each warp, [tokens] cosines and sines: pairs j = item*V + i and the next of a token at i/2*turned + item,
+  // both cosines and then both sines, so that lanes read 16 bytes side by side; in their place the warps' sums of the weights' gradients, when
+  // the block is done
   extern __shared__ float4 shared[];
   const uint32_t which = blockIdx.x >= a.side[0].blocks, block = which ? blockIdx.x - a.side[0].blocks : blockIdx.x;
   const RotarySide &d = a.side[which];
-  const uint32_t wlane = threadIdx.x & 31, warp = threadIdx.x >> 5, lane = wlane & (a.lanes - 1), group = wlane / a.lanes, groups = 32 / a.lanes;
-  const uint32_t half = a.rot / 2, heads = d.heads;
-  Raw *ring = reinterpret_cast<Raw *>(shared) + threadIdx.x;
-  float2 *table = reinterpret_cast<float2 *>(reinterpret_cast<char *>(shared) + ring_bytes(V, IT, BOTH, sizeof(T))) + (size_t)warp * d.tokens * half;
+  const uint32_t wlane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / a.lanes, group = wlane / a.lanes, lane = wlane - group * a.lanes;
+  const uint32_t half = a.rot / 2;
+  const bool interleaved = a.interleaved;
+  double *rates = reinterpret_cast<double *>(shared);
+  Raw *ring = reinterpret_cast<Raw *>(shared + half / 2) + threadIdx.x;
+  float4 *table = shared + half / 2 + ring_bytes(V, IT, BOTH, sizeof(T)) / 16 + (size_t)warp * d.tokens * half / 2;
   // this lane's items: two vectors, at e0 and e1
   uint32_t e0[IT], e1[IT];
   bool has[IT], second[IT], turns[IT];
@@ -139,64 +218,55 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM && BWD)) r
     const uint32_t p = lane + k * a.lanes;
     turns[k] = p < a.turned;
     has[k] = p < a.items;
-    e0[k] = !turns[k] ? a.rot + (p - a.turned) * 2 * V : a.interleaved ? p * 2 * V : p * V;
-    e1[k] = turns[k] && !a.interleaved ? half + p * V : e0[k] + V;
+    e0[k] = !turns[k] ? a.rot + (p - a.turned) * 2 * V : interleaved ? p * 2 * V : p * V;
+    e1[k] = turns[k] && !interleaved ? half + p * V : e0[k] + V;
     second[k] = has[k] && e1[k] < a.dim;
   }
   pdl_wait();
-  float g[NORM ? IT : 1][2 * V], acc[NORM && BWD ? IT : 1][2 * V];
-  if constexpr (NORM) {
-    const bool aligned_gamma = ((uintptr_t)d.gamma.p & 15) == 0;
+  make_rates(a, rates);
+  const bool aligned_gamma = ((uintptr_t)d.gamma.p & 15) == 0;
+  auto weights = [&](int k, float2 *g) {
+    float v[2 * V];
 #pragma unroll
-    for (int k = 0; k < IT; ++k)
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t e = j ? e1[k] : e0[k];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const bool any = j ? second[k] : has[k];
-        const uint32_t e = j ? e1[k] : e0[k];
+      for (int i = 0; i < V; ++i) v[j * V + i] = 0.0f;
+      if (!(j ? second[k] : has[k])) continue;
+      if (aligned_gamma) d.gamma.load<V>(e, v + j * V);
+      else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) { g[k][j * V + i] = 0.0f; if constexpr (BWD) acc[k][j * V + i] = 0.0f; }
-        if (!any) continue;
-        if (V > 1 && aligned_gamma) { if constexpr (V > 1) d.gamma.load<V>(e, g[k] + j * V); }
-        else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) g[k][j * V + i] = d.gamma.at(e + i);
-        }
+        for (int i = 0; i < V; ++i) v[j * V + i] = d.gamma.at(e + i);
       }
+    }
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+      g[j] = interleaved ? make_float2(v[4 * j], v[4 * j + 2]) : make_float2(v[2 * j], v[2 * j + 1]);
+      g[V / 2 + j] = interleaved ? make_float2(v[4 * j + 1], v[4 * j + 3]) : make_float2(v[V + 2 * j], v[V + 2 * j + 1]);
+    }
+  };
+  float2 g[NORM ? IT : 1][V], acc[BOTH ? IT : 1][V];
+  if constexpr (NORM) {
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+      weights(k, g[k]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) if constexpr (BOTH) acc[k][i] = both(0.0f);
+    }
   }
-  struct Head { Few<T, V> in[IT][2], x[BOTH ? IT : 1][2]; } now, next;
-  // (what a lane does not have is never loaded, and counts as zeros)
+  // (what a lane does not have is never copied, and counts as zeros)
 #pragma unroll
   for (int k = 0; k < IT; ++k)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if constexpr (V == 1) {
-        now.in[k][j].clear(); next.in[k][j].clear();
-        if constexpr (BOTH) { now.x[k][j].clear(); next.x[k][j].clear(); }
-      } else if (!(j ? second[k] : has[k])) {
+    for (int j = 0; j < 2; ++j)
+      if (!(j ? second[k] : has[k]))
         for (int i = 0; i < DEPTH; ++i) {
           ring[(i * PIECES + 2 * k + j) * kThreads] = Raw{};
           if constexpr (BOTH) ring[(i * PIECES + 2 * IT + 2 * k + j) * kThreads] = Raw{};
         }
-      }
-    }
-  // Where this group is: the unit, its head (none: from `end` on), the passes that the unit has left, and addresses
-  struct Place { uint32_t unit, head, end, left; const T *p, *x; };
-  const uint32_t step = d.blocks * kWarps, mine = d.tokens > 1 ? group / heads : 0;      // mine: of the unit's tokens
-  const uint64_t hop = d.in.head * groups, hop_x = BOTH ? d.x.head * groups : 0, hop_out = d.out.head * groups;
-  auto enter = [&](Place &w, const HeadArray &p, const HeadArray *x) {       // the first head of its unit
-    if (w.unit >= d.units) { w.head = w.end = 0; w.left = 1; return; }
-    const uint32_t first = d.parts > 1 ? w.unit / d.parts : w.unit * d.tokens, low = d.parts > 1 ? (w.unit - first * d.parts) * d.span : 0;
-    const uint32_t token = first + mine;
-    w.end = min(heads, low + d.span);
-    w.left = d.tokens > 1 ? 1 : (w.end - low + groups - 1) / groups;
-    w.head = low + group - mine * heads;
-    if (mine >= d.tokens || token >= a.total) w.head = w.end;
-    const uint32_t b = a.batch == 1 ? 0 : token / a.seq, s = token - b * a.seq;
-    w.p = static_cast<const T *>(p.p) + b * p.batch + s * p.seq + w.head * p.head;
-    if (x) w.x = static_cast<const T *>(x->p) + b * x->batch + s * x->seq + w.head * x->head;
-  };
-  uint32_t turn_in = 0;                  // the ring's place that is filled next
-  auto load = [&](const Place &w) {
+  const Walk<T> walk(a, d, group, groups);
+  uint32_t turn_in = 0, turn_out = 0;        // the ring's places that are filled and emptied next
+  auto load = [&](const Place<T> &w) {
     if (w.head < w.end) {
 #pragma unroll
       for (int k = 0; k < IT; ++k)
@@ -204,163 +274,332 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM && BWD)) r
         for (int j = 0; j < 2; ++j) {
           if (!(j ? second[k] : has[k])) continue;
           const uint32_t e = j ? e1[k] : e0[k];
-          if constexpr (V == 1) {
-            next.in[k][j].load(w.p + e);
-            if constexpr (BOTH) next.x[k][j].load(w.x + e);
-          } else {
-            copy_async<V * sizeof(T)>(ring + (turn_in * PIECES + 2 * k + j) * kThreads, w.p + e);
-            if constexpr (BOTH) copy_async<V * sizeof(T)>(ring + (turn_in * PIECES + 2 * IT + 2 * k + j) * kThreads, w.x + e);
-          }
+          copy_async<V * sizeof(T)>(ring + (turn_in * PIECES + 2 * k + j) * kThreads, w.p + e);
+          if constexpr (BOTH) copy_async<V * sizeof(T)>(ring + (turn_in * PIECES + 2 * IT + 2 * k + j) * kThreads, w.x + e);
         }
     }
-    if constexpr (V > 1) {
-      copies_commit();
-      turn_in = turn_in + 1 == DEPTH ? 0 : turn_in + 1;
-    }
+    copies_commit();
+    turn_in = (turn_in + 1) & (DEPTH - 1);
   };
-  auto advance = [&](Place &w, uint64_t hop, uint64_t hop_x, const HeadArray &p, const HeadArray *x) {
-    if (--w.left) { w.head += groups; w.p += hop; if (x) w.x += hop_x; }
-    else { w.unit += step; enter(w, p, x); }
-  };
-  float2 w[KEEP ? IT : 1][V];
-  auto fetch = [&](int k, uint32_t t, float2 *w) {
-    const uint32_t p = lane + k * a.lanes;
-    const float2 *cs = table + t * half;
-    if constexpr (V == 1) w[0] = cs[p];
-    else {
+  // f -> f*straight + (its partner)*across, with the forward pass's weights in it
+  struct Turn { float2 straight[V], across[V]; };
+  const uint32_t row = min(walk.mine, d.tokens - 1);       // (a group without a token reads another's: it stays within the table)
+  auto coefficients = [&](int k, Turn &o) {
+    const float2 *by = g[NORM ? k : 0];
 #pragma unroll
-      for (int i = 0; i < V; i += 2) *reinterpret_cast<float4 *>(w + i) = *reinterpret_cast<const float4 *>(cs + (i / 2 * a.turned + p) * 2);
+    for (int i = 0; i < V / 2; ++i) {
+      float4 t = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
+      if (turns[k]) t = table[row * half / 2 + i * a.turned + lane + k * a.lanes];
+      const float2 c = make_float2(t.x, t.y), s = make_float2(t.z, t.w), minus = make_float2(-t.z, -t.w);
+      if constexpr (NORM && !BWD) {
+        o.straight[i] = mul2(by[i], c); o.across[i] = mul2(by[V / 2 + i], minus);
+        o.straight[V / 2 + i] = mul2(by[V / 2 + i], c); o.across[V / 2 + i] = mul2(by[i], s);
+      } else {
+        o.straight[i] = c; o.across[i] = minus;
+        o.straight[V / 2 + i] = c; o.across[V / 2 + i] = s;
+      }
     }
   };
-  Place at, ahead;
+  auto turn = [&](int k, float2 *f, const Turn &o) {
+    if (turns[k]) {
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {
+        const float2 u = f[j], v = f[V / 2 + j];
+        f[j] = fma2(v, o.across[j], mul2(u, o.straight[j]));
+        f[V / 2 + j] = fma2(u, o.across[V / 2 + j], mul2(v, o.straight[V / 2 + j]));
+      }
+    } else if (NORM && !BWD) {      // (elements that pass have no partner: its infinity would be a NaN here)
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = mul2(f[j], o.straight[j]);
+    }
+  };
+  Turn kept[KEEP ? IT : 1];
+  const HeadArray *from = BOTH ? &d.x : nullptr;
+  Place<T> at, ahead;
   at.unit = ahead.unit = block * kWarps + warp;
-  enter(at, d.out, nullptr);
-  enter(ahead, d.in, BOTH ? &d.x : nullptr);
-  uint32_t turn_out = 0;
+  walk.enter(at, d.out, nullptr);
+  walk.enter(ahead, d.in, from);
+  long long position = position_of(a, walk.token(at.unit), d.tokens, wlane);
 #pragma unroll
-  for (int i = 0; i < (V == 1 ? 1 : DEPTH - 1); ++i) {
+  for (int i = 0; i < DEPTH - 1; ++i) {
     load(ahead);
-    advance(ahead, hop, hop_x, d.in, BOTH ? &d.x : nullptr);
+    walk.advance(ahead, d.in, from);
   }
-  for (; at.unit < d.units;) {
+  __syncthreads();
+  while (at.unit < d.units) {
     // the unit's cosines and sines
-    const uint32_t first = d.parts > 1 ? at.unit / d.parts : at.unit * d.tokens, count = min(d.tokens, a.total - first) * half;
     __syncwarp();
-    for (uint32_t i = wlane; i < count; i += 32) {
-      const uint32_t t = d.tokens > 1 ? i / half : 0, j = i - t * half, item = j / V, k = j % V;
-      table[t * half + (V == 1 ? item : (k / 2 * a.turned + item) * 2 + k % 2)] = turn_of(position_of(a, first + t), a.freq[j], a.amplitude, a.way);
-    }
+    make_table(a, rates, d.tokens, position, [&](uint32_t t, uint32_t j, float2 cs) {
+      float *to = reinterpret_cast<float *>(table + t * half / 2 + j % V / 2 * a.turned + j / V) + j % 2;
+      to[0] = cs.x; to[2] = cs.y;
+    });
+    position = position_of(a, walk.token(at.unit + walk.step), d.tokens, wlane);
     __syncwarp();
-    if (KEEP && at.head < at.end) {
+    if constexpr (KEEP) {
 #pragma unroll
-      for (int k = 0; k < IT; ++k) if (turns[k]) fetch(k, mine, w[KEEP ? k : 0]);
+      for (int k = 0; k < IT; ++k) coefficients(k, kept[k]);
     }
-    // heads of this unit, as many at a time as the warp has groups
     for (const uint32_t unit = at.unit; at.unit == unit;) {
       const bool live = at.head < at.end;
-      if constexpr (V == 1) now = next;
       load(ahead);
-      advance(ahead, hop, hop_x, d.in, BOTH ? &d.x : nullptr);
-      if constexpr (V > 1) {
-        copies_wait<DEPTH - 1>();
+      walk.advance(ahead, d.in, from);
+      copies_wait<DEPTH - 1>();
+      float2 f[IT][V], sq2 = both(0.0f);
+#pragma unroll
+      for (int k = 0; k < IT; ++k) {
+        Few<T, V> in[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) in[j].raw = ring[(turn_out * PIECES + 2 * k + j) * kThreads];
+        spread(in, interleaved, f[k]);
+      }
+      if constexpr (NORM && !BWD) {
 #pragma unroll
         for (int k = 0; k < IT; ++k)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            now.in[k][j].raw = ring[(turn_out * PIECES + 2 * k + j) * kThreads];
-            if constexpr (BOTH) now.x[k][j].raw = ring[(turn_out * PIECES + 2 * IT + 2 * k + j) * kThreads];
-          }
-        turn_out = turn_out + 1 == DEPTH ? 0 : turn_out + 1;
+          for (int i = 0; i < V; ++i) sq2 = fma2(f[k][i], f[k][i], sq2);
+        const float2 r = both(rsqrtf(group_sum(sq2.x + sq2.y, a.lanes, wlane - lane) * a.inv_dim + a.epsilon));
+#pragma unroll
+        for (int k = 0; k < IT; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) f[k][i] = mul2(f[k][i], r);
       }
-      float f[IT][2 * V], sq = 0.0f;
 #pragma unroll
-      for (int k = 0; k < IT; ++k) { now.in[k][0].floats(f[k]); now.in[k][1].floats(f[k] + V); }
-      auto turn = [&](int k) {
-        if (!live || !turns[k]) return;
-        float2 own[V];
-        if constexpr (!KEEP) fetch(k, mine, own);
-        const float2 *cs = KEEP ? w[KEEP ? k : 0] : own;
-        if (a.interleaved) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float u = f[k][2 * i], v = f[k][2 * i + 1];
-            f[k][2 * i] = u * cs[i].x - v * cs[i].y; f[k][2 * i + 1] = u * cs[i].y + v * cs[i].x;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float u = f[k][i], v = f[k][V + i];
-            f[k][i] = u * cs[i].x - v * cs[i].y; f[k][V + i] = u * cs[i].y + v * cs[i].x;
-          }
+      for (int k = 0; k < IT; ++k) {
+        if constexpr (KEEP) turn(k, f[k], kept[KEEP ? k : 0]);
+        else {
+          Turn own;
+          coefficients(k, own);
+          turn(k, f[k], own);
         }
-      };
-      if constexpr (!BWD) {
-        if constexpr (NORM) {
-#pragma unroll
-          for (int k = 0; k < IT; ++k)
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) sq = fmaf(f[k][i], f[k][i], sq);
-          for (uint32_t o = a.lanes / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-          const float r = rsqrtf(sq * a.inv_dim + a.epsilon);
-#pragma unroll
-          for (int k = 0; k < IT; ++k)
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) f[k][i] *= r * g[k][i];
-        }
-#pragma unroll
-        for (int k = 0; k < IT; ++k) turn(k);
-      } else {
-#pragma unroll
-        for (int k = 0; k < IT; ++k) turn(k);
-        float x[IT][2 * V], dot = 0.0f;
+      }
+      if constexpr (BOTH) {
+        float2 x[IT][V], dot2 = both(0.0f);
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
-          now.x[k][0].floats(x[k]);
-          now.x[k][1].floats(x[k] + V);
+          Few<T, V> in[2];
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) { sq = fmaf(x[k][i], x[k][i], sq); dot = fmaf(f[k][i] * g[k][i], x[k][i], dot); }
+          for (int j = 0; j < 2; ++j) in[j].raw = ring[(turn_out * PIECES + 2 * IT + 2 * k + j) * kThreads];
+          spread(in, interleaved, x[k]);
+#pragma unroll
+          for (int i = 0; i < V; ++i) { sq2 = fma2(x[k][i], x[k][i], sq2); dot2 = fma2(mul2(f[k][i], g[k][i]), x[k][i], dot2); }
         }
-        for (uint32_t o = a.lanes / 2; o > 0; o >>= 1) {
-          sq += __shfl_xor_sync(0xffffffffu, sq, o);
-          dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        }
-        const float r = rsqrtf(sq * a.inv_dim + a.epsilon), c = dot * r * r * r * a.inv_dim;
+        const float r = rsqrtf(group_sum(sq2.x + sq2.y, a.lanes, wlane - lane) * a.inv_dim + a.epsilon);
+        const float2 r2 = both(r), c = both(-group_sum(dot2.x + dot2.y, a.lanes, wlane - lane) * r * r * r * a.inv_dim);
         if (live) {
 #pragma unroll
           for (int k = 0; k < IT; ++k)
 #pragma unroll
-            for (int i = 0; i < 2 * V; ++i) {
-              acc[k][i] = fmaf(f[k][i], x[k][i] * r, acc[k][i]);
-              f[k][i] = f[k][i] * (g[k][i] * r) - x[k][i] * c;
+            for (int i = 0; i < V; ++i) {
+              const float2 fr = mul2(f[k][i], r2);
+              acc[k][i] = fma2(fr, x[k][i], acc[k][i]);
+              f[k][i] = fma2(fr, g[k][i], mul2(x[k][i], c));
             }
         }
       }
+      turn_out = (turn_out + 1) & (DEPTH - 1);
       if (live) {
         T *out = const_cast<T *>(at.p);
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
-          Few<T, V> o;
-          if (has[k]) { o.of(f[k]); o.store(out + e0[k]); }
-          if (second[k]) { o.of(f[k] + V); o.store(out + e1[k]); }
+          Few<T, V> o[2];
+          gather(o, interleaved, f[k]);
+          if (has[k]) *reinterpret_cast<Raw *>(out + e0[k]) = o[0].raw;
+          if (second[k]) *reinterpret_cast<Raw *>(out + e1[k]) = o[1].raw;
         }
       }
-      advance(at, hop_out, 0, d.out, nullptr);
+      walk.advance(at, d.out, nullptr);
     }
   }
-  if constexpr (BWD && NORM) {
+  if constexpr (BOTH) {
     if (!d.want) return;
-    // the groups' sums join within the warp, the warps' in shared memory
+    // the warp's groups add their sums in turn, then the warps'
     float *sums = reinterpret_cast<float *>(shared);
-    if constexpr (V > 1) copies_wait<0>();
+    copies_wait<0>();
     __syncthreads();
+    for (uint32_t n = 0; n < groups; ++n) {
+      if (group == n) {
 #pragma unroll
-    for (int k = 0; k < IT; ++k)
+        for (int k = 0; k < IT; ++k)
 #pragma unroll
-      for (int j = 0; j < 2 * V; ++j) {
-        for (uint32_t o = a.lanes; o < 32; o *= 2) acc[k][j] += __shfl_xor_sync(0xffffffffu, acc[k][j], o);
-        const bool any = j < V ? has[k] : second[k];
-        if (group == 0 && any) sums[(size_t)warp * a.dim + (j < V ? e0[k] + j : e1[k] + j - V)] = acc[k][j];
+          for (int j = 0; j < 2 * V; ++j) {
+            // element j of the item, of the pairs as spread() has them
+            const float2 v2 = interleaved ? acc[k][(j % 2) * (V / 2) + j / 4] : acc[k][(j / V) * (V / 2) + j % V / 2];
+            const float v = (interleaved ? j / 2 % 2 : j % 2) ? v2.y : v2.x;
+            if (!(j < V ? has[k] : second[k])) continue;
+            float *to = sums + (size_t)warp * a.dim + (j < V ? e0[k] + j : e1[k] + j - V);
+            *to = n ? *to + v : v;
+          }
       }
+      __syncwarp();
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.dim; i += kThreads) {
+      float sum = 0.0f;
+#pragma unroll
+      for (uint32_t n = 0; n < kWarps; ++n) sum += sums[(size_t)n * a.dim + i];
+      a.partial[(uint64_t)blockIdx.x * a.dim + i] = sum;
+    }
+  }
+}
+
+// Heads whose pairs lie anywhere.  They are copied as they lie, `copy` bytes at a time, into places of `slot` bytes; a lane has IT pairs, lanes
+// side by side, or as many elements that pass.  DEPTH places to a group: the next head is on its way while one is worked on.
+template <typename T, int IT, bool NORM, bool BWD>
+__global__ void __launch_bounds__(kThreads, IT > 8 ? 1 : 2) rotary_pairs_kernel(const RotaryArgs a)
+{
+  constexpr bool BOTH = NORM && BWD;
+  constexpr int DEPTH = 2, ARRAYS = BOTH ? 2 : 1;
+  // each pair's turns per position; of each warp, the heads' places [depth][array][group] and the cosines and sines [tokens][rot/2]; then the
+  // sums of the weights' gradients
+  extern __shared__ float4 shared[];
+  const uint32_t which = blockIdx.x >= a.side[0].blocks, block = which ? blockIdx.x - a.side[0].blocks : blockIdx.x;
+  const RotarySide &d = a.side[which];
+  const uint32_t wlane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / a.lanes, group = wlane / a.lanes, lane = wlane - group * a.lanes;
+  const uint32_t half = a.rot / 2, bytes = a.dim * (uint32_t)sizeof(T);
+  double *rates = reinterpret_cast<double *>(shared);
+  char *base = reinterpret_cast<char *>(shared + (half + 1) / 2), *places = base + (size_t)warp * DEPTH * ARRAYS * groups * a.slot;
+  float2 *table = reinterpret_cast<float2 *>(base + (size_t)kWarps * DEPTH * ARRAYS * groups * a.slot) + (size_t)warp * d.tokens * half;
+  auto place = [&](uint32_t turn, int array) { return places + ((turn * ARRAYS + array) * groups + group) * a.slot; };
+  uint32_t e0[IT], e1[IT];
+  bool has[IT], second[IT], turns[IT];
+#pragma unroll
+  for (int k = 0; k < IT; ++k) {
+    const uint32_t p = lane + k * a.lanes;
+    turns[k] = p < half;
+    has[k] = p < a.items;
+    e0[k] = !turns[k] ? a.rot + (p - half) * 2 : a.interleaved ? p * 2 : p;
+    e1[k] = turns[k] && !a.interleaved ? half + p : e0[k] + 1;
+    second[k] = has[k] && e1[k] < a.dim;
+  }
+  pdl_wait();
+  make_rates(a, rates);
+  float2 g[NORM ? IT : 1], acc[BOTH ? IT : 1];
+  if constexpr (NORM) {
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+      g[k] = make_float2(has[k] ? d.gamma.at(e0[k]) : 0.0f, second[k] ? d.gamma.at(e1[k]) : 0.0f);
+      if constexpr (BOTH) acc[k] = both(0.0f);
+    }
+  }
+  const Walk<T> walk(a, d, group, groups);
+  const HeadArray *from = BOTH ? &d.x : nullptr;
+  uint32_t turn_in = 0, turn_out = 0;
+  auto load = [&](const Place<T> &w) {
+    if (w.head < w.end) {
+#pragma unroll
+      for (int n = 0; n < ARRAYS; ++n) {
+        char *to = place(turn_in, n);
+        const char *p = reinterpret_cast<const char *>(n ? w.x : w.p);
+        for (uint32_t i = lane * a.copy; i < bytes; i += a.lanes * a.copy) {
+          if (a.copy == 16) copy_async<16>(to + i, p + i);
+          else if (a.copy == 8) copy_async<8>(to + i, p + i);
+          else if (a.copy == 4) copy_async<4>(to + i, p + i);
+          else *reinterpret_cast<uint16_t *>(to + i) = *reinterpret_cast<const uint16_t *>(p + i);
+        }
+      }
+    }
+    copies_commit();
+    turn_in ^= 1;
+  };
+  Place<T> at, ahead;
+  at.unit = ahead.unit = block * kWarps + warp;
+  walk.enter(at, d.out, nullptr);
+  walk.enter(ahead, d.in, from);
+  long long position = position_of(a, walk.token(at.unit), d.tokens, wlane);
+  load(ahead);
+  walk.advance(ahead, d.in, from);
+  __syncthreads();
+  while (at.unit < d.units) {
+    __syncwarp();
+    make_table(a, rates, d.tokens, position, [&](uint32_t t, uint32_t j, float2 cs) { table[t * half + j] = cs; });
+    position = position_of(a, walk.token(at.unit + walk.step), d.tokens, wlane);
+    __syncwarp();
+    const float2 *cs = table + walk.mine * half;
+    for (const uint32_t unit = at.unit; at.unit == unit;) {
+      const bool live = at.head < at.end;
+      load(ahead);
+      walk.advance(ahead, d.in, from);
+      copies_wait<DEPTH - 1>();
+      __syncwarp();                       // (lanes read what others copied)
+      T *in = reinterpret_cast<T *>(place(turn_out, 0));
+      const T *xin = BOTH ? reinterpret_cast<const T *>(place(turn_out, 1)) : nullptr;
+      float2 f[IT];
+      float sq = 0.0f, dot = 0.0f;
+#pragma unroll
+      for (int k = 0; k < IT; ++k) f[k] = make_float2(live && has[k] ? to_float(in[e0[k]]) : 0.0f, live && second[k] ? to_float(in[e1[k]]) : 0.0f);
+      auto turned = [&](int k) {
+        if (!live || !turns[k]) return;
+        const float2 w = cs[lane + k * a.lanes], v = f[k];
+        f[k] = make_float2(v.x * w.x - v.y * w.y, v.x * w.y + v.y * w.x);
+      };
+      if constexpr (NORM && !BWD) {
+#pragma unroll
+        for (int k = 0; k < IT; ++k) sq = fmaf(f[k].x, f[k].x, fmaf(f[k].y, f[k].y, sq));
+        const float r = rsqrtf(group_sum(sq, a.lanes, wlane - lane) * a.inv_dim + a.epsilon);
+#pragma unroll
+        for (int k = 0; k < IT; ++k) f[k] = mul2(f[k], mul2(g[k], both(r)));
+      }
+#pragma unroll
+      for (int k = 0; k < IT; ++k) turned(k);
+      if constexpr (BOTH) {
+        float2 x[IT];
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+          x[k] = make_float2(live && has[k] ? to_float(xin[e0[k]]) : 0.0f, live && second[k] ? to_float(xin[e1[k]]) : 0.0f);
+          sq = fmaf(x[k].x, x[k].x, fmaf(x[k].y, x[k].y, sq));
+          dot = fmaf(f[k].x * g[k].x, x[k].x, fmaf(f[k].y * g[k].y, x[k].y, dot));
+        }
+        const float r = rsqrtf(group_sum(sq, a.lanes, wlane - lane) * a.inv_dim + a.epsilon);
+        const float2 r2 = both(r), c = both(-group_sum(dot, a.lanes, wlane - lane) * r * r * r * a.inv_dim);
+        if (live) {
+#pragma unroll
+          for (int k = 0; k < IT; ++k) {
+            const float2 fr = mul2(f[k], r2);
+            acc[k] = fma2(fr, x[k], acc[k]);
+            f[k] = fma2(fr, g[k], mul2(x[k], c));
+          }
+        }
+      }
+      // back into the place, each element by the lane that read it, and out as it was copied in
+      if (live) {
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+          if (has[k]) in[e0[k]] = from_float<T>(f[k].x);
+          if (second[k]) in[e1[k]] = from_float<T>(f[k].y);
+        }
+      }
+      __syncwarp();
+      if (live) {
+        char *out = reinterpret_cast<char *>(const_cast<T *>(at.p));
+        const char *p = reinterpret_cast<const char *>(in);
+        for (uint32_t i = lane * a.copy; i < bytes; i += a.lanes * a.copy) {
+          if (a.copy == 16) *reinterpret_cast<uint4 *>(out + i) = *reinterpret_cast<const uint4 *>(p + i);
+          else if (a.copy == 8) *reinterpret_cast<uint2 *>(out + i) = *reinterpret_cast<const uint2 *>(p + i);
+          else if (a.copy == 4) *reinterpret_cast<uint32_t *>(out + i) = *reinterpret_cast<const uint32_t *>(p + i);
+          else *reinterpret_cast<uint16_t *>(out + i) = *reinterpret_cast<const uint16_t *>(p + i);
+        }
+      }
+      turn_out ^= 1;
+      walk.advance(at, d.out, nullptr);
+      // (the place is filled anew by copies of the lanes that emptied it, and the array beside it after every lane has passed the barrier above)
+    }
+  }
+  if constexpr (BOTH) {
+    if (!d.want) return;
+    float *sums = reinterpret_cast<float *>(shared);
+    copies_wait<0>();
+    __syncthreads();
+    for (uint32_t n = 0; n < groups; ++n) {
+      if (group == n) {
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+          float *to = sums + (size_t)warp * a.dim;
+          if (has[k]) to[e0[k]] = n ? to[e0[k]] + acc[k].x : acc[k].x;
+          if (second[k]) to[e1[k]] = n ? to[e1[k]] + acc[k].y : acc[k].y;
+        }
+      }
+      __syncwarp();
+    }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < a.dim; i += kThreads) {
       float sum = 0.0f;
@@ -418,11 +657,19 @@ inline bool same_place(const AnodeHeads *o, const AnodeHeads *i, uint32_t batch,
 
 #define TRY(call) do { const int rc_ = (call); if (rc_) return rc_; } while (0)
 
+// V = 1: pairs anywhere
 template <typename T, int V, int IT, bool NORM, bool BWD>
 int launch_rotary(const RotaryArgs &a, uint32_t blocks, size_t tables, size_t sums, cudaStream_t stream)
 {
-  const auto kernel = rotary_heads_kernel<T, V, IT, NORM, BWD>;
-  size_t shared = ring_bytes(V, IT, NORM && BWD, sizeof(T)) + tables;
+  void (*kernel)(RotaryArgs);
+  size_t shared;
+  if constexpr (V == 1) {
+    kernel = rotary_pairs_kernel<T, IT, NORM, BWD>;
+    shared = (size_t)kWarps * 2 * (NORM && BWD ? 2 : 1) * (32 / a.lanes) * a.slot + tables;
+  } else {
+    kernel = rotary_heads_kernel<T, V, IT, NORM, BWD>;
+    shared = ring_bytes(V, IT, NORM && BWD, sizeof(T)) + tables;
+  }
   if (shared < sums) shared = sums;
   static SharedMemory allowed;
   if (!allowed.up_to((const void *)kernel, shared)) return ANODE_E_LAUNCH;
@@ -501,18 +748,34 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
   a.way = c.bwd ? -1.0f : 1.0f;
   a.turned = a.rot / 2 / v;
   a.items = a.turned + (a.dim - a.rot + 2 * v - 1) / (2 * v);
+  // lanes of a head's group: as many as it has items, in a power of two where others would not make more groups of a warp
+  const uint32_t per_lane = v == 1 ? 8 : 1, wide = (a.items + per_lane - 1) / per_lane;
   a.lanes = 1;
-  while (a.lanes < 32 && a.lanes < a.items) a.lanes *= 2;
+  while (a.lanes < 32 && a.lanes < wide) a.lanes *= 2;
+  if (wide < 32 && 32 / wide > 32 / a.lanes) a.lanes = wide;
   const uint32_t each = (a.items + a.lanes - 1) / a.lanes, groups = 32 / a.lanes;
+  if (v == 1) {
+    a.copy = 16;
+    auto copies = [&](uint32_t n) {
+      if (a.dim * e % n) return false;
+      for (int k = 0; k < 1 + two; ++k)
+        for (const AnodeHeads *h : {c.in[k], c.out[k], c.bwd && a.norm ? c.x[k] : nullptr})
+          if (h && (!aligned_to(h->data, n) || (a.batch > 1 && h->batch_stride * e % n) || (a.seq > 1 && h->seq_stride * e % n) || (h->heads > 1 && h->head_stride * e % n)))
+            return false;
+      return true;
+    };
+    while (a.copy > e && !copies(a.copy)) a.copy /= 2;
+    a.slot = (uint32_t)((a.dim * e + 15) / 16 * 16 + 16);      // (16 more, so that groups side by side read other banks)
+  }
   // blocks that the device holds; both arrays' warps work side by side, as many on either as its share of the heads asks for
-  const uint32_t room = sm_count() * (c.bwd && a.norm ? 2 : 3);
+  const uint32_t room = sm_count() * (uint32_t)(v == 1 ? each > 8 ? 1 : 2 : resident((int)(2 * v * each), a.norm));
   uint32_t blocks = 0, most = 1, units[2] = {0, 0}, passes[2];
   double cost[2] = {0.0, 0.0};
   for (int k = 0; k < 1 + two; ++k) {
     RotarySide &d = a.side[k];
     // a warp has tokens that fill it, or a token's heads
     d.tokens = d.heads < groups ? groups / d.heads : 1;
-    while (d.tokens > 1 && d.tokens * a.rot / 2 > 512) --d.tokens;
+    while (d.tokens > 1 && d.tokens * (a.rot / 2) > 512) --d.tokens;
     units[k] = (a.total - 1) / d.tokens + 1;
     passes[k] = (d.heads + groups - 1) / groups;
     if (d.tokens > most) most = d.tokens;
@@ -534,7 +797,8 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
     d.blocks = need < share ? need : share ? share : 1;
     blocks += d.blocks;
   }
-  const size_t tables = (size_t)kWarps * most * a.rot / 2 * 8, sums = wants ? (size_t)kWarps * a.dim * 4 : 0;
+  const size_t tables = (size_t)kWarps * most * (a.rot / 2) * 8 + (a.rot / 2 + 1) / 2 * 16,      // and the pairs' rates
+                sums = wants ? (size_t)kWarps * a.dim * 4 : 0;
   TRY(by_type(c.type, [&](auto t) {
     using T = decltype(t);
     auto with = [&](auto norm, auto bwd) {
@@ -543,8 +807,7 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
         if (v == 8) return each == 1 ? launch_rotary<T, 8, 1, N, B>(a, blocks, tables, sums, stream) : launch_rotary<T, 8, 2, N, B>(a, blocks, tables, sums, stream);
       if (v == 4) return each == 1 ? launch_rotary<T, 4, 1, N, B>(a, blocks, tables, sums, stream)
                        : each == 2 ? launch_rotary<T, 4, 2, N, B>(a, blocks, tables, sums, stream) : launch_rotary<T, 4, 4, N, B>(a, blocks, tables, sums, stream);
-      return each == 1 ? launch_rotary<T, 1, 1, N, B>(a, blocks, tables, sums, stream) : each == 2 ? launch_rotary<T, 1, 2, N, B>(a, blocks, tables, sums, stream)
-           : each <= 4 ? launch_rotary<T, 1, 4, N, B>(a, blocks, tables, sums, stream) : launch_rotary<T, 1, 16, N, B>(a, blocks, tables, sums, stream);
+      return each <= 8 ? launch_rotary<T, 1, 8, N, B>(a, blocks, tables, sums, stream) : launch_rotary<T, 1, 16, N, B>(a, blocks, tables, sums, stream);
     };
     const std::true_type yes;
     const std::false_type no;

@@ -64,6 +64,30 @@ __device__ __forceinline__ void put_weight(void *p, int type, uint32_t i, float 
   else static_cast<__nv_bfloat16 *>(p)[i] = from_float<__nv_bfloat16>(v);
 }
 
+// Two floats at a time, in one instruction each
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long &>(d))
+      : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)), "l"(reinterpret_cast<unsigned long long &>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d))
+      : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d))
+      : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // 16 bytes of an array: V elements
 template <typename T> struct Vec {
   static constexpr int V = 16 / sizeof(T);

@@ -28,7 +28,7 @@ struct NormArgs {
   uint64_t y_stride, total_stride;
   float *inv_rms;
   // in 8 bits
-  uint32_t block;                      // columns of a group (the whole row: cols)
+  uint32_t block;                      // columns of a group (0: the whole row)
   float *scale;
   uint64_t scale_row, scale_group;
 };
@@ -62,12 +62,13 @@ template <typename T, bool QUANT> __global__ void __launch_bounds__(kThreads) rm
     } else {
       // a warp per group; bits of |y| in the order of unsigned numbers, a NaN's above all
       uint8_t *q = static_cast<uint8_t *>(a.y) + row * a.y_stride;
-      const bool whole = a.block == a.cols;
+      const bool whole = a.block == 0;
+      const uint32_t width = whole ? a.cols : a.block;
       const uint32_t lane = whole ? threadIdx.x : threadIdx.x & 31, lanes = whole ? kThreads : 32, warp = threadIdx.x >> 5;
       __syncthreads();       // (the sum is stored by other threads than read it here)
-      for (uint64_t base = whole ? 0 : (uint64_t)warp * a.block, group = whole ? 0 : warp; base < a.cols;
-           base += (uint64_t)a.block * (kThreads / 32), group += kThreads / 32) {
-        const uint32_t end = (uint32_t)(base + a.block < a.cols ? base + a.block : a.cols);
+      for (uint64_t base = whole ? 0 : (uint64_t)warp * width, group = whole ? 0 : warp; base < a.cols;
+           base += (uint64_t)width * (kThreads / 32), group += kThreads / 32) {
+        const uint32_t end = (uint32_t)(base + width < a.cols ? base + width : a.cols);
         uint32_t top = 0;
         for (uint32_t c = (uint32_t)base + lane; c < end; c += lanes) top = max(top, __float_as_uint(value(c)) & 0x7fffffffu);
         top = __reduce_max_sync(0xffffffffu, top);
@@ -89,19 +90,27 @@ template <typename T, bool QUANT> __global__ void __launch_bounds__(kThreads) rm
 // The launch of the kernels that hold their rows
 struct Held {
   uint32_t team, chunks;     // threads of a row, slots of each
-  uint32_t slots;            // 16-byte slots of a row
   uint32_t groups;           // of 128 columns, where 8-bit rows have them
 };
 
-// Rows held in registers: a team of threads (4 to 32 lanes of a warp, or a block) has a row, a thread CH slots of 16 bytes, so that the
-// row is read once.  SHIFT: rows that begin anywhere or are no whole number of slots, as long as all arrays' rows begin at the same place of a slot:
-// slots are those of the addresses, the first and the last are moved element by element.
-constexpr uint32_t most_threads(int chunks) { return chunks <= 2 ? 1024u : chunks == 4 ? 512u : 640u; }
+__host__ __device__ constexpr uint32_t most_threads(int chunks) { return chunks <= 2 ? 1024u : chunks == 4 ? 512u : 640u; }
 
-template <typename T, int CH, bool SHIFT, bool QUANT>
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// Rows held in registers: a team of threads (4 to 32 lanes of a warp, or a block) has a row, a thread CH slots of 16 bytes, so that the
+// row is read once.  SHIFT: rows that begin anywhere or are no whole number of slots, as long as all arrays' rows begin at the same place of a
+// slot: slots are then those of the addresses, and the elements before the first whole one and after the last have a lane each.
+// QUANT: 0 none, else an output in 8 bits with a scale for each row (1) or for each 128 columns (2).
+// What bounds it: memory; so a thread's loads are all in flight at once.
+template <typename T, int CH, bool SHIFT, int QUANT>
 __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const NormArgs a, const Held h)
 {
-  constexpr int V = Vec<T>::V;
+  constexpr int V = Vec<T>::V, H = V / 2;
   __shared__ float buf[2][32];
   extern __shared__ uint32_t tops[];            // bits of the largest |y| of each group, where groups are not whole slots
   const uint32_t per_block = blockDim.x / h.team, mine = threadIdx.x / h.team, at = threadIdx.x - mine * h.team;
@@ -109,183 +118,179 @@ __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const N
   const bool live = row < a.rows;               // (all threads take part in the teams' sums)
   const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
   const T *res = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
-  const int ph = SHIFT ? (int)(((uintptr_t)x & 15) / sizeof(T)) : 0;
+  T *total = a.total ? static_cast<T *>(a.total) + row * a.total_stride : nullptr;
+  // the row's head: columns before its first whole slot; then `slots` of them, and a tail
+  const uint32_t head = SHIFT ? min(a.cols, (uint32_t)(-(int)((uintptr_t)x / sizeof(T)) & (V - 1))) : 0, slots = (a.cols - head) / V;
+  const uint32_t start = head + at * V, hop = h.team * V;      // this thread's slots: columns start + k*hop
+  const uint32_t mine_slots = live && at < slots ? (slots - at + h.team - 1) / h.team : 0;
+  // the lane's element of the head or the tail
+  const uint32_t tail = a.cols - head - slots * V, edge = at < head ? at : a.cols - tail + (at - head);
+  const bool on_edge = SHIFT && live && at < head + tail;
   uint32_t *top = tops + mine * h.groups;
-  const bool lines = QUANT && a.block != a.cols;
-  if (SHIFT && lines) for (uint32_t i = at; i < h.groups; i += h.team) top[i] = 0;
+  constexpr bool LINES = QUANT == 2;
+  if (SHIFT && LINES) for (uint32_t i = at; i < h.groups; i += h.team) top[i] = 0;
+  const bool aligned_gamma = ((uintptr_t)a.gamma.p & 15) == 0;
   pdl_wait();
   Vec<T> t[CH], r[CH];
-  // slot k of this thread: columns from `col` on, the elements [first, end) of it belong to the row
-  auto col = [&](int k) { return (int)((at + k * h.team) * V) - ph; };
-  auto first = [&](int k) { return SHIFT ? max(0, -col(k)) : 0; };
-  auto end = [&](int k) { return SHIFT ? min(V, (int)a.cols - col(k)) : V; };
-  auto has = [&](int k) { return live && at + k * h.team < h.slots && (!SHIFT || end(k) > 0); };
-  auto whole = [&](int k) { return !SHIFT || (first(k) == 0 && end(k) == V); };
-  auto load = [&](const T *p, int k) { return whole(k) ? Vec<T>::load(p + col(k)) : Vec<T>::load_some(p + col(k), first(k), end(k)); };
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     t[k].bits = make_uint4(0, 0, 0, 0);
-    if (has(k)) t[k] = load(x, k);
+    if (k < mine_slots) t[k] = Vec<T>::load(x + start + k * hop);
   }
   if (res) {
 #pragma unroll
-    for (int k = 0; k < CH; ++k) if (has(k)) r[k] = load(res, k);
+    for (int k = 0; k < CH; ++k) if (k < mine_slots) r[k] = Vec<T>::load(res + start + k * hop);
+  }
+  float te = 0.0f, ge = 1.0f;
+  if (on_edge) {
+    te = to_float(x[edge]);
+    if (res) te = to_float(from_float<T>(te + to_float(res[edge])));
+    ge = a.gamma.at(edge);
   }
   // the weights of few slots are loaded ahead of the sum, those of many when they are needed: they would take the registers
   constexpr bool AHEAD = CH <= 2;
-  float g[AHEAD ? CH : 1][V];
-  auto weights = [&](int k, float *w) {
-    if (!SHIFT) a.gamma.load<V>(col(k), w);
-    else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = i >= first(k) && i < end(k) ? a.gamma.at(col(k) + i) : 0.0f;
-    }
+  float2 g[AHEAD ? CH : 1][H];
+  auto weights = [&](int k, float2 *w) {
+    float *f = reinterpret_cast<float *>(w);
+    const uint32_t c = start + k * hop;
+    if (!SHIFT) a.gamma.load<V>(c, f);
+    else if (aligned_gamma) a.gamma.load_any<V>(c, a.cols, f);
+    else a.gamma.load_each<V>(c, f);
   };
   if (AHEAD) {
 #pragma unroll
-    for (int k = 0; k < CH; ++k) if (has(k)) weights(k, g[AHEAD ? k : 0]);
+    for (int k = 0; k < CH; ++k) if (k < mine_slots) weights(k, g[AHEAD ? k : 0]);
   }
-  float sq = 0.0f;
+  float2 sq2 = make_float2(te * te, 0.0f);
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
-    if (!has(k)) continue;
-    float f[V];
-    t[k].floats(f);
-    if (res) {
-      float e[V];
-      r[k].floats(e);
+    float2 f[H];
+    if (res && k < mine_slots) {
+      float2 e[H];
+      t[k].floats(reinterpret_cast<float *>(f));
+      r[k].floats(reinterpret_cast<float *>(e));
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] += e[i];
-      t[k] = Vec<T>::of(f);
-      t[k].floats(f);
-      if (a.total) {
-        T *p = static_cast<T *>(a.total) + row * a.total_stride + col(k);
-        if (whole(k)) t[k].store(p); else t[k].store_some(p, first(k), end(k));
-      }
+      for (int i = 0; i < H; ++i) f[i] = add2(f[i], e[i]);
+      t[k] = Vec<T>::of(reinterpret_cast<const float *>(f));
+      if (total) t[k].store(total + start + k * hop);
     }
+    t[k].floats(reinterpret_cast<float *>(f));
 #pragma unroll
-    for (int i = 0; i < V; ++i) sq = fmaf(f[i], f[i], sq);
+    for (int i = 0; i < H; ++i) sq2 = fma2(f[i], f[i], sq2);
   }
-  const float inv = 1.0f / sqrtf(team_sum_all(sq, h.team, buf[0]) * a.inv_cols + a.epsilon);
+  if (on_edge && total) total[edge] = from_float<T>(te);
+  const float inv = 1.0f / sqrtf(team_sum_all(sq2.x + sq2.y, h.team, buf[0]) * a.inv_cols + a.epsilon);
   if (live && a.inv_rms && at == 0) a.inv_rms[row] = inv;
-  auto values = [&](int k, float *y) {
-    float f[V];
-    t[k].floats(f);
-    if (AHEAD) {
+  const float2 inv2 = both(inv);
+  auto values = [&](int k, float2 *y) {
+    float2 f[H];
+    t[k].floats(reinterpret_cast<float *>(f));
+    if (!AHEAD) weights(k, y);
 #pragma unroll
-      for (int i = 0; i < V; ++i) y[i] = f[i] * inv * g[AHEAD ? k : 0][i];
-    } else {
-      weights(k, y);
-#pragma unroll
-      for (int i = 0; i < V; ++i) y[i] *= f[i] * inv;
-    }
+    for (int i = 0; i < H; ++i) y[i] = mul2(mul2(f[i], inv2), AHEAD ? g[AHEAD ? k : 0][i] : y[i]);
   };
-  if (!QUANT) {
+  const float ye = te * inv * ge;
+  if constexpr (!QUANT) {
+    T *y = static_cast<T *>(a.y) + row * a.y_stride;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      if (!has(k)) continue;
-      float f[V];
+      if (k >= mine_slots) continue;
+      float2 f[H];
       values(k, f);
-      T *p = static_cast<T *>(a.y) + row * a.y_stride + col(k);
-      const Vec<T> y = Vec<T>::of(f);
-      if (whole(k)) y.store(p); else y.store_some(p, first(k), end(k));
+      Vec<T>::of(reinterpret_cast<const float *>(f)).store(y + start + k * hop);
     }
+    if (on_edge) y[edge] = from_float<T>(ye);
     return;
   }
   // bits of |y| in the order of unsigned numbers: a NaN's lie above all
-  auto largest = [&](const float *y, int from, int to) {
-    uint32_t m = 0;
+  auto bits_of = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
+  auto largest = [&](const float2 *y) {
+    float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) if (!SHIFT || (i >= from && i < to)) m = max(m, __float_as_uint(y[i]) & 0x7fffffffu);
-    return m;
+    for (int i = 0; i < H; ++i) m = max_nan(max_nan(m, fabsf(y[i].x)), fabsf(y[i].y));
+    return bits_of(m);
   };
-  auto scale_of = [&](uint32_t m) { return __uint_as_float(max(m, __float_as_uint(kTiny))) / kE4M3; };
-  // V values to 8 bits: those before `edge` times `one`, the others times `two`
-  auto put = [&](int k, const float *y, float one, float two, int edge) {
-    uint8_t *q = static_cast<uint8_t *>(a.y) + row * a.y_stride + col(k);
+  auto scale_of = [&](uint32_t m) { return __uint_as_float(max(m, __float_as_uint(kTiny))) * (1.0f / kE4M3); };
+  auto inverse = [&](float scale) { return __fdividef(1.0f, scale); };      // (a scale is no smaller than 2^-105: nothing is flushed)
+  uint8_t *q = static_cast<uint8_t *>(a.y) + row * a.y_stride;
+  auto eight = [](float u, float v) { return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(u, v), __NV_SATFINITE, __NV_E4M3); };
+  // a slot to 8 bits: its elements before `border` times `one`, the others times `two`
+  auto put = [&](int k, const float2 *y, float one, float two, int border) {
     uint32_t w[V / 4];
 #pragma unroll
     for (int i = 0; i < V / 4; ++i) {
-      float f[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] = y[4 * i + j] * (SHIFT && 4 * i + j >= edge ? two : one);
-      w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3) |
-             (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+      const float2 u = mul2(y[2 * i], SHIFT && LINES ? make_float2(4 * i >= border ? two : one, 4 * i + 1 >= border ? two : one) : both(one));
+      const float2 v = mul2(y[2 * i + 1], SHIFT && LINES ? make_float2(4 * i + 2 >= border ? two : one, 4 * i + 3 >= border ? two : one) : both(one));
+      w[i] = eight(u.x, u.y) | eight(v.x, v.y) << 16;
     }
-    if (whole(k)) {
-      if constexpr (V == 8) *reinterpret_cast<uint2 *>(q) = make_uint2(w[0], w[V / 4 - 1]);
-      else *reinterpret_cast<uint32_t *>(q) = w[0];
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) if (i >= first(k) && i < end(k)) q[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
-    }
+    if constexpr (V == 8) *reinterpret_cast<uint2 *>(q + start + k * hop) = make_uint2(w[0], w[V / 4 - 1]);
+    else *reinterpret_cast<uint32_t *>(q + start + k * hop) = w[0];
   };
-  if (lines && !SHIFT) {
+  if constexpr (LINES && !SHIFT) {
     // 128 columns: 128/V lanes with a slot each
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      float y[V];
+      float2 y[H];
       uint32_t m = 0;
-      if (has(k)) { values(k, y); m = largest(y, 0, V); }
+      if (k < mine_slots) { values(k, y); m = largest(y); }
 #pragma unroll
       for (int o = 64 / V; o > 0; o >>= 1)
         if (o < (int)h.team) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));      // (a smaller team has one group)
-      if (!has(k)) continue;
-      const float scale = scale_of(m), one = 1.0f / scale;
-      if (col(k) % 128 == 0) a.scale[row * a.scale_row + (uint32_t)col(k) / 128 * a.scale_group] = scale;
+      if (k >= mine_slots) continue;
+      const float scale = scale_of(m), one = inverse(scale);
+      const uint32_t c = start + k * hop;
+      if (c % 128 == 0) a.scale[row * a.scale_row + c / 128 * a.scale_group] = scale;
       put(k, y, one, one, V);
     }
     return;
   }
-  if (!lines) {
-    uint32_t all = 0;
+  float2 y[CH][H];
 #pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      if (!has(k)) continue;
-      float y[V];
-      values(k, y);
-      all = max(all, largest(y, first(k), end(k)));
-    }
+  for (int k = 0; k < CH; ++k) if (k < mine_slots) values(k, y[k]);
+  if constexpr (!LINES) {
+    uint32_t all = on_edge ? bits_of(ye) : 0;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) if (k < mine_slots) all = max(all, largest(y[k]));
     for (uint32_t o = min(h.team, 32u) / 2; o > 0; o >>= 1) all = max(all, __shfl_xor_sync(0xffffffffu, all, o));
     if (h.team > 32) {
       if ((threadIdx.x & 31) == 0) buf[1][threadIdx.x >> 5] = __uint_as_float(all);
       __syncthreads();
       all = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < blockDim.x / 32 ? __float_as_uint(buf[1][threadIdx.x & 31]) : 0u);
     }
-    const float scale = scale_of(all), one = 1.0f / scale;
+    const float scale = scale_of(all), one = inverse(scale);
     if (live && at == 0) a.scale[row * a.scale_row] = scale;
 #pragma unroll
+    for (int k = 0; k < CH; ++k) if (k < mine_slots) put(k, y[k], one, one, V);
+    if (on_edge) q[edge] = (uint8_t)eight(ye * one, 0.0f);
+  } else {
+    // groups that end inside of slots: elements of a slot before `border` are of its first group
+    auto sync = [&] { if (h.team > 32) __syncthreads(); else __syncwarp(); };
+    sync();
+#pragma unroll
     for (int k = 0; k < CH; ++k) {
-      if (!has(k)) continue;
-      float y[V];
-      values(k, y);
-      put(k, y, one, one, V);
+      if (k >= mine_slots) continue;
+      const uint32_t c = start + k * hop, border = 128 - c % 128;
+      if (border >= V) { atomicMax(top + c / 128, largest(y[k])); continue; }
+      float m[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float v = fabsf(i % 2 ? y[k][i / 2].y : y[k][i / 2].x);
+        if (i < border) m[0] = max_nan(m[0], v); else m[1] = max_nan(m[1], v);
+      }
+      atomicMax(top + c / 128, bits_of(m[0]));
+      atomicMax(top + c / 128 + 1, bits_of(m[1]));
     }
-    return;
-  }
-  // groups that end inside of slots: elements of a slot before `edge` are of its first group
-  auto edge = [&](int k) { return 128 - (col(k) + first(k)) % 128 + first(k); };
-  auto sync = [&] { if (h.team > 32) __syncthreads(); else __syncwarp(); };
-  sync();
+    if (on_edge) atomicMax(top + edge / 128, bits_of(ye));
+    sync();
+    if (live) for (uint32_t i = at; i < h.groups; i += h.team) a.scale[row * a.scale_row + i * a.scale_group] = scale_of(top[i]);
 #pragma unroll
-  for (int k = 0; k < CH; ++k) {
-    if (!has(k)) continue;
-    float y[V];
-    values(k, y);
-    const uint32_t group = (uint32_t)(col(k) + first(k)) / 128;
-    atomicMax(top + group, largest(y, first(k), min(end(k), edge(k))));
-    if (end(k) > edge(k)) atomicMax(top + group + 1, largest(y, edge(k), end(k)));
-  }
-  sync();
-  if (live) for (uint32_t i = at; i < h.groups; i += h.team) a.scale[row * a.scale_row + i * a.scale_group] = scale_of(top[i]);
-#pragma unroll
-  for (int k = 0; k < CH; ++k) {
-    if (!has(k)) continue;
-    float y[V];
-    values(k, y);
-    const uint32_t group = (uint32_t)(col(k) + first(k)) / 128;
-    const float one = 1.0f / scale_of(top[group]);
-    put(k, y, one, end(k) > edge(k) ? 1.0f / scale_of(top[group + 1]) : one, edge(k));
+    for (int k = 0; k < CH; ++k) {
+      if (k >= mine_slots) continue;
+      const uint32_t c = start + k * hop, border = 128 - c % 128;
+      const float one = inverse(scale_of(top[c / 128]));
+      put(k, y[k], one, border < V ? inverse(scale_of(top[c / 128 + 1])) : one, border);
+    }
+    if (on_edge) q[edge] = (uint8_t)eight(ye * inverse(scale_of(top[edge / 128])), 0.0f);
   }
 }
 
@@ -304,115 +309,190 @@ struct GradArgs {
   uint32_t parts;
 };
 
-// How the adjoint's rows are held: `teams` teams of `team` threads to a block, each with a row at a time
-struct HeldGrad { uint32_t team, teams, slots; };
+// How the adjoint's rows are held: `teams` teams of `team` threads to a block, each with a row at a time, `depth` rows on their way or at work;
+// `padded` floats of a row of sums in shared memory
+struct HeldGrad { uint32_t team, teams, depth, padded; };
 
-constexpr uint32_t kGradThreads = 512;
-
-// W elements of a row: 16 bytes, or one element
-template <typename T, int W> struct Piece {
-  Vec<T> v;
-  __device__ __forceinline__ static Piece load(const T *p) { return Piece{Vec<T>::load(p)}; }
-  __device__ __forceinline__ void floats(float *f) const { v.floats(f); }
-  __device__ __forceinline__ static void store(T *p, const float *f) { Vec<T>::of(f).store(p); }
-};
-template <typename T> struct Piece<T, 1> {
-  T v;
-  __device__ __forceinline__ static Piece load(const T *p) { return Piece{*p}; }
-  __device__ __forceinline__ void floats(float *f) const { f[0] = to_float(v); }
-  __device__ __forceinline__ static void store(T *p, const float *f) { *p = from_float<T>(f[0]); }
-};
-
-// The adjoint with its rows held in registers: a team of threads walks down rows, each thread with the same columns of all of them, so that
-// one pass over the arrays gives dx and, in the threads' registers, dgamma's sums.  PRE: the next row is on its way while one is worked on.
-// The teams' sums join in shared memory and the blocks' in a second launch, both in a fixed order.
-template <typename T, int W, int CH, bool PRE>
-__global__ void __launch_bounds__(kGradThreads) rms_norm_grad_kernel(const GradArgs a, const HeldGrad h)
+// The adjoint with its rows held on chip: a team of threads (4 to 32 lanes of a warp, or more warps) walks down rows, a thread with CH slots of 16
+// bytes of each array, so that one pass gives dx and dgamma's sums.  The next rows are on their way by asynchronous copies, each thread into a
+// ring of its own: a thread waits for nothing but its own copies and, once per row, its team's sum.
+// A thread's columns are the same in all rows, and dgamma's sums are in its registers; SHIFT, as in rms_norm_held_kernel: the columns
+// move with the rows' beginnings, and sums and weights are in shared memory, where column c is at c + c/V, so that threads with V
+// columns each meet in no bank.  Both kinds join in a fixed order, the blocks' in a second launch.
+template <typename T, int CH, int NT, bool SHIFT>
+__global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, const HeldGrad h)
 {
-  __shared__ float buf[2][kGradThreads / 32];
-  extern __shared__ float sums[];               // [teams][cols]
+  constexpr int V = Vec<T>::V, H = V / 2;
+  __shared__ float buf[2][32];
+  extern __shared__ float4 shared[];            // the rings [depth][CH][3][thread]; SHIFT: weights [padded], sums [teams][padded]; at last the sums [teams][cols]
   const uint32_t mine = threadIdx.x / h.team, at = threadIdx.x - mine * h.team, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool works = mine < h.teams;
-  auto col = [&](int k) { return (at + k * h.team) * W; };
-  auto has = [&](int k) { return works && at + k * h.team < h.slots; };
+  const uint32_t lanes = h.team < 32 ? ((1u << h.team) - 1) << (lane & ~(h.team - 1)) : 0xffffffffu;      // of this warp in the team
+  uint4 *ring = reinterpret_cast<uint4 *>(shared) + threadIdx.x;
+  float *weights = reinterpret_cast<float *>(shared + (size_t)h.depth * CH * 3 * NT), *sums = weights + h.padded, *own = sums + (size_t)mine * h.padded;
+  const uint32_t hop = h.team * V;
   pdl_wait();
-  float acc[CH][W], g[CH][W];
+  float2 acc[SHIFT ? 1 : CH][H], g[SHIFT ? 1 : CH][H];
+  if constexpr (SHIFT) {
+    for (uint32_t c = threadIdx.x; c < a.cols; c += NT) weights[c + c / V] = a.gamma.at(c);
+    for (uint32_t c = threadIdx.x; c < h.teams * h.padded; c += NT) sums[c] = 0.0f;
+    __syncthreads();
+  } else {
 #pragma unroll
-  for (int k = 0; k < CH; ++k) {
+    for (int k = 0; k < CH; ++k) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) { acc[k][i] = 0.0f; g[k][i] = 0.0f; }
-    if (!has(k)) continue;
-    if constexpr (W > 1) a.gamma.load<W>(col(k), g[k]); else g[k][0] = a.gamma.at(col(k));
+      for (int i = 0; i < H; ++i) acc[k][i] = both(0.0f);
+      if (works && at * V + k * hop < a.cols) a.gamma.load<V>(at * V + k * hop, reinterpret_cast<float *>(g[k]));
+    }
   }
-  typedef Piece<T, W> Some;
-  struct Row { Some dy[CH], t[CH], dt[CH]; float r; } now, next;
-  auto load = [&](Row &w, uint64_t row) {
-    const T *dy = static_cast<const T *>(a.dy) + row * a.dy_stride, *t = static_cast<const T *>(a.total) + row * a.total_stride;
-    const T *dt = a.dtotal ? static_cast<const T *>(a.dtotal) + row * a.dtotal_stride : nullptr;
-    w.r = a.inv_rms[row];
+  // a row of this team: its head, this thread's slots, and its element of the head or the tail
+  struct Row { uint32_t head, start, slots, edge; bool on_edge; };
+  auto shape = [&](uint64_t row) {
+    Row w;
+    w.head = SHIFT ? min(a.cols, (uint32_t)(-(int)((uintptr_t)(static_cast<const T *>(a.dy) + row * a.dy_stride) / sizeof(T)) & (V - 1))) : 0;
+    const uint32_t slots = (a.cols - w.head) / V, tail = a.cols - w.head - slots * V;
+    w.start = w.head + at * V;
+    w.slots = at < slots ? (slots - at + h.team - 1) / h.team : 0;
+    w.edge = at < w.head ? at : a.cols - tail + (at - w.head);
+    w.on_edge = SHIFT && at < w.head + tail;
+    return w;
+  };
+  auto dy_of = [&](uint64_t row) { return static_cast<const T *>(a.dy) + row * a.dy_stride; };
+  auto t_of = [&](uint64_t row) { return static_cast<const T *>(a.total) + row * a.total_stride; };
+  auto dt_of = [&](uint64_t row) { return static_cast<const T *>(a.dtotal) + row * a.dtotal_stride; };
+  uint32_t in = 0, out = 0;
+  auto copy = [&](uint64_t row) {
+    if (works && row < a.rows) {
+      const Row w = shape(row);
+      const T *dy = dy_of(row) + w.start, *t = t_of(row) + w.start, *dt = dt_of(row) + w.start;
+      uint4 *to = ring + in * (CH * 3 * NT);
 #pragma unroll
-    for (int k = 0; k < CH; ++k)
-      if (has(k)) { w.dy[k] = Some::load(dy + col(k)); w.t[k] = Some::load(t + col(k)); }
-    if (dt) {
-#pragma unroll
-      for (int k = 0; k < CH; ++k) if (has(k)) w.dt[k] = Some::load(dt + col(k));
+      for (int k = 0; k < CH; ++k) {
+        if (k >= w.slots) continue;
+        copy_async<16>(to + (3 * k) * NT, dy + k * hop);
+        copy_async<16>(to + (3 * k + 1) * NT, t + k * hop);
+        if (a.dtotal) copy_async<16>(to + (3 * k + 2) * NT, dt + k * hop);
+      }
+    }
+    copies_commit();
+    in = in + 1 == h.depth ? 0 : in + 1;
+  };
+  // what does not go through the ring: 1/rms, and an element of the head or the tail
+  struct Side { float r, dy, t, dt; } now = {}, next = {};
+  auto side = [&](Side &o, uint64_t row) {
+    if (!works || row >= a.rows) return;
+    o.r = a.inv_rms[row];
+    if constexpr (SHIFT) {
+      const Row w = shape(row);
+      o.dy = o.t = o.dt = 0.0f;
+      if (w.on_edge) {
+        o.dy = to_float(dy_of(row)[w.edge]); o.t = to_float(t_of(row)[w.edge]);
+        if (a.dtotal) o.dt = to_float(dt_of(row)[w.edge]);
+      }
     }
   };
   const uint64_t step = (uint64_t)gridDim.x * h.teams;
   uint64_t row = (uint64_t)blockIdx.x * h.teams + mine;
+  for (uint32_t i = 0; i + 1 < h.depth; ++i) copy(row + i * step);
+  side(next, row);
   uint32_t turn = 0;
-  if (PRE && works && row < a.rows) load(now, row);
   for (; works && row < a.rows; row += step, turn ^= 1) {
-    if (PRE) { if (row + step < a.rows) load(next, row + step); }
-    else load(now, row);
-    float dot = 0.0f;
+    now = next;
+    copy(row + (h.depth - 1) * step);
+    side(next, row + step);
+    if (h.depth == 1) copies_wait<0>(); else if (h.depth == 2) copies_wait<1>(); else if (h.depth == 3) copies_wait<2>(); else copies_wait<3>();
+    const Row w = shape(row);
+    const uint4 *from = ring + out * (CH * 3 * NT);
+    out = out + 1 == h.depth ? 0 : out + 1;
+    // where the columns' weights and sums are: element i of slot k at pad + k*hop_pad + i, one further from the next multiple of V on
+    const uint32_t pad = w.start + at, hop_pad = hop + h.team, wrap = V - w.head;
+    auto place = [&](int k, int i) { return pad + k * hop_pad + i + (i >= wrap); };
+    float2 dot2 = both(0.0f);
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      if (!has(k)) continue;
-      float dy[W], t[W];
-      now.dy[k].floats(dy); now.t[k].floats(t);
+      if (k >= w.slots) continue;
+      float2 dy[H], t[H];
+      Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(dy));
+      Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(t));
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const float xh = t[i] * now.r;
-        acc[k][i] = fmaf(dy[i], xh, acc[k][i]);
-        dot = fmaf(dy[i] * g[k][i], xh, dot);
+      for (int i = 0; i < H; ++i) {
+        float2 v;
+        if constexpr (SHIFT) v = make_float2(weights[place(k, 2 * i)], weights[place(k, 2 * i + 1)]); else v = g[k][i];
+        dot2 = fma2(mul2(dy[i], v), t[i], dot2);
       }
     }
-    dot = warp_sum_all(dot);
-    if (h.team > 32) {
-      if (lane == 0) buf[turn][warp] = dot;
-      asm volatile("bar.sync %0, %1;" ::"r"(mine + 1), "r"(h.team) : "memory");
-      const uint32_t first = mine * h.team / 32, warps = h.team / 32;
-      dot = warp_sum_all(lane < warps ? buf[turn][first + lane] : 0.0f);
+    float dot = dot2.x + dot2.y, ge = 0.0f;
+    const uint32_t pe = w.edge + w.edge / V;
+    if (w.on_edge) { ge = weights[pe]; dot = fmaf(now.dy * ge, now.t, dot); }
+    if (h.team >= 32) {
+      dot = warp_sum_all(dot);
+      if (h.team > 32) {
+        if (lane == 0) buf[turn][warp] = dot;
+        asm volatile("bar.sync %0, %1;" ::"r"(mine + 1), "r"(h.team) : "memory");
+        const uint32_t first = mine * h.team / 32, warps = h.team / 32;
+        dot = warp_sum_all(lane < warps ? buf[turn][first + lane] : 0.0f);
+      } else if (SHIFT) __syncwarp();           // (another lane has had these columns in the row before)
+    } else {
+      for (uint32_t o = h.team / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(lanes, dot, o);
+      if (SHIFT) __syncwarp(lanes);
     }
-    dot *= a.inv_cols;
+    const float2 r = both(now.r), c = both(-now.r * now.r * now.r * dot * a.inv_cols);
     T *dx = static_cast<T *>(a.dx) + row * a.dx_stride;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      if (!has(k)) continue;
-      float dy[W], t[W], dt[W];
-      now.dy[k].floats(dy); now.t[k].floats(t);
-      if (a.dtotal) now.dt[k].floats(dt);
+      if (k >= w.slots) continue;
+      float2 dy[H], t[H], dt[H];
+      Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(dy));
+      Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(t));
+      if (a.dtotal) Vec<T>{from[(3 * k + 2) * NT]}.floats(reinterpret_cast<float *>(dt));
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const float v = now.r * (dy[i] * g[k][i] - t[i] * now.r * dot);
-        dy[i] = a.dtotal ? v + dt[i] : v;
+      for (int i = 0; i < H; ++i) {
+        const float2 dyr = mul2(dy[i], r);
+        float2 v;
+        if constexpr (SHIFT) {
+          const float2 p = mul2(dyr, t[i]);
+          own[place(k, 2 * i)] += p.x;
+          own[place(k, 2 * i + 1)] += p.y;
+          v = make_float2(weights[place(k, 2 * i)], weights[place(k, 2 * i + 1)]);
+        } else {
+          acc[k][i] = fma2(dyr, t[i], acc[k][i]);
+          v = g[k][i];
+        }
+        dy[i] = fma2(dyr, v, mul2(t[i], c));
+        if (a.dtotal) dy[i] = add2(dy[i], dt[i]);
       }
-      Some::store(dx + col(k), dy);
+      Vec<T>::of(reinterpret_cast<const float *>(dy)).store(dx + w.start + k * hop);
     }
-    if (PRE) now = next;
+    if (w.on_edge) {
+      own[pe] += now.dy * now.r * now.t;
+      dx[w.edge] = from_float<T>(fmaf(now.dy * now.r, ge, now.t * c.x) + now.dt);
+    }
   }
   if (!a.dgamma) return;
-#pragma unroll
-  for (int k = 0; k < CH; ++k) {
-    if (!has(k)) continue;
-#pragma unroll
-    for (int i = 0; i < W; ++i) sums[(size_t)mine * a.cols + col(k) + i] = acc[k][i];
-  }
+  copies_wait<0>();
   __syncthreads();
-  for (uint32_t c = threadIdx.x; c < a.cols; c += kGradThreads) {
+  uint32_t parts = h.teams;
+  if constexpr (!SHIFT) {
+    // the teams of a warp join first
+    sums = reinterpret_cast<float *>(shared);
+    if (h.team < 32) parts = (h.teams * h.team + 31) / 32;
+    const uint32_t part = h.team < 32 ? warp : mine;
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float v = reinterpret_cast<const float *>(acc[k])[i];
+        for (uint32_t o = h.team; o < 32; o *= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+        const uint32_t c = at * V + k * hop + i;
+        if (part < parts && c < a.cols && (h.team >= 32 || lane < h.team)) sums[(size_t)part * a.cols + c] = v;
+      }
+    __syncthreads();
+  }
+  const uint32_t apart = SHIFT ? h.padded : a.cols;
+  for (uint32_t c = threadIdx.x; c < a.cols; c += NT) {
+    const uint32_t i = SHIFT ? c + c / V : c;
     float sum = 0.0f;
-    for (uint32_t t = 0; t < h.teams; ++t) sum += sums[(size_t)t * a.cols + c];
+    for (uint32_t t = 0; t < parts; ++t) sum += sums[(size_t)t * apart + i];
     a.partial[(uint64_t)blockIdx.x * a.cols + c] = sum;
   }
 }
@@ -504,17 +584,16 @@ bool held_plan(const NormArgs &a, int type, int gamma_type, bool quant, Held &h,
   if (!in_step(a.residual, e, a.residual_stride, v, a.x, e, a.x_stride, a.rows) || !in_step(a.total, e, a.total_stride, v, a.x, e, a.x_stride, a.rows) ||
       !in_step(a.y, quant ? 1 : e, a.y_stride, v, a.x, e, a.x_stride, a.rows)) return false;
   shift = !aligned_to(a.x, 16) || a.cols % v || (a.rows > 1 && a.x_stride % v) || !aligned_to(a.gamma.p, 16);
-  const uint64_t slots = shift ? ((uint64_t)a.cols + 2 * v - 2) / v : a.cols / v;
+  const uint32_t slots = a.cols / v;
   if (slots > 8 * most_threads(8)) return false;
-  h.slots = (uint32_t)slots;
-  h.groups = quant && a.block != a.cols ? (a.cols + 127) / 128 : 0;
+  h.groups = quant && a.block ? (a.cols + 127) / 128 : 0;
   if (slots <= 128) {
-    h.team = 4;
+    h.team = shift ? 16 : 4;              // (a lane for each element before and after whole slots)
     while (h.team < 32 && h.team < slots) h.team *= 2;
-    h.chunks = slots <= 32 ? 1 : slots <= 64 ? 2 : 4;
+    h.chunks = slots <= h.team ? 1 : slots <= 64 ? 2 : 4;
   } else {
     h.chunks = a.rows <= 2 * 148 && slots <= 2048 ? (slots <= 1024 ? 1 : 2) : slots <= 4 * most_threads(4) ? 4 : 8;
-    h.team = (h.slots + h.chunks * 32 - 1) / (h.chunks * 32) * 32;
+    h.team = (slots + h.chunks * 32 - 1) / (h.chunks * 32) * 32;
   }
   return true;
 }
@@ -524,37 +603,48 @@ template <typename T, int CH> int launch_held(const NormArgs &a, const Held &h, 
   const uint32_t threads = h.team > 32 ? h.team : 128, per_block = threads / h.team;
   const dim3 grid((uint32_t)((a.rows + per_block - 1) / per_block));
   const size_t shared = shift ? (size_t)per_block * h.groups * 4 : 0;
-  if (quant) return shift ? launch(rms_norm_held_kernel<T, CH, true, true>, grid, threads, shared, stream, a, h)
-                          : launch(rms_norm_held_kernel<T, CH, false, true>, grid, threads, shared, stream, a, h);
-  return shift ? launch(rms_norm_held_kernel<T, CH, true, false>, grid, threads, shared, stream, a, h)
-               : launch(rms_norm_held_kernel<T, CH, false, false>, grid, threads, shared, stream, a, h);
+  auto go = [&](auto plain, auto shifted) { return launch(shift ? shifted : plain, grid, threads, shared, stream, a, h); };
+  if (!quant) return go(rms_norm_held_kernel<T, CH, false, 0>, rms_norm_held_kernel<T, CH, true, 0>);
+  return h.groups ? go(rms_norm_held_kernel<T, CH, false, 2>, rms_norm_held_kernel<T, CH, true, 2>)
+                  : go(rms_norm_held_kernel<T, CH, false, 1>, rms_norm_held_kernel<T, CH, true, 1>);
 }
 
-// How the rows of an adjoint are held in registers: pieces of 16 bytes or of one element, `chunks` of them to a thread; false where they are not
-bool grad_plan(const GradArgs &a, int type, HeldGrad &h, uint32_t &width, uint32_t &chunks)
+// How the rows of an adjoint are held on chip: chunks*threads of the kernel; false where they are not
+bool grad_plan(const GradArgs &a, int type, HeldGrad &h, uint32_t &chunks, uint32_t &threads, bool &shift)
 {
   const size_t e = type_bytes(type);
-  const uint32_t v = (uint32_t)(16 / e);
-  auto fits = [&](const void *p, uint64_t stride) { return !p || (aligned_to(p, 16) && (a.rows <= 1 || stride % v == 0)); };
-  width = a.cols % v == 0 && fits(a.dy, a.dy_stride) && fits(a.total, a.total_stride) && fits(a.dtotal, a.dtotal_stride) && fits(a.dx, a.dx_stride) &&
-          aligned_to(a.gamma.p, 16) ? v : 1;
-  h.slots = a.cols / width;
-  const uint32_t most = width > 1 ? 4 : 16;
-  if (h.slots > most * kGradThreads) return false;
-  chunks = width > 1 ? (h.slots <= 32 ? 1 : h.slots <= 2 * kGradThreads ? 2 : 4) : h.slots <= 64 ? 2 : h.slots <= 8 * kGradThreads ? 8 : 16;
-  h.team = (h.slots + chunks * 32 - 1) / (chunks * 32) * 32;
-  h.teams = kGradThreads / h.team;
-  if (a.rows < (uint64_t)h.teams * sm_count()) h.teams = (uint32_t)((a.rows + sm_count() - 1) / sm_count());     // a row per block first
+  const uint32_t v = (uint32_t)(16 / e), slots = a.cols / v;
+  if (!in_step(a.total, e, a.total_stride, v, a.dy, e, a.dy_stride, a.rows) || !in_step(a.dtotal, e, a.dtotal_stride, v, a.dy, e, a.dy_stride, a.rows) ||
+      !in_step(a.dx, e, a.dx_stride, v, a.dy, e, a.dy_stride, a.rows)) return false;
+  shift = !aligned_to(a.dy, 16) || a.cols % v || (a.rows > 1 && a.dy_stride % v) || !aligned_to(a.gamma.p, 16);
+  chunks = slots <= 1024 ? 1 : 4;
+  threads = slots > 1024 && slots <= 2048 && v == 8 ? 512 : 1024;
+  if (slots > (v == 8 ? 2048u : 4096u)) return false;
+  h.team = (slots + chunks * 32 - 1) / (chunks * 32) * 32;
+  if (slots <= 16) {
+    h.team = shift ? 16 : 4;              // (a lane for each element before and after whole slots)
+    while (h.team < slots) h.team *= 2;
+  }
+  if (h.team < 32 && slots > 16) h.team = 32;
+  h.teams = threads / h.team;
+  if (h.team > 32 && h.teams > 15) h.teams = 15;      // (a named barrier each)
+  const uint32_t sms = sm_count();
+  if (a.rows < (uint64_t)h.teams * sms) h.teams = (uint32_t)((a.rows + sms - 1) / sms);     // a row per block first
+  h.padded = shift ? (a.cols + a.cols / v + 4) / 4 * 4 : 0;
+  const size_t fixed = (size_t)h.padded * 4 * (1 + h.teams), each = (size_t)threads * chunks * 48, room = 226 * 1024;
+  if (fixed + each > room) return false;
+  h.depth = (uint32_t)((room - fixed) / each);
+  if (h.depth > 4) h.depth = 4;
   return true;
 }
 
-template <typename T, int W, int CH, bool PRE> int launch_grad(const GradArgs &a, const HeldGrad &h, cudaStream_t stream)
+template <typename T, int CH, int NT> int launch_grad(const GradArgs &a, const HeldGrad &h, bool shift, cudaStream_t stream)
 {
-  const auto kernel = rms_norm_grad_kernel<T, W, CH, PRE>;
-  const size_t shared = a.dgamma ? (size_t)h.teams * a.cols * 4 : 0;
-  static SharedMemory allowed;
-  if (!allowed.up_to((const void *)kernel, shared)) return ANODE_E_LAUNCH;
-  return launch(kernel, dim3(a.parts), kGradThreads, shared, stream, a, h);
+  const auto kernel = shift ? rms_norm_grad_kernel<T, CH, NT, true> : rms_norm_grad_kernel<T, CH, NT, false>;
+  const size_t shared = (size_t)h.depth * CH * NT * 48 + (shift ? (size_t)h.padded * 4 * (1 + h.teams) : 0);
+  static SharedMemory allowed[2];
+  if (!allowed[shift].up_to((const void *)kernel, shared)) return ANODE_E_LAUNCH;
+  return launch(kernel, dim3(a.parts), NT, shared, stream, a, h);
 }
 
 int norm_forward(const NormArgs &a, int type, int gamma_type, bool quant, cudaStream_t stream)
@@ -624,7 +714,7 @@ extern "C" int anode_gpu_rms_norm_add_quant_fwd(
   if ((many && !scale_row_stride) || (wide && !scale_group_stride) ||
       (many && wide && scale_row_stride < groups * scale_group_stride && scale_group_stride < rows * scale_row_stride)) return ANODE_E_STRIDE;
   NormArgs a = {rows, cols, epsilon, 1.0f / (float)cols, x, residual, x_stride, residual_stride, {gamma, gamma_type}, q, total, q_stride,
-                total_stride, nullptr, block ? block : cols, scale, scale_row_stride, scale_group_stride};
+                total_stride, nullptr, block, scale, scale_row_stride, scale_group_stride};
   return norm_forward(a, type, gamma_type, true, stream);
 }
 
@@ -659,19 +749,18 @@ extern "C" int anode_gpu_rms_norm_add_bwd(
   GradArgs a = {rows, cols, 1.0f / (float)cols, dy, total, dtotal, dy_stride, total_stride, dtotal_stride, inv_rms, {gamma, gamma_type},
                 dx, dx_stride, dgamma, static_cast<float *>(workspace), parts_of(rows)};
   HeldGrad h = {};
-  uint32_t width = 0, chunks = 0;
-  const bool held = grad_plan(a, type, h, width, chunks);
+  uint32_t chunks = 0, threads = 0;
+  bool shift = false;
+  const bool held = grad_plan(a, type, h, chunks, threads, shift);
   const uint32_t wide = (uint32_t)(((uint64_t)cols + kThreads - 1) / kThreads), narrow = (uint32_t)(((uint64_t)cols + 31) / 32);
   return by_type(type, [&](auto t) {
     using T = decltype(t);
-    constexpr int V = Vec<T>::V;
     if (held) {
       const uint64_t blocks = (rows + h.teams - 1) / h.teams;
       if (a.parts > blocks) a.parts = (uint32_t)blocks;
-      TRY(width > 1 ? (chunks == 1 ? launch_grad<T, V, 1, true>(a, h, stream) : chunks == 2 ? launch_grad<T, V, 2, true>(a, h, stream)
-                                   : launch_grad<T, V, 4, false>(a, h, stream))
-                    : (chunks == 2 ? launch_grad<T, 1, 2, true>(a, h, stream) : chunks == 8 ? launch_grad<T, 1, 8, true>(a, h, stream)
-                                   : launch_grad<T, 1, 16, false>(a, h, stream)));
+      if (chunks == 1) TRY((launch_grad<T, 1, 1024>(a, h, shift, stream)));
+      else if constexpr (sizeof(T) == 2) TRY((launch_grad<T, 4, 512>(a, h, shift, stream)));
+      else TRY((launch_grad<T, 4, 1024>(a, h, shift, stream)));
       return dgamma ? launch(join_columns_kernel, dim3(narrow), kThreads, 0, stream, cols, a.parts, a.partial, dgamma, gamma_type) : (int)ANODE_OK;
     }
     if (dgamma) {

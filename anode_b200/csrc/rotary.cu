@@ -101,15 +101,6 @@ template <typename T, int V> __device__ __forceinline__ void gather(Few<T, V> (&
   }
 }
 
-template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const void *from)
-{
-  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
-
 // The position of a unit's token `lane` (lanes beyond its tokens: 0), as it is asked for a unit ahead
 __device__ __forceinline__ long long position_of(const RotaryArgs &a, uint32_t first, uint32_t tokens, uint32_t lane)
 {

@@ -50,6 +50,62 @@ struct Weights {
       }
     }
   }
+  // N of them from column c on, one by one
+  template <int N> __device__ __forceinline__ void load_each(uint32_t c, float *f) const
+  {
+    if (!p) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = 1.0f;
+    } else if (type == ANODE_TYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = static_cast<const float *>(p)[c + i];
+    } else {
+      uint16_t w[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = static_cast<const uint16_t *>(p)[c + i];
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = type == ANODE_TYPE_F16 ? __half2float(__ushort_as_half(w[i])) : __uint_as_float((uint32_t)w[i] << 16);
+    }
+  }
+  // N of them from any column c on, out of `cols`: those of 16 bytes of the vector, two by two aligned pieces shifted together
+  template <int N> __device__ __forceinline__ void load_any(uint32_t c, uint32_t cols, float *f) const
+  {
+    const uint32_t o = c % N, first = c - o;
+    if (!p || o == 0) { load<N>(c, f); return; }
+    if (first + 2 * N > cols) { load_each<N>(c, f); return; }
+    if (type == ANODE_TYPE_F32) {
+      uint32_t w[2 * N];
+#pragma unroll
+      for (int i = 0; i < 2 * N; i += 4) *reinterpret_cast<uint4 *>(w + i) = *reinterpret_cast<const uint4 *>(static_cast<const float *>(p) + first + i);
+#pragma unroll
+      for (int b = N / 2; b > 0; b /= 2)
+#pragma unroll
+        for (int i = 0; i + b < 2 * N; ++i) w[i] = o & b ? w[i + b] : w[i];
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = __uint_as_float(w[i]);
+    } else {
+      uint32_t w[N];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint16_t *from = static_cast<const uint16_t *>(p) + first + i * N;
+        if constexpr (N == 8) *reinterpret_cast<uint4 *>(w + 4 * i) = *reinterpret_cast<const uint4 *>(from);
+        else *reinterpret_cast<uint2 *>(w + 2 * i) = *reinterpret_cast<const uint2 *>(from);
+      }
+#pragma unroll
+      for (int b = N / 2; b > 1; b /= 2)
+#pragma unroll
+        for (int i = 0; i + b / 2 < N; ++i) w[i] = o & b ? w[i + b / 2] : w[i];
+      const uint32_t by = o & 1 ? 0x5432u : 0x3210u;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        const uint32_t v = __byte_perm(w[i], w[i + 1], by);
+        if (type == ANODE_TYPE_F16) {
+          const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&v));
+          f[2 * i] = x.x; f[2 * i + 1] = x.y;
+        } else { f[2 * i] = __uint_as_float(v << 16); f[2 * i + 1] = __uint_as_float(v & 0xffff0000u); }
+      }
+    }
+  }
   __device__ __forceinline__ float at(uint32_t i) const
   {
     if (!p) return 1.0f;
@@ -63,6 +119,16 @@ __device__ __forceinline__ void put_weight(void *p, int type, uint32_t i, float 
   else if (type == ANODE_TYPE_F16) static_cast<__half *>(p)[i] = from_float<__half>(v);
   else static_cast<__nv_bfloat16 *>(p)[i] = from_float<__nv_bfloat16>(v);
 }
+
+// Copies into shared memory that a thread waits for itself
+template <int BYTES> __device__ __forceinline__ void copy_async(void *to, const void *from)
+{
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 // Two floats at a time, in one instruction each
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
@@ -117,21 +183,6 @@ template <typename T> struct Vec {
       else { const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]); w[i] = *reinterpret_cast<const uint32_t *>(&v); }
     }
     return Vec{make_uint4(w[0], w[1], w[2], w[3])};
-  }
-  // element by element, those of [first, end); the others are zero, or stay
-  __device__ __forceinline__ static Vec load_some(const T *p, int first, int end)
-  {
-    float f[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = i >= first && i < end ? to_float(p[i]) : 0.0f;
-    return of(f);
-  }
-  __device__ __forceinline__ void store_some(T *p, int first, int end) const
-  {
-    float f[V];
-    floats(f);
-#pragma unroll
-    for (int i = 0; i < V; ++i) if (i >= first && i < end) p[i] = from_float<T>(f[i]);
   }
 };
 

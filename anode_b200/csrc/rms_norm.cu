@@ -131,6 +131,7 @@ __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const N
   if (SHIFT && LINES) for (uint32_t i = at; i < h.groups; i += h.team) top[i] = 0;
   const bool aligned_gamma = ((uintptr_t)a.gamma.p & 15) == 0;
   pdl_wait();
+  pdl_trigger();        // (the next kernel's blocks wait as these did: 0.1 to 0.3 us of a call of few rows)
   Vec<T> t[CH], r[CH];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
@@ -345,80 +346,90 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
       if (works && at * V + k * hop < a.cols) a.gamma.load<V>(at * V + k * hop, reinterpret_cast<float *>(g[k]));
     }
   }
-  // a row of this team: its head, this thread's slots, and its element of the head or the tail
-  struct Row { uint32_t head, start, slots, edge; bool on_edge; };
-  auto shape = [&](uint64_t row) {
+  // a row of this team, from where its dy is: columns before its first whole slot, slots, and this thread's element of the head or the tail
+  struct Row { uint32_t head, slots, edge; bool on_edge; };
+  auto shape = [&](const T *dy) {
     Row w;
-    w.head = SHIFT ? min(a.cols, (uint32_t)(-(int)((uintptr_t)(static_cast<const T *>(a.dy) + row * a.dy_stride) / sizeof(T)) & (V - 1))) : 0;
-    const uint32_t slots = (a.cols - w.head) / V, tail = a.cols - w.head - slots * V;
-    w.start = w.head + at * V;
-    w.slots = at < slots ? (slots - at + h.team - 1) / h.team : 0;
+    w.head = SHIFT ? min(a.cols, (0u - (uint32_t)((uintptr_t)dy / sizeof(T))) & (V - 1)) : 0;
+    w.slots = (a.cols - w.head) / V;
+    const uint32_t tail = a.cols - w.head - w.slots * V;
     w.edge = at < w.head ? at : a.cols - tail + (at - w.head);
     w.on_edge = SHIFT && at < w.head + tail;
     return w;
   };
-  auto dy_of = [&](uint64_t row) { return static_cast<const T *>(a.dy) + row * a.dy_stride; };
-  auto t_of = [&](uint64_t row) { return static_cast<const T *>(a.total) + row * a.total_stride; };
-  auto dt_of = [&](uint64_t row) { return static_cast<const T *>(a.dtotal) + row * a.dtotal_stride; };
+  const uint64_t step = (uint64_t)gridDim.x * h.teams, row0 = (uint64_t)blockIdx.x * h.teams + mine;
+  // rows that this team has: at work, and to be copied
+  uint32_t left = works && row0 < a.rows ? (uint32_t)((a.rows - row0 + step - 1) / step) : 0, ahead = left;
+  const T *dy = static_cast<const T *>(a.dy) + row0 * a.dy_stride, *t = static_cast<const T *>(a.total) + row0 * a.total_stride;
+  const T *dt = static_cast<const T *>(a.dtotal) + row0 * a.dtotal_stride;
+  T *dx = static_cast<T *>(a.dx) + row0 * a.dx_stride;
+  const float *inv = a.inv_rms + row0;
+  const uint64_t dy_step = step * a.dy_stride, t_step = step * a.total_stride, dt_step = step * a.dtotal_stride, dx_step = step * a.dx_stride;
   uint32_t in = 0, out = 0;
-  auto copy = [&](uint64_t row) {
-    if (works && row < a.rows) {
-      const Row w = shape(row);
-      const T *dy = dy_of(row) + w.start, *t = t_of(row) + w.start, *dt = dt_of(row) + w.start;
+  auto copy = [&] {                     // the next row to be copied
+    if (ahead) {
+      const Row w = shape(dy);
+      const uint32_t start = w.head + at * V;
       uint4 *to = ring + in * (CH * 3 * NT);
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
-        if (k >= w.slots) continue;
-        copy_async<16>(to + (3 * k) * NT, dy + k * hop);
-        copy_async<16>(to + (3 * k + 1) * NT, t + k * hop);
-        if (a.dtotal) copy_async<16>(to + (3 * k + 2) * NT, dt + k * hop);
+        if (at + k * h.team >= w.slots) continue;
+        copy_async<16>(to + (3 * k) * NT, dy + start + k * hop);
+        copy_async<16>(to + (3 * k + 1) * NT, t + start + k * hop);
+        if (a.dtotal) copy_async<16>(to + (3 * k + 2) * NT, dt + start + k * hop);
       }
+      --ahead;
+      dy += dy_step; t += t_step; dt += dt_step;
     }
     copies_commit();
     in = in + 1 == h.depth ? 0 : in + 1;
   };
-  // what does not go through the ring: 1/rms, and an element of the head or the tail
+  // what does not go through the ring: 1/rms, and an element of the head or the tail, of the row that is worked on next
   struct Side { float r, dy, t, dt; } now = {}, next = {};
-  auto side = [&](Side &o, uint64_t row) {
-    if (!works || row >= a.rows) return;
-    o.r = a.inv_rms[row];
+  const T *dy1 = dy, *t1 = t, *dt1 = dt;
+  auto side = [&](Side &o) {
+    o.r = *inv;
+    inv += step;
     if constexpr (SHIFT) {
-      const Row w = shape(row);
+      const Row w = shape(dy1);
       o.dy = o.t = o.dt = 0.0f;
       if (w.on_edge) {
-        o.dy = to_float(dy_of(row)[w.edge]); o.t = to_float(t_of(row)[w.edge]);
-        if (a.dtotal) o.dt = to_float(dt_of(row)[w.edge]);
+        o.dy = to_float(dy1[w.edge]); o.t = to_float(t1[w.edge]);
+        if (a.dtotal) o.dt = to_float(dt1[w.edge]);
       }
+      dy1 += dy_step; t1 += t_step; dt1 += dt_step;
     }
   };
-  const uint64_t step = (uint64_t)gridDim.x * h.teams;
-  uint64_t row = (uint64_t)blockIdx.x * h.teams + mine;
-  for (uint32_t i = 0; i + 1 < h.depth; ++i) copy(row + i * step);
-  side(next, row);
+  for (uint32_t i = 1; i < h.depth; ++i) copy();
+  if (left) side(next);
   uint32_t turn = 0;
-  for (; works && row < a.rows; row += step, turn ^= 1) {
+  for (; left; --left, turn ^= 1) {
     now = next;
-    copy(row + (h.depth - 1) * step);
-    side(next, row + step);
-    if (h.depth == 1) copies_wait<0>(); else if (h.depth == 2) copies_wait<1>(); else if (h.depth == 3) copies_wait<2>(); else copies_wait<3>();
-    const Row w = shape(row);
+    copy();
+    if (left > 1) side(next);
+    if (h.depth == 4) copies_wait<3>(); else if (h.depth == 3) copies_wait<2>(); else if (h.depth == 2) copies_wait<1>(); else copies_wait<0>();
+    const Row w = shape(dx);              // (begins at the same place of a slot as dy)
     const uint4 *from = ring + out * (CH * 3 * NT);
     out = out + 1 == h.depth ? 0 : out + 1;
     // where the columns' weights and sums are: element i of slot k at pad + k*hop_pad + i, one further from the next multiple of V on
-    const uint32_t pad = w.start + at, hop_pad = hop + h.team, wrap = V - w.head;
-    auto place = [&](int k, int i) { return pad + k * hop_pad + i + (i >= wrap); };
+    const uint32_t pad = w.head + at * (V + 1), hop_pad = hop + h.team, wrap = V - w.head;
     float2 dot2 = both(0.0f);
+    // a single slot stays in registers between the two passes over the row, more are read again
+    constexpr bool ONE = CH == 1;
+    float2 u[H], v[H];
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      if (k >= w.slots) continue;
-      float2 dy[H], t[H];
-      Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(dy));
-      Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(t));
+      if (at + k * h.team >= w.slots) continue;
+      Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(u));
+      Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(v));
 #pragma unroll
       for (int i = 0; i < H; ++i) {
-        float2 v;
-        if constexpr (SHIFT) v = make_float2(weights[place(k, 2 * i)], weights[place(k, 2 * i + 1)]); else v = g[k][i];
-        dot2 = fma2(mul2(dy[i], v), t[i], dot2);
+        float2 gi;
+        if constexpr (SHIFT) {
+          const float *p = weights + pad + k * hop_pad;
+          gi = make_float2((2 * i >= wrap ? p + 1 : p)[2 * i], (2 * i + 1 >= wrap ? p + 1 : p)[2 * i + 1]);
+        } else gi = g[k][i];
+        dot2 = fma2(mul2(u[i], gi), v[i], dot2);
       }
     }
     float dot = dot2.x + dot2.y, ge = 0.0f;
@@ -437,55 +448,67 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
       if (SHIFT) __syncwarp(lanes);
     }
     const float2 r = both(now.r), c = both(-now.r * now.r * now.r * dot * a.inv_cols);
-    T *dx = static_cast<T *>(a.dx) + row * a.dx_stride;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      if (k >= w.slots) continue;
-      float2 dy[H], t[H], dt[H];
-      Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(dy));
-      Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(t));
-      if (a.dtotal) Vec<T>{from[(3 * k + 2) * NT]}.floats(reinterpret_cast<float *>(dt));
+      if (at + k * h.team >= w.slots) continue;
+      if (!ONE) {
+        Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(u));
+        Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(v));
+      }
+      float2 e[H];
 #pragma unroll
       for (int i = 0; i < H; ++i) {
-        const float2 dyr = mul2(dy[i], r);
-        float2 v;
+        const float2 ur = mul2(u[i], r);
+        float2 gi;
         if constexpr (SHIFT) {
-          const float2 p = mul2(dyr, t[i]);
-          own[place(k, 2 * i)] += p.x;
-          own[place(k, 2 * i + 1)] += p.y;
-          v = make_float2(weights[place(k, 2 * i)], weights[place(k, 2 * i + 1)]);
+          const float *p = weights + pad + k * hop_pad;
+          float *s = own + pad + k * hop_pad;
+          const float2 add = mul2(ur, v[i]);
+          (2 * i >= wrap ? s + 1 : s)[2 * i] += add.x;
+          (2 * i + 1 >= wrap ? s + 1 : s)[2 * i + 1] += add.y;
+          gi = make_float2((2 * i >= wrap ? p + 1 : p)[2 * i], (2 * i + 1 >= wrap ? p + 1 : p)[2 * i + 1]);
         } else {
-          acc[k][i] = fma2(dyr, t[i], acc[k][i]);
-          v = g[k][i];
+          acc[k][i] = fma2(ur, v[i], acc[k][i]);
+          gi = g[k][i];
         }
-        dy[i] = fma2(dyr, v, mul2(t[i], c));
-        if (a.dtotal) dy[i] = add2(dy[i], dt[i]);
+        e[i] = fma2(ur, gi, mul2(v[i], c));
       }
-      Vec<T>::of(reinterpret_cast<const float *>(dy)).store(dx + w.start + k * hop);
+      if (a.dtotal) {
+        Vec<T>{from[(3 * k + 2) * NT]}.floats(reinterpret_cast<float *>(v));
+#pragma unroll
+        for (int i = 0; i < H; ++i) e[i] = add2(e[i], v[i]);
+      }
+      Vec<T>::of(reinterpret_cast<const float *>(e)).store(dx + w.head + at * V + k * hop);
     }
     if (w.on_edge) {
       own[pe] += now.dy * now.r * now.t;
       dx[w.edge] = from_float<T>(fmaf(now.dy * now.r, ge, now.t * c.x) + now.dt);
     }
+    dx += dx_step;
   }
   if (!a.dgamma) return;
+  pdl_trigger();
   copies_wait<0>();
   __syncthreads();
   uint32_t parts = h.teams;
   if constexpr (!SHIFT) {
-    // the teams of a warp join first
+    // the teams of a warp join first; a block of one team has its sums in registers
     sums = reinterpret_cast<float *>(shared);
     if (h.team < 32) parts = (h.teams * h.team + 31) / 32;
     const uint32_t part = h.team < 32 ? warp : mine;
+    float *to = parts == 1 ? a.partial + (uint64_t)blockIdx.x * a.cols : sums + (size_t)part * a.cols;
 #pragma unroll
-    for (int k = 0; k < CH; ++k)
+    for (int k = 0; k < CH; ++k) {
+      float *v = reinterpret_cast<float *>(acc[k]);
+      for (uint32_t o = h.team; o < 32; o *= 2)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float v = reinterpret_cast<const float *>(acc[k])[i];
-        for (uint32_t o = h.team; o < 32; o *= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-        const uint32_t c = at * V + k * hop + i;
-        if (part < parts && c < a.cols && (h.team >= 32 || lane < h.team)) sums[(size_t)part * a.cols + c] = v;
-      }
+        for (int i = 0; i < V; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+      const uint32_t c = at * V + k * hop;
+      if (part >= parts || c >= a.cols || (h.team < 32 && lane >= h.team)) continue;
+#pragma unroll
+      for (int i = 0; i < V; i += 4) *reinterpret_cast<float4 *>(to + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    }
+    if (parts == 1) return;
     __syncthreads();
   }
   const uint32_t apart = SHIFT ? h.padded : a.cols;
@@ -510,25 +533,25 @@ template <typename T> __global__ void __launch_bounds__(kThreads) rms_norm_dgamm
   a.partial[(uint64_t)blockIdx.y * a.cols + c] = sum;
 }
 
-// The blocks' sums: a lane has a column, a warp every eighth part of it
-__global__ void __launch_bounds__(kThreads) join_columns_kernel(uint32_t cols, uint32_t parts, const float *partial, void *out, int type)
+// The blocks' sums: a lane has a column, a warp every 32nd block, all of whose sums are asked for at once
+__global__ void __launch_bounds__(1024) join_columns_kernel(uint32_t cols, uint32_t parts, const float *partial, void *out, int type)
 {
-  constexpr uint32_t kWarps = kThreads / 32;
-  __shared__ float sums[kWarps][33];
+  constexpr uint32_t kEach = (kMostParts + 31) / 32;
+  __shared__ float sums[32][33];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;
   pdl_wait();
-  float sum = 0.0f;
-  if (c < cols) {
-#pragma unroll 4
-    for (uint32_t p = warp; p < parts; p += kWarps) sum += partial[(uint64_t)p * cols + c];
-  }
+  float v[kEach], sum = 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) v[i] = c < cols && warp + 32 * i < parts ? partial[(uint64_t)(warp + 32 * i) * cols + c] : 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) sum += v[i];
   sums[warp][lane] = sum;
   __syncthreads();
-  if (warp || c >= cols) return;
-#pragma unroll
-  for (uint32_t w = 1; w < kWarps; ++w) sum += sums[w][lane];
-  put_weight(out, type, (uint32_t)c, sum);
+  // a warp per column: a lane's term of each
+  sum = warp_sum_all(sums[lane][warp]);
+  const uint64_t mine = (uint64_t)blockIdx.x * 32 + warp;
+  if (lane == 0 && mine < cols) put_weight(out, type, (uint32_t)mine, sum);
 }
 
 template <typename T> __global__ void __launch_bounds__(kThreads) rms_norm_dx_kernel(const GradArgs a)
@@ -617,8 +640,8 @@ bool grad_plan(const GradArgs &a, int type, HeldGrad &h, uint32_t &chunks, uint3
   if (!in_step(a.total, e, a.total_stride, v, a.dy, e, a.dy_stride, a.rows) || !in_step(a.dtotal, e, a.dtotal_stride, v, a.dy, e, a.dy_stride, a.rows) ||
       !in_step(a.dx, e, a.dx_stride, v, a.dy, e, a.dy_stride, a.rows)) return false;
   shift = !aligned_to(a.dy, 16) || a.cols % v || (a.rows > 1 && a.dy_stride % v) || !aligned_to(a.gamma.p, 16);
-  chunks = slots <= 1024 ? 1 : 4;
-  threads = slots > 1024 && slots <= 2048 && v == 8 ? 512 : 1024;
+  chunks = slots <= 32 ? 1 : slots < 128 ? 2 : 4;
+  threads = slots <= 2048 ? 512 : 1024;
   if (slots > (v == 8 ? 2048u : 4096u)) return false;
   h.team = (slots + chunks * 32 - 1) / (chunks * 32) * 32;
   if (slots <= 16) {
@@ -650,7 +673,7 @@ template <typename T, int CH, int NT> int launch_grad(const GradArgs &a, const H
 int norm_forward(const NormArgs &a, int type, int gamma_type, bool quant, cudaStream_t stream)
 {
   if (!known_type(type) || (a.gamma.p && !known_type(gamma_type))) return ANODE_E_TYPE;
-  if (a.cols == 0 || a.rows >> 40) return ANODE_E_DIMS;
+  if (a.cols == 0 || a.rows >> 36) return ANODE_E_DIMS;
   if (a.rows == 0) return ANODE_OK;
   const size_t e = type_bytes(type);
   TRY(check_rows(a.x, e, a.rows, a.cols, a.x_stride, false));
@@ -729,7 +752,7 @@ extern "C" int anode_gpu_rms_norm_add_bwd(
 {
   (void)cfg;
   if (!known_type(type) || ((gamma || dgamma) && !known_type(gamma_type))) return ANODE_E_TYPE;
-  if (cols == 0 || rows >> 40) return ANODE_E_DIMS;
+  if (cols == 0 || rows >> 36) return ANODE_E_DIMS;
   if (gamma && !aligned_to(gamma, type_bytes(gamma_type))) return ANODE_E_ALIGN;
   if (dgamma) {
     if (!aligned_to(dgamma, type_bytes(gamma_type))) return ANODE_E_ALIGN;
@@ -758,14 +781,15 @@ extern "C" int anode_gpu_rms_norm_add_bwd(
     if (held) {
       const uint64_t blocks = (rows + h.teams - 1) / h.teams;
       if (a.parts > blocks) a.parts = (uint32_t)blocks;
-      if (chunks == 1) TRY((launch_grad<T, 1, 1024>(a, h, shift, stream)));
-      else if constexpr (sizeof(T) == 2) TRY((launch_grad<T, 4, 512>(a, h, shift, stream)));
-      else TRY((launch_grad<T, 4, 1024>(a, h, shift, stream)));
-      return dgamma ? launch(join_columns_kernel, dim3(narrow), kThreads, 0, stream, cols, a.parts, a.partial, dgamma, gamma_type) : (int)ANODE_OK;
+      if (chunks == 1) TRY((launch_grad<T, 1, 512>(a, h, shift, stream)));
+      else if (chunks == 2) TRY((launch_grad<T, 2, 512>(a, h, shift, stream)));
+      else if (threads == 512) TRY((launch_grad<T, 4, 512>(a, h, shift, stream)));
+      else if constexpr (sizeof(T) == 4) TRY((launch_grad<T, 4, 1024>(a, h, shift, stream)));
+      return dgamma ? launch(join_columns_kernel, dim3(narrow), 1024, 0, stream, cols, a.parts, a.partial, dgamma, gamma_type) : (int)ANODE_OK;
     }
     if (dgamma) {
       TRY(launch(rms_norm_dgamma_kernel<T>, dim3(wide, a.parts), kThreads, 0, stream, a));
-      TRY(launch(join_columns_kernel, dim3(narrow), kThreads, 0, stream, cols, a.parts, a.partial, dgamma, gamma_type));
+      TRY(launch(join_columns_kernel, dim3(narrow), 1024, 0, stream, cols, a.parts, a.partial, dgamma, gamma_type));
     }
     return launch(rms_norm_dx_kernel<T>, dim3(row_blocks(rows)), kThreads, 0, stream, a);
   });

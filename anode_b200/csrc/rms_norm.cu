@@ -311,94 +311,86 @@ struct GradArgs {
 };
 
 // How the adjoint's rows are held: `teams` teams of `team` threads to a block, each with a row at a time, `depth` rows on their way or at work;
-// `padded` floats of a row of sums in shared memory
-struct HeldGrad { uint32_t team, teams, depth, padded; };
+// a team's rows lie `step` apart
+struct HeldGrad {
+  uint32_t team, teams, depth;
+  uint64_t step;
+};
 
 // The adjoint with its rows held on chip: a team of threads (4 to 32 lanes of a warp, or more warps) walks down rows, a thread with CH slots of 16
 // bytes of each array, so that one pass gives dx and dgamma's sums.  The next rows are on their way by asynchronous copies, each thread into a
 // ring of its own: a thread waits for nothing but its own copies and, once per row, its team's sum.
-// A thread's columns are the same in all rows, and dgamma's sums are in its registers; SHIFT, as in rms_norm_held_kernel: the columns
-// move with the rows' beginnings, and sums and weights are in shared memory, where column c is at c + c/V, so that threads with V
-// columns each meet in no bank.  Both kinds join in a fixed order, the blocks' in a second launch.
+// A thread's columns are the same in all of its team's rows: weights and dgamma's sums are in its registers.  SHIFT, as in
+// rms_norm_held_kernel: rows that begin at different places of a slot do so in turns of at most V, so a team's rows lie a multiple of V
+// apart and begin at the same one.
+// The sums join in a fixed order, the teams' in shared memory and the blocks' in a second launch.
 template <typename T, int CH, int NT, bool SHIFT>
 __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, const HeldGrad h)
 {
   constexpr int V = Vec<T>::V, H = V / 2;
   __shared__ float buf[2][32];
-  extern __shared__ float4 shared[];            // the rings [depth][CH][3][thread]; SHIFT: weights [padded], sums [teams][padded]; at last the sums [teams][cols]
+  extern __shared__ float4 shared[];            // the rings [depth][CH][3][thread]; at last the sums [teams][cols]
   const uint32_t mine = threadIdx.x / h.team, at = threadIdx.x - mine * h.team, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool works = mine < h.teams;
+  const uint64_t row0 = (uint64_t)blockIdx.x * h.teams + mine;
+  const bool works = mine < h.teams && row0 < h.step && row0 < a.rows;
   const uint32_t lanes = h.team < 32 ? ((1u << h.team) - 1) << (lane & ~(h.team - 1)) : 0xffffffffu;      // of this warp in the team
   uint4 *ring = reinterpret_cast<uint4 *>(shared) + threadIdx.x;
-  float *weights = reinterpret_cast<float *>(shared + (size_t)h.depth * CH * 3 * NT), *sums = weights + h.padded, *own = sums + (size_t)mine * h.padded;
-  const uint32_t hop = h.team * V;
-  pdl_wait();
-  float2 acc[SHIFT ? 1 : CH][H], g[SHIFT ? 1 : CH][H];
-  if constexpr (SHIFT) {
-    for (uint32_t c = threadIdx.x; c < a.cols; c += NT) weights[c + c / V] = a.gamma.at(c);
-    for (uint32_t c = threadIdx.x; c < h.teams * h.padded; c += NT) sums[c] = 0.0f;
-    __syncthreads();
-  } else {
-#pragma unroll
-    for (int k = 0; k < CH; ++k) {
-#pragma unroll
-      for (int i = 0; i < H; ++i) acc[k][i] = both(0.0f);
-      if (works && at * V + k * hop < a.cols) a.gamma.load<V>(at * V + k * hop, reinterpret_cast<float *>(g[k]));
-    }
-  }
-  // a row of this team, from where its dy is: columns before its first whole slot, slots, and this thread's element of the head or the tail
-  struct Row { uint32_t head, slots, edge; bool on_edge; };
-  auto shape = [&](const T *dy) {
-    Row w;
-    w.head = SHIFT ? min(a.cols, (0u - (uint32_t)((uintptr_t)dy / sizeof(T))) & (V - 1)) : 0;
-    w.slots = (a.cols - w.head) / V;
-    const uint32_t tail = a.cols - w.head - w.slots * V;
-    w.edge = at < w.head ? at : a.cols - tail + (at - w.head);
-    w.on_edge = SHIFT && at < w.head + tail;
-    return w;
-  };
-  const uint64_t step = (uint64_t)gridDim.x * h.teams, row0 = (uint64_t)blockIdx.x * h.teams + mine;
-  // rows that this team has: at work, and to be copied
-  uint32_t left = works && row0 < a.rows ? (uint32_t)((a.rows - row0 + step - 1) / step) : 0, ahead = left;
   const T *dy = static_cast<const T *>(a.dy) + row0 * a.dy_stride, *t = static_cast<const T *>(a.total) + row0 * a.total_stride;
   const T *dt = static_cast<const T *>(a.dtotal) + row0 * a.dtotal_stride;
   T *dx = static_cast<T *>(a.dx) + row0 * a.dx_stride;
   const float *inv = a.inv_rms + row0;
-  const uint64_t dy_step = step * a.dy_stride, t_step = step * a.total_stride, dt_step = step * a.dtotal_stride, dx_step = step * a.dx_stride;
-  uint32_t in = 0, out = 0;
+  // a row's columns before its first whole slot, and what remains behind the last one; this thread's slots, and its element of those
+  const uint32_t head = SHIFT ? min(a.cols, (0u - (uint32_t)((uintptr_t)dy / sizeof(T))) & (V - 1)) : 0, slots = (a.cols - head) / V;
+  const uint32_t tail = a.cols - head - slots * V, edge = at < head ? at : a.cols - tail + (at - head), start = head + at * V, hop = h.team * V;
+  const bool on_edge = SHIFT && works && at < head + tail;
+  auto has = [&](int k) { return works && at + k * h.team < slots; };
+  pdl_wait();
+  float2 acc[CH][H], g[CH][H];
+  float acc_edge = 0.0f, g_edge = on_edge ? a.gamma.at(edge) : 0.0f;
+  const bool aligned_gamma = ((uintptr_t)a.gamma.p & 15) == 0;
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) acc[k][i] = g[k][i] = both(0.0f);
+    if (!has(k)) continue;
+    float *w = reinterpret_cast<float *>(g[k]);
+    if (!SHIFT) a.gamma.load<V>(start + k * hop, w);
+    else if (aligned_gamma) a.gamma.load_any<V>(start + k * hop, a.cols, w);
+    else a.gamma.load_each<V>(start + k * hop, w);
+  }
+  // rows that this team has: at work, and to be copied
+  uint32_t left = works ? (uint32_t)((a.rows - row0 + h.step - 1) / h.step) : 0, ahead = left, in = 0, out = 0;
+  const uint64_t dy_step = h.step * a.dy_stride, t_step = h.step * a.total_stride, dt_step = h.step * a.dtotal_stride, dx_step = h.step * a.dx_stride;
+  // what does not go through the ring, of the row that is worked on next: 1/rms, and an element of the head or the tail
+  struct Side { float r, dy, t, dt; } now = {}, next = {};
+  const T *dy1 = dy + edge, *t1 = t + edge, *dt1 = dt + edge;
+  auto side = [&](Side &o) {
+    o.r = *inv;
+    inv += h.step;
+    if constexpr (SHIFT) {
+      if (on_edge) {
+        o.dy = to_float(*dy1); o.t = to_float(*t1);
+        if (a.dtotal) o.dt = to_float(*dt1);
+      }
+      dy1 += dy_step; t1 += t_step; dt1 += dt_step;
+    }
+  };
+  dy += start; t += start; dt += start;
   auto copy = [&] {                     // the next row to be copied
     if (ahead) {
-      const Row w = shape(dy);
-      const uint32_t start = w.head + at * V;
       uint4 *to = ring + in * (CH * 3 * NT);
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
-        if (at + k * h.team >= w.slots) continue;
-        copy_async<16>(to + (3 * k) * NT, dy + start + k * hop);
-        copy_async<16>(to + (3 * k + 1) * NT, t + start + k * hop);
-        if (a.dtotal) copy_async<16>(to + (3 * k + 2) * NT, dt + start + k * hop);
+        if (!has(k)) continue;
+        copy_async<16>(to + (3 * k) * NT, dy + k * hop);
+        copy_async<16>(to + (3 * k + 1) * NT, t + k * hop);
+        if (a.dtotal) copy_async<16>(to + (3 * k + 2) * NT, dt + k * hop);
       }
       --ahead;
       dy += dy_step; t += t_step; dt += dt_step;
     }
     copies_commit();
     in = in + 1 == h.depth ? 0 : in + 1;
-  };
-  // what does not go through the ring: 1/rms, and an element of the head or the tail, of the row that is worked on next
-  struct Side { float r, dy, t, dt; } now = {}, next = {};
-  const T *dy1 = dy, *t1 = t, *dt1 = dt;
-  auto side = [&](Side &o) {
-    o.r = *inv;
-    inv += step;
-    if constexpr (SHIFT) {
-      const Row w = shape(dy1);
-      o.dy = o.t = o.dt = 0.0f;
-      if (w.on_edge) {
-        o.dy = to_float(dy1[w.edge]); o.t = to_float(t1[w.edge]);
-        if (a.dtotal) o.dt = to_float(dt1[w.edge]);
-      }
-      dy1 += dy_step; t1 += t_step; dt1 += dt_step;
-    }
   };
   for (uint32_t i = 1; i < h.depth; ++i) copy();
   if (left) side(next);
@@ -408,33 +400,21 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
     copy();
     if (left > 1) side(next);
     if (h.depth == 4) copies_wait<3>(); else if (h.depth == 3) copies_wait<2>(); else if (h.depth == 2) copies_wait<1>(); else copies_wait<0>();
-    const Row w = shape(dx);              // (begins at the same place of a slot as dy)
     const uint4 *from = ring + out * (CH * 3 * NT);
     out = out + 1 == h.depth ? 0 : out + 1;
-    // where the columns' weights and sums are: element i of slot k at pad + k*hop_pad + i, one further from the next multiple of V on
-    const uint32_t pad = w.head + at * (V + 1), hop_pad = hop + h.team, wrap = V - w.head;
-    float2 dot2 = both(0.0f);
+    float2 dot2 = make_float2(SHIFT ? now.dy * g_edge * now.t : 0.0f, 0.0f);
     // a single slot stays in registers between the two passes over the row, more are read again
     constexpr bool ONE = CH == 1;
     float2 u[H], v[H];
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      if (at + k * h.team >= w.slots) continue;
+      if (!has(k)) continue;
       Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(u));
       Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(v));
 #pragma unroll
-      for (int i = 0; i < H; ++i) {
-        float2 gi;
-        if constexpr (SHIFT) {
-          const float *p = weights + pad + k * hop_pad;
-          gi = make_float2((2 * i >= wrap ? p + 1 : p)[2 * i], (2 * i + 1 >= wrap ? p + 1 : p)[2 * i + 1]);
-        } else gi = g[k][i];
-        dot2 = fma2(mul2(u[i], gi), v[i], dot2);
-      }
+      for (int i = 0; i < H; ++i) dot2 = fma2(mul2(u[i], g[k][i]), v[i], dot2);
     }
-    float dot = dot2.x + dot2.y, ge = 0.0f;
-    const uint32_t pe = w.edge + w.edge / V;
-    if (w.on_edge) { ge = weights[pe]; dot = fmaf(now.dy * ge, now.t, dot); }
+    float dot = dot2.x + dot2.y;
     if (h.team >= 32) {
       dot = warp_sum_all(dot);
       if (h.team > 32) {
@@ -442,15 +422,12 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
         asm volatile("bar.sync %0, %1;" ::"r"(mine + 1), "r"(h.team) : "memory");
         const uint32_t first = mine * h.team / 32, warps = h.team / 32;
         dot = warp_sum_all(lane < warps ? buf[turn][first + lane] : 0.0f);
-      } else if (SHIFT) __syncwarp();           // (another lane has had these columns in the row before)
-    } else {
-      for (uint32_t o = h.team / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(lanes, dot, o);
-      if (SHIFT) __syncwarp(lanes);
-    }
+      }
+    } else for (uint32_t o = h.team / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(lanes, dot, o);
     const float2 r = both(now.r), c = both(-now.r * now.r * now.r * dot * a.inv_cols);
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      if (at + k * h.team >= w.slots) continue;
+      if (!has(k)) continue;
       if (!ONE) {
         Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(u));
         Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(v));
@@ -459,30 +436,19 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
 #pragma unroll
       for (int i = 0; i < H; ++i) {
         const float2 ur = mul2(u[i], r);
-        float2 gi;
-        if constexpr (SHIFT) {
-          const float *p = weights + pad + k * hop_pad;
-          float *s = own + pad + k * hop_pad;
-          const float2 add = mul2(ur, v[i]);
-          (2 * i >= wrap ? s + 1 : s)[2 * i] += add.x;
-          (2 * i + 1 >= wrap ? s + 1 : s)[2 * i + 1] += add.y;
-          gi = make_float2((2 * i >= wrap ? p + 1 : p)[2 * i], (2 * i + 1 >= wrap ? p + 1 : p)[2 * i + 1]);
-        } else {
-          acc[k][i] = fma2(ur, v[i], acc[k][i]);
-          gi = g[k][i];
-        }
-        e[i] = fma2(ur, gi, mul2(v[i], c));
+        acc[k][i] = fma2(ur, v[i], acc[k][i]);
+        e[i] = fma2(ur, g[k][i], mul2(v[i], c));
       }
       if (a.dtotal) {
         Vec<T>{from[(3 * k + 2) * NT]}.floats(reinterpret_cast<float *>(v));
 #pragma unroll
         for (int i = 0; i < H; ++i) e[i] = add2(e[i], v[i]);
       }
-      Vec<T>::of(reinterpret_cast<const float *>(e)).store(dx + w.head + at * V + k * hop);
+      Vec<T>::of(reinterpret_cast<const float *>(e)).store(dx + start + k * hop);
     }
-    if (w.on_edge) {
-      own[pe] += now.dy * now.r * now.t;
-      dx[w.edge] = from_float<T>(fmaf(now.dy * now.r, ge, now.t * c.x) + now.dt);
+    if (on_edge) {
+      acc_edge = fmaf(now.dy * now.r, now.t, acc_edge);
+      dx[edge] = from_float<T>(fmaf(now.dy * now.r, g_edge, now.t * c.x) + now.dt);
     }
     dx += dx_step;
   }
@@ -490,10 +456,25 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
   pdl_trigger();
   copies_wait<0>();
   __syncthreads();
+  float *sums = reinterpret_cast<float *>(shared);
   uint32_t parts = h.teams;
-  if constexpr (!SHIFT) {
+  const uint32_t apart = SHIFT ? a.cols + a.cols / V + 1 : a.cols;
+  if constexpr (SHIFT) {
+    // column c at c + c/V, so that threads with V columns each meet in no bank (a team without a row has zeros)
+    if (mine < h.teams) {
+      float *to = sums + (size_t)mine * apart;
+      for (uint32_t c = at; !works && c < apart; c += h.team) to[c] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        if (!has(k)) continue;
+        float *p = to + start + k * hop + at + k * h.team;
+#pragma unroll
+        for (int i = 0; i < V; ++i) (head + i < V ? p : p + 1)[i] = reinterpret_cast<const float *>(acc[k])[i];
+      }
+      if (on_edge) to[edge + edge / V] = acc_edge;
+    }
+  } else {
     // the teams of a warp join first; a block of one team has its sums in registers
-    sums = reinterpret_cast<float *>(shared);
     if (h.team < 32) parts = (h.teams * h.team + 31) / 32;
     const uint32_t part = h.team < 32 ? warp : mine;
     float *to = parts == 1 ? a.partial + (uint64_t)blockIdx.x * a.cols : sums + (size_t)part * a.cols;
@@ -503,19 +484,17 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
       for (uint32_t o = h.team; o < 32; o *= 2)
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-      const uint32_t c = at * V + k * hop;
+      const uint32_t c = start + k * hop;
       if (part >= parts || c >= a.cols || (h.team < 32 && lane >= h.team)) continue;
 #pragma unroll
       for (int i = 0; i < V; i += 4) *reinterpret_cast<float4 *>(to + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     }
     if (parts == 1) return;
-    __syncthreads();
   }
-  const uint32_t apart = SHIFT ? h.padded : a.cols;
+  __syncthreads();
   for (uint32_t c = threadIdx.x; c < a.cols; c += NT) {
-    const uint32_t i = SHIFT ? c + c / V : c;
     float sum = 0.0f;
-    for (uint32_t t = 0; t < parts; ++t) sum += sums[(size_t)t * apart + i];
+    for (uint32_t t = 0; t < parts; ++t) sum += sums[(size_t)t * apart + (SHIFT ? c + c / V : c)];
     a.partial[(uint64_t)blockIdx.x * a.cols + c] = sum;
   }
 }
@@ -653,10 +632,7 @@ bool grad_plan(const GradArgs &a, int type, HeldGrad &h, uint32_t &chunks, uint3
   if (h.team > 32 && h.teams > 15) h.teams = 15;      // (a named barrier each)
   const uint32_t sms = sm_count();
   if (a.rows < (uint64_t)h.teams * sms) h.teams = (uint32_t)((a.rows + sms - 1) / sms);     // a row per block first
-  h.padded = shift ? (a.cols + a.cols / v + 4) / 4 * 4 : 0;
-  const size_t fixed = (size_t)h.padded * 4 * (1 + h.teams), each = (size_t)threads * chunks * 48, room = 226 * 1024;
-  if (fixed + each > room) return false;
-  h.depth = (uint32_t)((room - fixed) / each);
+  h.depth = (uint32_t)(226 * 1024 / ((size_t)threads * chunks * 48));
   if (h.depth > 4) h.depth = 4;
   return true;
 }
@@ -664,7 +640,9 @@ bool grad_plan(const GradArgs &a, int type, HeldGrad &h, uint32_t &chunks, uint3
 template <typename T, int CH, int NT> int launch_grad(const GradArgs &a, const HeldGrad &h, bool shift, cudaStream_t stream)
 {
   const auto kernel = shift ? rms_norm_grad_kernel<T, CH, NT, true> : rms_norm_grad_kernel<T, CH, NT, false>;
-  const size_t shared = (size_t)h.depth * CH * NT * 48 + (shift ? (size_t)h.padded * 4 * (1 + h.teams) : 0);
+  size_t shared = (size_t)h.depth * CH * NT * 48;
+  const size_t sums = (size_t)h.teams * (a.cols + (shift ? a.cols / Vec<T>::V + 1 : 0)) * 4;
+  if (shared < sums) shared = sums;
   static SharedMemory allowed[2];
   if (!allowed[shift].up_to((const void *)kernel, shared)) return ANODE_E_LAUNCH;
   return launch(kernel, dim3(a.parts), NT, shared, stream, a, h);
@@ -778,9 +756,12 @@ extern "C" int anode_gpu_rms_norm_add_bwd(
   const uint32_t wide = (uint32_t)(((uint64_t)cols + kThreads - 1) / kThreads), narrow = (uint32_t)(((uint64_t)cols + 31) / 32);
   return by_type(type, [&](auto t) {
     using T = decltype(t);
+    constexpr uint32_t V = Vec<T>::V;
     if (held) {
       const uint64_t blocks = (rows + h.teams - 1) / h.teams;
       if (a.parts > blocks) a.parts = (uint32_t)blocks;
+      h.step = (uint64_t)a.parts * h.teams;
+      if (shift && rows > h.step) h.step = h.step / V * V;
       if (chunks == 1) TRY((launch_grad<T, 1, 512>(a, h, shift, stream)));
       else if (chunks == 2) TRY((launch_grad<T, 2, 512>(a, h, shift, stream)));
       else if (threads == 512) TRY((launch_grad<T, 4, 512>(a, h, shift, stream)));

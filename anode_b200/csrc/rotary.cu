@@ -8,7 +8,7 @@
 // own, and goes through the heads with the next ones' data on their way by asynchronous copies: no warp waits for another.
 //
 // rotary_heads_kernel: the pairs' places divide by 16 (or 8) bytes.  A lane has ITEMS of 2V elements each: V pairs, or 2V elements that pass.
-// In the half layout an item is two vectors rot/2 apart, so that both elements of a pair are in one lane and the turn needs no exchange;
+// An item is two vectors rot/2 apart, so that both elements of a pair are in one lane in either layout and the turn needs no exchange;
 // only the norm's sums go across the group.  What a lane computes with is what it copied itself.  Lanes keep their items from head to head,
 // and with them the weights and the sums of the weights' gradients.
 // rotary_pairs_kernel: pairs anywhere.  Heads are copied as they lie, a lane has single pairs of them and puts the results in their place.
@@ -32,6 +32,7 @@ struct RotarySide {
   Weights gamma;
   uint32_t heads;
   uint32_t tokens, parts, span;        // a unit of a warp: `tokens` tokens, or one of the `parts` spans of a token's heads
+  uint32_t passes, last;               // heads of a group in a span, and in a token's last one
   uint32_t units;
   uint32_t blocks, want;               // blocks of the grid; whether the weights' gradient is asked for
 };
@@ -74,9 +75,9 @@ template <typename T, int V> struct Few {
   }
 };
 // An item's 2V elements as pairs of floats: f[0..V/2) the first elements of the pairs that turn together, f[V/2..V) the second ones
-template <typename T, int V> __device__ __forceinline__ void spread(const Few<T, V> (&in)[2], bool interleaved, float2 *f)
+template <bool interleaved, typename T, int V> __device__ __forceinline__ void spread(const Few<T, V> (&in)[2], float2 *f)
 {
-  if (interleaved) {
+  if constexpr (interleaved) {
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) {
       const float2 a = in[2 * j / (V / 2)].two(2 * j % (V / 2)), b = in[(2 * j + 1) / (V / 2)].two((2 * j + 1) % (V / 2));
@@ -87,9 +88,9 @@ template <typename T, int V> __device__ __forceinline__ void spread(const Few<T,
     for (int j = 0; j < V / 2; ++j) { f[j] = in[0].two(j); f[V / 2 + j] = in[1].two(j); }
   }
 }
-template <typename T, int V> __device__ __forceinline__ void gather(Few<T, V> (&out)[2], bool interleaved, const float2 *f)
+template <bool interleaved, typename T, int V> __device__ __forceinline__ void gather(Few<T, V> (&out)[2], const float2 *f)
 {
-  if (interleaved) {
+  if constexpr (interleaved) {
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) {
       out[2 * j / (V / 2)].put(2 * j % (V / 2), f[j].x, f[V / 2 + j].x);
@@ -145,22 +146,33 @@ template <typename T> struct Walk {
   // the first head of the unit
   __device__ __forceinline__ void enter(Place<T> &w, const HeadArray &p, const HeadArray *x) const
   {
-    if (w.unit >= d.units) { w.head = w.end = 0; w.left = 1; return; }
-    const uint32_t first = token(w.unit), low = d.parts > 1 ? (w.unit - first * d.parts) * d.span : 0, token = first + mine;
-    w.end = min(d.heads, low + d.span);
-    w.left = d.tokens > 1 ? 1 : (w.end - low + groups - 1) / groups;
-    w.head = low + group - mine * d.heads;
-    if (mine >= d.tokens || token >= a.total || group >= groups) w.head = w.end = 0;
-    const uint32_t b = a.batch == 1 ? 0 : token / a.seq, s = token - b * a.seq;
-    w.p = static_cast<const T *>(p.p) + b * p.batch + s * p.seq + w.head * p.head;
-    if (x) w.x = static_cast<const T *>(x->p) + b * x->batch + s * x->seq + w.head * x->head;
+    w.left = 1;
+    w.head = w.end = 0;
+    if (w.unit >= d.units) return;
+    uint32_t token = w.unit * d.tokens + mine, low = 0;
+    if (d.parts > 1) {
+      token = w.unit / d.parts;
+      const uint32_t part = w.unit - token * d.parts;
+      low = part * d.span;
+      w.left = part + 1 < d.parts ? d.passes : d.last;
+    } else if (d.tokens == 1) w.left = d.last;
+    const uint32_t head = low + group - mine * d.heads;
+    uint32_t b = 0, s = token;
+    if (a.batch > 1) { b = token / a.seq; s = token - b * a.seq; }
+    w.p = static_cast<const T *>(p.p) + s * p.seq + head * p.head;
+    if (x) w.x = static_cast<const T *>(x->p) + s * x->seq + head * x->head;
+    if (a.batch > 1) {
+      w.p += b * p.batch;
+      if (x) w.x += b * x->batch;
+    }
+    if (mine < d.tokens && token < a.total && group < groups) { w.head = head; w.end = min(d.heads, low + d.span); }
   }
-  __device__ __forceinline__ void advance(Place<T> &w, const HeadArray &p, const HeadArray *x) const
+  // to the group's next head, `hop` further
+  __device__ __forceinline__ void advance(Place<T> &w, const HeadArray &p, uint64_t hop, const HeadArray *x, uint64_t hop_x) const
   {
     if (--w.left) {
-      // (a group beyond the last stays there: its end is 0)
-      w.head += groups; w.p += p.head * groups;
-      if (x) w.x += x->head * groups;
+      w.head += groups; w.p += hop;         // (a group without a head stays without: its end is 0)
+      if (x) w.x += hop_x;
     } else { w.unit += step; enter(w, p, x); }
   }
 };
@@ -168,7 +180,8 @@ template <typename T> struct Walk {
 __device__ __forceinline__ float group_sum(float v, uint32_t lanes, uint32_t first)
 {
   if ((lanes & (lanes - 1)) == 0) {
-    for (uint32_t o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+    for (uint32_t o = 1; o < 32; o *= 2) if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
   }
   float sum = 0.0f;
@@ -182,14 +195,14 @@ __host__ __device__ constexpr int resident(int floats, bool norm) { return float
 __host__ __device__ constexpr int ring_depth(int it) { return it == 1 ? 4 : 2; }
 __host__ __device__ constexpr size_t ring_bytes(int v, int it, bool both, size_t e) { return (size_t)ring_depth(it) * kThreads * it * 2 * v * e * (both ? 2 : 1); }
 
-template <typename T, int V, int IT, bool NORM, bool BWD>
+template <typename T, int V, int IT, bool NORM, bool BWD, bool interleaved>
 __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_heads_kernel(const RotaryArgs a)
 {
   constexpr bool BOTH = NORM && BWD;        // two arrays are read
   constexpr bool KEEP = V * IT <= (BOTH ? 4 : 8);       // a lane's cosines and sines stay in its registers from head to head
-  constexpr int DEPTH = ring_depth(IT), PIECES = IT * 2 * (BOTH ? 2 : 1);
+  constexpr int DEPTH = ring_depth(IT), PIECES = IT * 2 * (BOTH ? 2 : 1), H = V / 2;
   typedef typename Few<T, V>::Raw Raw;
-  // each pair's turns per position; the rings, [depth][piece][thread]; of each warp, [tokens] cosines and sines: pairs j = item*V + i and the next of a token at i/2*turned + item,
+  // each pair's turns per position; the rings, [depth][piece][thread]; of each warp, [tokens] cosines and sines: pairs n and n + 1 of an item of a token at n/2*turned + item,
   // both cosines and then both sines, so that lanes read 16 bytes side by side; in their place the warps' sums of the weights' gradients, when
   // the block is done
   extern __shared__ float4 shared[];
@@ -197,7 +210,6 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_h
   const RotarySide &d = a.side[which];
   const uint32_t wlane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = 32 / a.lanes, group = wlane / a.lanes, lane = wlane - group * a.lanes;
   const uint32_t half = a.rot / 2;
-  const bool interleaved = a.interleaved;
   double *rates = reinterpret_cast<double *>(shared);
   Raw *ring = reinterpret_cast<Raw *>(shared + half / 2) + threadIdx.x;
   float4 *table = shared + half / 2 + ring_bytes(V, IT, BOTH, sizeof(T)) / 16 + (size_t)warp * d.tokens * half / 2;
@@ -209,8 +221,9 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_h
     const uint32_t p = lane + k * a.lanes;
     turns[k] = p < a.turned;
     has[k] = p < a.items;
-    e0[k] = !turns[k] ? a.rot + (p - a.turned) * 2 * V : interleaved ? p * 2 * V : p * V;
-    e1[k] = turns[k] && !interleaved ? half + p * V : e0[k] + V;
+    // (interleaved pairs are whole in either vector: these two lie apart, too, so that lanes side by side move 16 bytes side by side)
+    e0[k] = turns[k] ? p * V : a.rot + (p - a.turned) * 2 * V;
+    e1[k] = turns[k] ? half + p * V : e0[k] + V;
     second[k] = has[k] && e1[k] < a.dim;
   }
   pdl_wait();
@@ -256,6 +269,7 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_h
           if constexpr (BOTH) ring[(i * PIECES + 2 * IT + 2 * k + j) * kThreads] = Raw{};
         }
   const Walk<T> walk(a, d, group, groups);
+  const uint64_t hop = d.in.head * groups, hop_x = BOTH ? d.x.head * groups : 0, hop_out = d.out.head * groups;
   uint32_t turn_in = 0, turn_out = 0;        // the ring's places that are filled and emptied next
   auto load = [&](const Place<T> &w) {
     if (w.head < w.end) {
@@ -272,34 +286,38 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_h
     copies_commit();
     turn_in = (turn_in + 1) & (DEPTH - 1);
   };
-  // f -> f*straight + (its partner)*across, with the forward pass's weights in it
-  struct Turn { float2 straight[V], across[V]; };
+  // f -> f*straight + (its partner)*across, with the forward pass's weights in it (without them the two halves share their cosines, and
+  // across holds the sines)
+  constexpr bool WEIGHED = NORM && !BWD;
+  struct Turn { float2 straight[WEIGHED ? V : H], across[WEIGHED ? V : H]; };
   const uint32_t row = min(walk.mine, d.tokens - 1);       // (a group without a token reads another's: it stays within the table)
   auto coefficients = [&](int k, Turn &o) {
     const float2 *by = g[NORM ? k : 0];
+    const uint32_t from = row * half / 2 + (turns[k] ? lane + k * a.lanes : 0);
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      float4 t = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
-      if (turns[k]) t = table[row * half / 2 + i * a.turned + lane + k * a.lanes];
-      const float2 c = make_float2(t.x, t.y), s = make_float2(t.z, t.w), minus = make_float2(-t.z, -t.w);
-      if constexpr (NORM && !BWD) {
-        o.straight[i] = mul2(by[i], c); o.across[i] = mul2(by[V / 2 + i], minus);
-        o.straight[V / 2 + i] = mul2(by[V / 2 + i], c); o.across[V / 2 + i] = mul2(by[i], s);
+    for (int i = 0; i < H; ++i) {
+      float4 t = table[from + i * a.turned];
+      if constexpr (WEIGHED) {
+        if (!turns[k]) t = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
+        const float2 c = make_float2(t.x, t.y), s = make_float2(t.z, t.w), minus = make_float2(-t.z, -t.w);
+        o.straight[i] = mul2(by[i], c); o.across[i] = mul2(by[H + i], minus);
+        o.straight[H + i] = mul2(by[H + i], c); o.across[H + i] = mul2(by[i], s);
       } else {
-        o.straight[i] = c; o.across[i] = minus;
-        o.straight[V / 2 + i] = c; o.across[V / 2 + i] = s;
+        o.straight[i] = make_float2(t.x, t.y);
+        o.across[i] = make_float2(t.z, t.w);
       }
     }
   };
   auto turn = [&](int k, float2 *f, const Turn &o) {
     if (turns[k]) {
 #pragma unroll
-      for (int j = 0; j < V / 2; ++j) {
-        const float2 u = f[j], v = f[V / 2 + j];
-        f[j] = fma2(v, o.across[j], mul2(u, o.straight[j]));
-        f[V / 2 + j] = fma2(u, o.across[V / 2 + j], mul2(v, o.straight[V / 2 + j]));
+      for (int j = 0; j < H; ++j) {
+        const float2 u = f[j], v = f[H + j];
+        if constexpr (WEIGHED) f[j] = fma2(v, o.across[j], mul2(u, o.straight[j]));
+        else f[j] = fma2(mul2(v, o.across[j]), both(-1.0f), mul2(u, o.straight[j]));
+        f[H + j] = fma2(u, o.across[WEIGHED ? H + j : j], mul2(v, o.straight[WEIGHED ? H + j : j]));
       }
-    } else if (NORM && !BWD) {      // (elements that pass have no partner: its infinity would be a NaN here)
+    } else if (WEIGHED) {      // (elements that pass have no partner: its infinity would be a NaN here)
 #pragma unroll
       for (int j = 0; j < V; ++j) f[j] = mul2(f[j], o.straight[j]);
     }
@@ -314,14 +332,17 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_h
 #pragma unroll
   for (int i = 0; i < DEPTH - 1; ++i) {
     load(ahead);
-    walk.advance(ahead, d.in, from);
+    walk.advance(ahead, d.in, hop, from, hop_x);
   }
   __syncthreads();
   while (at.unit < d.units) {
     // the unit's cosines and sines
     __syncwarp();
     make_table(a, rates, d.tokens, position, [&](uint32_t t, uint32_t j, float2 cs) {
-      float *to = reinterpret_cast<float *>(table + t * half / 2 + j % V / 2 * a.turned + j / V) + j % 2;
+      // pair n of item `item`
+      const uint32_t late = interleaved && j >= half / 2, of = interleaved ? j - late * (half / 2) : j;
+      const uint32_t item = of / (interleaved ? H : V), n = interleaved ? late * H + of % H : of % V;
+      float *to = reinterpret_cast<float *>(table + t * half / 2 + n / 2 * a.turned + item) + n % 2;
       to[0] = cs.x; to[2] = cs.y;
     });
     position = position_of(a, walk.token(at.unit + walk.step), d.tokens, wlane);
@@ -333,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_h
     for (const uint32_t unit = at.unit; at.unit == unit;) {
       const bool live = at.head < at.end;
       load(ahead);
-      walk.advance(ahead, d.in, from);
+      walk.advance(ahead, d.in, hop, from, hop_x);
       copies_wait<DEPTH - 1>();
       float2 f[IT][V], sq2 = both(0.0f);
 #pragma unroll
@@ -341,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_h
         Few<T, V> in[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) in[j].raw = ring[(turn_out * PIECES + 2 * k + j) * kThreads];
-        spread(in, interleaved, f[k]);
+        spread<interleaved>(in, f[k]);
       }
       if constexpr (NORM && !BWD) {
 #pragma unroll
@@ -370,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_h
           Few<T, V> in[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) in[j].raw = ring[(turn_out * PIECES + 2 * IT + 2 * k + j) * kThreads];
-          spread(in, interleaved, x[k]);
+          spread<interleaved>(in, x[k]);
 #pragma unroll
           for (int i = 0; i < V; ++i) { sq2 = fma2(x[k][i], x[k][i], sq2); dot2 = fma2(mul2(f[k][i], g[k][i]), x[k][i], dot2); }
         }
@@ -393,12 +414,12 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_h
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
           Few<T, V> o[2];
-          gather(o, interleaved, f[k]);
+          gather<interleaved>(o, f[k]);
           if (has[k]) *reinterpret_cast<Raw *>(out + e0[k]) = o[0].raw;
           if (second[k]) *reinterpret_cast<Raw *>(out + e1[k]) = o[1].raw;
         }
       }
-      walk.advance(at, d.out, nullptr);
+      walk.advance(at, d.out, hop_out, nullptr, 0);
     }
   }
   if constexpr (BOTH) {
@@ -473,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, IT > 8 ? 1 : 2) rotary_pairs_kernel(
     }
   }
   const Walk<T> walk(a, d, group, groups);
+  const uint64_t hop = d.in.head * groups, hop_x = BOTH ? d.x.head * groups : 0, hop_out = d.out.head * groups;
   const HeadArray *from = BOTH ? &d.x : nullptr;
   uint32_t turn_in = 0, turn_out = 0;
   auto load = [&](const Place<T> &w) {
@@ -498,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, IT > 8 ? 1 : 2) rotary_pairs_kernel(
   walk.enter(ahead, d.in, from);
   long long position = position_of(a, walk.token(at.unit), d.tokens, wlane);
   load(ahead);
-  walk.advance(ahead, d.in, from);
+  walk.advance(ahead, d.in, hop, from, hop_x);
   __syncthreads();
   while (at.unit < d.units) {
     __syncwarp();
@@ -509,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, IT > 8 ? 1 : 2) rotary_pairs_kernel(
     for (const uint32_t unit = at.unit; at.unit == unit;) {
       const bool live = at.head < at.end;
       load(ahead);
-      walk.advance(ahead, d.in, from);
+      walk.advance(ahead, d.in, hop, from, hop_x);
       copies_wait<DEPTH - 1>();
       __syncwarp();                       // (lanes read what others copied)
       T *in = reinterpret_cast<T *>(place(turn_out, 0));
@@ -571,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, IT > 8 ? 1 : 2) rotary_pairs_kernel(
         }
       }
       turn_out ^= 1;
-      walk.advance(at, d.out, nullptr);
+      walk.advance(at, d.out, hop_out, nullptr, 0);
       // (the place is filled anew by copies of the lanes that emptied it, and the array beside it after every lane has passed the barrier above)
     }
   }
@@ -658,12 +680,12 @@ int launch_rotary(const RotaryArgs &a, uint32_t blocks, size_t tables, size_t su
     kernel = rotary_pairs_kernel<T, IT, NORM, BWD>;
     shared = (size_t)kWarps * 2 * (NORM && BWD ? 2 : 1) * (32 / a.lanes) * a.slot + tables;
   } else {
-    kernel = rotary_heads_kernel<T, V, IT, NORM, BWD>;
+    kernel = a.interleaved ? rotary_heads_kernel<T, V, IT, NORM, BWD, true> : rotary_heads_kernel<T, V, IT, NORM, BWD, false>;
     shared = ring_bytes(V, IT, NORM && BWD, sizeof(T)) + tables;
   }
   if (shared < sums) shared = sums;
-  static SharedMemory allowed;
-  if (!allowed.up_to((const void *)kernel, shared)) return ANODE_E_LAUNCH;
+  static SharedMemory allowed[2];
+  if (!allowed[a.interleaved].up_to((const void *)kernel, shared)) return ANODE_E_LAUNCH;
   return launch(kernel, dim3(blocks), kThreads, shared, stream, a);
 }
 
@@ -779,8 +801,10 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
     if (d.parts < 1 || d.tokens > 1) d.parts = 1;
     d.span = (passes[k] + d.parts - 1) / d.parts * groups;
     d.parts = (d.heads + d.span - 1) / d.span;
+    d.passes = d.span / groups;
+    d.last = (d.heads - (d.parts - 1) * d.span + groups - 1) / groups;
     d.units = units[k] * d.parts;
-    cost[k] = (double)units[k] * (passes[k] + 1.5 * d.parts);        // (the cosines and sines cost a unit about one and a half passes)
+    cost[k] = (double)units[k] * (passes[k] + 2.5 * d.parts);        // (the cosines and sines cost a unit about two and a half passes)
   }
   for (int k = 0; k < 1 + two; ++k) {
     RotarySide &d = a.side[k];

@@ -189,14 +189,14 @@ __device__ __forceinline__ float group_sum(float v, uint32_t lanes, uint32_t fir
   return sum;
 }
 
-// Registers: two or three blocks of a multiprocessor
-__host__ __device__ constexpr int resident(int floats, bool norm) { return floats > 16 ? 1 : norm ? 2 : 3; }
+// Blocks of a multiprocessor: with three, which the forms without a norm would have registers for, the same heads took 62.3 us in the place of 58.7
+__host__ __device__ constexpr int resident(int floats) { return floats > 16 ? 1 : 2; }
 // Heads of a lane's ring, and its bytes
 __host__ __device__ constexpr int ring_depth(int it) { return it == 1 ? 4 : 2; }
 __host__ __device__ constexpr size_t ring_bytes(int v, int it, bool both, size_t e) { return (size_t)ring_depth(it) * kThreads * it * 2 * v * e * (both ? 2 : 1); }
 
 template <typename T, int V, int IT, bool NORM, bool BWD, bool interleaved>
-__global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_heads_kernel(const RotaryArgs a)
+__global__ void __launch_bounds__(kThreads, resident(2 * V * IT)) rotary_heads_kernel(const RotaryArgs a)
 {
   constexpr bool BOTH = NORM && BWD;        // two arrays are read
   constexpr bool KEEP = V * IT <= (BOTH ? 4 : 8);       // a lane's cosines and sines stay in its registers from head to head
@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT, NORM)) rotary_h
     turns[k] = p < a.turned;
     has[k] = p < a.items;
     // (interleaved pairs are whole in either vector: these two lie apart, too, so that lanes side by side move 16 bytes side by side)
-    e0[k] = turns[k] ? p * V : a.rot + (p - a.turned) * 2 * V;
-    e1[k] = turns[k] ? half + p * V : e0[k] + V;
+    e0[k] = turns[k] ? p * V : a.rot + (p - a.turned) * V;
+    e1[k] = turns[k] ? half + p * V : e0[k] + (a.items - a.turned) * V;
     second[k] = has[k] && e1[k] < a.dim;
   }
   pdl_wait();
@@ -781,7 +781,7 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
     a.slot = (uint32_t)((a.dim * e + 15) / 16 * 16 + 16);      // (16 more, so that groups side by side read other banks)
   }
   // blocks that the device holds; both arrays' warps work side by side, as many on either as its share of the heads asks for
-  const uint32_t room = sm_count() * (uint32_t)(v == 1 ? each > 8 ? 1 : 2 : resident((int)(2 * v * each), a.norm));
+  const uint32_t room = sm_count() * (uint32_t)(v == 1 ? each > 8 ? 1 : 2 : resident((int)(2 * v * each)));
   uint32_t blocks = 0, most = 1, units[2] = {0, 0}, passes[2];
   double cost[2] = {0.0, 0.0};
   for (int k = 0; k < 1 + two; ++k) {

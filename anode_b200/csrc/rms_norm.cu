@@ -107,7 +107,7 @@ __device__ __forceinline__ float max_nan(float a, float b)
 // slot: slots are then those of the addresses, and the elements before the first whole one and after the last have a lane each.
 // QUANT: 0 none, else an output in 8 bits with a scale for each row (1) or for each 128 columns (2).
 // What bounds it: memory; so a thread's loads are all in flight at once.
-template <typename T, int CH, bool SHIFT, int QUANT>
+template <typename T, int CH, bool SHIFT, int QUANT, bool RES>
 __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const NormArgs a, const Held h)
 {
   constexpr int V = Vec<T>::V, H = V / 2;
@@ -117,8 +117,8 @@ __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const N
   const uint64_t row = (uint64_t)blockIdx.x * per_block + mine;
   const bool live = row < a.rows;               // (all threads take part in the teams' sums)
   const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
-  const T *res = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
-  T *total = a.total ? static_cast<T *>(a.total) + row * a.total_stride : nullptr;
+  const T *res = RES ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
+  T *total = RES && a.total ? static_cast<T *>(a.total) + row * a.total_stride : nullptr;
   // the row's head: columns before its first whole slot; then `slots` of them, and a tail
   const uint32_t head = SHIFT ? min(a.cols, (uint32_t)(-(int)((uintptr_t)x / sizeof(T)) & (V - 1))) : 0, slots = (a.cols - head) / V;
   const uint32_t start = head + at * V, hop = h.team * V;      // this thread's slots: columns start + k*hop
@@ -132,20 +132,20 @@ __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const N
   const bool aligned_gamma = ((uintptr_t)a.gamma.p & 15) == 0;
   pdl_wait();
   pdl_trigger();        // (the next kernel's blocks wait as these did: 0.1 to 0.3 us of a call of few rows)
-  Vec<T> t[CH], r[CH];
+  Vec<T> t[CH], r[RES ? CH : 1];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     t[k].bits = make_uint4(0, 0, 0, 0);
     if (k < mine_slots) t[k] = Vec<T>::load(x + start + k * hop);
   }
-  if (res) {
+  if constexpr (RES) {
 #pragma unroll
     for (int k = 0; k < CH; ++k) if (k < mine_slots) r[k] = Vec<T>::load(res + start + k * hop);
   }
   float te = 0.0f, ge = 1.0f;
   if (on_edge) {
     te = to_float(x[edge]);
-    if (res) te = to_float(from_float<T>(te + to_float(res[edge])));
+    if (RES) te = to_float(from_float<T>(te + to_float(res[edge])));
     ge = a.gamma.at(edge);
   }
   // the weights of few slots are loaded ahead of the sum, those of many when they are needed: they would take the registers
@@ -166,10 +166,10 @@ __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const N
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     float2 f[H];
-    if (res && k < mine_slots) {
+    if (RES && k < mine_slots) {
       float2 e[H];
       t[k].floats(reinterpret_cast<float *>(f));
-      r[k].floats(reinterpret_cast<float *>(e));
+      r[RES ? k : 0].floats(reinterpret_cast<float *>(e));
 #pragma unroll
       for (int i = 0; i < H; ++i) f[i] = add2(f[i], e[i]);
       t[k] = Vec<T>::of(reinterpret_cast<const float *>(f));
@@ -589,12 +589,12 @@ bool held_plan(const NormArgs &a, int type, int gamma_type, bool quant, Held &h,
   const uint32_t slots = a.cols / v;
   if (slots > 8 * most_threads(8)) return false;
   h.groups = quant && a.block ? (a.cols + 127) / 128 : 0;
-  if (slots <= 128) {
+  if (slots <= (shift ? 128u : 64u)) {
     h.team = shift ? 16 : 4;              // (a lane for each element before and after whole slots)
     while (h.team < 32 && h.team < slots) h.team *= 2;
     h.chunks = slots <= h.team ? 1 : slots <= 64 ? 2 : 4;
   } else {
-    h.chunks = a.rows <= 2 * 148 && slots <= 2048 ? (slots <= 1024 ? 1 : 2) : slots <= 4 * most_threads(4) ? 4 : 8;
+    h.chunks = a.rows <= 2 * 148 && slots <= 2048 ? (slots <= 1024 ? 1 : 2) : slots <= 256 ? 2 : slots <= 4 * most_threads(4) ? 4 : 8;
     h.team = (slots + h.chunks * 32 - 1) / (h.chunks * 32) * 32;
   }
   return true;
@@ -605,10 +605,12 @@ template <typename T, int CH> int launch_held(const NormArgs &a, const Held &h, 
   const uint32_t threads = h.team > 32 ? h.team : 128, per_block = threads / h.team;
   const dim3 grid((uint32_t)((a.rows + per_block - 1) / per_block));
   const size_t shared = shift ? (size_t)per_block * h.groups * 4 : 0;
-  auto go = [&](auto plain, auto shifted) { return launch(shift ? shifted : plain, grid, threads, shared, stream, a, h); };
-  if (!quant) return go(rms_norm_held_kernel<T, CH, false, 0>, rms_norm_held_kernel<T, CH, true, 0>);
-  return h.groups ? go(rms_norm_held_kernel<T, CH, false, 2>, rms_norm_held_kernel<T, CH, true, 2>)
-                  : go(rms_norm_held_kernel<T, CH, false, 1>, rms_norm_held_kernel<T, CH, true, 1>);
+  auto go = [&](auto form) {
+    constexpr int Q = decltype(form)::value;
+    return launch(a.residual ? (shift ? rms_norm_held_kernel<T, CH, true, Q, true> : rms_norm_held_kernel<T, CH, false, Q, true>)
+                             : (shift ? rms_norm_held_kernel<T, CH, true, Q, false> : rms_norm_held_kernel<T, CH, false, Q, false>), grid, threads, shared, stream, a, h);
+  };
+  return !quant ? go(std::integral_constant<int, 0>()) : h.groups ? go(std::integral_constant<int, 2>()) : go(std::integral_constant<int, 1>());
 }
 
 // How the rows of an adjoint are held on chip: chunks*threads of the kernel; false where they are not

@@ -18,9 +18,9 @@
 namespace anode_b200 {
 namespace rows {
 
-constexpr uint32_t kThreads = 256, kMostDim = 1024;
+constexpr uint32_t kThreads = 128, kMostDim = 1024;
 constexpr uint32_t kWarps = kThreads / 32;
-constexpr uint32_t kMostParts = 148 * 4;      // blocks that have sums of the weights' gradients
+constexpr uint32_t kMostParts = 148 * 8;      // blocks that have sums of the weights' gradients
 
 struct HeadArray {
   void *p;
@@ -189,8 +189,9 @@ __device__ __forceinline__ float group_sum(float v, uint32_t lanes, uint32_t fir
   return sum;
 }
 
-// Blocks of a multiprocessor: with three, which the forms without a norm would have registers for, the same heads took 62.3 us in the place of 58.7
-__host__ __device__ constexpr int resident(int floats) { return floats > 16 ? 1 : 2; }
+// Blocks of a multiprocessor: with more, which the forms without a norm would have registers for, [16384,40,128] took 62.3 us in the place of 58.7,
+// with a norm 62.7 in the place of 56.5
+__host__ __device__ constexpr int resident(int floats) { return floats > 16 ? 2 : 4; }
 // Heads of a lane's ring, and its bytes
 __host__ __device__ constexpr int ring_depth(int it) { return it == 1 ? 4 : 2; }
 __host__ __device__ constexpr size_t ring_bytes(int v, int it, bool both, size_t e) { return (size_t)ring_depth(it) * kThreads * it * 2 * v * e * (both ? 2 : 1); }
@@ -454,13 +455,15 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT)) rotary_heads_k
   }
 }
 
+constexpr int kPairsDepth = 4;
+
 // Heads whose pairs lie anywhere.  They are copied as they lie, `copy` bytes at a time, into places of `slot` bytes; a lane has IT pairs, lanes
-// side by side, or as many elements that pass.  DEPTH places to a group: the next head is on its way while one is worked on.
+// side by side, or as many elements that pass.  DEPTH places to a group: the next heads are on their way while one is worked on.
 template <typename T, int IT, bool NORM, bool BWD>
-__global__ void __launch_bounds__(kThreads, IT > 8 ? 1 : 2) rotary_pairs_kernel(const RotaryArgs a)
+__global__ void __launch_bounds__(kThreads, IT > 8 ? 2 : 4) rotary_pairs_kernel(const RotaryArgs a)
 {
   constexpr bool BOTH = NORM && BWD;
-  constexpr int DEPTH = 2, ARRAYS = BOTH ? 2 : 1;
+  constexpr int DEPTH = kPairsDepth, ARRAYS = BOTH ? 2 : 1;
   // each pair's turns per position; of each warp, the heads' places [depth][array][group] and the cosines and sines [tokens][rot/2]; then the
   // sums of the weights' gradients
   extern __shared__ float4 shared[];
@@ -471,7 +474,8 @@ __global__ void __launch_bounds__(kThreads, IT > 8 ? 1 : 2) rotary_pairs_kernel(
   double *rates = reinterpret_cast<double *>(shared);
   char *base = reinterpret_cast<char *>(shared + (half + 1) / 2), *places = base + (size_t)warp * DEPTH * ARRAYS * groups * a.slot;
   float2 *table = reinterpret_cast<float2 *>(base + (size_t)kWarps * DEPTH * ARRAYS * groups * a.slot) + (size_t)warp * d.tokens * half;
-  auto place = [&](uint32_t turn, int array) { return places + ((turn * ARRAYS + array) * groups + group) * a.slot; };
+  // (lanes beyond the last group read, and drop, what it has)
+  auto place = [&](uint32_t turn, int array) { return places + ((turn * ARRAYS + array) * groups + min(group, groups - 1)) * a.slot; };
   uint32_t e0[IT], e1[IT];
   bool has[IT], second[IT], turns[IT];
 #pragma unroll
@@ -512,22 +516,25 @@ __global__ void __launch_bounds__(kThreads, IT > 8 ? 1 : 2) rotary_pairs_kernel(
       }
     }
     copies_commit();
-    turn_in ^= 1;
+    turn_in = (turn_in + 1) & (DEPTH - 1);
   };
   Place<T> at, ahead;
   at.unit = ahead.unit = block * kWarps + warp;
   walk.enter(at, d.out, nullptr);
   walk.enter(ahead, d.in, from);
   long long position = position_of(a, walk.token(at.unit), d.tokens, wlane);
-  load(ahead);
-  walk.advance(ahead, d.in, hop, from, hop_x);
+#pragma unroll
+  for (int i = 0; i < DEPTH - 1; ++i) {
+    load(ahead);
+    walk.advance(ahead, d.in, hop, from, hop_x);
+  }
   __syncthreads();
   while (at.unit < d.units) {
     __syncwarp();
     make_table(a, rates, d.tokens, position, [&](uint32_t t, uint32_t j, float2 cs) { table[t * half + j] = cs; });
     position = position_of(a, walk.token(at.unit + walk.step), d.tokens, wlane);
     __syncwarp();
-    const float2 *cs = table + walk.mine * half;
+    const float2 *cs = table + min(walk.mine, d.tokens - 1) * half;
     for (const uint32_t unit = at.unit; at.unit == unit;) {
       const bool live = at.head < at.end;
       load(ahead);
@@ -539,9 +546,9 @@ __global__ void __launch_bounds__(kThreads, IT > 8 ? 1 : 2) rotary_pairs_kernel(
       float2 f[IT];
       float sq = 0.0f, dot = 0.0f;
 #pragma unroll
-      for (int k = 0; k < IT; ++k) f[k] = make_float2(live && has[k] ? to_float(in[e0[k]]) : 0.0f, live && second[k] ? to_float(in[e1[k]]) : 0.0f);
+      for (int k = 0; k < IT; ++k) f[k] = make_float2(has[k] ? to_float(in[e0[k]]) : 0.0f, second[k] ? to_float(in[e1[k]]) : 0.0f);
       auto turned = [&](int k) {
-        if (!live || !turns[k]) return;
+        if (!turns[k]) return;
         const float2 w = cs[lane + k * a.lanes], v = f[k];
         f[k] = make_float2(v.x * w.x - v.y * w.y, v.x * w.y + v.y * w.x);
       };
@@ -558,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, IT > 8 ? 1 : 2) rotary_pairs_kernel(
         float2 x[IT];
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
-          x[k] = make_float2(live && has[k] ? to_float(xin[e0[k]]) : 0.0f, live && second[k] ? to_float(xin[e1[k]]) : 0.0f);
+          x[k] = make_float2(has[k] ? to_float(xin[e0[k]]) : 0.0f, second[k] ? to_float(xin[e1[k]]) : 0.0f);
           sq = fmaf(x[k].x, x[k].x, fmaf(x[k].y, x[k].y, sq));
           dot = fmaf(f[k].x * g[k].x, x[k].x, fmaf(f[k].y * g[k].y, x[k].y, dot));
         }
@@ -592,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, IT > 8 ? 1 : 2) rotary_pairs_kernel(
           else *reinterpret_cast<uint16_t *>(out + i) = *reinterpret_cast<const uint16_t *>(p + i);
         }
       }
-      turn_out ^= 1;
+      turn_out = (turn_out + 1) & (DEPTH - 1);
       walk.advance(at, d.out, hop_out, nullptr, 0);
       // (the place is filled anew by copies of the lanes that emptied it, and the array beside it after every lane has passed the barrier above)
     }
@@ -678,7 +685,7 @@ int launch_rotary(const RotaryArgs &a, uint32_t blocks, size_t tables, size_t su
   size_t shared;
   if constexpr (V == 1) {
     kernel = rotary_pairs_kernel<T, IT, NORM, BWD>;
-    shared = (size_t)kWarps * 2 * (NORM && BWD ? 2 : 1) * (32 / a.lanes) * a.slot + tables;
+    shared = (size_t)kWarps * kPairsDepth * (NORM && BWD ? 2 : 1) * (32 / a.lanes) * a.slot + tables;
   } else {
     kernel = a.interleaved ? rotary_heads_kernel<T, V, IT, NORM, BWD, true> : rotary_heads_kernel<T, V, IT, NORM, BWD, false>;
     shared = ring_bytes(V, IT, NORM && BWD, sizeof(T)) + tables;
@@ -781,7 +788,7 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
     a.slot = (uint32_t)((a.dim * e + 15) / 16 * 16 + 16);      // (16 more, so that groups side by side read other banks)
   }
   // blocks that the device holds; both arrays' warps work side by side, as many on either as its share of the heads asks for
-  const uint32_t room = sm_count() * (uint32_t)(v == 1 ? each > 8 ? 1 : 2 : resident((int)(2 * v * each)));
+  const uint32_t room = sm_count() * (uint32_t)(v == 1 ? each > 8 ? 2 : 4 : resident((int)(2 * v * each)));
   uint32_t blocks = 0, most = 1, units[2] = {0, 0}, passes[2];
   double cost[2] = {0.0, 0.0};
   for (int k = 0; k < 1 + two; ++k) {

@@ -425,11 +425,23 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT)) rotary_heads_k
   }
   if constexpr (BOTH) {
     if (!d.want) return;
-    // the warp's groups add their sums in turn, then the warps'
+    // the groups' sums join within the warp (those of other than a power of two lanes add theirs in turn), then the warps'
     float *sums = reinterpret_cast<float *>(shared);
     copies_wait<0>();
+    pdl_trigger();
+    const bool even = (a.lanes & (a.lanes - 1)) == 0;
+    if (even) {
+#pragma unroll
+      for (int k = 0; k < IT; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          for (uint32_t o = a.lanes; o < 32; o *= 2) {
+            acc[k][i].x += __shfl_xor_sync(0xffffffffu, acc[k][i].x, o);
+            acc[k][i].y += __shfl_xor_sync(0xffffffffu, acc[k][i].y, o);
+          }
+    }
     __syncthreads();
-    for (uint32_t n = 0; n < groups; ++n) {
+    for (uint32_t n = 0; n < (even ? 1 : groups); ++n) {
       if (group == n) {
 #pragma unroll
         for (int k = 0; k < IT; ++k)
@@ -638,17 +650,23 @@ __global__ void __launch_bounds__(1024) rotary_join_kernel(uint32_t dim, uint32_
   void *out = k ? dk : dq;
   pdl_wait();
   if (!out) return;
+  // (half of the blocks that there may be are asked for at once)
+  constexpr uint32_t kEach = kMostParts / 64;
+  const uint32_t end = k ? blocks : q_blocks;
   float sum = 0.0f;
-  if (i < dim) {
-#pragma unroll 4
-    for (uint32_t b = (k ? q_blocks : 0) + warp; b < (k ? blocks : q_blocks); b += 32) sum += partial[(uint64_t)b * dim + i];
+  for (uint32_t first = (k ? q_blocks : 0) + warp; first < end; first += 32 * kEach) {
+    float v[kEach];
+#pragma unroll
+    for (uint32_t n = 0; n < kEach; ++n) v[n] = i < dim && first + 32 * n < end ? partial[(uint64_t)(first + 32 * n) * dim + i] : 0.0f;
+#pragma unroll
+    for (uint32_t n = 0; n < kEach; ++n) sum += v[n];
   }
   sums[warp][lane] = sum;
   __syncthreads();
-  if (warp || i >= dim) return;
-#pragma unroll
-  for (uint32_t w = 1; w < 32; ++w) sum += sums[w][lane];
-  put_weight(out, type, i, sum);
+  // a warp per element: a lane's term of each
+  sum = warp_sum_all(sums[lane][warp]);
+  const uint32_t mine = (blockIdx.x - k * wide) * 32 + warp;
+  if (lane == 0 && mine < dim) put_weight(out, type, mine, sum);
 }
 
 // An array of heads: pointer and alignment; an output's heads do not overlap
@@ -789,7 +807,8 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
   }
   // blocks that the device holds; both arrays' warps work side by side, as many on either as its share of the heads asks for
   const uint32_t room = sm_count() * (uint32_t)(v == 1 ? each > 8 ? 2 : 4 : resident((int)(2 * v * each)));
-  uint32_t blocks = 0, most = 1, units[2] = {0, 0}, passes[2];
+  uint64_t all_passes = 0;
+  uint32_t blocks = 0, most = 1, units[2], passes[2];
   double cost[2] = {0.0, 0.0};
   for (int k = 0; k < 1 + two; ++k) {
     RotarySide &d = a.side[k];
@@ -799,14 +818,13 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
     units[k] = (a.total - 1) / d.tokens + 1;
     passes[k] = (d.heads + groups - 1) / groups;
     if (d.tokens > most) most = d.tokens;
+    all_passes += (uint64_t)units[k] * passes[k];
   }
+  const uint64_t each_passes = (all_passes - 1) / (room * kWarps) + 1;
   for (int k = 0; k < 1 + two; ++k) {
     RotarySide &d = a.side[k];
     // or, where that leaves warps of the device idle, a span of them
-    d.parts = room * kWarps / ((uint64_t)units[0] + units[1]);
-    if (d.parts > passes[k]) d.parts = passes[k];
-    if (d.parts < 1 || d.tokens > 1) d.parts = 1;
-    d.span = (passes[k] + d.parts - 1) / d.parts * groups;
+    d.span = (d.tokens > 1 || each_passes > passes[k] ? passes[k] : (uint32_t)each_passes) * groups;
     d.parts = (d.heads + d.span - 1) / d.span;
     d.passes = d.span / groups;
     d.last = (d.heads - (d.parts - 1) * d.span + groups - 1) / groups;

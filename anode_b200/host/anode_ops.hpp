@@ -11,6 +11,7 @@
 //   x.batch_normalize_2d(axes, online, avg_rate, eps) (src/ops.rs:999-1014)        ->  anode::batch_normalize_2d
 //   the adjoint wiring of the three ops (src/ops_gpu.rs:3785-3796, 3994-4005, 4340-4357) -> anode::batch_normalize_adjoint
 //   BatchNormalize2dFusedOp / BatchNormalize2dBwdFusedOp (declared, never built: src/ops.rs:105-106) -> same names here
+//   normalization over rows and rotary positions (no counterpart)                  ->  anode_rows.hpp
 // Error behaviour: the reference's entry points return void and `unimplemented!()` on anything
 // that is not packed or not over the leading axes; here that is an anode::Error, as is a negative
 // return code of the new entry points.
@@ -264,3 +265,4 @@ struct PositiveClipBwdOp {
 }  // namespace anode
 
 #include "anode_layers.hpp"
+#include "anode_rows.hpp"

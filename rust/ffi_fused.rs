@@ -19,6 +19,17 @@ use gpudevicemem::ffi::routines_gpu::KernelConfig;
 #[repr(C)]
 pub struct AnodeSyncComm { _private: [u8; 0] }
 
+/// Heads of a [batch, seq, heads, dim] array; strides in elements, dim packed.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct AnodeHeads {
+  pub data: *mut c_void,
+  pub batch_stride: u64,
+  pub seq_stride: u64,
+  pub head_stride: u64,
+  pub heads: u32,
+}
+
 pub const ANODE_OK: c_int = 0;
 pub const ANODE_E_NULL: c_int = -1;
 pub const ANODE_E_DIMS: c_int = -2;
@@ -27,6 +38,11 @@ pub const ANODE_E_LAUNCH: c_int = -4;
 pub const ANODE_E_COMM: c_int = -5;
 pub const ANODE_E_ALIGN: c_int = -6;
 pub const ANODE_E_TOO_LARGE: c_int = -7;
+pub const ANODE_E_TYPE: c_int = -8;
+pub const ANODE_E_STRIDE: c_int = -9;
+pub const ANODE_TYPE_F32: c_int = 0;
+pub const ANODE_TYPE_F16: c_int = 1;
+pub const ANODE_TYPE_BF16: c_int = 2;
 pub const ANODE_ST_WAIT_STATS: u32 = 1;
 pub const ANODE_ST_WAIT_PEER: u32 = 2;
 pub const ANODE_ST_ABORTED: u32 = 4;
@@ -435,6 +451,136 @@ extern "C" {
     dgamma: *mut f32,
     dbeta: *mut f32,
     comm: *mut AnodeSyncComm,
+    workspace: *mut c_void,
+    workspace_bytes: usize,
+    cfg: *const KernelConfig,
+    stream: *mut CUstream_st,
+  ) -> c_int;
+  // normalization over rows, and rotary positions
+  pub fn anode_gpu_rms_norm_add_fwd(
+    type_: c_int,
+    rows: u64,
+    cols: u32,
+    epsilon: f32,
+    x: *const c_void,
+    x_stride: u64,
+    residual: *const c_void,
+    residual_stride: u64,
+    gamma: *const c_void,
+    gamma_type: c_int,
+    y: *mut c_void,
+    y_stride: u64,
+    total: *mut c_void,
+    total_stride: u64,
+    inv_rms: *mut f32,
+    cfg: *const KernelConfig,
+    stream: *mut CUstream_st,
+  ) -> c_int;
+  pub fn anode_gpu_rms_norm_add_bwd_workspace_bytes(
+    rows: u64,
+    cols: u32,
+  ) -> usize;
+  pub fn anode_gpu_rms_norm_add_bwd(
+    type_: c_int,
+    rows: u64,
+    cols: u32,
+    dy: *const c_void,
+    dy_stride: u64,
+    total: *const c_void,
+    total_stride: u64,
+    inv_rms: *const f32,
+    gamma: *const c_void,
+    gamma_type: c_int,
+    dtotal: *const c_void,
+    dtotal_stride: u64,
+    dx: *mut c_void,
+    dx_stride: u64,
+    dgamma: *mut c_void,
+    workspace: *mut c_void,
+    workspace_bytes: usize,
+    cfg: *const KernelConfig,
+    stream: *mut CUstream_st,
+  ) -> c_int;
+  pub fn anode_gpu_rms_norm_add_quant_fwd(
+    type_: c_int,
+    rows: u64,
+    cols: u32,
+    epsilon: f32,
+    block: u32,
+    x: *const c_void,
+    x_stride: u64,
+    residual: *const c_void,
+    residual_stride: u64,
+    gamma: *const c_void,
+    gamma_type: c_int,
+    q: *mut u8,
+    q_stride: u64,
+    scale: *mut f32,
+    scale_row_stride: u64,
+    scale_group_stride: u64,
+    total: *mut c_void,
+    total_stride: u64,
+    cfg: *const KernelConfig,
+    stream: *mut CUstream_st,
+  ) -> c_int;
+  pub fn anode_gpu_rotary_positions_fwd(
+    type_: c_int,
+    batch: u32,
+    seq: u32,
+    dim: u32,
+    rot: u32,
+    interleaved: c_int,
+    amplitude: f32,
+    freq: *const f64,
+    positions: *const c_void,
+    position_bytes: c_int,
+    pos_batch_stride: u64,
+    pos_seq_stride: u64,
+    norm: c_int,
+    epsilon: f32,
+    gamma_q: *const c_void,
+    gamma_k: *const c_void,
+    gamma_type: c_int,
+    q: *const AnodeHeads,
+    k: *const AnodeHeads,
+    q_out: *const AnodeHeads,
+    k_out: *const AnodeHeads,
+    cfg: *const KernelConfig,
+    stream: *mut CUstream_st,
+  ) -> c_int;
+  pub fn anode_gpu_rotary_positions_bwd_workspace_bytes(
+    batch: u32,
+    seq: u32,
+    q_heads: u32,
+    k_heads: u32,
+    dim: u32,
+  ) -> usize;
+  pub fn anode_gpu_rotary_positions_bwd(
+    type_: c_int,
+    batch: u32,
+    seq: u32,
+    dim: u32,
+    rot: u32,
+    interleaved: c_int,
+    amplitude: f32,
+    freq: *const f64,
+    positions: *const c_void,
+    position_bytes: c_int,
+    pos_batch_stride: u64,
+    pos_seq_stride: u64,
+    norm: c_int,
+    epsilon: f32,
+    gamma_q: *const c_void,
+    gamma_k: *const c_void,
+    gamma_type: c_int,
+    dq_out: *const AnodeHeads,
+    dk_out: *const AnodeHeads,
+    q: *const AnodeHeads,
+    k: *const AnodeHeads,
+    dq: *const AnodeHeads,
+    dk: *const AnodeHeads,
+    dgamma_q: *mut c_void,
+    dgamma_k: *mut c_void,
     workspace: *mut c_void,
     workspace_bytes: usize,
     cfg: *const KernelConfig,

@@ -283,15 +283,21 @@ __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const N
     }
     if (on_edge) atomicMax(top + edge / 128, bits_of(ye));
     sync();
-    if (live) for (uint32_t i = at; i < h.groups; i += h.team) a.scale[row * a.scale_row + i * a.scale_group] = scale_of(top[i]);
+    // a group's scale is made once, and its inverse takes the peak's place
+    for (uint32_t i = at; i < h.groups; i += h.team) {
+      const float scale = scale_of(top[i]);
+      if (live) a.scale[row * a.scale_row + i * a.scale_group] = scale;
+      top[i] = __float_as_uint(inverse(scale));
+    }
+    sync();
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       if (k >= mine_slots) continue;
       const uint32_t c = start + k * hop, border = 128 - c % 128;
-      const float one = inverse(scale_of(top[c / 128]));
-      put(k, y[k], one, border < V ? inverse(scale_of(top[c / 128 + 1])) : one, border);
+      const float one = __uint_as_float(top[c / 128]);
+      put(k, y[k], one, border < V ? __uint_as_float(top[c / 128 + 1]) : one, border);
     }
-    if (on_edge) q[edge] = (uint8_t)eight(ye * inverse(scale_of(top[edge / 128])), 0.0f);
+    if (on_edge) q[edge] = (uint8_t)eight(ye * __uint_as_float(top[edge / 128]), 0.0f);
   }
 }
 
@@ -313,7 +319,7 @@ struct GradArgs {
 // How the adjoint's rows are held: `teams` teams of `team` threads to a block, each with a row at a time, `depth` rows on their way or at work;
 // a team's rows lie `step` apart
 struct HeldGrad {
-  uint32_t team, teams, depth;
+  uint32_t team, teams, depth, threads;
   uint64_t step;
 };
 
@@ -334,6 +340,7 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
   const uint64_t row0 = (uint64_t)blockIdx.x * h.teams + mine;
   const bool works = mine < h.teams && row0 < h.step && row0 < a.rows;
   const uint32_t lanes = h.team < 32 ? ((1u << h.team) - 1) << (lane & ~(h.team - 1)) : 0xffffffffu;      // of this warp in the team
+  const uint32_t nt = blockDim.x;
   uint4 *ring = reinterpret_cast<uint4 *>(shared) + threadIdx.x;
   const T *dy = static_cast<const T *>(a.dy) + row0 * a.dy_stride, *t = static_cast<const T *>(a.total) + row0 * a.total_stride;
   const T *dt = static_cast<const T *>(a.dtotal) + row0 * a.dtotal_stride;
@@ -378,13 +385,13 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
   dy += start; t += start; dt += start;
   auto copy = [&] {                     // the next row to be copied
     if (ahead) {
-      uint4 *to = ring + in * (CH * 3 * NT);
+      uint4 *to = ring + in * (CH * 3) * nt;
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
         if (!has(k)) continue;
-        copy_async<16>(to + (3 * k) * NT, dy + k * hop);
-        copy_async<16>(to + (3 * k + 1) * NT, t + k * hop);
-        if (a.dtotal) copy_async<16>(to + (3 * k + 2) * NT, dt + k * hop);
+        copy_async<16>(to + (3 * k) * nt, dy + k * hop);
+        copy_async<16>(to + (3 * k + 1) * nt, t + k * hop);
+        if (a.dtotal) copy_async<16>(to + (3 * k + 2) * nt, dt + k * hop);
       }
       --ahead;
       dy += dy_step; t += t_step; dt += dt_step;
@@ -400,7 +407,7 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
     copy();
     if (left > 1) side(next);
     if (h.depth == 4) copies_wait<3>(); else if (h.depth == 3) copies_wait<2>(); else if (h.depth == 2) copies_wait<1>(); else copies_wait<0>();
-    const uint4 *from = ring + out * (CH * 3 * NT);
+    const uint4 *from = ring + out * (CH * 3) * nt;
     out = out + 1 == h.depth ? 0 : out + 1;
     float2 dot2 = make_float2(SHIFT ? now.dy * g_edge * now.t : 0.0f, 0.0f);
     // a single slot stays in registers between the two passes over the row, more are read again
@@ -409,8 +416,8 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       if (!has(k)) continue;
-      Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(u));
-      Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(v));
+      Vec<T>{from[(3 * k) * nt]}.floats(reinterpret_cast<float *>(u));
+      Vec<T>{from[(3 * k + 1) * nt]}.floats(reinterpret_cast<float *>(v));
 #pragma unroll
       for (int i = 0; i < H; ++i) dot2 = fma2(mul2(u[i], g[k][i]), v[i], dot2);
     }
@@ -429,8 +436,8 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
     for (int k = 0; k < CH; ++k) {
       if (!has(k)) continue;
       if (!ONE) {
-        Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(u));
-        Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(v));
+        Vec<T>{from[(3 * k) * nt]}.floats(reinterpret_cast<float *>(u));
+        Vec<T>{from[(3 * k + 1) * nt]}.floats(reinterpret_cast<float *>(v));
       }
       float2 e[H];
 #pragma unroll
@@ -440,7 +447,7 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
         e[i] = fma2(ur, g[k][i], mul2(v[i], c));
       }
       if (a.dtotal) {
-        Vec<T>{from[(3 * k + 2) * NT]}.floats(reinterpret_cast<float *>(v));
+        Vec<T>{from[(3 * k + 2) * nt]}.floats(reinterpret_cast<float *>(v));
 #pragma unroll
         for (int i = 0; i < H; ++i) e[i] = add2(e[i], v[i]);
       }
@@ -477,7 +484,8 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
     // the teams of a warp join first; a block of one team has its sums in registers
     if (h.team < 32) parts = (h.teams * h.team + 31) / 32;
     const uint32_t part = h.team < 32 ? warp : mine;
-    float *to = parts == 1 ? a.partial + (uint64_t)blockIdx.x * a.cols : sums + (size_t)part * a.cols;
+    const bool direct = parts == 1 && gridDim.x > 1;
+    float *to = direct ? a.partial + (uint64_t)blockIdx.x * a.cols : sums + (size_t)part * a.cols;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       float *v = reinterpret_cast<float *>(acc[k]);
@@ -489,13 +497,14 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
 #pragma unroll
       for (int i = 0; i < V; i += 4) *reinterpret_cast<float4 *>(to + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     }
-    if (parts == 1) return;
+    if (direct) return;
   }
   __syncthreads();
-  for (uint32_t c = threadIdx.x; c < a.cols; c += NT) {
+  for (uint32_t c = threadIdx.x; c < a.cols; c += nt) {
     float sum = 0.0f;
     for (uint32_t t = 0; t < parts; ++t) sum += sums[(size_t)t * apart + (SHIFT ? c + c / V : c)];
-    a.partial[(uint64_t)blockIdx.x * a.cols + c] = sum;
+    if (gridDim.x == 1) put_weight(a.dgamma, a.gamma.type, c, sum);        // (nothing to join with)
+    else a.partial[(uint64_t)blockIdx.x * a.cols + c] = sum;
   }
 }
 
@@ -512,25 +521,40 @@ template <typename T> __global__ void __launch_bounds__(kThreads) rms_norm_dgamm
   a.partial[(uint64_t)blockIdx.y * a.cols + c] = sum;
 }
 
-// The blocks' sums: a lane has a column, a warp every 32nd block, all of whose sums are asked for at once
-__global__ void __launch_bounds__(1024) join_columns_kernel(uint32_t cols, uint32_t parts, const float *partial, void *out, int type)
+// The blocks' sums, of few blocks: a thread has a column
+constexpr uint32_t kFewParts = 16;
+__global__ void __launch_bounds__(kThreads) join_few_kernel(uint32_t cols, uint32_t parts, const float *partial, void *out, int type)
 {
-  constexpr uint32_t kEach = (kMostParts + 31) / 32;
-  __shared__ float sums[32][33];
+  const uint64_t c = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+  pdl_wait();
+  if (c >= cols) return;
+  float v[kFewParts], sum = 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < kFewParts; ++i) v[i] = i < parts ? partial[(uint64_t)i * cols + c] : 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < kFewParts; ++i) sum += v[i];
+  put_weight(out, type, (uint32_t)c, sum);
+}
+
+// The blocks' sums: a lane has a column, a warp every eighth block, all of whose sums are asked for at once
+__global__ void __launch_bounds__(kThreads) join_columns_kernel(uint32_t cols, uint32_t parts, const float *partial, void *out, int type)
+{
+  constexpr uint32_t kWarps = kThreads / 32, kEach = (kMostParts + kWarps - 1) / kWarps;
+  __shared__ float sums[kWarps][33];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;
   pdl_wait();
   float v[kEach], sum = 0.0f;
 #pragma unroll
-  for (uint32_t i = 0; i < kEach; ++i) v[i] = c < cols && warp + 32 * i < parts ? partial[(uint64_t)(warp + 32 * i) * cols + c] : 0.0f;
+  for (uint32_t i = 0; i < kEach; ++i) v[i] = c < cols && warp + kWarps * i < parts ? partial[(uint64_t)(warp + kWarps * i) * cols + c] : 0.0f;
 #pragma unroll
   for (uint32_t i = 0; i < kEach; ++i) sum += v[i];
   sums[warp][lane] = sum;
   __syncthreads();
-  // a warp per column: a lane's term of each
-  sum = warp_sum_all(sums[lane][warp]);
-  const uint64_t mine = (uint64_t)blockIdx.x * 32 + warp;
-  if (lane == 0 && mine < cols) put_weight(out, type, (uint32_t)mine, sum);
+  if (warp || c >= cols) return;
+#pragma unroll
+  for (uint32_t w = 1; w < kWarps; ++w) sum += sums[w][lane];
+  put_weight(out, type, (uint32_t)c, sum);
 }
 
 template <typename T> __global__ void __launch_bounds__(kThreads) rms_norm_dx_kernel(const GradArgs a)
@@ -621,8 +645,10 @@ bool grad_plan(const GradArgs &a, int type, HeldGrad &h, uint32_t &chunks, uint3
   if (!in_step(a.total, e, a.total_stride, v, a.dy, e, a.dy_stride, a.rows) || !in_step(a.dtotal, e, a.dtotal_stride, v, a.dy, e, a.dy_stride, a.rows) ||
       !in_step(a.dx, e, a.dx_stride, v, a.dy, e, a.dy_stride, a.rows)) return false;
   shift = !aligned_to(a.dy, 16) || a.cols % v || (a.rows > 1 && a.dy_stride % v) || !aligned_to(a.gamma.p, 16);
-  chunks = slots <= 32 ? 1 : slots < 128 ? 2 : 4;
-  threads = slots <= 2048 ? 512 : 1024;
+  // four slots to a thread, but two where that would be a single team of few warps ([8192,8704] 110 us with four, 97 with two)
+  const bool single = v == 8 && slots > 1024 && slots <= 1536;
+  chunks = slots <= 32 ? 1 : slots < 128 || single ? 2 : 4;
+  threads = single ? 768 : slots <= 2048 ? 512 : 1024;
   if (slots > (v == 8 ? 2048u : 4096u)) return false;
   h.team = (slots + chunks * 32 - 1) / (chunks * 32) * 32;
   if (slots <= 16) {
@@ -633,21 +659,33 @@ bool grad_plan(const GradArgs &a, int type, HeldGrad &h, uint32_t &chunks, uint3
   h.teams = threads / h.team;
   if (h.team > 32 && h.teams > 15) h.teams = 15;      // (a named barrier each)
   const uint32_t sms = sm_count();
-  if (a.rows < (uint64_t)h.teams * sms) h.teams = (uint32_t)((a.rows + sms - 1) / sms);     // a row per block first
-  h.depth = (uint32_t)(226 * 1024 / ((size_t)threads * chunks * 48));
+  // few rows: all in one block, which has nothing to join, or else a row per block first
+  if (a.rows <= h.teams) h.teams = (uint32_t)a.rows;
+  else if (a.rows < (uint64_t)h.teams * sms) h.teams = (uint32_t)((a.rows + sms - 1) / sms);
+  // a single team of many rows leaves out the threads beyond it, whose rings' place gives it more rows ahead; otherwise they help with the sums
+  h.threads = h.teams == 1 && a.rows > 4ull * sms ? h.team : threads;
+  h.depth = (uint32_t)(226 * 1024 / ((size_t)h.threads * chunks * 48));
   if (h.depth > 4) h.depth = 4;
   return true;
+}
+
+int join(const GradArgs &a, int type, cudaStream_t stream)
+{
+  const uint64_t cols = a.cols;
+  return a.parts <= kFewParts ? launch(join_few_kernel, dim3((uint32_t)((cols + kThreads - 1) / kThreads)), kThreads, 0, stream, a.cols, a.parts, a.partial, a.dgamma, type)
+                              : launch(join_columns_kernel, dim3((uint32_t)((cols + 31) / 32)), kThreads, 0, stream, a.cols, a.parts, a.partial, a.dgamma, type);
 }
 
 template <typename T, int CH, int NT> int launch_grad(const GradArgs &a, const HeldGrad &h, bool shift, cudaStream_t stream)
 {
   const auto kernel = shift ? rms_norm_grad_kernel<T, CH, NT, true> : rms_norm_grad_kernel<T, CH, NT, false>;
-  size_t shared = (size_t)h.depth * CH * NT * 48;
+  const uint32_t threads = h.threads;
+  size_t shared = (size_t)h.depth * CH * threads * 48;
   const size_t sums = (size_t)h.teams * (a.cols + (shift ? a.cols / Vec<T>::V + 1 : 0)) * 4;
   if (shared < sums) shared = sums;
   static SharedMemory allowed[2];
   if (!allowed[shift].up_to((const void *)kernel, shared)) return ANODE_E_LAUNCH;
-  return launch(kernel, dim3(a.parts), NT, shared, stream, a, h);
+  return launch(kernel, dim3(a.parts), threads, shared, stream, a, h);
 }
 
 int norm_forward(const NormArgs &a, int type, int gamma_type, bool quant, cudaStream_t stream)
@@ -755,7 +793,7 @@ extern "C" int anode_gpu_rms_norm_add_bwd(
   uint32_t chunks = 0, threads = 0;
   bool shift = false;
   const bool held = grad_plan(a, type, h, chunks, threads, shift);
-  const uint32_t wide = (uint32_t)(((uint64_t)cols + kThreads - 1) / kThreads), narrow = (uint32_t)(((uint64_t)cols + 31) / 32);
+  const uint32_t wide = (uint32_t)(((uint64_t)cols + kThreads - 1) / kThreads);
   return by_type(type, [&](auto t) {
     using T = decltype(t);
     constexpr uint32_t V = Vec<T>::V;
@@ -765,14 +803,15 @@ extern "C" int anode_gpu_rms_norm_add_bwd(
       h.step = (uint64_t)a.parts * h.teams;
       if (shift && rows > h.step) h.step = h.step / V * V;
       if (chunks == 1) TRY((launch_grad<T, 1, 512>(a, h, shift, stream)));
-      else if (chunks == 2) TRY((launch_grad<T, 2, 512>(a, h, shift, stream)));
+      else if (chunks == 2 && threads == 512) TRY((launch_grad<T, 2, 512>(a, h, shift, stream)));
+      else if (chunks == 2) { if constexpr (sizeof(T) == 2) TRY((launch_grad<T, 2, 768>(a, h, shift, stream))); }
       else if (threads == 512) TRY((launch_grad<T, 4, 512>(a, h, shift, stream)));
       else if constexpr (sizeof(T) == 4) TRY((launch_grad<T, 4, 1024>(a, h, shift, stream)));
-      return dgamma ? launch(join_columns_kernel, dim3(narrow), 1024, 0, stream, cols, a.parts, a.partial, dgamma, gamma_type) : (int)ANODE_OK;
+      return dgamma && a.parts > 1 ? join(a, gamma_type, stream) : (int)ANODE_OK;
     }
     if (dgamma) {
       TRY(launch(rms_norm_dgamma_kernel<T>, dim3(wide, a.parts), kThreads, 0, stream, a));
-      TRY(launch(join_columns_kernel, dim3(narrow), 1024, 0, stream, cols, a.parts, a.partial, dgamma, gamma_type));
+      TRY(join(a, gamma_type, stream));
     }
     return launch(rms_norm_dx_kernel<T>, dim3(row_blocks(rows)), kThreads, 0, stream, a);
   });

@@ -239,10 +239,7 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT)) rotary_heads_k
       for (int i = 0; i < V; ++i) v[j * V + i] = 0.0f;
       if (!(j ? second[k] : has[k])) continue;
       if (aligned_gamma) d.gamma.load<V>(e, v + j * V);
-      else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[j * V + i] = d.gamma.at(e + i);
-      }
+      else d.gamma.load_each<V>(e, v + j * V);
     }
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) {
@@ -503,11 +500,14 @@ __global__ void __launch_bounds__(kThreads, IT > 8 ? 2 : 4) rotary_pairs_kernel(
   make_rates(a, rates);
   float2 g[NORM ? IT : 1], acc[BOTH ? IT : 1];
   if constexpr (NORM) {
+    uint32_t column[2 * IT];
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-      g[k] = make_float2(has[k] ? d.gamma.at(e0[k]) : 0.0f, second[k] ? d.gamma.at(e1[k]) : 0.0f);
+      column[2 * k] = has[k] ? e0[k] : a.dim;
+      column[2 * k + 1] = second[k] ? e1[k] : a.dim;
       if constexpr (BOTH) acc[k] = both(0.0f);
     }
+    d.gamma.gather<2 * IT>(column, a.dim, reinterpret_cast<float *>(g));
   }
   const Walk<T> walk(a, d, group, groups);
   const uint64_t hop = d.in.head * groups, hop_x = BOTH ? d.x.head * groups : 0, hop_out = d.out.head * groups;
@@ -787,7 +787,10 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
   a.turned = a.rot / 2 / v;
   a.items = a.turned + (a.dim - a.rot + 2 * v - 1) / (2 * v);
   // lanes of a head's group: as many as it has items, in a power of two where others would not make more groups of a warp
-  const uint32_t per_lane = v == 1 ? 8 : 1, wide = (a.items + per_lane - 1) / per_lane;
+  // (pairs anywhere: eight to a lane where the heads fill the device, else two, which a warp is done with sooner: backward, 64 tokens
+  // of 40 heads, 62 of 128 turned, 12.5 us and 7.5)
+  const bool few = (uint64_t)a.batch * a.seq * (a.side[0].heads + a.side[1].heads) < 64ull * sm_count();
+  const uint32_t per_lane = v > 1 ? 1 : few && a.items <= 64 ? 2 : a.items > 32 ? 8 : (a.items + 3) / 4, wide = (a.items + per_lane - 1) / per_lane;
   a.lanes = 1;
   while (a.lanes < 32 && a.lanes < wide) a.lanes *= 2;
   if (wide < 32 && 32 / wide > 32 / a.lanes) a.lanes = wide;
@@ -847,7 +850,7 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
         if (v == 8) return each == 1 ? launch_rotary<T, 8, 1, N, B>(a, blocks, tables, sums, stream) : launch_rotary<T, 8, 2, N, B>(a, blocks, tables, sums, stream);
       if (v == 4) return each == 1 ? launch_rotary<T, 4, 1, N, B>(a, blocks, tables, sums, stream)
                        : each == 2 ? launch_rotary<T, 4, 2, N, B>(a, blocks, tables, sums, stream) : launch_rotary<T, 4, 4, N, B>(a, blocks, tables, sums, stream);
-      return each <= 8 ? launch_rotary<T, 1, 8, N, B>(a, blocks, tables, sums, stream) : launch_rotary<T, 1, 16, N, B>(a, blocks, tables, sums, stream);
+      return each <= 2 ? launch_rotary<T, 1, 2, N, B>(a, blocks, tables, sums, stream) : each <= 8 ? launch_rotary<T, 1, 8, N, B>(a, blocks, tables, sums, stream) : launch_rotary<T, 1, 16, N, B>(a, blocks, tables, sums, stream);
     };
     const std::true_type yes;
     const std::false_type no;

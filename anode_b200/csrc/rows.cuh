@@ -51,6 +51,20 @@ struct Weights {
       }
     }
   }
+  // N of them at any columns, those of columns below `end`, the others 0: all asked for before any is used
+  template <int N> __device__ __forceinline__ void gather(const uint32_t *c, uint32_t end, float *f) const
+  {
+    if (!p || type == ANODE_TYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = c[i] >= end ? 0.0f : p ? static_cast<const float *>(p)[c[i]] : 1.0f;
+    } else {
+      uint16_t w[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = c[i] < end ? static_cast<const uint16_t *>(p)[c[i]] : (uint16_t)0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = type == ANODE_TYPE_F16 ? __half2float(__ushort_as_half(w[i])) : __uint_as_float((uint32_t)w[i] << 16);
+    }
+  }
   // N of them from column c on, one by one
   template <int N> __device__ __forceinline__ void load_each(uint32_t c, float *f) const
   {
@@ -222,12 +236,13 @@ template <typename F> inline int by_type(int type, F f)
   return type == ANODE_TYPE_F32 ? f(float()) : type == ANODE_TYPE_F16 ? f(__half()) : f(__nv_bfloat16());
 }
 
-// A kernel's leave to use more dynamic shared memory than 48 KB, asked for once per device and for all that a block may have
+// A kernel's leave to use more shared memory than 48 KB (its own arrays, of a few KB here, among them), asked for once per device and for all that
+// a block may have
 class SharedMemory {
  public:
   bool up_to(const void *kernel, size_t bytes)
   {
-    if (bytes <= 48 * 1024) return true;
+    if (bytes <= 40 * 1024) return true;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
     if (done_.load(std::memory_order_relaxed) >> dev & 1) return true;

@@ -12,7 +12,7 @@ from tests.test_gpu_rms_norm import EPS, make, saved, weights
 pytestmark = pytest.mark.gpu
 
 # rows, cols: by the slots of 16 bytes of a row (up to 32, up to 127, up to 2048, more), whole and ragged, several rows to each team
-MANY = [(40000, 32), (25000, 33), (20000, 200), (12000, 257), (5000, 640), (5001, 643), (2500, 1536), (2500, 1535), (1300, 5000), (1301, 5003), (700, 9001), (500, 16384)]
+MANY = [(40000, 32), (25000, 33), (20000, 200), (12000, 257), (5000, 640), (5001, 643), (2500, 1536), (2500, 1535), (1300, 5000), (1301, 5003), (700, 9001), (400, 10240), (500, 16384)]
 F32 = [(500, 12288), (500, 12289), (300, 16380), (301, 16381)]
 
 

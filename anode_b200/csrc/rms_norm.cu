@@ -369,15 +369,16 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
   uint32_t left = works ? (uint32_t)((a.rows - row0 + h.step - 1) / h.step) : 0, ahead = left, in = 0, out = 0;
   const uint64_t dy_step = h.step * a.dy_stride, t_step = h.step * a.total_stride, dt_step = h.step * a.dtotal_stride, dx_step = h.step * a.dx_stride;
   // what does not go through the ring, of the row that is worked on next: 1/rms, and an element of the head or the tail
-  struct Side { float r, dy, t, dt; } now = {}, next = {};
+  // (as it lies in memory: nothing waits for it before its row's turn)
+  struct Side { float r; T dy, t, dt; } now = {}, next = {};
   const T *dy1 = dy + edge, *t1 = t + edge, *dt1 = dt + edge;
   auto side = [&](Side &o) {
     o.r = *inv;
     inv += h.step;
     if constexpr (SHIFT) {
       if (on_edge) {
-        o.dy = to_float(*dy1); o.t = to_float(*t1);
-        if (a.dtotal) o.dt = to_float(*dt1);
+        o.dy = *dy1; o.t = *t1;
+        if (a.dtotal) o.dt = *dt1;
       }
       dy1 += dy_step; t1 += t_step; dt1 += dt_step;
     }
@@ -409,7 +410,8 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
     if (h.depth == 4) copies_wait<3>(); else if (h.depth == 3) copies_wait<2>(); else if (h.depth == 2) copies_wait<1>(); else copies_wait<0>();
     const uint4 *from = ring + out * (CH * 3) * nt;
     out = out + 1 == h.depth ? 0 : out + 1;
-    float2 dot2 = make_float2(SHIFT ? now.dy * g_edge * now.t : 0.0f, 0.0f);
+    const float dy_edge = to_float(now.dy), t_edge = to_float(now.t);
+    float2 dot2 = make_float2(SHIFT ? dy_edge * g_edge * t_edge : 0.0f, 0.0f);
     // a single slot stays in registers between the two passes over the row, more are read again
     constexpr bool ONE = CH == 1;
     float2 u[H], v[H];
@@ -454,8 +456,8 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
       Vec<T>::of(reinterpret_cast<const float *>(e)).store(dx + start + k * hop);
     }
     if (on_edge) {
-      acc_edge = fmaf(now.dy * now.r, now.t, acc_edge);
-      dx[edge] = from_float<T>(fmaf(now.dy * now.r, g_edge, now.t * c.x) + now.dt);
+      acc_edge = fmaf(dy_edge * now.r, t_edge, acc_edge);
+      dx[edge] = from_float<T>(fmaf(dy_edge * now.r, g_edge, t_edge * c.x) + to_float(now.dt));
     }
     dx += dx_step;
   }
@@ -646,7 +648,7 @@ bool grad_plan(const GradArgs &a, int type, HeldGrad &h, uint32_t &chunks, uint3
       !in_step(a.dx, e, a.dx_stride, v, a.dy, e, a.dy_stride, a.rows)) return false;
   shift = !aligned_to(a.dy, 16) || a.cols % v || (a.rows > 1 && a.dy_stride % v) || !aligned_to(a.gamma.p, 16);
   // four slots to a thread, but two where that would be a single team of few warps ([8192,8704] 110 us with four, 97 with two)
-  const bool single = v == 8 && slots > 1024 && slots <= 1536;
+  const bool single = !shift && v == 8 && slots > 1024 && slots <= 1536;
   chunks = slots <= 32 ? 1 : slots < 128 || single ? 2 : 4;
   threads = single ? 768 : slots <= 2048 ? 512 : 1024;
   if (slots > (v == 8 ? 2048u : 4096u)) return false;
@@ -678,7 +680,8 @@ int join(const GradArgs &a, int type, cudaStream_t stream)
 
 template <typename T, int CH, int NT> int launch_grad(const GradArgs &a, const HeldGrad &h, bool shift, cudaStream_t stream)
 {
-  const auto kernel = shift ? rms_norm_grad_kernel<T, CH, NT, true> : rms_norm_grad_kernel<T, CH, NT, false>;
+  auto kernel = rms_norm_grad_kernel<T, CH, NT, false>;
+  if constexpr (NT != 768) { if (shift) kernel = rms_norm_grad_kernel<T, CH, NT, true>; }       // (ragged rows had no registers for that form)
   const uint32_t threads = h.threads;
   size_t shared = (size_t)h.depth * CH * threads * 48;
   const size_t sums = (size_t)h.teams * (a.cols + (shift ? a.cols / Vec<T>::V + 1 : 0)) * 4;

@@ -615,7 +615,7 @@ inline bool in_step(const void *p, size_t bytes, uint64_t stride, uint32_t v, co
 }
 
 // How the rows of a call are held in registers; false where they are not
-bool held_plan(const NormArgs &a, int type, int gamma_type, bool quant, Held &h, bool &shift)
+bool held_plan(const NormArgs &a, int type, bool quant, Held &h, bool &shift)
 {
   const size_t e = type_bytes(type);
   const uint32_t v = (uint32_t)(16 / e);
@@ -722,7 +722,7 @@ int norm_forward(const NormArgs &a, int type, int gamma_type, bool quant, cudaSt
   if (a.inv_rms && !aligned_to(a.inv_rms, 4)) return ANODE_E_ALIGN;
   Held h = {};
   bool shift = false;
-  const bool held = a.rows < (1ull << 30) && held_plan(a, type, gamma_type, quant, h, shift);
+  const bool held = a.rows < (1ull << 30) && held_plan(a, type, quant, h, shift);
   return by_type(type, [&](auto t) {
     using T = decltype(t);
     if (held) return h.chunks == 1 ? launch_held<T, 1>(a, h, shift, quant, stream) : h.chunks == 2 ? launch_held<T, 2>(a, h, shift, quant, stream)

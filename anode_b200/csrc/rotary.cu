@@ -752,6 +752,14 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
       if (c.dgamma[k] && cudaMemsetAsync(c.dgamma[k], 0, ge * a.dim, stream) != cudaSuccess) return ANODE_E_LAUNCH;
     return ANODE_OK;
   }
+  // queries and keys are worked on side by side: no output of one is in the place of an array of the other
+  if (two) {
+    if (c.dgamma[0] && c.dgamma[0] == c.dgamma[1]) return ANODE_E_STRIDE;
+    for (int k = 0; k < 2; ++k) {
+      const void *out = c.out[k]->data;
+      if (out && (out == c.out[!k]->data || out == c.in[!k]->data || (c.bwd && a.norm && out == c.x[!k]->data))) return ANODE_E_STRIDE;
+    }
+  }
   if (!a.freq || !a.positions) return ANODE_E_NULL;
   if (!aligned_to(a.freq, 8) || !aligned_to(a.positions, (size_t)c.position_bytes)) return ANODE_E_ALIGN;
   for (int k = 0; k < 1 + two; ++k) {

@@ -643,7 +643,7 @@ class RotaryPositionsOp:
     norm): the pair (u, v) of the head becomes amplitude*(u cos a - v sin a, u sin a + v cos a), a = position*freq[i], for the
     pairs (i, i + rot/2) or, interleaved, (2i, 2i + 1), i < rot/2 = len(freq); elements from rot on pass.  q, k: [tokens,
     heads, dim] or [batch, seq, heads, dim] at any strides (k None: one array only); positions: int32 or int64, [tokens], [batch, seq] or [seq]; freq: float64
-    (rotary_frequencies).  q_out may be q, k_out may be k."""
+    (rotary_frequencies).  q_out may be q, k_out may be k; neither may be the other's array."""
     @staticmethod
     def apply(positions, freq, q, k, q_out, k_out, interleaved=False, amplitude=1.0, epsilon=None, gamma_q=None, gamma_k=None, cfg=None, stream=None):
         _hint(cfg)
@@ -656,7 +656,7 @@ class RotaryPositionsOp:
     def adjoint(positions, freq, dq_out, dk_out, dq, dk, interleaved=False, amplitude=1.0, epsilon=None, q=None, k=None, gamma_q=None, gamma_k=None,
                 dgamma_q=None, dgamma_k=None, workspace=None, cfg=None, stream=None):
         """dq, dk from the gradients of q_out, k_out; with a norm also from q and k, the forward pass's inputs, and then the gradients of
-        the norm's weights where they are asked for.  dq may be dq_out, dk may be dk_out.  workspace: a tensor of rotary_workspace_bytes,
+        the norm's weights where they are asked for.  dq may be dq_out, dk may be dk_out; neither may be an array of the other's.  workspace: a tensor of rotary_workspace_bytes,
         needed for those only; None has one made on the call's stream."""
         _hint(cfg)
         rc = native().rotary_bwd(positions, freq, dq_out, dk_out, dq, dk, interleaved, amplitude, epsilon, q, k, gamma_q, gamma_k, dgamma_q, dgamma_k,

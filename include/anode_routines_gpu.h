@@ -174,7 +174,7 @@ void anode_gpu_positive_clip_flat_map_bwd_f32(
 #define ANODE_E_ALIGN      -6   /* tensor pointers must be 4-byte aligned */
 #define ANODE_E_TOO_LARGE  -7   /* the problem needs more scratch than the library's built-in array holds */
 #define ANODE_E_TYPE       -8   /* an element type that the call does not take */
-#define ANODE_E_STRIDE     -9   /* strides that overlap in an output, or an output in the place of an input with other strides */
+#define ANODE_E_STRIDE     -9   /* strides that overlap in an output, or an output in a place that it may not have */
 
 /* Bits of the device status word. */
 #define ANODE_ST_WAIT_STATS   1u  /* a wait for a channel's statistics ran out */
@@ -510,7 +510,8 @@ int anode_gpu_sync_batch_norm_add_act_bwd_3d1_packed_f32(
  * Conventions that differ from the above: the element type is an argument (ANODE_TYPE_*; f16 and bf16 beside f32), rows
  * and heads may lie apart (strides in elements; the innermost dimension is packed), and no rows or no tokens are a call
  * that does nothing (gradients of weights are then zero).  All arithmetic is in f32, angles in f64; every output is
- * rounded once.  An output may be an input's array (same pointer and strides); other overlaps are not allowed.
+ * rounded once.  An output may be an input's array (same pointer and strides), a query's not a
+ * key's; other overlaps are not allowed.
  * Tensors are aligned to their elements; 16-byte aligned ones of such strides are faster.  Nothing synchronises, nothing
  * is allocated, and no state is kept in a workspace from call to call: it is written before it is read in every call, and
  * calls that may overlap on the device take one each.

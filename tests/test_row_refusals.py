@@ -86,6 +86,17 @@ def test_the_c_calls_refuse(call, change, code):
     assert call(**change) == code
 
 
+@pytest.mark.parametrize("call, change", [
+    (rotary, dict(k_out=heads(7 * P, 2))), (rotary, dict(q_out=heads(6 * P))), (rotary, dict(k_out=heads(5 * P, 2))),
+    (rotary, dict(k=heads(5 * P, 2), q_out=heads(5 * P))),
+    (rotary_grad, dict(dk=heads(9 * P, 2))), (rotary_grad, dict(dq=heads(6 * P))), (rotary_grad, dict(dk=heads(5 * P, 2))),
+    (rotary_grad, dict(dq=heads(8 * P))), (rotary_grad, dict(dk=heads(7 * P, 2))), (rotary_grad, dict(dgamma_k=11 * P)),
+])
+def test_queries_and_keys_side_by_side_share_no_output(call, change):
+    """The two are worked on at the same time: an output in the place of any array of the other one has no defined result."""
+    assert call(**change) == STRIDE
+
+
 def test_no_rows_and_no_tokens_do_nothing():
     assert norm(rows=0, x=None, residual=None, total=None, y=None) == 0
     assert quant(rows=0, scale=None, x=None, q=None, residual=None, total=None) == 0

@@ -196,7 +196,7 @@ ERRORS = {
     -6: "ANODE_E_ALIGN: tensor pointers must be 4-byte aligned",
     -7: "ANODE_E_TOO_LARGE: the problem needs more scratch than the library's built-in array holds",
     -8: "ANODE_E_TYPE: an element type that the call does not take",
-    -9: "ANODE_E_STRIDE: strides that overlap in an output, or an output in the place of an input with other strides",
+    -9: "ANODE_E_STRIDE: strides that overlap in an output, or an output in a place that it may not have",
 }
 
 

@@ -688,6 +688,12 @@ def rotary_frequencies(rot, base=10000.0, factor=1.0, context=None, slow=1.0, fa
     return freq.to(device)
 
 
+def _refuse_overwriting(kept, *outs):
+    """What a layer's backward pass reads is not the place of its forward pass's output."""
+    if any(out is not None and t is not None and t.numel() and out.data_ptr() == t.data_ptr() for out in outs for t in kept):
+        raise ValueError("the output would overwrite what the backward pass reads (infer may be in place)")
+
+
 class RmsNormAdd:
     """An RMS-norm layer with the residual's addition that keeps its weights and what its backward pass needs: a training loop makes
     two calls per step, forward(x, residual) and backward(dy, dtotal); serving calls infer or infer_quant."""
@@ -720,6 +726,8 @@ class RmsNormAdd:
 
     def forward(self, x, residual=None, out=None, total=None):
         """infer, keeping the sum and 1/rms for the backward pass.  The sum (x without a residual) has to stay as it is until then."""
+        if residual is None:
+            _refuse_overwriting((x,), out)
         y = out if out is not None else torch.empty_like(x)
         if residual is not None and total is None:
             total = torch.empty_like(x)
@@ -761,6 +769,8 @@ class RotaryPositions:
 
     def forward(self, q, k, positions, q_out=None, k_out=None):
         """infer, keeping the positions and, with a norm, q and k for the backward pass: they have to stay as they are until then."""
+        if self.epsilon is not None:
+            _refuse_overwriting((q, k), q_out, k_out)
         out = self.infer(q, k, positions, q_out, k_out)
         self._saved = (positions, q, k) if self.epsilon is not None else (positions, None, None)
         return out

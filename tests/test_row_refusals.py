@@ -195,3 +195,19 @@ def test_frequencies():
     assert torch.allclose(s[turns > 4], plain[turns > 4], rtol=1e-15, atol=0) and torch.allclose(s[turns < 1], plain[turns < 1] / 8, rtol=1e-15, atol=0)
     between = (turns > 1) & (turns < 4)
     assert between.any() and ((s < plain) & (s > plain / 8))[between].all()
+
+
+def test_layers_keep_what_their_backward_pass_reads():
+    """forward in place would leave the backward pass with the norm in the place of its input; infer may be in place."""
+    x, pos, q = torch.zeros(4, 8), torch.arange(4), torch.zeros(4, 2, 8)
+    with pytest.raises(ValueError, match="backward pass"):
+        ops.RmsNormAdd(8, device="cpu").forward(x, out=x)
+    turn = ops.RotaryPositions(8, norm=True, device="cpu")
+    with pytest.raises(ValueError, match="backward pass"):
+        turn.forward(q, None, pos, q_out=q)
+    with pytest.raises(ValueError, match="backward pass"):
+        turn.forward(q, q.clone(), pos, None, q.view(4, 2, 8))
+    for call in (lambda: ops.RmsNormAdd(8, device="cpu").infer(x, out=x), lambda: turn.infer(q, None, pos, q_out=q),
+                 lambda: ops.RotaryPositions(8, device="cpu").forward(q, None, pos, q_out=q), lambda: ops.RmsNormAdd(8, device="cpu").forward(x, x.clone(), out=x)):
+        with pytest.raises(ValueError, match="CUDA tensor"):      # (as far as a machine without a device goes)
+            call()

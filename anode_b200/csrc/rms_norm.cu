@@ -443,7 +443,9 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
         dot = warp_sum_all(lane < warps ? buf[turn][first + lane] : 0.0f);
       }
     } else for (uint32_t o = h.team / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(lanes, dot, o);
-    const float2 r = both(now.r), c = both(-now.r * now.r * now.r * dot * a.inv_cols);
+    // (1/rms meets the sum, a row's element and the bracket one at a time: its powers alone would leave f32's range where rows are large or tiny)
+    const float m = dot * now.r * a.inv_cols;
+    const float2 r = both(now.r), minus = both(-m);
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       if (!has(k)) continue;
@@ -454,20 +456,24 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
       float2 e[H];
 #pragma unroll
       for (int i = 0; i < H; ++i) {
-        const float2 ur = mul2(u[i], r);
-        acc[k][i] = fma2(ur, v[i], acc[k][i]);
-        e[i] = fma2(ur, g[k][i], mul2(v[i], c));
+        const float2 xh = mul2(v[i], r);
+        acc[k][i] = fma2(u[i], xh, acc[k][i]);
+        e[i] = fma2(u[i], g[k][i], mul2(xh, minus));
       }
       if (a.dtotal) {
         Vec<T>{from[(3 * k + 2) * nt]}.floats(reinterpret_cast<float *>(v));
 #pragma unroll
-        for (int i = 0; i < H; ++i) e[i] = add2(e[i], v[i]);
+        for (int i = 0; i < H; ++i) e[i] = fma2(e[i], r, v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < H; ++i) e[i] = mul2(e[i], r);
       }
       Vec<T>::of(reinterpret_cast<const float *>(e)).store(dx + start + k * hop);
     }
     if (on_edge) {
-      acc_edge = fmaf(dy_edge * now.r, t_edge, acc_edge);
-      dx[edge] = from_float<T>(fmaf(dy_edge * now.r, g_edge, t_edge * c.x) + to_float(now.dt));
+      const float xh = t_edge * now.r;
+      acc_edge = fmaf(dy_edge, xh, acc_edge);
+      dx[edge] = from_float<T>(fmaf(fmaf(dy_edge, g_edge, -xh * m), now.r, to_float(now.dt)));
     }
     dx += dx_step;
   }

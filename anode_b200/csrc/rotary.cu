@@ -399,15 +399,16 @@ __global__ void __launch_bounds__(kThreads, resident(2 * V * IT)) rotary_heads_k
           for (int i = 0; i < V; ++i) { sq2 = fma2(x[k][i], x[k][i], sq2); dot2 = fma2(mul2(f[k][i], g[k][i]), x[k][i], dot2); }
         }
         const float r = rsqrtf(group_sum(sq2.x + sq2.y, a.lanes, wlane - lane) * a.inv_dim + a.epsilon);
-        const float2 r2 = both(r), c = both(-group_sum(dot2.x + dot2.y, a.lanes, wlane - lane) * r * r * r * a.inv_dim);
+        // (1/rms meets the sum, the head's elements and the bracket one at a time: its powers alone may leave f32's range)
+        const float2 r2 = both(r), minus = both(-group_sum(dot2.x + dot2.y, a.lanes, wlane - lane) * r * a.inv_dim);
         if (live) {
 #pragma unroll
           for (int k = 0; k < IT; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              const float2 fr = mul2(f[k][i], r2);
-              acc[k][i] = fma2(fr, x[k][i], acc[k][i]);
-              f[k][i] = fma2(fr, g[k][i], mul2(x[k][i], c));
+              const float2 xh = mul2(x[k][i], r2);
+              acc[k][i] = fma2(f[k][i], xh, acc[k][i]);
+              f[k][i] = mul2(fma2(f[k][i], g[k][i], mul2(xh, minus)), r2);
             }
         }
       }
@@ -587,13 +588,13 @@ __global__ void __launch_bounds__(kThreads, IT > 8 ? 2 : 4) rotary_pairs_kernel(
           dot = fmaf(f[k].x * g[k].x, x[k].x, fmaf(f[k].y * g[k].y, x[k].y, dot));
         }
         const float r = rsqrtf(group_sum(sq, a.lanes, wlane - lane) * a.inv_dim + a.epsilon);
-        const float2 r2 = both(r), c = both(-group_sum(dot, a.lanes, wlane - lane) * r * r * r * a.inv_dim);
+        const float2 r2 = both(r), minus = both(-group_sum(dot, a.lanes, wlane - lane) * r * a.inv_dim);
         if (live) {
 #pragma unroll
           for (int k = 0; k < IT; ++k) {
-            const float2 fr = mul2(f[k], r2);
-            acc[k] = fma2(fr, x[k], acc[k]);
-            f[k] = fma2(fr, g[k], mul2(x[k], c));
+            const float2 xh = mul2(x[k], r2);
+            acc[k] = fma2(f[k], xh, acc[k]);
+            f[k] = mul2(fma2(f[k], g[k], mul2(xh, minus)), r2);
           }
         }
       }

@@ -189,7 +189,7 @@ def native():
 
 ERRORS = {
     -1: "ANODE_E_NULL: a required pointer is NULL",
-    -2: "ANODE_E_DIMS: a dimension is 0 or the tensor has 2^32 or more elements",
+    -2: "ANODE_E_DIMS: a dimension is 0, or too large for the call (a tensor of 2^32 or more elements, a row of 2^31 or more)",
     -3: "ANODE_E_WORKSPACE: workspace missing, misaligned or too small",
     -4: "ANODE_E_LAUNCH: the CUDA runtime refused the launch",
     -5: "ANODE_E_COMM: communicator missing, inconsistent, or NCCL failure",

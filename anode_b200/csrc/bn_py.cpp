@@ -585,7 +585,7 @@ bool cols_of(RowArgs &a, int i, const at::Tensor &t, U8 &rows, uint32_t &cols)
 {
   U8 stride;
   const int64_t c = t.size(t.dim() - 1);
-  if (c > 0xffffffffll) return a.fail(i, "too many columns");
+  if (c > 0x7fffffffll) return a.fail(i, "too many columns");
   cols = (uint32_t)c;
   return a.collapse(i, t, t.dim() - 1, rows, stride);
 }

@@ -598,6 +598,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads) rms_norm_dx_ke
 inline uint32_t parts_of(uint64_t rows) { return (uint32_t)(rows < kMostParts ? (rows ? rows : 1) : kMostParts); }
 inline uint32_t row_blocks(uint64_t rows) { return (uint32_t)(rows < (1u << 30) ? rows : (1u << 30)); }
 
+// Columns are counted in 32 bits, up to a block's threads beyond the last one
+inline bool served(uint64_t rows, uint32_t cols) { return cols != 0 && !(cols >> 31) && !(rows >> 36); }
+
 // An array of rows: a pointer of the type's alignment; an output's rows do not overlap
 inline int check_rows(const void *p, size_t bytes, uint64_t rows, uint32_t cols, uint64_t stride, bool output)
 {
@@ -710,7 +713,7 @@ template <typename T, int CH, int NT> int launch_grad(const GradArgs &a, const H
 int norm_forward(const NormArgs &a, int type, int gamma_type, bool quant, cudaStream_t stream)
 {
   if (!known_type(type) || (a.gamma.p && !known_type(gamma_type))) return ANODE_E_TYPE;
-  if (a.cols == 0 || a.rows >> 36) return ANODE_E_DIMS;
+  if (!served(a.rows, a.cols)) return ANODE_E_DIMS;
   if (a.rows == 0) return ANODE_OK;
   const size_t e = type_bytes(type);
   TRY(check_rows(a.x, e, a.rows, a.cols, a.x_stride, false));
@@ -789,7 +792,7 @@ extern "C" int anode_gpu_rms_norm_add_bwd(
 {
   (void)cfg;
   if (!known_type(type) || ((gamma || dgamma) && !known_type(gamma_type))) return ANODE_E_TYPE;
-  if (cols == 0 || rows >> 36) return ANODE_E_DIMS;
+  if (!served(rows, cols)) return ANODE_E_DIMS;
   if (gamma && !aligned_to(gamma, type_bytes(gamma_type))) return ANODE_E_ALIGN;
   if (dgamma) {
     if (!aligned_to(dgamma, type_bytes(gamma_type))) return ANODE_E_ALIGN;

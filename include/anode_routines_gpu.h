@@ -167,7 +167,7 @@ void anode_gpu_positive_clip_flat_map_bwd_f32(
 
 #define ANODE_OK            0
 #define ANODE_E_NULL       -1   /* a required pointer is NULL */
-#define ANODE_E_DIMS       -2   /* a dimension is 0 or dim0*dim1*dim2 >= 2^32 */
+#define ANODE_E_DIMS       -2   /* a dimension is 0, dim0*dim1*dim2 >= 2^32, or what section 4 says of its sizes */
 #define ANODE_E_WORKSPACE  -3   /* workspace missing, misaligned or too small */
 #define ANODE_E_LAUNCH     -4   /* the CUDA runtime refused the launch */
 #define ANODE_E_COMM       -5   /* communicator missing / inconsistent / NCCL failure */
@@ -512,6 +512,7 @@ int anode_gpu_sync_batch_norm_add_act_bwd_3d1_packed_f32(
  * that does nothing (gradients of weights are then zero).  All arithmetic is in f32, angles in f64; every output is
  * rounded once.  An output may be an input's array (same pointer and strides), a query's not a
  * key's; other overlaps are not allowed.
+ * Sizes: fewer than 2^36 rows of fewer than 2^31 columns, fewer than 2^31 tokens of at most 65535 heads; beyond them ANODE_E_DIMS.
  * Tensors are aligned to their elements; 16-byte aligned ones of such strides are faster.  Nothing synchronises, nothing
  * is allocated, and no state is kept in a workspace from call to call: it is written before it is read in every call, and
  * calls that may overlap on the device take one each.

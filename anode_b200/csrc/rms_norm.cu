@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(NT) rms_norm_grad_kernel(const GradArgs a, con
   }
 }
 
-// Any rows: dgamma's partial sums, a thread has a column and every `parts`-th row; ahead of the kernel below, whose dx may be dy
+// Any rows: dgamma's partial sums, a thread has a column and every `parts`-th row
 template <typename T> __global__ void __launch_bounds__(kThreads) rms_norm_dgamma_kernel(const GradArgs a)
 {
   pdl_wait();
@@ -831,10 +831,9 @@ extern "C" int anode_gpu_rms_norm_add_bwd(
       else if constexpr (sizeof(T) == 4) TRY((launch_grad<T, 4, 1024>(a, h, shift, stream)));
       return dgamma && a.parts > 1 ? join(a, gamma_type, stream) : (int)ANODE_OK;
     }
-    if (dgamma) {
-      TRY(launch(rms_norm_dgamma_kernel<T>, dim3(wide, a.parts), kThreads, 0, stream, a));
-      TRY(join(a, gamma_type, stream));
-    }
-    return launch(rms_norm_dx_kernel<T>, dim3(row_blocks(rows)), kThreads, 0, stream, a);
+    // dgamma's parts ahead of dx, which may be dy; dgamma, which may be gamma, behind it
+    if (dgamma) TRY(launch(rms_norm_dgamma_kernel<T>, dim3(wide, a.parts), kThreads, 0, stream, a));
+    TRY(launch(rms_norm_dx_kernel<T>, dim3(row_blocks(rows)), kThreads, 0, stream, a));
+    return dgamma ? join(a, gamma_type, stream) : (int)ANODE_OK;
   });
 }

@@ -102,6 +102,7 @@ struct RotaryPositionsOp {
                     DeviceArray &q_out, DeviceArray *k_out, const DeviceArray *gamma_q, const DeviceArray *gamma_k, cudaStream_t s = 0)
   {
     const Shape d = shape(q, k, positions);
+    if (!k != !k_out) throw Error(ANODE_E_NULL, "k and k_out are given together");
     want_len(q_out, q.len(), "q_out"); if (k) want_len(*k_out, k->len(), "k_out");
     want_opt(gamma_q, d.dim, "gamma_q"); want_opt(gamma_k, d.dim, "gamma_k");
     const AnodeHeads a = heads(q), b = k ? heads(*k) : AnodeHeads{}, ao = heads(q_out), bo = k ? heads(*k_out) : AnodeHeads{};
@@ -119,6 +120,7 @@ struct RotaryPositionsOp {
                       const DeviceArray *gamma_k, DeviceArray *dgamma_q, DeviceArray *dgamma_k, RowScratch *scratch, cudaStream_t s = 0)
   {
     const Shape d = shape(dq_out, dk_out, positions);
+    if (!dk_out != !dk) throw Error(ANODE_E_NULL, "dk_out and dk are given together");
     want_len(dq, dq_out.len(), "dq"); if (dk_out) want_len(*dk, dk_out->len(), "dk");
     if (f.norm) { if (!q || (dk_out && !k)) throw Error(ANODE_E_NULL, "q, k"); want_len(*q, dq.len(), "q"); if (dk_out) want_len(*k, dk->len(), "k"); }
     want_opt(gamma_q, d.dim, "gamma_q"); want_opt(gamma_k, d.dim, "gamma_k"); want_opt(dgamma_q, d.dim, "dgamma_q"); want_opt(dgamma_k, d.dim, "dgamma_k");

@@ -103,7 +103,7 @@ struct RotaryPositionsOp {
   {
     const Shape d = shape(q, k, positions);
     if (!k != !k_out) throw Error(ANODE_E_NULL, "k and k_out are given together");
-    want_len(q_out, q.len(), "q_out"); if (k) want_len(*k_out, k->len(), "k_out");
+    want_heads(q_out, q, "q_out"); if (k) want_heads(*k_out, *k, "k_out");
     want_opt(gamma_q, d.dim, "gamma_q"); want_opt(gamma_k, d.dim, "gamma_k");
     const AnodeHeads a = heads(q), b = k ? heads(*k) : AnodeHeads{}, ao = heads(q_out), bo = k ? heads(*k_out) : AnodeHeads{};
     check(anode_gpu_rotary_positions_fwd(ANODE_TYPE_F32, 1, d.tokens, d.dim, 2 * (uint32_t)freq.len(), f.interleaved, f.amplitude, freq.ptr(), positions.ptr(), 8,
@@ -112,6 +112,7 @@ struct RotaryPositionsOp {
   }
   static size_t scratch_bytes(const DeviceArray &q, const DeviceArray *k)
   {
+    if (q.size().size() != 3 || (k && k->size().size() != 3)) throw Error(ANODE_E_DIMS, "heads need [dim, heads, tokens]");
     return anode_gpu_rotary_positions_bwd_workspace_bytes(1, q.size()[2], q.size()[1], k ? k->size()[1] : 0, q.size()[0]);
   }
   // q and k (the forward pass's inputs) are read where there is a norm
@@ -121,8 +122,8 @@ struct RotaryPositionsOp {
   {
     const Shape d = shape(dq_out, dk_out, positions);
     if (!dk_out != !dk) throw Error(ANODE_E_NULL, "dk_out and dk are given together");
-    want_len(dq, dq_out.len(), "dq"); if (dk_out) want_len(*dk, dk_out->len(), "dk");
-    if (f.norm) { if (!q || (dk_out && !k)) throw Error(ANODE_E_NULL, "q, k"); want_len(*q, dq.len(), "q"); if (dk_out) want_len(*k, dk->len(), "k"); }
+    want_heads(dq, dq_out, "dq"); if (dk_out) want_heads(*dk, *dk_out, "dk");
+    if (f.norm) { if (!q || (dk_out && !k)) throw Error(ANODE_E_NULL, "q, k"); want_heads(*q, dq_out, "q"); if (dk_out) want_heads(*k, *dk_out, "k"); }
     want_opt(gamma_q, d.dim, "gamma_q"); want_opt(gamma_k, d.dim, "gamma_k"); want_opt(dgamma_q, d.dim, "dgamma_q"); want_opt(dgamma_k, d.dim, "dgamma_k");
     const AnodeHeads a = heads(dq_out), b = dk_out ? heads(*dk_out) : AnodeHeads{}, ao = heads(dq), bo = dk_out ? heads(*dk) : AnodeHeads{};
     const AnodeHeads x = f.norm ? heads(*q) : AnodeHeads{}, z = f.norm && dk_out ? heads(*k) : AnodeHeads{};
@@ -141,6 +142,12 @@ struct RotaryPositionsOp {
       throw Error(ANODE_E_DIMS, "heads need [dim, heads, tokens] of one dim and one number of tokens");
     if (positions.len() != q.size()[2]) throw Error(ANODE_E_DIMS, "positions: one per token");
     return Shape{q.size()[0], q.size()[2]};
+  }
+  // heads of `like`'s sizes, the tokens behind them in as many dimensions as they please
+  static void want_heads(const DeviceArray &a, const DeviceArray &like, const char *what)
+  {
+    want_len(a, like.len(), what);
+    if (a.size().size() < 2 || a.size()[0] != like.size()[0] || a.size()[1] != like.size()[1]) throw Error(ANODE_E_DIMS, std::string(what) + ": expected [dim, heads, tokens]");
   }
   static AnodeHeads heads(const DeviceArray &x)
   {

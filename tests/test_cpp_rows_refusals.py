@@ -7,7 +7,7 @@ import pytest
 from tests.test_cpp_host import CPP, build
 
 
-@pytest.mark.parametrize("which", ["missing"])
+@pytest.mark.parametrize("which", ["missing", "shapes"])
 def test_refused_before_anything_is_asked_of_a_device(which):
     build()
     r = subprocess.run([os.path.join(CPP, "test_host_rows_refusals"), which], capture_output=True, text=True, timeout=120)

@@ -105,6 +105,18 @@ struct Held {
 
 __host__ __device__ constexpr uint32_t most_threads(int chunks) { return chunks <= 2 ? 1024u : chunks == 4 ? 512u : 640u; }
 
+// A group's scale, from the bits of its largest |y|: a product is within a step of the quotient, which the remainder that it leaves gives rounded to
+// nearest (Markstein 1990; an infinity leaves none).  Only the lane that stores the scale makes it so; values are multiplied by the reciprocal of the
+// product.  All of it in every lane took 78.2 us in the place of 76.2 for [8192,8192], divisions 81.5.
+__device__ __forceinline__ float peak_of(uint32_t largest) { return __uint_as_float(max(largest, __float_as_uint(kTiny))); }
+__device__ __forceinline__ float scale_of(uint32_t largest)
+{
+  constexpr float c = 1.0f / kE4M3;
+  const float a = peak_of(largest), s = a * c;
+  return a == __uint_as_float(0x7f800000u) ? a : fmaf(fmaf(-s, kE4M3, a), c, s);
+}
+__device__ __forceinline__ float inverse_of(uint32_t largest) { return __fdividef(1.0f, peak_of(largest) * (1.0f / kE4M3)); }      // (of 2^-105 to 2^120: nothing is flushed)
+
 __device__ __forceinline__ float max_nan(float a, float b)
 {
   float d;
@@ -221,8 +233,6 @@ __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const N
     for (int i = 0; i < H; ++i) m = max_nan(max_nan(m, fabsf(y[i].x)), fabsf(y[i].y));
     return bits_of(m);
   };
-  auto scale_of = [&](uint32_t m) { return __uint_as_float(max(m, __float_as_uint(kTiny))) * (1.0f / kE4M3); };
-  auto inverse = [&](float scale) { return __fdividef(1.0f, scale); };      // (a scale is no smaller than 2^-105: nothing is flushed)
   uint8_t *q = static_cast<uint8_t *>(a.y) + row * a.y_stride;
   auto eight = [](float u, float v) { return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(u, v), __NV_SATFINITE, __NV_E4M3); };
   // a slot to 8 bits: its elements before `border` times `one`, the others times `two`
@@ -248,9 +258,9 @@ __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const N
       for (int o = 64 / V; o > 0; o >>= 1)
         if (o < (int)h.team) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));      // (a smaller team has one group)
       if (k >= mine_slots) continue;
-      const float scale = scale_of(m), one = inverse(scale);
+      const float one = inverse_of(m);
       const uint32_t c = start + k * hop;
-      if (c % 128 == 0) a.scale[row * a.scale_row + c / 128 * a.scale_group] = scale;
+      if (c % 128 == 0) a.scale[row * a.scale_row + c / 128 * a.scale_group] = scale_of(m);
       put(k, y, one, one, V);
     }
     return;
@@ -268,8 +278,8 @@ __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const N
       __syncthreads();
       all = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < blockDim.x / 32 ? __float_as_uint(buf[1][threadIdx.x & 31]) : 0u);
     }
-    const float scale = scale_of(all), one = inverse(scale);
-    if (live && at == 0) a.scale[row * a.scale_row] = scale;
+    const float one = inverse_of(all);
+    if (live && at == 0) a.scale[row * a.scale_row] = scale_of(all);
 #pragma unroll
     for (int k = 0; k < CH; ++k) if (k < mine_slots) put(k, y[k], one, one, V);
     if (on_edge) q[edge] = (uint8_t)eight(ye * one, 0.0f);
@@ -295,9 +305,8 @@ __global__ void __launch_bounds__(most_threads(CH)) rms_norm_held_kernel(const N
     sync();
     // a group's scale is made once, and its inverse takes the peak's place
     for (uint32_t i = at; i < h.groups; i += h.team) {
-      const float scale = scale_of(top[i]);
-      if (live) a.scale[row * a.scale_row + i * a.scale_group] = scale;
-      top[i] = __float_as_uint(inverse(scale));
+      if (live) a.scale[row * a.scale_row + i * a.scale_group] = scale_of(top[i]);
+      top[i] = __float_as_uint(inverse_of(top[i]));
     }
     sync();
 #pragma unroll

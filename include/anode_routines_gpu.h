@@ -526,8 +526,8 @@ int anode_gpu_sync_batch_norm_add_act_bwd_3d1_packed_f32(
  *   r     = (sum(total^2)/cols + epsilon)^-1/2   per row (stored where inv_rms is not NULL)
  *   y     = total * r * gamma                    (gamma NULL: 1)
  * The norm reads the sum as it is stored, so that the backward pass sees the same numbers.  total without residual is
- * refused (it would be a copy).  Squares are summed in f32: rows with elements beyond 1e19 give y = 0, rows that hold a NaN
- * or an infinity give NaN where the formula does. */
+ * refused (it would be a copy).  Squares are summed in f32: rows whose rms reaches 2^64/sqrt(cols) (1.4e17 at 16384 columns)
+ * give r = 0 and y = 0, rows that hold a NaN or an infinity give NaN where the formula does. */
 int anode_gpu_rms_norm_add_fwd(
     int type, uint64_t rows, uint32_t cols, float epsilon,
     const void *x, uint64_t x_stride, const void *residual, uint64_t residual_stride,
@@ -578,7 +578,7 @@ struct AnodeHeads {
  *   (n[u], n[v]) -> (n[u]*c - n[v]*s, n[u]*s + n[v]*c);   n[rot..dim) passes as it is
  * (u, v) = (i, i + rot/2), or (2i, 2i + 1) where interleaved != 0.  rot is even, 2 <= rot <= dim <= 1024.  freq: rot/2 doubles on the
  * device (for long contexts stretched as the caller likes).  Angles are formed and reduced in f64, so that far positions
- * keep their digits.  positions[b*pos_batch_stride + s*pos_seq_stride]: signed integers of position_bytes (4 or 8) bytes. */
+ * keep their digits.  A head's squares are summed in f32, as a row's are above.  positions[b*pos_batch_stride + s*pos_seq_stride]: signed integers of position_bytes (4 or 8) bytes. */
 int anode_gpu_rotary_positions_fwd(
     int type, uint32_t batch, uint32_t seq, uint32_t dim, uint32_t rot, int interleaved, float amplitude,
     const double *freq, const void *positions, int position_bytes, uint64_t pos_batch_stride, uint64_t pos_seq_stride,

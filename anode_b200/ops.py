@@ -688,9 +688,31 @@ def rotary_frequencies(rot, base=10000.0, factor=1.0, context=None, slow=1.0, fa
     return freq.to(device)
 
 
+def _meets(levels, apart):
+    """Whether steps from -behind to ahead of each (stride, ahead, behind), the largest stride first, add up to `apart`."""
+    if not levels:
+        return apart == 0
+    (stride, ahead, behind), rest = levels[0], levels[1:]
+    up, down = (sum(level[0] * level[k] for level in rest) for k in (1, 2))
+    first, last = max(-behind, -((up - apart) // stride)), min(ahead, (apart + down) // stride)
+    return any(_meets(rest, apart - stride * n) for n in range(first, last + 1))
+
+
+def _share_memory(a, b):
+    """Whether two arrays have a byte in common, at whatever strides they lie."""
+    if a.device != b.device or not a.numel() or not b.numel():
+        return False
+    reach = {1: [a.element_size() - 1, b.element_size() - 1]}          # by stride in bytes: how far a and b go
+    for k, t in enumerate((a, b)):
+        for size, stride in zip(t.shape, t.stride()):
+            if size > 1 and stride:
+                reach.setdefault(stride * t.element_size(), [0, 0])[k] += size - 1
+    return _meets([(stride, *reach[stride]) for stride in sorted(reach, reverse=True)], b.data_ptr() - a.data_ptr())
+
+
 def _refuse_overwriting(kept, *outs):
-    """What a layer's backward pass reads is not the place of its forward pass's output."""
-    if any(out is not None and t is not None and t.numel() and out.data_ptr() == t.data_ptr() for out in outs for t in kept):
+    """What a layer's backward pass reads is no place for its forward pass's output."""
+    if any(out is not None and t is not None and _share_memory(t, out) for out in outs for t in kept):
         raise ValueError("the output would overwrite what the backward pass reads (infer may be in place)")
 
 
@@ -705,7 +727,7 @@ class RmsNormAdd:
         self._saved = None
 
     def infer(self, x, residual=None, out=None, total=None):
-        """(y, total): the norm of the sum, and the sum, which is x itself without a residual."""
+        """(y, total): the norm of the sum, and the sum, which is x itself without a residual (with out=x, then, y's array: the sum is gone)."""
         y = out if out is not None else torch.empty_like(x)
         if residual is not None and total is None:
             total = torch.empty_like(x)
@@ -726,8 +748,7 @@ class RmsNormAdd:
 
     def forward(self, x, residual=None, out=None, total=None):
         """infer, keeping the sum and 1/rms for the backward pass.  The sum (x without a residual) has to stay as it is until then."""
-        if residual is None:
-            _refuse_overwriting((x,), out)
+        _refuse_overwriting((x if residual is None else total,), out)
         y = out if out is not None else torch.empty_like(x)
         if residual is not None and total is None:
             total = torch.empty_like(x)

@@ -622,7 +622,7 @@ class RmsNormalizeAddOp:
 class RmsNormalizeAddQuantOp:
     """RmsNormalizeAddOp with its output in 8 bits, for a product that takes e4m3 operands: q = e4m3(y/scale), float8_e4m3fn, with
     scale = max(max |y|, 2^-96)/448 over the row (scale of x.shape[:-1]) or over each 128 columns of it (scale of
-    x.shape[:-1] + (ceil(cols/128),), any strides).  y is not rounded in between, and the quotient is taken in f32 (within 8*2^-24)."""
+    x.shape[:-1] + (ceil(cols/128),), any strides).  y is not rounded in between, and the quotient is taken in f32 (within 3*2^-24)."""
     @staticmethod
     def apply(epsilon, x, q, scale, gamma=None, residual=None, total=None, cfg=None, stream=None):
         _hint(cfg)

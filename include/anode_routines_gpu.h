@@ -552,8 +552,8 @@ int anode_gpu_rms_norm_add_bwd(
 /* The forward pass with its output in 8 bits, for a product that takes e4m3 operands:
  *   a = max |y| over the row (block = 0) or over each 128 columns of it (block = 128; the last may be shorter)
  *   scale = max(a, 2^-96)/448,  q = e4m3(y/scale)   (nearest, ties to even; |q| <= 448)
- * The scale is rounded to nearest; the quotient of a value is a product with the scale's reciprocal in f32, within 8*2^-24 of itself, so that what is as close as
- * that to the middle of two e4m3 values may become either.
+ * The scale is rounded to nearest; the quotient of a value is y*(448/a) in f32, both rounded to nearest, within 3*2^-24 of
+ * y/scale, so that what is as close as that to the middle of two e4m3 values may become either.
  * y itself is not rounded in between.  scale[row*scale_row_stride + group*scale_group_stride]; a scale is never 0, and a
  * group that holds a NaN has NaN for its scale and its values. */
 int anode_gpu_rms_norm_add_quant_fwd(

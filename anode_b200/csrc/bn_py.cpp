@@ -487,9 +487,10 @@ struct RowArgs {
   {
     rows = 1; stride = 0;
     bool first = true;
+    for (int64_t d = 0; d < lead; ++d)
+      if (t.size(d) == 0) { rows = 0; return true; }
     for (int64_t d = lead - 1; d >= 0; --d) {
       const int64_t n = t.size(d);
-      if (n == 0) { rows = 0; return true; }
       if (n == 1) continue;
       if (first) { stride = (U8)t.stride(d); first = false; }
       else if ((U8)t.stride(d) != stride * rows) return fail(i, "its rows do not lie at one distance");

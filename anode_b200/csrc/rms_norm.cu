@@ -8,12 +8,15 @@
 //
 // All of it is bound by memory where there are many rows (a handful of operations per element), and by the chain launch -> load -> sum -> store
 // where there are few.  Measured on one B200 against its copy bandwidth of 6539 GB/s, bf16 with residual, rows of 8192:
-//   forward            [16384,8192] 158 us (1.04 of it), without a residual 92 us (0.89); ragged rows of 4095 84 us (0.98); [1,4096] 1.6 us
-//   8 bits, per 128    [8192,8192] 76 us (0.95), ragged rows of 8191 106 us (0.68: a slot's two groups are chosen element by element)
-//   adjoint            [8192,4096] 46.5 us (0.88), [8192,16384] 162 us (1.01), ragged rows of 4095 55 us (0.74)
+//   forward            [16384,8192] 158 us (1.04 of it), without a residual 92 us (0.89); ragged rows of 4095 84 us (0.98); [1,4096] 1.7 us
+//   8 bits, per 128    [8192,8192] 77 us (0.93), ragged rows of 8191 107 us (0.67: a slot's two groups are chosen element by element)
+//   8 bits, per row    [8192,8192] 72.5 us (0.99)
+//   adjoint            [8192,4096] 46.5 us (0.88), [8192,16384] 160 us (1.02), ragged rows of 4095 56 us (0.73); f32 [4096,16384] 181 us (0.91),
+//                      [4096,16381] 279 us (0.59: 64 registers to a thread of a row of 4096 slots, and spills)
 // Three kernels: rms_norm_held_kernel (forward: a row per team of threads, many small blocks, whose loads and stores overlap one another's;
 // persistent teams with the next row on its way took 191 us for the first of these and 87.5 for the fourth), rms_norm_grad_kernel (persistent
-// teams, since dgamma's sums stay in registers), and the plain ones below for rows that are too wide or do not begin in step.
+// teams, since dgamma's sums stay in registers), and the plain ones below for rows that are too wide or do not begin in step: element by element, two
+// or three reads of each.  Those take 221 us forward for [8192,8192] out of step (0.37), 289 in 8 bits (0.25), 220 back for [8192,4096] (0.19).
 #include <cuda_fp8.h>
 
 #include "bn_host.h"

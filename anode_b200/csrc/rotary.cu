@@ -13,10 +13,10 @@
 // and with them the weights and the sums of the weights' gradients.
 // rotary_pairs_kernel: pairs anywhere.  Heads are copied as they lie, a lane has single pairs of them and puts the results in their place.
 //
-// What bounds it: memory, and the instructions of a pass over a warp's heads (161 of a warp with a norm, 121 without, some 300 backward, for
+// What bounds it: memory, and the instructions of a pass over a warp's heads (161 of a warp with a norm, 121 without, some 330 backward, for
 // 32 lanes' 16 elements each) and of a token's cosines and sines (some 550, which is why a warp has all of a token's heads).  On one B200, of
-// 6539 GB/s, bf16, 40 heads of 128: 16384 tokens forward 56.7 us with a norm (0.91) and 60 without (0.85); 8192 tokens backward 50.9 us with a
-// norm (0.76) and 29 without (0.88); 62 of 128 elements turned (pairs anywhere) 116 and 114 us; 32 tokens 2.7 us.
+// 6539 GB/s, bf16, 40 heads of 128: 16384 tokens forward 56.7 us with a norm (0.91) and 60 without (0.85); 8192 tokens backward 51.7 us with a
+// norm (0.74) and 29 without (0.88); 62 of 128 elements turned (pairs anywhere) 116 us either way; 32 tokens 2.7 us.
 #include "bn_host.h"
 #include "rows.cuh"
 

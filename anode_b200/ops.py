@@ -700,7 +700,9 @@ def _meets(levels, apart):
 
 def _share_memory(a, b):
     """Whether two arrays have a byte in common, at whatever strides they lie."""
-    if a.device != b.device or not a.numel() or not b.numel():
+    s, t = a.untyped_storage(), b.untyped_storage()
+    p, q = s.data_ptr(), t.data_ptr()
+    if p + s.nbytes() <= q or q + t.nbytes() <= p or a.device != b.device or not a.numel() or not b.numel():
         return False
     reach = {1: [a.element_size() - 1, b.element_size() - 1]}          # by stride in bytes: how far a and b go
     for k, t in enumerate((a, b)):

@@ -510,8 +510,8 @@ int anode_gpu_sync_batch_norm_add_act_bwd_3d1_packed_f32(
  * Conventions that differ from the above: the element type is an argument (ANODE_TYPE_*; f16 and bf16 beside f32), rows
  * and heads may lie apart (strides in elements; the innermost dimension is packed), and no rows or no tokens are a call
  * that does nothing (gradients of weights are then zero).  All arithmetic is in f32, angles in f64; every output is
- * rounded once.  An output may be an input's array (same pointer and strides), a query's not a
- * key's; other overlaps are not allowed.
+ * rounded once.  An output may be an input's array of its kind (rows for rows, heads for heads, a weight's gradient for the
+ * weight; same pointer and strides), a query's not a key's; other overlaps are not allowed.
  * Sizes: fewer than 2^36 rows of fewer than 2^31 columns, fewer than 2^31 tokens of at most 65535 heads; beyond them ANODE_E_DIMS.
  * Tensors are aligned to their elements; 16-byte aligned ones of such strides are faster.  Nothing synchronises, nothing
  * is allocated, and no state is kept in a workspace from call to call: it is written before it is read in every call, and

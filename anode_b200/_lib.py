@@ -109,6 +109,19 @@ SIGNATURES = {
     "anode_gpu_rotary_positions_fwd": (c_int, _R + [_H] * 4 + _T),
     "anode_gpu_rotary_positions_bwd_workspace_bytes": (size_t, [u32] * 5),
     "anode_gpu_rotary_positions_bwd": (c_int, _R + [_H] * 6 + [vp, vp, vp, size_t] + _T),
+    "anode_gpu_layer_norm_add_fwd":
+        (c_int, [c_int, u64, u32, f32, vp, u64, vp, u64, vp, vp, c_int, vp, u64, vp, u64, vp, vp] + _T),
+    "anode_gpu_layer_norm_add_bwd_workspace_bytes": (size_t, [u64, u32]),
+    "anode_gpu_layer_norm_add_bwd":
+        (c_int, [c_int, u64, u32, vp, u64, vp, u64, vp, vp, vp, c_int, vp, u64, vp, u64, vp, vp, vp, size_t] + _T),
+    "anode_gpu_embed_tokens_fwd": (c_int, [c_int, u64, u32, u32, f32, vp, c_int, vp, u64, vp, u64] + _T),
+    "anode_gpu_embed_tokens_bwd_workspace_bytes": (size_t, [u64, u32, u32]),
+    "anode_gpu_embed_tokens_bwd":
+        (c_int, [c_int, u64, u32, u32, f32, vp, c_int, vp, u64, vp, u64, c_int, c_int, vp, size_t] + _T),
+    "anode_gpu_token_log_probs_fwd":
+        (c_int, [c_int, u64, u32, f32, vp, u64, vp, c_int, vp, vp, vp, u32, vp, vp, c_int] + _T),
+    "anode_gpu_token_log_probs_bwd":
+        (c_int, [c_int, u64, u32, f32, vp, u64, vp, c_int, vp, vp, vp, vp, vp, u64] + _T),
     "anode_gpu_batch_norm_fused_plan": (c_int, _D + [c_int, u32, u32, u32, ctypes.POINTER(u32), u32]),
     "anode_gpu_batch_norm_fused_plan_walk":
         (c_int, _D + [c_int, u32, u32, u32, u32, u32, ctypes.POINTER(ctypes.c_uint64)]),
@@ -197,6 +210,7 @@ ERRORS = {
     -7: "ANODE_E_TOO_LARGE: the problem needs more scratch than the library's built-in array holds",
     -8: "ANODE_E_TYPE: an element type that the call does not take",
     -9: "ANODE_E_STRIDE: strides that overlap in an output, or an output in a place that it may not have",
+    -10: "ANODE_E_VALUE: a number that the call does not take",
 }
 
 

@@ -38,7 +38,8 @@ struct KernelConfig { uint32_t block_sz, max_block_ct; };
 
 // addresses of the C ABI, in the order of kNames
 enum { F_FWD, F_FWD_ACT, F_FWD_ADD, F_BWD, F_BWD_ACT, F_BWD_ADD, F_INFER, F_NORMALIZE, F_ADJOINT,
-       F_RMS_FWD, F_RMS_BWD, F_RMS_BWD_BYTES, F_RMS_QUANT, F_ROTARY_FWD, F_ROTARY_BWD, F_ROTARY_BWD_BYTES, F_COUNT };
+       F_RMS_FWD, F_RMS_BWD, F_RMS_BWD_BYTES, F_RMS_QUANT, F_ROTARY_FWD, F_ROTARY_BWD, F_ROTARY_BWD_BYTES,
+       F_LAYER_FWD, F_LAYER_BWD, F_LAYER_BWD_BYTES, F_EMBED_FWD, F_EMBED_BWD, F_EMBED_BWD_BYTES, F_PROBS_FWD, F_PROBS_BWD, F_COUNT };
 const char *const kNames[F_COUNT] = {
     "anode_gpu_batch_norm_relu_fused_fwd_3d1_packed_f32", "anode_gpu_batch_norm_act_fused_fwd_3d1_packed_f32",
     "anode_gpu_batch_norm_add_act_fused_fwd_3d1_packed_f32", "anode_gpu_batch_norm_relu_fused_bwd_3d1_packed_f32",
@@ -46,7 +47,10 @@ const char *const kNames[F_COUNT] = {
     "anode_gpu_batch_norm_act_infer_3d1_packed_f32", "anode_gpu_batch_normalize_3d1_packed_f32",
     "anode_gpu_batch_normalize_adjoint_3d1_packed_f32", "anode_gpu_rms_norm_add_fwd", "anode_gpu_rms_norm_add_bwd",
     "anode_gpu_rms_norm_add_bwd_workspace_bytes", "anode_gpu_rms_norm_add_quant_fwd", "anode_gpu_rotary_positions_fwd",
-    "anode_gpu_rotary_positions_bwd", "anode_gpu_rotary_positions_bwd_workspace_bytes"};
+    "anode_gpu_rotary_positions_bwd", "anode_gpu_rotary_positions_bwd_workspace_bytes", "anode_gpu_layer_norm_add_fwd",
+    "anode_gpu_layer_norm_add_bwd", "anode_gpu_layer_norm_add_bwd_workspace_bytes", "anode_gpu_embed_tokens_fwd",
+    "anode_gpu_embed_tokens_bwd", "anode_gpu_embed_tokens_bwd_workspace_bytes", "anode_gpu_token_log_probs_fwd",
+    "anode_gpu_token_log_probs_bwd"};
 void *g_fn[F_COUNT] = {};
 
 typedef const float *In;
@@ -441,6 +445,13 @@ typedef int (*RotaryFwdFn)(int, uint32_t, uint32_t, uint32_t, uint32_t, int, flo
 typedef int (*RotaryBwdFn)(int, uint32_t, uint32_t, uint32_t, uint32_t, int, float, const double *, CV, int, U8, U8, int, float, CV, CV, int, H, H, H, H, H, H,
                            P, P, P, size_t, K, P);
 typedef size_t (*RotaryBytesFn)(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t);
+typedef int (*LayerFwdFn)(int, U8, uint32_t, float, CV, U8, CV, U8, CV, CV, int, P, U8, P, U8, float *, float *, K, P);
+typedef int (*LayerBwdFn)(int, U8, uint32_t, CV, U8, CV, U8, const float *, const float *, CV, int, CV, U8, P, U8, P, P, P, size_t, K, P);
+typedef int (*EmbedFwdFn)(int, U8, uint32_t, uint32_t, float, CV, int, CV, U8, P, U8, K, P);
+typedef size_t (*EmbedBytesFn)(U8, uint32_t, uint32_t);
+typedef int (*EmbedBwdFn)(int, U8, uint32_t, uint32_t, float, CV, int, CV, U8, P, U8, int, int, P, size_t, K, P);
+typedef int (*ProbsFwdFn)(int, U8, uint32_t, float, CV, U8, CV, int, float *, float *, float *, uint32_t, float *, P, int, K, P);
+typedef int (*ProbsBwdFn)(int, U8, uint32_t, float, CV, U8, CV, int, const float *, const float *, const float *, const float *, P, U8, K, P);
 
 int type_code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kHalf ? 1 : t == at::kBFloat16 ? 2 : -1; }
 
@@ -532,6 +543,16 @@ struct RowArgs {
     const at::Tensor *t = tensor(i, null_ok);
     if (!t) return nullptr;
     if (t->scalar_type() != as || t->numel() != n || !t->is_contiguous()) { fail(i, what); return nullptr; }
+    return data(i, *t);
+  }
+  // a packed array of n whole numbers of 4 or 8 bytes; n < 0: of any number, which it is set to
+  void *whole(int i, int64_t &n, const char *what, int &bytes, bool null_ok)
+  {
+    const at::Tensor *t = tensor(i, null_ok);
+    if (!t) return nullptr;
+    bytes = t->scalar_type() == at::kLong ? 8 : t->scalar_type() == at::kInt ? 4 : 0;
+    if (n < 0) n = t->numel();
+    if (!bytes || t->numel() != n || !t->is_contiguous()) { fail(i, what); return nullptr; }
     return data(i, *t);
   }
   double f(int i)
@@ -854,6 +875,258 @@ PyObject *py_rotary_bwd(PyObject *, PyObject *const *v, Py_ssize_t n)
   END_GUARDED
 }
 
+// layer_fwd(epsilon, x, y, gamma, beta, residual, total, mean, inv_std, stream)
+PyObject *py_layer_fwd(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  GUARDED
+  if (!want_args(n, 10)) return nullptr;
+  static const char *const names[] = {"epsilon", "x", "y", "gamma", "beta", "residual", "total", "mean", "inv_std", "stream"};
+  RowArgs a{v, names};
+  U8 rows = 0, sx, sy, sr, st;
+  uint32_t cols = 0;
+  const double eps = a.f(0);
+  CV x = a.rows(1, nullptr, sx);
+  if (!a.ok) return nullptr;
+  const at::Tensor &like = THPVariable_Unpack(v[1]);
+  const int type = a.type(1, like);
+  int wt = -1;
+  if (!a.ok || !cols_of(a, 1, like, rows, cols)) return nullptr;
+  P y = a.rows(2, &like, sy);
+  CV g = a.weights(3, cols, wt), b = a.weights(4, cols, wt), r = a.rows(5, &like, sr, true);
+  P t = a.rows(6, &like, st, true);
+  if (a.ok && a.given(6) && !a.given(5)) a.fail(6, "is the sum with a residual: without one it would be a copy of x");
+  float *stats[2];
+  for (int i = 0; i < 2; ++i) stats[i] = (float *)a.packed(7 + i, at::kFloat, (int64_t)rows, "expected a packed float32 array, one value per row", true);
+  void *s = a.stream(9);
+  if (!a.ok || !bound(F_LAYER_FWD)) return nullptr;
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)a.device));
+  int rc;
+  {
+    Unlocked unlocked;
+    rc = ((LayerFwdFn)g_fn[F_LAYER_FWD])(type, rows, cols, (float)eps, x, sx, r, sr, g, b, wt, y, sy, t, st, stats[0], stats[1], &kDefaultCfg, s);
+  }
+  return PyLong_FromLong(rc);
+  END_GUARDED
+}
+
+// layer_bwd(dy, total, mean, inv_std, dx, gamma, dtotal, dgamma, dbeta, accumulate, workspace, stream)
+PyObject *py_layer_bwd(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  GUARDED
+  if (!want_args(n, 12)) return nullptr;
+  static const char *const names[] = {"dy", "total", "mean", "inv_std", "dx", "gamma", "dtotal", "dgamma", "dbeta", "cap", "workspace", "stream"};
+  RowArgs a{v, names};
+  U8 rows = 0, sy, st, sx, sd;
+  uint32_t cols = 0;
+  CV dy = a.rows(0, nullptr, sy);
+  if (!a.ok) return nullptr;
+  const at::Tensor &like = THPVariable_Unpack(v[0]);
+  const int type = a.type(0, like);
+  int wt = -1;
+  if (!a.ok || !cols_of(a, 0, like, rows, cols)) return nullptr;
+  CV t = a.rows(1, &like, st);
+  const float *stats[2];
+  for (int i = 0; i < 2; ++i) stats[i] = (const float *)a.packed(2 + i, at::kFloat, (int64_t)rows, "expected a packed float32 array, one value per row", false);
+  P dx = a.rows(4, &like, sx);
+  CV g = a.weights(5, cols, wt), dt = a.rows(6, &like, sd, true);
+  P dg = a.weights(7, cols, wt), db = a.weights(8, cols, wt);
+  if (a.truth(9)) {
+    if (a.ok && a.given(6)) a.fail(9, "Accumulate adds into dx, which takes the place of dtotal: give one of them");
+    dt = dx; sd = sx;
+  }
+  void *s = a.stream(11);
+  if (!a.ok || !bound(F_LAYER_BWD) || !bound(F_LAYER_BWD_BYTES)) return nullptr;
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)a.device));
+  size_t bytes = dg || db ? ((RmsBytesFn)g_fn[F_LAYER_BWD_BYTES])(rows, cols) : 0;
+  at::Tensor own;
+  void *ws = a.workspace(10, 11, s, bytes, own);
+  if (!a.ok) return nullptr;
+  int rc;
+  {
+    Unlocked unlocked;
+    rc = ((LayerBwdFn)g_fn[F_LAYER_BWD])(type, rows, cols, dy, sy, t, st, stats[0], stats[1], g, wt, dt, sd, dx, sx, dg, db, ws, bytes, &kDefaultCfg, s);
+  }
+  return PyLong_FromLong(rc);
+  END_GUARDED
+}
+
+// The arguments that both directions of the table by tokens have: the tokens, the table or its gradient, and a row for each token
+struct EmbedArgs {
+  RowArgs &a;
+  int64_t tokens = -1;
+  int token_bytes = 0;
+  uint32_t vocab = 0, cols = 0;
+  CV token = nullptr;
+  P table = nullptr, rows = nullptr;
+  U8 table_stride = 0, rows_stride = 0;
+  const at::Tensor *table_like = nullptr, *rows_like = nullptr;
+
+  bool take(int at_token, int at_table, int at_rows)
+  {
+    token = a.whole(at_token, tokens, "expected a packed int32 or int64 array", token_bytes, false);
+    table = a.rows(at_table, nullptr, table_stride);
+    rows = a.rows(at_rows, nullptr, rows_stride);
+    if (!a.ok) return false;
+    const at::Tensor &t = THPVariable_Unpack(a.v[at_token]);
+    table_like = &THPVariable_Unpack(a.v[at_table]);
+    rows_like = &THPVariable_Unpack(a.v[at_rows]);
+    if (table_like->dim() != 2) return a.fail(at_table, "expected an array [vocab, cols]");
+    if (table_like->size(0) > 0x7fffffffll || table_like->size(1) > 0x7fffffffll) return a.fail(at_table, "too many rows or columns");
+    vocab = (uint32_t)table_like->size(0); cols = (uint32_t)table_like->size(1);
+    bool fits = rows_like->dim() == t.dim() + 1 && rows_like->size(t.dim()) == (int64_t)cols;
+    for (int64_t d = 0; fits && d < t.dim(); ++d) fits = rows_like->size(d) == t.size(d);
+    return fits || a.fail(at_rows, "expected a row of the table's columns for each token");
+  }
+};
+
+// embed_fwd(tokens, table, y, scale, stream)
+PyObject *py_embed_fwd(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  GUARDED
+  if (!want_args(n, 5)) return nullptr;
+  static const char *const names[] = {"tokens", "table", "y", "scale", "stream"};
+  RowArgs a{v, names};
+  EmbedArgs e{a};
+  if (!e.take(0, 1, 2)) return nullptr;
+  const int type = a.type(1, *e.table_like);
+  if (a.ok && e.rows_like->scalar_type() != e.table_like->scalar_type()) a.fail(2, "has another type than the table");
+  const double scale = a.f(3);
+  void *s = a.stream(4);
+  if (!a.ok || !bound(F_EMBED_FWD)) return nullptr;
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)a.device));
+  int rc;
+  {
+    Unlocked unlocked;
+    rc = ((EmbedFwdFn)g_fn[F_EMBED_FWD])(type, (U8)e.tokens, e.vocab, e.cols, (float)scale, e.token, e.token_bytes, e.table, e.table_stride, e.rows,
+                                         e.rows_stride, &kDefaultCfg, s);
+  }
+  return PyLong_FromLong(rc);
+  END_GUARDED
+}
+
+// embed_bwd(tokens, dy, dtable, scale, accumulate, workspace, stream)
+PyObject *py_embed_bwd(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  GUARDED
+  if (!want_args(n, 7)) return nullptr;
+  static const char *const names[] = {"tokens", "dy", "dtable", "scale", "cap", "workspace", "stream"};
+  RowArgs a{v, names};
+  EmbedArgs e{a};
+  if (!e.take(0, 2, 1)) return nullptr;
+  const int type = a.type(1, *e.rows_like), dtable_type = a.type(2, *e.table_like);
+  if (a.ok && dtable_type != type && dtable_type != 0) a.fail(2, "expected dy's type or float32");
+  const double scale = a.f(3);
+  const int accumulate = a.truth(4);
+  void *s = a.stream(6);
+  if (!a.ok || !bound(F_EMBED_BWD) || !bound(F_EMBED_BWD_BYTES)) return nullptr;
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)a.device));
+  size_t bytes = e.tokens ? ((EmbedBytesFn)g_fn[F_EMBED_BWD_BYTES])((U8)e.tokens, e.vocab, e.cols) : 0;
+  at::Tensor own;
+  void *ws = a.workspace(5, 6, s, bytes, own);
+  if (!a.ok) return nullptr;
+  int rc;
+  {
+    Unlocked unlocked;
+    rc = ((EmbedBwdFn)g_fn[F_EMBED_BWD])(type, (U8)e.tokens, e.vocab, e.cols, (float)scale, e.token, e.token_bytes, e.rows, e.rows_stride, e.table,
+                                         e.table_stride, dtable_type, accumulate, ws, bytes, &kDefaultCfg, s);
+  }
+  return PyLong_FromLong(rc);
+  END_GUARDED
+}
+
+// probs_fwd(logits, tokens, logprob, entropy, stats, top_logprob, top_token, scale, stream)
+PyObject *py_probs_fwd(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  GUARDED
+  if (!want_args(n, 9)) return nullptr;
+  static const char *const names[] = {"logits", "tokens", "logprob", "entropy", "stats", "top_logprob", "top_token", "scale", "stream"};
+  RowArgs a{v, names};
+  U8 rows = 0, sx;
+  uint32_t vocab = 0;
+  CV x = a.rows(0, nullptr, sx);
+  if (!a.ok) return nullptr;
+  const at::Tensor &like = THPVariable_Unpack(v[0]);
+  const int type = a.type(0, like);
+  if (!a.ok || !cols_of(a, 0, like, rows, vocab)) return nullptr;
+  int64_t count = (int64_t)rows;
+  int token_bytes = 0, top_bytes = 0;
+  static const char *const each = "expected a packed float32 array, one value per row";
+  CV token = a.whole(1, count, "expected a packed int32 or int64 array, one token per row", token_bytes, true);
+  float *logprob = (float *)a.packed(2, at::kFloat, count, each, true), *entropy = (float *)a.packed(3, at::kFloat, count, each, true);
+  if (a.ok && a.given(2) && !a.given(1)) a.fail(1, "expected the tokens whose log probabilities are asked for");
+  float *stats = (float *)a.packed(4, at::kFloat, 2 * count, "expected a packed float32 array, two values per row", true);
+  // [*, top] beside logits of [*, vocab]
+  int64_t top = 0;
+  float *top_logprob = nullptr;
+  P top_token = nullptr;
+  for (int i = 5; i < 7 && a.ok; ++i) {
+    const at::Tensor *t = a.tensor(i, true);
+    if (!t) continue;
+    bool fits = t->dim() == like.dim() && t->is_contiguous() && (i == 5 ? t->scalar_type() == at::kFloat : t->scalar_type() == at::kLong || t->scalar_type() == at::kInt);
+    for (int64_t d = 0; fits && d + 1 < like.dim(); ++d) fits = t->size(d) == like.size(d);
+    const int64_t k = fits ? t->size(like.dim() - 1) : 0;
+    if (!fits || (i == 6 && a.given(5) && k != top)) {
+      a.fail(i, i == 5 ? "expected a packed float32 array [*, top]" : "expected a packed int32 or int64 array [*, top], of top_logprob's sizes where both are given");
+      break;
+    }
+    if (k > (int64_t)vocab || k > 128) { a.fail(i, "more alternatives than a row has logits, or more than 128"); break; }
+    top = k;
+    if (i == 5) top_logprob = (float *)a.data(i, *t);
+    else { top_token = a.data(i, *t); top_bytes = t->scalar_type() == at::kLong ? 8 : 4; }
+  }
+  const double scale = a.f(7);
+  void *s = a.stream(8);
+  if (!a.ok || !bound(F_PROBS_FWD)) return nullptr;
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)a.device));
+  int rc;
+  {
+    Unlocked unlocked;
+    rc = ((ProbsFwdFn)g_fn[F_PROBS_FWD])(type, rows, vocab, (float)scale, x, sx, token, token_bytes, logprob, entropy, stats, (uint32_t)top, top_logprob,
+                                         top_token, top_bytes, &kDefaultCfg, s);
+  }
+  return PyLong_FromLong(rc);
+  END_GUARDED
+}
+
+// probs_bwd(logits, tokens, stats, dlogprob, dlogits, entropy, dentropy, scale, stream)
+PyObject *py_probs_bwd(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+  GUARDED
+  if (!want_args(n, 9)) return nullptr;
+  static const char *const names[] = {"logits", "tokens", "stats", "dlogprob", "dlogits", "entropy", "dentropy", "scale", "stream"};
+  RowArgs a{v, names};
+  U8 rows = 0, sx, sd;
+  uint32_t vocab = 0;
+  CV x = a.rows(0, nullptr, sx);
+  if (!a.ok) return nullptr;
+  const at::Tensor &like = THPVariable_Unpack(v[0]);
+  const int type = a.type(0, like);
+  if (!a.ok || !cols_of(a, 0, like, rows, vocab)) return nullptr;
+  int64_t count = (int64_t)rows;
+  int token_bytes = 0;
+  static const char *const each = "expected a packed float32 array, one value per row";
+  CV token = a.whole(1, count, "expected a packed int32 or int64 array, one token per row", token_bytes, true);
+  const float *stats = (const float *)a.packed(2, at::kFloat, 2 * count, "expected a packed float32 array, two values per row", false);
+  const float *dlogprob = (const float *)a.packed(3, at::kFloat, count, each, true);
+  P dlogits = a.rows(4, &like, sd);
+  const float *entropy = (const float *)a.packed(5, at::kFloat, count, each, true), *dentropy = (const float *)a.packed(6, at::kFloat, count, each, true);
+  if (a.ok && a.given(3) && !a.given(1)) a.fail(1, "expected the tokens of dlogprob");
+  if (a.ok && a.given(6) && !a.given(5)) a.fail(5, "expected the entropies that the forward pass stored");
+  if (a.ok && !a.given(3) && !a.given(6)) a.fail(3, "expected dlogprob, dentropy or both");
+  const double scale = a.f(7);
+  void *s = a.stream(8);
+  if (!a.ok || !bound(F_PROBS_BWD)) return nullptr;
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)a.device));
+  int rc;
+  {
+    Unlocked unlocked;
+    rc = ((ProbsBwdFn)g_fn[F_PROBS_BWD])(type, rows, vocab, (float)scale, x, sx, token, token_bytes, stats, entropy, dlogprob, dentropy, dlogits, sd,
+                                         &kDefaultCfg, s);
+  }
+  return PyLong_FromLong(rc);
+  END_GUARDED
+}
+
 // bind({name: address}): the C ABI's functions
 PyObject *py_bind(PyObject *, PyObject *const *v, Py_ssize_t n)
 {
@@ -884,6 +1157,12 @@ PyMethodDef kMethods[] = {
     {"rms_quant", (PyCFunction)(void *)py_rms_quant, METH_FASTCALL, nullptr},
     {"rotary_fwd", (PyCFunction)(void *)py_rotary_fwd, METH_FASTCALL, nullptr},
     {"rotary_bwd", (PyCFunction)(void *)py_rotary_bwd, METH_FASTCALL, nullptr},
+    {"layer_fwd", (PyCFunction)(void *)py_layer_fwd, METH_FASTCALL, nullptr},
+    {"layer_bwd", (PyCFunction)(void *)py_layer_bwd, METH_FASTCALL, nullptr},
+    {"embed_fwd", (PyCFunction)(void *)py_embed_fwd, METH_FASTCALL, nullptr},
+    {"embed_bwd", (PyCFunction)(void *)py_embed_bwd, METH_FASTCALL, nullptr},
+    {"probs_fwd", (PyCFunction)(void *)py_probs_fwd, METH_FASTCALL, nullptr},
+    {"probs_bwd", (PyCFunction)(void *)py_probs_bwd, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", "Fast paths of anode_b200.ops into the C ABI.", -1, kMethods};
 

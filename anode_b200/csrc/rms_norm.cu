@@ -615,32 +615,6 @@ template <typename T> __global__ void __launch_bounds__(kThreads) rms_norm_dx_ke
 }
 
 inline uint32_t parts_of(uint64_t rows) { return (uint32_t)(rows < kMostParts ? (rows ? rows : 1) : kMostParts); }
-inline uint32_t row_blocks(uint64_t rows) { return (uint32_t)(rows < (1u << 30) ? rows : (1u << 30)); }
-
-// Columns are counted in 32 bits, up to a block's threads beyond the last one
-inline bool served(uint64_t rows, uint32_t cols) { return cols != 0 && !(cols >> 31) && !(rows >> 36); }
-
-// An array of rows: a pointer of the type's alignment; an output's rows do not overlap
-inline int check_rows(const void *p, size_t bytes, uint64_t rows, uint32_t cols, uint64_t stride, bool output)
-{
-  if (!p) return ANODE_E_NULL;
-  if (!aligned_to(p, bytes)) return ANODE_E_ALIGN;
-  if (output && rows > 1 && stride < cols) return ANODE_E_STRIDE;
-  return ANODE_OK;
-}
-// An output in an input's place has its strides
-inline bool apart(const void *out, uint64_t out_stride, const void *in, uint64_t in_stride, uint64_t rows)
-{
-  return out != in || out_stride == in_stride || rows <= 1;
-}
-
-#define TRY(call) do { const int rc_ = (call); if (rc_) return rc_; } while (0)
-
-// Whether an array's rows all begin at the same place of a slot of `v` elements as those of the first one
-inline bool in_step(const void *p, size_t bytes, uint64_t stride, uint32_t v, const void *p0, size_t bytes0, uint64_t stride0, uint64_t rows)
-{
-  return !p || ((uintptr_t)p / bytes % v == (uintptr_t)p0 / bytes0 % v && (rows <= 1 || stride % v == stride0 % v));
-}
 
 // How the rows of a call are held in registers; false where they are not
 bool held_plan(const NormArgs &a, int type, bool quant, Held &h, bool &shift)

@@ -699,8 +699,6 @@ inline bool same_place(const AnodeHeads *o, const AnodeHeads *i, uint32_t batch,
   return (batch < 2 || o->batch_stride == i->batch_stride) && (seq < 2 || o->seq_stride == i->seq_stride) && (o->heads < 2 || o->head_stride == i->head_stride);
 }
 
-#define TRY(call) do { const int rc_ = (call); if (rc_) return rc_; } while (0)
-
 // V = 1: pairs anywhere
 template <typename T, int V, int IT, bool NORM, bool BWD>
 int launch_rotary(const RotaryArgs &a, uint32_t blocks, size_t tables, size_t sums, cudaStream_t stream)

@@ -671,6 +671,88 @@ def rotary_workspace_bytes(batch, seq, q_heads, k_heads, dim):
     return int(_lib.load().anode_gpu_rotary_positions_bwd_workspace_bytes(batch, seq, q_heads, k_heads, dim))
 
 
+class LayerNormalizeAddOp:
+    """Layer norm over rows with the residual's addition in one launch: total = round(x + residual), y = (total - mu)*r*gamma + beta with
+    mu = mean(total), r = (mean((total - mu)^2) + epsilon)^-1/2 over the last dimension.  Arrays as RmsNormalizeAddOp's; gamma and beta are of one
+    type.  mean, inv_std: float32, one value per row, for the adjoint.  y may be x or residual, total may be either, too, but not y's array."""
+    @staticmethod
+    def apply(epsilon, x, y, gamma=None, beta=None, residual=None, total=None, mean=None, inv_std=None, cfg=None, stream=None):
+        _hint(cfg)
+        rc = native().layer_fwd(epsilon, x, y, gamma, beta, residual, total, mean, inv_std, stream)
+        if rc:
+            check(rc, "anode_gpu_layer_norm_add_fwd")
+        return y
+
+    @staticmethod
+    def adjoint(dy, total, mean, inv_std, dx, gamma=None, dtotal=None, dgamma=None, dbeta=None, cap=WriteCap.Assign, workspace=None, cfg=None, stream=None):
+        """dx = r*(g - mean(g) - xh*mean(g*xh)) + dtotal with g = dy*gamma, xh = (total - mu)*r: the gradient of x and of the residual alike;
+        dgamma = sum over rows of dy*xh, dbeta = sum over rows of dy, in the weights' type.  dtotal, dx, Accumulate and the workspace (of
+        layer_norm_workspace_bytes, needed for dgamma and dbeta only) as in RmsNormalizeAddOp.adjoint."""
+        _hint(cfg)
+        rc = native().layer_bwd(dy, total, mean, inv_std, dx, gamma, dtotal, dgamma, dbeta, cap is WriteCap.Accumulate, workspace, stream)
+        if rc:
+            check(rc, "anode_gpu_layer_norm_add_bwd")
+        return dx
+
+
+def layer_norm_workspace_bytes(rows, cols):
+    """Bytes that LayerNormalizeAddOp.adjoint needs for dgamma and dbeta (see rms_norm_workspace_bytes)."""
+    return int(_lib.load().anode_gpu_layer_norm_add_bwd_workspace_bytes(rows, cols))
+
+
+class EmbedTokensOp:
+    """Rows of a table by tokens: y[i] = scale*table[tokens[i]].  tokens: int32 or int64, packed, of any sizes [*]; table: [vocab, cols], y: [*, cols] of its
+    type, rows at one distance each.  A token outside of [0, vocab) stands for none: its row is zeros, and it has no gradient."""
+    @staticmethod
+    def apply(tokens, table, y, scale=1.0, cfg=None, stream=None):
+        _hint(cfg)
+        rc = native().embed_fwd(tokens, table, y, scale, stream)
+        if rc:
+            check(rc, "anode_gpu_embed_tokens_fwd")
+        return y
+
+    @staticmethod
+    def adjoint(tokens, dy, dtable, scale=1.0, cap=WriteCap.Assign, workspace=None, cfg=None, stream=None):
+        """dtable[v] = scale * sum of dy[i] over tokens[i] = v, every row of it (zeros where no token names it); Accumulate adds that to the rows that
+        tokens name and leaves the others alone.  dtable has dy's type or is float32; sums are float32, in an order that follows from the tokens: the same
+        call gives the same bits.  workspace: a tensor of embed_workspace_bytes; None has one made on the call's stream."""
+        _hint(cfg)
+        rc = native().embed_bwd(tokens, dy, dtable, scale, cap is WriteCap.Accumulate, workspace, stream)
+        if rc:
+            check(rc, "anode_gpu_embed_tokens_bwd")
+        return dtable
+
+
+def embed_workspace_bytes(tokens, vocab, cols):
+    """Bytes that EmbedTokensOp.adjoint needs (see rms_norm_workspace_bytes)."""
+    return int(_lib.load().anode_gpu_embed_tokens_bwd_workspace_bytes(tokens, vocab, cols))
+
+
+class TokenLogProbsOp:
+    """Log probabilities over rows of logits [*, vocab], at a temperature of 1/scale, in one launch and one pass: with m = max x, z = scale*(x - m),
+    L = log(sum(exp(z))), logprob = z[token] - L of the given tokens (int32 or int64, one per row; one outside of [0, vocab) stands for none and has 0),
+    entropy = L - sum(z*exp(z))/sum(exp(z)), and the up to 128 likeliest tokens with their log probabilities, [*, top], the largest logit first, of equal ones
+    the lowest index.  stats: float32, two values per row, (m, L), for the adjoint.  What is None is not computed.
+    A logit of -infinity has probability 0; a row of nothing else has log probabilities of -infinity and entropy 0; one that holds a NaN or +infinity, NaN."""
+    @staticmethod
+    def apply(logits, tokens, logprob, entropy=None, stats=None, top_logprob=None, top_token=None, scale=1.0, cfg=None, stream=None):
+        _hint(cfg)
+        rc = native().probs_fwd(logits, tokens, logprob, entropy, stats, top_logprob, top_token, scale, stream)
+        if rc:
+            check(rc, "anode_gpu_token_log_probs_fwd")
+        return logprob
+
+    @staticmethod
+    def adjoint(logits, tokens, stats, dlogprob, dlogits, entropy=None, dentropy=None, scale=1.0, cfg=None, stream=None):
+        """dlogits = scale*(dlogprob*([token] - p) - dentropy*p*(z - L + entropy)), p = exp(z - L), from the forward pass's logits, tokens and scale, and the
+        stats and entropies that it stored.  dlogprob or dentropy may be None; a row without a token has no part of dlogprob.  dlogits may be logits."""
+        _hint(cfg)
+        rc = native().probs_bwd(logits, tokens, stats, dlogprob, dlogits, entropy, dentropy, scale, stream)
+        if rc:
+            check(rc, "anode_gpu_token_log_probs_bwd")
+        return dlogits
+
+
 def rotary_frequencies(rot, base=10000.0, factor=1.0, context=None, slow=1.0, fast=4.0, device="cuda"):
     """Angles per position, base^(-2i/rot) for i < rot/2, as float64.  For a context stretched by `factor`: all of them divided by it
     (context None), or, where `context` is the length that the model was trained at, those that turn fewer than `slow`
@@ -808,6 +890,107 @@ class RotaryPositions:
         dk = dk if dk is not None or not two else torch.empty_like(dk_out)
         return RotaryPositionsOp.adjoint(positions, self.freq, dq_out, dk_out, dq, dk, self.interleaved, self.amplitude, self.epsilon, q, k, self.gamma_q,
                                          self.gamma_k if two else None, self.dgamma_q, self.dgamma_k if two else None)
+
+
+class LayerNormAdd:
+    """A layer-norm layer with the residual's addition that keeps its weights and what its backward pass needs, as RmsNormAdd does."""
+
+    def __init__(self, cols, epsilon=1e-5, affine=True, bias=True, dtype=torch.float32, device="cuda"):
+        self.epsilon = float(epsilon)
+        self.gamma = torch.ones(cols, device=device, dtype=dtype) if affine else None
+        self.dgamma = torch.zeros(cols, device=device, dtype=dtype) if affine else None
+        self.beta, self.dbeta = (torch.zeros(cols, device=device, dtype=dtype) if affine and bias else None for _ in range(2))
+        self._saved = None
+
+    def infer(self, x, residual=None, out=None, total=None):
+        """(y, total): the norm of the sum, and the sum, which is x itself without a residual (with out=x, then, y's array: the sum is gone)."""
+        y = out if out is not None else torch.empty_like(x)
+        if residual is not None and total is None:
+            total = torch.empty_like(x)
+        LayerNormalizeAddOp.apply(self.epsilon, x, y, self.gamma, self.beta, residual, total)
+        return y, x if residual is None else total
+
+    def forward(self, x, residual=None, out=None, total=None):
+        """infer, keeping the sum, its mean and 1/std for the backward pass.  The sum (x without a residual) has to stay as it is until then."""
+        _refuse_overwriting((x if residual is None else total,), out)
+        y = out if out is not None else torch.empty_like(x)
+        if residual is not None and total is None:
+            total = torch.empty_like(x)
+        mean, inv_std = (torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32) for _ in range(2))
+        LayerNormalizeAddOp.apply(self.epsilon, x, y, self.gamma, self.beta, residual, total, mean, inv_std)
+        total = x if residual is None else total
+        self._saved = total, mean, inv_std
+        return y, total
+
+    def backward(self, dy, dtotal=None, out=None):
+        """The gradient of x, which is the residual's, too; those of gamma and beta are left in dgamma and dbeta."""
+        if self._saved is None:
+            raise RuntimeError("backward before forward")
+        total, mean, inv_std = self._saved
+        dx = out if out is not None else torch.empty_like(dy)
+        return LayerNormalizeAddOp.adjoint(dy, total, mean, inv_std, dx, self.gamma, dtotal, self.dgamma, self.dbeta)
+
+
+class TokenEmbedding:
+    """A table of rows by tokens as a layer that keeps it, its gradient (of its type, or float32) and the tokens of its forward pass."""
+
+    def __init__(self, vocab, cols, scale=1.0, dtype=torch.float32, grad_dtype=None, device="cuda"):
+        self.scale = float(scale)
+        self.table = torch.zeros(vocab, cols, device=device, dtype=dtype)
+        self.dtable = torch.zeros(vocab, cols, device=device, dtype=grad_dtype or dtype)
+        self._tokens = None
+
+    def infer(self, tokens, out=None):
+        y = out if out is not None else torch.empty(tokens.shape + self.table.shape[1:], device=self.table.device, dtype=self.table.dtype)
+        return EmbedTokensOp.apply(tokens, self.table, y, self.scale)
+
+    def forward(self, tokens, out=None):
+        """infer, keeping the tokens for the backward pass: they have to stay as they are until then."""
+        y = self.infer(tokens, out)
+        self._tokens = tokens
+        return y
+
+    def backward(self, dy, cap=WriteCap.Assign):
+        """The table's gradient, in dtable; Accumulate adds to what is there."""
+        if self._tokens is None:
+            raise RuntimeError("backward before forward")
+        return EmbedTokensOp.adjoint(self._tokens, dy, self.dtable, self.scale, cap)
+
+
+class TokenLogProbs:
+    """Log probabilities of tokens at a temperature of 1/scale, as a layer that keeps what its backward pass needs."""
+
+    def __init__(self, scale=1.0):
+        self.scale = float(scale)
+        self._saved = None
+
+    def infer(self, logits, tokens=None, top=0, entropy=False):
+        """(logprob, entropy, top_logprob, top_token), None for what is not asked for; the likeliest tokens are int64."""
+        rows = logits.shape[:-1]
+
+        def each(*more, dtype=torch.float32):
+            return torch.empty(rows + more, device=logits.device, dtype=dtype)
+        logprob, h = each() if tokens is not None else None, each() if entropy else None
+        best = (each(top), each(top, dtype=torch.int64)) if top else (None, None)
+        TokenLogProbsOp.apply(logits, tokens, logprob, h, None, *best, self.scale)
+        return logprob, h, *best
+
+    def forward(self, logits, tokens, entropy=True):
+        """(logprob, entropy); logits and tokens have to stay as they are until the backward pass.  Without the entropies there is no gradient of them."""
+        rows = logits.shape[:-1]
+        logprob, h = (torch.empty(rows, device=logits.device, dtype=torch.float32) if want else None for want in (True, entropy))
+        stats = torch.empty(rows + (2,), device=logits.device, dtype=torch.float32)
+        TokenLogProbsOp.apply(logits, tokens, logprob, h, stats, None, None, self.scale)
+        self._saved = logits, tokens, stats, h
+        return logprob, h
+
+    def backward(self, dlogprob, dentropy=None, out=None):
+        """The gradient of the logits, in whose place it may be (out=logits)."""
+        if self._saved is None:
+            raise RuntimeError("backward before forward")
+        logits, tokens, stats, h = self._saved
+        dlogits = out if out is not None else torch.empty_like(logits)
+        return TokenLogProbsOp.adjoint(logits, tokens, stats, dlogprob, dlogits, h if dentropy is not None else None, dentropy, self.scale)
 
 
 class SyncWorkspace(Workspace):

@@ -167,7 +167,7 @@ void anode_gpu_positive_clip_flat_map_bwd_f32(
 
 #define ANODE_OK            0
 #define ANODE_E_NULL       -1   /* a required pointer is NULL */
-#define ANODE_E_DIMS       -2   /* a dimension is 0, dim0*dim1*dim2 >= 2^32, or what section 4 says of its sizes */
+#define ANODE_E_DIMS       -2   /* a dimension is 0, dim0*dim1*dim2 >= 2^32, or what sections 4 and 5 say of their sizes */
 #define ANODE_E_WORKSPACE  -3   /* workspace missing, misaligned or too small */
 #define ANODE_E_LAUNCH     -4   /* the CUDA runtime refused the launch */
 #define ANODE_E_COMM       -5   /* communicator missing / inconsistent / NCCL failure */
@@ -175,6 +175,7 @@ void anode_gpu_positive_clip_flat_map_bwd_f32(
 #define ANODE_E_TOO_LARGE  -7   /* the problem needs more scratch than the library's built-in array holds */
 #define ANODE_E_TYPE       -8   /* an element type that the call does not take */
 #define ANODE_E_STRIDE     -9   /* strides that overlap in an output, or an output in a place that it may not have */
+#define ANODE_E_VALUE     -10   /* a number that the call does not take */
 
 /* Bits of the device status word. */
 #define ANODE_ST_WAIT_STATS   1u  /* a wait for a channel's statistics ran out */
@@ -599,6 +600,83 @@ int anode_gpu_rotary_positions_bwd(
     const struct AnodeHeads *dq_out, const struct AnodeHeads *dk_out, const struct AnodeHeads *q, const struct AnodeHeads *k,
     const struct AnodeHeads *dq, const struct AnodeHeads *dk, void *dgamma_q, void *dgamma_k,
     void *workspace, size_t workspace_bytes,
+    const struct KernelConfig *cfg, struct CUstream_st *stream);
+
+/* ===================================================================================
+ * 5. Layer norm, rows of a table by tokens, and log probabilities of tokens (new): the rest of a language model's rows outside of its
+ *    matrix products, from the tokens to the loss and back.
+ *
+ * Section 4's conventions hold: element types and strides are arguments, arithmetic is in f32, every output is rounded once, no rows
+ * are a call that does nothing, sums are taken in a fixed order, and workspaces hold nothing from call to call.  Tokens are packed signed
+ * integers of token_bytes (4 or 8) bytes; one outside of [0, vocab) stands for no token.
+ * Sizes: rows and columns as in section 4 (a table's rows and a row's logits count as columns do), fewer than 2^31 tokens of a table.
+ * =================================================================================== */
+
+/* Layer norm with the residual's addition, forward:
+ *   total = round(x + residual)                        (x where residual is NULL; stored where total is not NULL)
+ *   mu    = sum(total)/cols,  r = (sum((total - mu)^2)/cols + epsilon)^-1/2      per row (stored where mean, inv_std are not NULL)
+ *   y     = (total - mu) * r * gamma + beta            (gamma NULL: 1, beta NULL: 0; of one type)
+ * As in anode_gpu_rms_norm_add_fwd, the norm reads the sum as it is stored, and total without residual is refused. */
+int anode_gpu_layer_norm_add_fwd(
+    int type, uint64_t rows, uint32_t cols, float epsilon,
+    const void *x, uint64_t x_stride, const void *residual, uint64_t residual_stride,
+    const void *gamma, const void *beta, int weight_type,
+    void *y, uint64_t y_stride, void *total, uint64_t total_stride, float *mean, float *inv_std,
+    const struct KernelConfig *cfg, struct CUstream_st *stream);
+
+/* Its adjoint, from the stored total (x where there was no residual), mean and inv_std:
+ *   g = dy*gamma, xh = (total - mu)*r:  dx = r*(g - sum(g)/cols - xh*sum(g*xh)/cols) + dtotal
+ *   dgamma = sum over rows of dy*xh,  dbeta = sum over rows of dy
+ * dtotal and dx as in anode_gpu_rms_norm_add_bwd.  dgamma, dbeta NULL: not computed; they have weight_type and need the workspace
+ * (anode_gpu_layer_norm_add_bwd_workspace_bytes, 16-byte aligned). */
+size_t anode_gpu_layer_norm_add_bwd_workspace_bytes(uint64_t rows, uint32_t cols);
+int anode_gpu_layer_norm_add_bwd(
+    int type, uint64_t rows, uint32_t cols,
+    const void *dy, uint64_t dy_stride, const void *total, uint64_t total_stride, const float *mean, const float *inv_std,
+    const void *gamma, int weight_type, const void *dtotal, uint64_t dtotal_stride,
+    void *dx, uint64_t dx_stride, void *dgamma, void *dbeta, void *workspace, size_t workspace_bytes,
+    const struct KernelConfig *cfg, struct CUstream_st *stream);
+
+/* Rows of a table [vocab, cols]:  y[i] = scale * table[token[i]], zeros where token[i] is none.  y may not meet the table. */
+int anode_gpu_embed_tokens_fwd(
+    int type, uint64_t tokens, uint32_t vocab, uint32_t cols, float scale,
+    const void *token, int token_bytes, const void *table, uint64_t table_stride, void *y, uint64_t y_stride,
+    const struct KernelConfig *cfg, struct CUstream_st *stream);
+
+/* Its adjoint:  dtable[v] = scale * (sum of dy[i] over token[i] = v), every row of it, zeros where no token names it; with accumulate != 0
+ * that is added to what dtable holds, whose other rows are neither read nor written.  dtable's type is dy's or f32.  A row's terms are added in f32,
+ * in an order that follows from the tokens alone: the same call gives the same bits.  The workspace
+ * (anode_gpu_embed_tokens_bwd_workspace_bytes, 16-byte aligned) is needed wherever there are tokens. */
+size_t anode_gpu_embed_tokens_bwd_workspace_bytes(uint64_t tokens, uint32_t vocab, uint32_t cols);
+int anode_gpu_embed_tokens_bwd(
+    int type, uint64_t tokens, uint32_t vocab, uint32_t cols, float scale,
+    const void *token, int token_bytes, const void *dy, uint64_t dy_stride, void *dtable, uint64_t dtable_stride, int dtable_type, int accumulate,
+    void *workspace, size_t workspace_bytes,
+    const struct KernelConfig *cfg, struct CUstream_st *stream);
+
+/* Log probabilities over rows of logits x, at a temperature of 1/scale (scale positive and finite, or ANODE_E_VALUE):
+ *   m = max x,  z = scale*(x - m),  S = sum(exp(z)),  L = log(S)
+ *   logprob = z[token] - L    (0 where the token is none; NULL: not computed, token is not read)
+ *   entropy = L - sum(z*exp(z))/S                                        (NULL: not computed)
+ *   stats   = (m, L), 8-byte aligned: what the adjoint needs             (NULL: not stored)
+ *   top_token, top_logprob [rows, top]: the `top` <= min(vocab, 128) likeliest tokens, of top_token_bytes (4 or 8) bytes, and z - L of
+ *   them, the largest logit first, of equal ones the lowest index (a NaN counts as larger than all; either may be NULL)
+ * A logit of -infinity has probability 0.  A row of nothing else has log probabilities of -infinity, entropy 0 and stats (-infinity, 0); one
+ * that holds a NaN or +infinity has NaN for log probabilities and entropy.  At least one output is asked for. */
+int anode_gpu_token_log_probs_fwd(
+    int type, uint64_t rows, uint32_t vocab, float scale,
+    const void *logits, uint64_t logits_stride, const void *token, int token_bytes,
+    float *logprob, float *entropy, float *stats, uint32_t top, float *top_logprob, void *top_token, int top_token_bytes,
+    const struct KernelConfig *cfg, struct CUstream_st *stream);
+
+/* Its adjoint, from the same logits, tokens and scale, and what the forward pass stored:
+ *   p = exp(z - L):  dlogits = scale*(dlogprob*([token] - p) - dentropy*p*(z - L + entropy))
+ * dlogprob (NULL: zeros; token is then not read) has no part in a row whose token is none; dentropy NULL: zeros (entropy is then not read); one of
+ * them is given.  A row of nothing but -infinity has zeros.  dlogits may be logits. */
+int anode_gpu_token_log_probs_bwd(
+    int type, uint64_t rows, uint32_t vocab, float scale,
+    const void *logits, uint64_t logits_stride, const void *token, int token_bytes, const float *stats, const float *entropy,
+    const float *dlogprob, const float *dentropy, void *dlogits, uint64_t dlogits_stride,
     const struct KernelConfig *cfg, struct CUstream_st *stream);
 
 #ifdef __cplusplus

@@ -102,11 +102,11 @@ __global__ void __launch_bounds__(most_threads(CH)) layer_norm_held_kernel(const
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     t[k].bits = make_uint4(0, 0, 0, 0);
-    if (k < mine_slots) t[k] = Vec<T>::pass(x + start + k * hop);
+    if (k < mine_slots) t[k] = Vec<T>::load(x + start + k * hop);
   }
   if constexpr (RES) {
 #pragma unroll
-    for (int k = 0; k < CH; ++k) if (k < mine_slots) r[k] = Vec<T>::pass(res + start + k * hop);
+    for (int k = 0; k < CH; ++k) if (k < mine_slots) r[k] = Vec<T>::load(res + start + k * hop);
   }
   float te = 0.0f, ge = 1.0f, be = 0.0f;
   if (on_edge) {
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(most_threads(CH)) layer_norm_held_kernel(const
     else if (aligned) from.load_any<V>(c, a.cols, f);
     else from.load_each<V>(c, f);
   };
-  // the weights of few slots are loaded ahead of the sums, those of many when they are needed: they would take the registers
+  // the weights of few slots are loaded ahead of the sums, those of more when they are needed: they would take the registers
   constexpr bool AHEAD = CH <= 2;
   float2 g[AHEAD ? CH : 1][H], b[AHEAD ? CH : 1][H];
   auto both_weights = [&](int k) {
@@ -545,12 +545,14 @@ bool held_plan(const LayerArgs &a, int type, Held &h, bool &shift)
   shift = !aligned_to(a.x, 16) || a.cols % v || (a.rows > 1 && a.x_stride % v) || !aligned_to(a.gamma.p, 16) || !aligned_to(a.beta.p, 16);
   const uint32_t slots = a.cols / v;
   if (slots > 8 * most_threads(8)) return false;
-  if (slots <= (shift ? 128u : 64u)) {
+  if (slots <= 128) {
     h.team = shift ? 16 : 4;              // (a lane for each element before and after whole slots)
     while (h.team < 32 && h.team < slots) h.team *= 2;
     h.chunks = slots <= h.team ? 1 : slots <= 64 ? 2 : 4;
   } else {
-    h.chunks = a.rows <= 2 * 148 && slots <= 1024 ? 1 : slots <= 256 ? 2 : slots <= 4 * most_threads(4) ? 4 : 8;
+    // few rows: short chains with the weights ahead ([600,2000] bf16 4.4 us with two slots to a thread, 5.4 with four); many: more bytes in flight
+    // for a thread's registers ([16384,2048] 49.5 us with two, 43.1 with four)
+    h.chunks = a.rows <= 2 * 148 && slots <= 1024 ? 1 : a.rows <= 8 * 148 && slots <= 256 ? 2 : slots <= 4 * most_threads(4) ? 4 : 8;
     h.team = (slots + h.chunks * 32 - 1) / (h.chunks * 32) * 32;
   }
   return true;

@@ -45,12 +45,6 @@ struct ProbsGradArgs {
   uint64_t dstride;
 };
 
-// a row's token, or `vocab` for one outside of it
-__device__ __forceinline__ uint32_t token_at(const void *p, int bytes, uint64_t i, uint32_t vocab)
-{
-  const uint64_t t = bytes == 8 ? static_cast<const uint64_t *>(p)[i] : (uint64_t)(int64_t)static_cast<const int32_t *>(p)[i];
-  return t < vocab ? (uint32_t)t : vocab;
-}
 __device__ __forceinline__ float max_nan(float a, float b)
 {
   float d;

@@ -308,6 +308,48 @@ inline int launch(void (*kernel)(P...), dim3 grid, uint32_t threads, size_t shar
   if (cudaLaunchKernelEx(&cfg, kernel, P(args)...) != cudaSuccess) { (void)cudaGetLastError(); return ANODE_E_LAUNCH; }
   return ANODE_OK;
 }
+// The same of a grid of clusters of up to 8 blocks
+template <typename... P, typename... A>
+inline int launch_in_clusters(void (*kernel)(P...), dim3 grid, uint32_t cluster, uint32_t threads, size_t shared, cudaStream_t stream, A... args)
+{
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = shared; cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, kernel, P(args)...) != cudaSuccess) { (void)cudaGetLastError(); return ANODE_E_LAUNCH; }
+  return ANODE_OK;
+}
+
+// Of a cluster: this block's place in it, a barrier that also orders what was written, and another block's shared memory
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync()
+{
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_address(const void *p, uint32_t rank)
+{
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return remote;
+}
+__device__ __forceinline__ uint32_t peer_load(const uint32_t *p, uint32_t rank)
+{
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_address(p, rank)) : "memory");
+  return v;
+}
+
+// A token as a row of a table or a column of logits, or `vocab` for one outside of them
+__device__ __forceinline__ uint32_t token_at(const void *p, int bytes, uint64_t i, uint32_t vocab)
+{
+  const uint64_t t = bytes == 8 ? static_cast<const uint64_t *>(p)[i] : (uint64_t)(int64_t)static_cast<const int32_t *>(p)[i];
+  return t < vocab ? (uint32_t)t : vocab;
+}
 
 }  // namespace rows
 }  // namespace anode_b200

@@ -5,7 +5,8 @@
 // A token outside of the table has a row of zeros and no gradient.  Sums are f32, in an order that follows from the tokens alone.
 //
 // The gradient in three launches:
-//   1. one cluster sorts (token, place) by tokens, a stable radix sort, while the others write zeros to the rows that no token names;
+//   1. (token, place) are sorted by tokens, and equal ones by places, while other blocks write zeros to the whole table: few by counting for each how many come
+//      before it, more by a radix sort in one cluster;
 //   2. the sorted places are cut into pieces, and a thread per 16 bytes of columns walks down a piece's rows of dy: it writes the sum where a token's run
 //      of places ends.  A run of up to kLong places belongs to the piece where it begins; of a longer one each piece leaves its part in the workspace;
 //   3. the parts of each long run are joined, in order.
@@ -51,12 +52,21 @@ template <typename T, int N> __device__ __forceinline__ void put_floats(T *p, co
 #pragma unroll
   for (int i = 0; i < N; i += M) Unit<T, M>::of(f + i).store(p + i);
 }
-template <typename T, int N> __device__ __forceinline__ void get_floats(const T *p, float *f)
-{
-  constexpr int M = N * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
+// N elements as they lie in memory, in one piece or two
+template <typename T, int N> struct Held {
+  static constexpr int M = N * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
+  Unit<T, M> part[N / M];
+  __device__ __forceinline__ void load(const T *p)
+  {
 #pragma unroll
-  for (int i = 0; i < N; i += M) Unit<T, M>::load(p + i).floats(f + i);
-}
+    for (int i = 0; i < N / M; ++i) part[i] = Unit<T, M>::load(p + i * M);
+  }
+  __device__ __forceinline__ void floats(float *f) const
+  {
+#pragma unroll
+    for (int i = 0; i < N / M; ++i) part[i].floats(f + i * M);
+  }
+};
 
 struct EmbedArgs {
   uint64_t tokens;
@@ -102,8 +112,9 @@ template <typename T, int E, int M> __global__ void __launch_bounds__(128) embed
 
 constexpr uint32_t kCluster = 8, kSortThreads = 512, kSortWarps = kSortThreads / 32;
 constexpr uint32_t kMostBits = 9;                    // of a token to a pass of the sort
-constexpr uint32_t kRowsAtOnce = 65536;              // of the table, whose bits a block has
-constexpr uint32_t kLong = 32;                       // places of a run that one piece adds up
+constexpr uint32_t kZeros = 65536;                   // bytes of the table that a block sets to zero
+constexpr uint32_t kCounted = 8192;                  // tokens that are sorted by counting
+constexpr uint32_t kLong = 32;                       // places of a run that one piece adds up, at most
 constexpr uint32_t kMostPiece = 32;                  // places of a piece
 constexpr uint32_t kLeastLanes = 4;                  // threads of a piece
 
@@ -113,10 +124,11 @@ struct SortArgs {
   int token_bytes;
   uint32_t bits, passes;
   uint32_t *key[2], *place[2];          // the last pass writes the first of each
+  uint32_t sorting;                     // blocks that sort
   // rows of zeros
   void *dtable;
-  uint64_t stride;                      // in units
-  uint32_t units, rows;                 // units of a row, rows of a block at a time
+  uint64_t zero_rows, stride, row_bytes;        // in bytes
+  uint32_t rows, cuts;                          // of a block; a row's blocks
 };
 
 // The first cluster: passes of a radix sort, each over `bits` of the tokens.  A warp has a stretch of the places.  It counts its digits (lanes with the same
@@ -208,41 +220,72 @@ __device__ __forceinline__ void sort_tokens(const SortArgs &a, uint32_t (*count)
   }
 }
 
-// The other clusters: each block has rows of the table, and its cluster's blocks look through the tokens together for those that are named
-template <typename W> __device__ __forceinline__ void zero_rows(const SortArgs &a, uint32_t *named)
+// Zeros in kZeros bytes of the table: whole rows, or part of a long one.  Rows that tokens name get theirs, too: to leave them out, blocks had to know them, and
+// as many as could look through the tokens had shares that the slower ones ended late with ([32768,4096] bf16 52 us, 37 as it is: 7.2 TB/s).
+template <typename W> __device__ __forceinline__ void zero_part(const SortArgs &a)
 {
-  const uint32_t rank = cluster_rank(), clusters = gridDim.x / kCluster - 1, first = blockIdx.x / kCluster - 1, each = kCluster * a.rows;
+  const uint64_t block = blockIdx.x - a.sorting, first = block / a.cuts * a.rows, cut = (block % a.cuts) * kZeros;
+  const uint64_t bytes = a.cuts > 1 ? min((uint64_t)kZeros, a.row_bytes - cut) : a.row_bytes;
   uint32_t team = 1;
-  while (team < 32 && team < a.units) team *= 2;
+  while (team < kSortThreads && team * 16 < bytes) team *= 2;
   const uint32_t lane = threadIdx.x & (team - 1);
-  for (uint64_t begin = (uint64_t)first * each; begin < a.vocab; begin += (uint64_t)clusters * each) {
-    for (uint32_t i = threadIdx.x; i < (a.rows + 31) / 32; i += kSortThreads) named[i] = 0;
-    cluster_sync();
-    for (uint64_t i = rank * kSortThreads + threadIdx.x; i < a.n; i += kCluster * kSortThreads) {
-      const uint64_t t = token_at(a.token, a.token_bytes, i, a.vocab);
-      if (t < begin || t >= begin + each || t >= a.vocab) continue;
-      const uint32_t of = (uint32_t)(t - begin) / a.rows, row = (uint32_t)(t - begin) - of * a.rows;
-      asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(peer_address(named + row / 32, of)), "r"(1u << (row & 31)) : "memory");
-    }
-    cluster_sync();
-    const uint64_t mine = begin + (uint64_t)rank * a.rows;
-    for (uint32_t row = threadIdx.x / team; row < a.rows && mine + row < a.vocab; row += kSortThreads / team) {
-      if (named[row / 32] >> (row & 31) & 1) continue;
-      W *to = static_cast<W *>(a.dtable) + (mine + row) * a.stride;
-      for (uint32_t u = lane; u < a.units; u += team) to[u] = W{};
-    }
-    __syncthreads();
+  for (uint64_t row = first + threadIdx.x / team; row < first + a.rows && row < a.zero_rows; row += kSortThreads / team) {
+    char *to = static_cast<char *>(a.dtable) + row * a.stride + cut;
+    // whole 16 bytes of it, and what lies before and behind them
+    const uint32_t head = (uint32_t)min((uint64_t)(-(uintptr_t)to & 15), bytes), units = (uint32_t)((bytes - head) / 16);
+    uint4 *body = reinterpret_cast<uint4 *>(to + head);
+#pragma unroll 4
+    for (uint32_t u = lane; u < units; u += team) body[u] = make_uint4(0, 0, 0, 0);
+    W *behind = reinterpret_cast<W *>(body + units);
+    for (uint32_t i = lane; i < head / sizeof(W); i += team) reinterpret_cast<W *>(to)[i] = W{};
+    for (uint32_t i = lane; i < (bytes - head - (uint64_t)units * 16) / sizeof(W); i += team) behind[i] = W{};
   }
 }
 
 template <typename W> __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs a)
 {
   __shared__ uint32_t count[kSortWarps][1u << kMostBits], totals[1u << kMostBits], base[kSortThreads + kSortWarps];
-  static_assert(sizeof(count) >= kRowsAtOnce / 8 && kSortThreads >= 1u << kMostBits, "a bit per row, a thread per digit");
+  static_assert(kSortThreads >= 1u << kMostBits, "a thread per digit");
   pdl_wait();
   pdl_trigger();
-  if (blockIdx.x < kCluster) { if (a.n) sort_tokens(a, count, totals, base); }
-  else zero_rows<W>(a, count[0]);
+  if (blockIdx.x < a.sorting) sort_tokens(a, count, totals, base);
+  else zero_part<W>(a);
+}
+
+// Up to kCounted tokens: a block finds the places of 32 of them, a lane each, its warps each among a part of all tokens, of which those before it come before it if
+// they are no larger, and those behind it if they are smaller
+template <typename W> __global__ void __launch_bounds__(kSortThreads) embed_count_kernel(const SortArgs a)
+{
+  __shared__ __align__(16) uint32_t key[kCounted];
+  __shared__ uint32_t counts[kSortWarps][32];
+  pdl_wait();
+  pdl_trigger();
+  if (blockIdx.x >= a.sorting) { zero_part<W>(a); return; }
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, begin = blockIdx.x * 32, i = begin + lane;
+  const uint32_t part = (a.n + kSortWarps * 32 - 1) / (kSortWarps * 32) * 32;       // whole blocks' tokens of 32, so that none has tokens on both sides
+  for (uint32_t j = threadIdx.x; j < part * kSortWarps; j += kSortThreads) key[j] = j < a.n ? token_at(a.token, a.token_bytes, j, a.vocab) : ~0u;
+  __syncthreads();
+  const uint32_t mine = key[i], lo = warp * part, hi = lo + part;
+  uint32_t before = 0;
+  auto count_up = [&](uint32_t from, uint32_t to, uint32_t limit) {        // keys below `limit`
+#pragma unroll 4
+    for (uint32_t j = from; j < to; j += 4) {
+      const uint4 k = *reinterpret_cast<const uint4 *>(key + j);
+      before += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
+    }
+  };
+  count_up(lo, min(hi, max(lo, begin)), mine + 1);
+  if (begin >= lo && begin < hi) {
+    for (uint32_t j = 0; j < 32; ++j) before += key[begin + j] < (j < lane ? mine + 1 : mine);
+    count_up(begin + 32, hi, mine);
+  } else if (begin < lo) count_up(lo, hi, mine);
+  counts[warp][lane] = before;
+  __syncthreads();
+  if (warp || i >= a.n) return;
+#pragma unroll
+  for (uint32_t w = 1; w < kSortWarps; ++w) before += counts[w][lane];
+  a.key[0][before] = mine;
+  a.place[0][before] = i;
 }
 
 struct SumArgs {
@@ -253,8 +296,8 @@ struct SumArgs {
   uint64_t dy_stride;
   void *dtable;
   uint64_t stride;
-  uint32_t piece, pieces;
-  uint32_t *begins;                     // of each piece: whether a long run begins in it
+  uint32_t piece, pieces, longest;      // places of a piece; a run of more than `longest` (from `piece` to kLong) is long
+  uint32_t *begins;                     // of each piece: the parts of the long run that begins in it, or 0
   float *part;                          // [pieces][2][part_cols]: of a long run that begins before the piece, and of one that begins in it
   uint32_t part_cols;
   uint32_t lanes;                       // threads of a piece
@@ -263,10 +306,10 @@ struct SumArgs {
 // What a piece adds up: places [from, to), of which the runs of `head` and `tail` are long (else they are ~0)
 struct Piece { uint32_t from, to, head, tail; bool head_before; };
 
-// M units of E columns per thread; a block has kThreads/lanes pieces side by side.  All rows of a step are asked for before one is used, whatever runs they
-// belong to, and with them what the table holds where a run ends (ACC).
+// M units of E columns per thread; a block has kThreads/lanes pieces side by side.  The rows of one step are asked for before those of the step before it are
+// used, whatever runs they belong to, and with them what the table holds where a run ends (ACC).
 template <typename T, typename O, int E, int M, int STEP, bool ACC>
-__global__ void __launch_bounds__(kThreads) embed_sums_kernel(const SumArgs a)
+__global__ void __launch_bounds__(kThreads, ACC ? 2 : 3) embed_sums_kernel(const SumArgs a)
 {
   constexpr uint32_t PIECES = kThreads / kLeastLanes;
   __shared__ uint32_t key[PIECES * kMostPiece + 2 * kLong], place[PIECES * kMostPiece + 2 * kLong];
@@ -293,9 +336,9 @@ __global__ void __launch_bounds__(kThreads) embed_sums_kernel(const SumArgs a)
     Piece q = {at, at, ~0u, ~0u, false};
     if (size && key[at] < a.vocab) {
       const uint32_t k0 = key[at], before = run(k0, at - 1, -1), after = run(k0, at + 1, 1);
-      const bool long0 = before + 1 + after > kLong;
+      const bool long0 = before + 1 + after > a.longest;
       const uint32_t k1 = key[last], ahead = run(k1, last - 1, -1), behind = run(k1, last + 1, 1);
-      const bool long1 = k1 < a.vocab && ahead + 1 + behind > kLong, whole = k0 == k1;
+      const bool long1 = k1 < a.vocab && ahead + 1 + behind > a.longest, whole = k0 == k1;
       q.head_before = before > 0;
       if (before && !long0) q.from = at + 1 + after;             // (that run is an earlier piece's)
       if (long0) q.head = k0;
@@ -303,10 +346,20 @@ __global__ void __launch_bounds__(kThreads) embed_sums_kernel(const SumArgs a)
       q.to = long1 || k1 >= a.vocab ? last + 1 : last + 1 + behind;
       if (q.from > q.to || (whole && before && !long0)) q.to = q.from;
     }
-    if (lane == 0) {
-      piece[p] = q;
-      if (first + p < a.pieces && blockIdx.y == 0) a.begins[first + p] = q.tail != ~0u && !(q.tail == q.head && q.head_before);
+    if (lane == 0) piece[p] = q;
+    if (first + p >= a.pieces || blockIdx.y) continue;
+    // the parts of a run that begins here: this one, the pieces behind it that it fills, and one that it ends in
+    uint32_t parts = 0;
+    if (q.tail != ~0u && !(q.tail == q.head && q.head_before)) {
+      uint32_t filled = 32, r = first + p + 1;
+      for (; filled == 32; r += filled) {
+        const uint64_t end = (uint64_t)(r + lane + 1) * a.piece;
+        const uint32_t others = ~__ballot_sync(0xffffffffu, end <= a.n && a.key[end - 1] == q.tail);
+        filled = others ? (uint32_t)__ffs((int)others) - 1 : 32u;
+      }
+      parts = r - (first + p) + (r < a.pieces && a.key[(uint64_t)r * a.piece] == q.tail);
     }
+    if (lane == 0) a.begins[first + p] = parts;
   }
   __syncthreads();
   const uint32_t mine = threadIdx.x / a.lanes;
@@ -323,108 +376,119 @@ __global__ void __launch_bounds__(kThreads) embed_sums_kernel(const SumArgs a)
   for (int m = 0; m < M; ++m)
 #pragma unroll
     for (int j = 0; j < E; ++j) sum[m][j] = 0.0f;
-  for (uint32_t i = q.from; i < q.to; i += STEP) {
+  struct Stage {
+    uint32_t k[STEP + 1];               // the places' tokens, and the one behind them; ~0: none
     Unit<T, E> v[STEP][M];
-    float old[ACC ? STEP : 1][M][E];
-    uint32_t k[STEP + 1];
+    Held<O, E> old[ACC ? STEP : 1][M];
+  };
+  auto fetch = [&](Stage &g, uint32_t i) {
 #pragma unroll
-    for (int s = 0; s <= STEP; ++s) { k[s] = i + s < q.to ? key[i + s] : ~0u; if (k[s] >= a.vocab) k[s] = ~0u; }
+    for (int s = 0; s <= STEP; ++s) { g.k[s] = i + s < q.to ? key[i + s] : ~0u; if (g.k[s] >= a.vocab) g.k[s] = ~0u; }
 #pragma unroll
     for (int s = 0; s < STEP; ++s) {
-      if (k[s] == ~0u) continue;
+      if (g.k[s] == ~0u) continue;
       const T *row = dy + place[i + s] * a.dy_stride;
 #pragma unroll
-      for (int m = 0; m < M; ++m) if (has[m]) v[s][m] = Unit<T, E>::load(row + (uint64_t)m * a.lanes * E);
+      for (int m = 0; m < M; ++m) if (has[m]) g.v[s][m] = Unit<T, E>::load(row + (uint64_t)m * a.lanes * E);
     }
     if constexpr (ACC) {
 #pragma unroll
       for (int s = 0; s < STEP; ++s) {
-        if (k[s] == k[s + 1] || k[s] == ~0u) continue;
+        if (g.k[s] == g.k[s + 1]) continue;
 #pragma unroll
-        for (int m = 0; m < M; ++m) if (has[m]) get_floats<O, E>(out + k[s] * a.stride + (uint64_t)m * a.lanes * E, old[s][m]);
+        for (int m = 0; m < M; ++m) if (has[m]) g.old[s][m].load(out + g.k[s] * a.stride + (uint64_t)m * a.lanes * E);
       }
     }
+  };
+  auto use = [&](const Stage &g) {
 #pragma unroll
     for (int s = 0; s < STEP; ++s) {
-      if (k[s] == ~0u) continue;
+      if (g.k[s] == ~0u) continue;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         float f[E];
-        v[s][m].floats(f);
+        g.v[s][m].floats(f);
 #pragma unroll
         for (int j = 0; j < E; ++j) sum[m][j] += f[j];
       }
-      if (k[s] == k[s + 1]) continue;
+      if (g.k[s] == g.k[s + 1]) continue;
       // the run's end, or that of the piece's part of a long one
-      const bool is_long = k[s] == q.head || k[s] == q.tail;
-      float *to = part + (k[s] == q.head && q.head_before ? 0 : a.part_cols);
+      const bool is_long = g.k[s] == q.head || g.k[s] == q.tail;
+      float *to = part + (g.k[s] == q.head && q.head_before ? 0 : a.part_cols);
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         if (has[m] && is_long) {
 #pragma unroll
           for (int j = 0; j < E; ++j) to[(uint64_t)m * a.lanes * E + j] = sum[m][j];
         } else if (has[m]) {
+          float f[E];
+          if constexpr (ACC) g.old[s][m].floats(f);
 #pragma unroll
-          for (int j = 0; j < E; ++j) sum[m][j] = ACC ? fmaf(sum[m][j], a.scale, old[ACC ? s : 0][m][j]) : sum[m][j] * a.scale;
-          put_floats<O, E>(out + k[s] * a.stride + (uint64_t)m * a.lanes * E, sum[m]);
+          for (int j = 0; j < E; ++j) sum[m][j] = ACC ? fmaf(sum[m][j], a.scale, f[j]) : sum[m][j] * a.scale;
+          put_floats<O, E>(out + g.k[s] * a.stride + (uint64_t)m * a.lanes * E, sum[m]);
         }
 #pragma unroll
         for (int j = 0; j < E; ++j) sum[m][j] = 0.0f;
       }
     }
+  };
+  Stage one, two;
+  fetch(one, q.from);
+  for (uint32_t i = q.from; i < q.to; i += 2 * STEP) {
+    fetch(two, i + STEP);
+    use(one);
+    fetch(one, i + 2 * STEP);
+    use(two);
   }
 }
 
-// The parts of long runs: a block has 128 columns and every gridDim.y-th piece that such a run begins in; a warp adds an eighth of the run's parts, in order
+// The parts of long runs: a block has 128 columns and every gridDim.y-th such run; a warp adds an eighth of the run's parts, in order
 template <typename O> __global__ void __launch_bounds__(kThreads) embed_join_kernel(const SumArgs a, const int accumulate)
 {
-  __shared__ float sums[kThreads / 32][4][32];
+  constexpr uint32_t WARPS = kThreads / 32;
+  __shared__ float sums[WARPS][4][32];
+  __shared__ uint32_t counts[WARPS], mine[kThreads];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t c = ((uint64_t)blockIdx.x * 32 + lane) * 4;
   pdl_wait();
-  for (uint32_t group = blockIdx.y * kThreads; group < a.pieces; group += gridDim.y * kThreads)
-    for (uint32_t p = group; p < min(a.pieces, group + kThreads); ++p) {
-      // the next piece with such a run
-      const uint32_t look = p + threadIdx.x;
-      const bool here = look < min(a.pieces, group + kThreads) && a.begins[look];
-      __shared__ uint32_t next, end;
-      __syncthreads();
-      if (threadIdx.x == 0) { next = ~0u; end = ~0u; }
-      __syncthreads();
-      if (here) atomicMin(&next, look);
-      __syncthreads();
-      p = next;
-      if (p == ~0u) break;
-      // the pieces behind it that the run fills, and one that it ends in
-      const uint32_t k = a.key[(uint64_t)p * a.piece + a.piece - 1];
-      for (uint32_t from = p + 1; end == ~0u; from += kThreads) {
-        const uint32_t r = from + threadIdx.x;
-        const uint64_t last = (uint64_t)r * a.piece + a.piece - 1;
-        __syncthreads();
-        if (last >= a.n || a.key[last] != k) atomicMin(&end, r);
-        __syncthreads();
-      }
-      const uint32_t filled = end;
-      const uint32_t stop = filled < a.pieces && a.key[(uint64_t)filled * a.piece] == k ? filled + 1 : filled;
-      const uint32_t parts = stop - p, each = (parts + kThreads / 32 - 1) / (kThreads / 32), lo = min(parts, warp * each), hi = min(parts, lo + each);
+  uint32_t before = blockIdx.y;         // runs until this block's next one
+  for (uint32_t group = 0; group < a.pieces; group += kThreads) {
+    // the pieces in which this block's runs begin
+    const uint32_t look = group + threadIdx.x;
+    const bool here = look < a.pieces && a.begins[look];
+    const uint32_t votes = __ballot_sync(0xffffffffu, here);
+    if (lane == 0) counts[warp] = __popc(votes);
+    __syncthreads();
+    uint32_t rank = __popc(votes & ((1u << lane) - 1)), all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < WARPS; ++w) { rank += w < warp ? counts[w] : 0; all += counts[w]; }
+    if (here && rank >= before && (rank - before) % gridDim.y == 0) mine[(rank - before) / gridDim.y] = look;
+    const uint32_t runs = all > before ? (all - before + gridDim.y - 1) / gridDim.y : 0;
+    before = before + runs * gridDim.y - all;
+    __syncthreads();
+    for (uint32_t i = 0; i < runs; ++i) {
+      const uint32_t p = mine[i], k = a.key[(uint64_t)p * a.piece + a.piece - 1], parts = a.begins[p];
+      const uint32_t each = (parts + WARPS - 1) / WARPS, lo = min(parts, warp * each), hi = min(parts, lo + each);
       float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (c < a.cols) {
 #pragma unroll 8
-        for (uint32_t i = lo; i < hi; ++i) {
-          const float4 v = *reinterpret_cast<const float4 *>(a.part + ((uint64_t)(p + i) * 2 + (i == 0)) * a.part_cols + c);
+        for (uint32_t j = lo; j < hi; ++j) {
+          const float4 v = *reinterpret_cast<const float4 *>(a.part + ((uint64_t)(p + j) * 2 + (j == 0)) * a.part_cols + c);
           sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
         }
       }
       sums[warp][0][lane] = sum.x; sums[warp][1][lane] = sum.y; sums[warp][2][lane] = sum.z; sums[warp][3][lane] = sum.w;
       __syncthreads();
       if (warp < 4 && c + warp < a.cols) {
-        float all = 0.0f;
+        float total = 0.0f;
 #pragma unroll
-        for (uint32_t w = 0; w < kThreads / 32; ++w) all += sums[w][warp][lane];
+        for (uint32_t w = 0; w < WARPS; ++w) total += sums[w][warp][lane];
         O *to = static_cast<O *>(a.dtable) + k * a.stride + c + warp;
-        *to = from_float<O>(accumulate ? fmaf(all, a.scale, to_float(*to)) : all * a.scale);
+        *to = from_float<O>(accumulate ? fmaf(total, a.scale, to_float(*to)) : total * a.scale);
       }
+      __syncthreads();
     }
+  }
 }
 
 inline int check_tokens(const void *token, int bytes)
@@ -454,7 +518,7 @@ inline uint32_t power_up_to(uint64_t n, uint32_t most)
 }
 
 // Places of a piece: few where there are few, so that more threads have some
-inline uint32_t piece_of(uint64_t tokens) { return tokens >= 8192 ? 32 : tokens >= 4096 ? 16 : tokens >= 1024 ? 8 : 4; }
+inline uint32_t piece_of(uint64_t tokens) { return tokens >= 16384 ? 32 : tokens >= 8192 ? 16 : 8; }
 
 // Where the workspace's arrays begin
 struct Layout {
@@ -475,18 +539,18 @@ template <typename T, typename O, int E> int launch_sums(SumArgs a, int accumula
   if (a.lanes < kLeastLanes) a.lanes = kLeastLanes;
   const uint32_t per_block = kThreads / a.lanes, wide = (units + a.lanes * M - 1) / (a.lanes * M);
   const dim3 grid((a.pieces + per_block - 1) / per_block, wide);
-  return accumulate ? launch(embed_sums_kernel<T, O, E, M, M == 1 ? 4 : 2, true>, grid, kThreads, 0, stream, a)
-                    : launch(embed_sums_kernel<T, O, E, M, M == 1 ? 8 : 4, false>, grid, kThreads, 0, stream, a);
+  return accumulate ? launch(embed_sums_kernel<T, O, E, M, E == 2 ? 2 : 4, true>, grid, kThreads, 0, stream, a)
+                    : launch(embed_sums_kernel<T, O, E, M, E == 2 ? 2 : 4, false>, grid, kThreads, 0, stream, a);
 }
 template <typename T, typename O> int launch_sums(const SumArgs &a, uint32_t unit, int accumulate, cudaStream_t stream)
 {
   constexpr int V = 16 / sizeof(T);
   TRY((unit == (uint32_t)V ? launch_sums<T, O, V>(a, accumulate, stream) : unit == 2 ? launch_sums<T, O, 2>(a, accumulate, stream)
                                                                                       : launch_sums<T, O, 1>(a, accumulate, stream)));
-  // a run is long beyond kLong places
-  if (a.n <= kLong) return ANODE_OK;
-  const uint32_t groups = (a.pieces + kThreads - 1) / kThreads;
-  return launch(embed_join_kernel<O>, dim3((uint32_t)(((uint64_t)a.cols + 127) / 128), groups < 16 ? groups : 16), kThreads, 0, stream, a, accumulate);
+  if (a.n <= a.longest) return ANODE_OK;
+  // a run to a block, of the tokens of a training batch: some 50 of 16384 come more than 32 times
+  const uint32_t wide = (uint32_t)(((uint64_t)a.cols + 127) / 128), most = a.n / (a.longest + 1), blocks = (16 * sm_count() + wide - 1) / wide;
+  return launch(embed_join_kernel<O>, dim3(wide, blocks < most ? blocks : most), kThreads, 0, stream, a, accumulate);
 }
 
 }  // namespace rows
@@ -547,31 +611,30 @@ extern "C" int anode_gpu_embed_tokens_bwd(
   }
   const Layout l(tokens, cols);
   uint32_t *words = static_cast<uint32_t *>(workspace);
-  SortArgs s = {(uint32_t)tokens, vocab, token, token_bytes, 0, 0, {words, words + l.n}, {words + 2 * l.n, words + 3 * l.n}, dtable, 0, 0, 0};
+  SortArgs s = {(uint32_t)tokens, vocab, token, token_bytes, 0, 0, {words, words + l.n}, {words + 2 * l.n, words + 3 * l.n}, 0, dtable, 0, 0, 0, 1, 1};
   // tokens up to `vocab`, which stands for none
   uint32_t bits = 0;
   while (vocab >> bits) ++bits;
   s.passes = (bits + kMostBits - 1) / kMostBits;
   s.bits = (bits + s.passes - 1) / s.passes;
-  // rows of zeros in units of 16 bytes, or as many as their columns and places allow
-  uint32_t bytes = 16;
-  while ((uint64_t)cols * oe % bytes || (uint64_t)dtable_stride * oe % bytes || !aligned_to(dtable, bytes)) bytes /= 2;
-  s.units = (uint32_t)((uint64_t)cols * oe / bytes);
-  s.stride = dtable_stride * oe / bytes;
-  uint32_t clusters = 0;
+  const bool counted = tokens <= kCounted;
+  s.sorting = !tokens ? 0 : counted ? (uint32_t)((tokens + 31) / 32) : kCluster;
+  uint64_t blocks = 0;
   if (!accumulate) {
-    const uint64_t work = ((uint64_t)vocab * cols * oe + (kCluster << 15) - 1) / (kCluster << 15);      // 32 KB for a block
-    clusters = (uint32_t)(work < 24 ? work : 24);
-    const uint64_t rows = ((uint64_t)vocab + clusters * kCluster - 1) / (clusters * kCluster);
-    s.rows = (uint32_t)(rows < kRowsAtOnce ? rows : kRowsAtOnce);
+    s.zero_rows = vocab; s.stride = dtable_stride * oe; s.row_bytes = (uint64_t)cols * oe;
+    if (dtable_stride == cols) { s.row_bytes *= vocab; s.zero_rows = 1; }      // (one long row)
+    s.cuts = (uint32_t)((s.row_bytes + kZeros - 1) / kZeros);
+    s.rows = s.cuts > 1 ? 1 : (uint32_t)(kZeros / s.row_bytes);
+    blocks = (s.zero_rows + s.rows - 1) / s.rows * s.cuts;
+    if (!counted) blocks = (blocks + kCluster - 1) / kCluster * kCluster;
+    if (blocks >> 30) return ANODE_E_DIMS;
   }
-  const dim3 grid((clusters + 1) * kCluster);
-  TRY(bytes == 16 ? launch_in_clusters(embed_sort_kernel<uint4>, grid, kCluster, kSortThreads, 0, stream, s)
-    : bytes == 8 ? launch_in_clusters(embed_sort_kernel<uint2>, grid, kCluster, kSortThreads, 0, stream, s)
-    : bytes == 4 ? launch_in_clusters(embed_sort_kernel<uint32_t>, grid, kCluster, kSortThreads, 0, stream, s)
-                 : launch_in_clusters(embed_sort_kernel<uint16_t>, grid, kCluster, kSortThreads, 0, stream, s));
+  const dim3 grid(s.sorting + (uint32_t)blocks);
+  TRY((counted ? (oe == 4 ? launch(embed_count_kernel<uint32_t>, grid, kSortThreads, 0, stream, s) : launch(embed_count_kernel<uint16_t>, grid, kSortThreads, 0, stream, s))
+               : (oe == 4 ? launch_in_clusters(embed_sort_kernel<uint32_t>, grid, kCluster, kSortThreads, 0, stream, s)
+                          : launch_in_clusters(embed_sort_kernel<uint16_t>, grid, kCluster, kSortThreads, 0, stream, s))));
   if (!tokens) return ANODE_OK;
-  const SumArgs a = {(uint32_t)tokens, vocab, cols, scale, s.key[0], s.place[0], dy, dy_stride, dtable, dtable_stride, (uint32_t)l.piece, (uint32_t)l.pieces,
+  const SumArgs a = {(uint32_t)tokens, vocab, cols, scale, s.key[0], s.place[0], dy, dy_stride, dtable, dtable_stride, (uint32_t)l.piece, (uint32_t)l.pieces, l.piece == 8 ? 16u : kLong,
                      words + l.begins / 4, reinterpret_cast<float *>(static_cast<char *>(workspace) + l.part), (uint32_t)l.part_cols, 0};
   const uint32_t unit = unit_of(dy, e, dy_stride, tokens, dtable, oe, dtable_stride, vocab, cols);
   return by_type(type, [&](auto t) {

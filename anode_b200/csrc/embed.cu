@@ -125,6 +125,7 @@ struct SortArgs {
   uint32_t bits, passes;
   uint32_t *key[2], *place[2];          // the last pass writes the first of each
   uint32_t sorting;                     // blocks that sort
+  uint32_t *runs;                       // the count of long runs, set to 0
   // rows of zeros
   void *dtable;
   uint64_t zero_rows, stride, row_bytes;        // in bytes
@@ -224,7 +225,8 @@ __device__ __forceinline__ void sort_tokens(const SortArgs &a, uint32_t (*count)
 // as many as could look through the tokens had shares that the slower ones ended late with ([32768,4096] bf16 52 us, 37 as it is: 7.2 TB/s).
 template <typename W> __device__ __forceinline__ void zero_part(const SortArgs &a)
 {
-  const uint64_t block = blockIdx.x - a.sorting, first = block / a.cuts * a.rows, cut = (block % a.cuts) * kZeros;
+  // (from the end on, so that the common tokens' rows, which come first, are the last to leave the second-level cache before their sums are written)
+  const uint64_t block = gridDim.x - 1 - blockIdx.x, first = block / a.cuts * a.rows, cut = (block % a.cuts) * kZeros;
   const uint64_t bytes = a.cuts > 1 ? min((uint64_t)kZeros, a.row_bytes - cut) : a.row_bytes;
   uint32_t team = 1;
   while (team < kSortThreads && team * 16 < bytes) team *= 2;
@@ -248,6 +250,7 @@ template <typename W> __global__ void __launch_bounds__(kSortThreads) embed_sort
   static_assert(kSortThreads >= 1u << kMostBits, "a thread per digit");
   pdl_wait();
   pdl_trigger();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.runs = 0;
   if (blockIdx.x < a.sorting) sort_tokens(a, count, totals, base);
   else zero_part<W>(a);
 }
@@ -261,9 +264,17 @@ template <typename W> __global__ void __launch_bounds__(kSortThreads) embed_coun
   pdl_wait();
   pdl_trigger();
   if (blockIdx.x >= a.sorting) { zero_part<W>(a); return; }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.runs = 0;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, begin = blockIdx.x * 32, i = begin + lane;
   const uint32_t part = (a.n + kSortWarps * 32 - 1) / (kSortWarps * 32) * 32;       // whole blocks' tokens of 32, so that none has tokens on both sides
-  for (uint32_t j = threadIdx.x; j < part * kSortWarps; j += kSortThreads) key[j] = j < a.n ? token_at(a.token, a.token_bytes, j, a.vocab) : ~0u;
+  constexpr uint32_t AT_ONCE = 8;
+  for (uint32_t j = threadIdx.x; j < part * kSortWarps; j += AT_ONCE * kSortThreads) {
+    uint32_t k[AT_ONCE];
+#pragma unroll
+    for (uint32_t u = 0; u < AT_ONCE; ++u) k[u] = j + u * kSortThreads < a.n ? token_at(a.token, a.token_bytes, j + u * kSortThreads, a.vocab) : ~0u;
+#pragma unroll
+    for (uint32_t u = 0; u < AT_ONCE; ++u) if (j + u * kSortThreads < part * kSortWarps) key[j + u * kSortThreads] = k[u];
+  }
   __syncthreads();
   const uint32_t mine = key[i], lo = warp * part, hi = lo + part;
   uint32_t before = 0;
@@ -297,7 +308,8 @@ struct SumArgs {
   void *dtable;
   uint64_t stride;
   uint32_t piece, pieces, longest;      // places of a piece; a run of more than `longest` (from `piece` to kLong) is long
-  uint32_t *begins;                     // of each piece: the parts of the long run that begins in it, or 0
+  uint32_t *runs;                       // how many runs are long, in whatever order: each one's first piece, token and count of parts
+  uint4 *run;
   float *part;                          // [pieces][2][part_cols]: of a long run that begins before the piece, and of one that begins in it
   uint32_t part_cols;
   uint32_t lanes;                       // threads of a piece
@@ -309,7 +321,7 @@ struct Piece { uint32_t from, to, head, tail; bool head_before; };
 // M units of E columns per thread; a block has kThreads/lanes pieces side by side.  The rows of one step are asked for before those of the step before it are
 // used, whatever runs they belong to, and with them what the table holds where a run ends (ACC).
 template <typename T, typename O, int E, int M, int STEP, bool ACC>
-__global__ void __launch_bounds__(kThreads, ACC ? 2 : 3) embed_sums_kernel(const SumArgs a)
+__global__ void __launch_bounds__(kThreads, ACC && M == 1 ? 2 : 3) embed_sums_kernel(const SumArgs a)
 {
   constexpr uint32_t PIECES = kThreads / kLeastLanes;
   __shared__ uint32_t key[PIECES * kMostPiece + 2 * kLong], place[PIECES * kMostPiece + 2 * kLong];
@@ -348,8 +360,7 @@ __global__ void __launch_bounds__(kThreads, ACC ? 2 : 3) embed_sums_kernel(const
     }
     if (lane == 0) piece[p] = q;
     if (first + p >= a.pieces || blockIdx.y) continue;
-    // the parts of a run that begins here: this one, the pieces behind it that it fills, and one that it ends in
-    uint32_t parts = 0;
+    // the parts of a long run that begins here: this one, the pieces behind it that it fills, and one that it ends in
     if (q.tail != ~0u && !(q.tail == q.head && q.head_before)) {
       uint32_t filled = 32, r = first + p + 1;
       for (; filled == 32; r += filled) {
@@ -357,9 +368,9 @@ __global__ void __launch_bounds__(kThreads, ACC ? 2 : 3) embed_sums_kernel(const
         const uint32_t others = ~__ballot_sync(0xffffffffu, end <= a.n && a.key[end - 1] == q.tail);
         filled = others ? (uint32_t)__ffs((int)others) - 1 : 32u;
       }
-      parts = r - (first + p) + (r < a.pieces && a.key[(uint64_t)r * a.piece] == q.tail);
+      const uint32_t parts = r - (first + p) + (r < a.pieces && a.key[(uint64_t)r * a.piece] == q.tail);
+      if (lane == 0) a.run[atomicAdd(a.runs, 1u)] = make_uint4(first + p, q.tail, parts, 0);
     }
-    if (lane == 0) a.begins[first + p] = parts;
   }
   __syncthreads();
   const uint32_t mine = threadIdx.x / a.lanes;
@@ -442,52 +453,41 @@ __global__ void __launch_bounds__(kThreads, ACC ? 2 : 3) embed_sums_kernel(const
   }
 }
 
-// The parts of long runs: a block has 128 columns and every gridDim.y-th such run; a warp adds an eighth of the run's parts, in order
-template <typename O> __global__ void __launch_bounds__(kThreads) embed_join_kernel(const SumArgs a, const int accumulate)
+// The parts of long runs: a block has 128 columns and every gridDim.y-th such run; a warp adds a quarter of the run's parts, in order
+constexpr uint32_t kJoinThreads = 128;
+template <typename O> __global__ void __launch_bounds__(kJoinThreads) embed_join_kernel(const SumArgs a, const int accumulate)
 {
-  constexpr uint32_t WARPS = kThreads / 32;
+  constexpr uint32_t WARPS = kJoinThreads / 32;
   __shared__ float sums[WARPS][4][32];
-  __shared__ uint32_t counts[WARPS], mine[kThreads];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint64_t c = ((uint64_t)blockIdx.x * 32 + lane) * 4;
   pdl_wait();
-  uint32_t before = blockIdx.y;         // runs until this block's next one
-  for (uint32_t group = 0; group < a.pieces; group += kThreads) {
-    // the pieces in which this block's runs begin
-    const uint32_t look = group + threadIdx.x;
-    const bool here = look < a.pieces && a.begins[look];
-    const uint32_t votes = __ballot_sync(0xffffffffu, here);
-    if (lane == 0) counts[warp] = __popc(votes);
-    __syncthreads();
-    uint32_t rank = __popc(votes & ((1u << lane) - 1)), all = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < WARPS; ++w) { rank += w < warp ? counts[w] : 0; all += counts[w]; }
-    if (here && rank >= before && (rank - before) % gridDim.y == 0) mine[(rank - before) / gridDim.y] = look;
-    const uint32_t runs = all > before ? (all - before + gridDim.y - 1) / gridDim.y : 0;
-    before = before + runs * gridDim.y - all;
-    __syncthreads();
-    for (uint32_t i = 0; i < runs; ++i) {
-      const uint32_t p = mine[i], k = a.key[(uint64_t)p * a.piece + a.piece - 1], parts = a.begins[p];
-      const uint32_t each = (parts + WARPS - 1) / WARPS, lo = min(parts, warp * each), hi = min(parts, lo + each);
-      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (c < a.cols) {
+  const uint32_t runs = *a.runs;
+  for (uint32_t i = blockIdx.y; i < runs; i += gridDim.y) {
+    const uint4 run = a.run[i];
+    const uint32_t parts = run.z, each = (parts + WARPS - 1) / WARPS, lo = min(parts, warp * each), hi = min(parts, lo + each);
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (c < a.cols) {
 #pragma unroll 8
-        for (uint32_t j = lo; j < hi; ++j) {
-          const float4 v = *reinterpret_cast<const float4 *>(a.part + ((uint64_t)(p + j) * 2 + (j == 0)) * a.part_cols + c);
-          sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-        }
+      for (uint32_t j = lo; j < hi; ++j) {
+        const float4 v = *reinterpret_cast<const float4 *>(a.part + ((uint64_t)(run.x + j) * 2 + (j == 0)) * a.part_cols + c);
+        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
       }
-      sums[warp][0][lane] = sum.x; sums[warp][1][lane] = sum.y; sums[warp][2][lane] = sum.z; sums[warp][3][lane] = sum.w;
-      __syncthreads();
-      if (warp < 4 && c + warp < a.cols) {
-        float total = 0.0f;
-#pragma unroll
-        for (uint32_t w = 0; w < WARPS; ++w) total += sums[w][warp][lane];
-        O *to = static_cast<O *>(a.dtable) + k * a.stride + c + warp;
-        *to = from_float<O>(accumulate ? fmaf(total, a.scale, to_float(*to)) : total * a.scale);
-      }
-      __syncthreads();
     }
+    sums[warp][0][lane] = sum.x; sums[warp][1][lane] = sum.y; sums[warp][2][lane] = sum.z; sums[warp][3][lane] = sum.w;
+    // a warp writes 32 columns side by side
+    const uint32_t mine = warp * 32 + lane;
+    const uint64_t column = (uint64_t)blockIdx.x * 128 + mine;
+    O *to = static_cast<O *>(a.dtable) + run.y * a.stride + column;
+    const float old = accumulate && column < a.cols ? to_float(*to) : 0.0f;
+    __syncthreads();
+    if (column < a.cols) {
+      float total = 0.0f;
+#pragma unroll
+      for (uint32_t w = 0; w < WARPS; ++w) total += sums[w][mine & 3][mine >> 2];
+      *to = from_float<O>(accumulate ? fmaf(total, a.scale, old) : total * a.scale);
+    }
+    __syncthreads();
   }
 }
 
@@ -517,30 +517,35 @@ inline uint32_t power_up_to(uint64_t n, uint32_t most)
   return v;
 }
 
-// Places of a piece: few where there are few, so that more threads have some
-inline uint32_t piece_of(uint64_t tokens) { return tokens >= 16384 ? 32 : tokens >= 8192 ? 16 : 8; }
+// Places of a piece: as many as give each multiprocessor three blocks of a row's width; a run of more is long, or of more than 8
+inline uint32_t piece_of(uint64_t tokens)
+{
+  const uint64_t each = (tokens + 3 * 148 - 1) / (3 * 148);
+  return (uint32_t)(each < 4 ? 4 : each < kMostPiece ? each : kMostPiece);
+}
 
-// Where the workspace's arrays begin
+// Where the workspace's arrays begin, in bytes
 struct Layout {
-  uint64_t n, piece, pieces, part_cols, begins, part, bytes;
-  Layout(uint64_t tokens, uint32_t cols) : n((tokens + 3) / 4 * 4), piece(piece_of(tokens)), pieces((tokens + piece - 1) / piece), part_cols(((uint64_t)cols + 3) / 4 * 4)
+  uint64_t n, piece, longest, pieces, part_cols, runs, run, part, bytes;
+  Layout(uint64_t tokens, uint32_t cols) : n((tokens + 3) / 4 * 4), piece(piece_of(tokens)), longest(piece < 8 ? 8 : piece), pieces((tokens + piece - 1) / piece), part_cols(((uint64_t)cols + 3) / 4 * 4)
   {
-    begins = 16 * n;
-    part = begins + (pieces + 3) / 4 * 16;
+    runs = 16 * n;
+    run = runs + 16;
+    part = run + tokens / (longest + 1) * 16;
     bytes = part + pieces * 2 * part_cols * 4;
   }
 };
 
 template <typename T, typename O, int E> int launch_sums(SumArgs a, int accumulate, cudaStream_t stream)
 {
-  constexpr int M = E * sizeof(T) == 16 ? 1 : 4;
+  constexpr int M = E * sizeof(T) == 16 ? 1 : 2;
   const uint32_t units = a.cols / E;
   a.lanes = power_up_to((units + M - 1) / M, kThreads);
   if (a.lanes < kLeastLanes) a.lanes = kLeastLanes;
   const uint32_t per_block = kThreads / a.lanes, wide = (units + a.lanes * M - 1) / (a.lanes * M);
   const dim3 grid((a.pieces + per_block - 1) / per_block, wide);
-  return accumulate ? launch(embed_sums_kernel<T, O, E, M, E == 2 ? 2 : 4, true>, grid, kThreads, 0, stream, a)
-                    : launch(embed_sums_kernel<T, O, E, M, E == 2 ? 2 : 4, false>, grid, kThreads, 0, stream, a);
+  return accumulate ? launch(embed_sums_kernel<T, O, E, M, 4, true>, grid, kThreads, 0, stream, a)
+                    : launch(embed_sums_kernel<T, O, E, M, 4, false>, grid, kThreads, 0, stream, a);
 }
 template <typename T, typename O> int launch_sums(const SumArgs &a, uint32_t unit, int accumulate, cudaStream_t stream)
 {
@@ -550,7 +555,7 @@ template <typename T, typename O> int launch_sums(const SumArgs &a, uint32_t uni
   if (a.n <= a.longest) return ANODE_OK;
   // a run to a block, of the tokens of a training batch: some 50 of 16384 come more than 32 times
   const uint32_t wide = (uint32_t)(((uint64_t)a.cols + 127) / 128), most = a.n / (a.longest + 1), blocks = (16 * sm_count() + wide - 1) / wide;
-  return launch(embed_join_kernel<O>, dim3(wide, blocks < most ? blocks : most), kThreads, 0, stream, a, accumulate);
+  return launch(embed_join_kernel<O>, dim3(wide, blocks < most ? blocks : most), kJoinThreads, 0, stream, a, accumulate);
 }
 
 }  // namespace rows
@@ -611,7 +616,7 @@ extern "C" int anode_gpu_embed_tokens_bwd(
   }
   const Layout l(tokens, cols);
   uint32_t *words = static_cast<uint32_t *>(workspace);
-  SortArgs s = {(uint32_t)tokens, vocab, token, token_bytes, 0, 0, {words, words + l.n}, {words + 2 * l.n, words + 3 * l.n}, 0, dtable, 0, 0, 0, 1, 1};
+  SortArgs s = {(uint32_t)tokens, vocab, token, token_bytes, 0, 0, {words, words + l.n}, {words + 2 * l.n, words + 3 * l.n}, 0, words + l.runs / 4, dtable, 0, 0, 0, 1, 1};
   // tokens up to `vocab`, which stands for none
   uint32_t bits = 0;
   while (vocab >> bits) ++bits;
@@ -634,8 +639,8 @@ extern "C" int anode_gpu_embed_tokens_bwd(
                : (oe == 4 ? launch_in_clusters(embed_sort_kernel<uint32_t>, grid, kCluster, kSortThreads, 0, stream, s)
                           : launch_in_clusters(embed_sort_kernel<uint16_t>, grid, kCluster, kSortThreads, 0, stream, s))));
   if (!tokens) return ANODE_OK;
-  const SumArgs a = {(uint32_t)tokens, vocab, cols, scale, s.key[0], s.place[0], dy, dy_stride, dtable, dtable_stride, (uint32_t)l.piece, (uint32_t)l.pieces, l.piece == 8 ? 16u : kLong,
-                     words + l.begins / 4, reinterpret_cast<float *>(static_cast<char *>(workspace) + l.part), (uint32_t)l.part_cols, 0};
+  const SumArgs a = {(uint32_t)tokens, vocab, cols, scale, s.key[0], s.place[0], dy, dy_stride, dtable, dtable_stride, (uint32_t)l.piece, (uint32_t)l.pieces, (uint32_t)l.longest,
+                     words + l.runs / 4, reinterpret_cast<uint4 *>(static_cast<char *>(workspace) + l.run), reinterpret_cast<float *>(static_cast<char *>(workspace) + l.part), (uint32_t)l.part_cols, 0};
   const uint32_t unit = unit_of(dy, e, dy_stride, tokens, dtable, oe, dtable_stride, vocab, cols);
   return by_type(type, [&](auto t) {
     using T = decltype(t);

@@ -19,52 +19,102 @@ namespace rows {
 
 constexpr uint32_t kThreads = 256;
 
-// N elements side by side
-template <typename T, int N> struct Unit {
-  static constexpr int BYTES = N * (int)sizeof(T);
-  typedef typename std::conditional<BYTES == 16, uint4, typename std::conditional<BYTES == 8, uint2, typename std::conditional<BYTES == 4, uint32_t, uint16_t>::type>::type>::type Word;
-  Word w;
-  __device__ __forceinline__ static Unit load(const T *p) { return Unit{*reinterpret_cast<const Word *>(p)}; }
-  __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<Word *>(p) = w; }
+// 16 bytes' elements of a row from column c on, wherever they begin: two aligned pieces that are shifted together when they are used, or, where those would reach
+// beyond the row, elements apart, put together when they are used, too, so that nothing waits for a load before then (columns that the row does not have are 0)
+template <typename T> struct Shifted {
+  static constexpr int V = Vec<T>::V;
+  typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type Bits;
+  static constexpr uint32_t APART = 8;
+  uint32_t w[8], o;
+  __device__ __forceinline__ void load(const T *row, int64_t c, uint32_t cols)
+  {
+    const T *p = row + c;
+    o = (uint32_t)((uintptr_t)p & 15) / sizeof(T);
+    if (c >= (int64_t)o && c - o + (o ? 2 * V : V) <= (int64_t)cols) {
+      *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(p - o);
+      if (o) *reinterpret_cast<uint4 *>(w + 4) = *reinterpret_cast<const uint4 *>(p - o + V);
+      return;
+    }
+    o = APART;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = c + i >= 0 && c + i < cols ? reinterpret_cast<const Bits *>(p)[i] : Bits(0);
+  }
   __device__ __forceinline__ void floats(float *f) const
   {
-    if constexpr (BYTES == 16) Vec<T>{w}.floats(f);
-    else {
+    if (o == APART) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = to_float(reinterpret_cast<const T *>(&w)[i]);
-    }
+      for (int i = 0; i < V; ++i) { const Bits bits = (Bits)w[i]; f[i] = to_float(*reinterpret_cast<const T *>(&bits)); }
+    } else shifted(f);
   }
-  __device__ __forceinline__ static Unit of(const float *f)
+  __device__ __forceinline__ void shifted(float *f) const
   {
-    Unit u;
-    if constexpr (BYTES == 16) u.w = Vec<T>::of(f).bits;
-    else {
+    // (words, and half a word)
+    const uint32_t by = sizeof(T) == 4 ? o : o / 2;
+    uint32_t v[6], u[5];
 #pragma unroll
-      for (int i = 0; i < N; ++i) reinterpret_cast<T *>(&u.w)[i] = from_float<T>(f[i]);
+    for (int i = 0; i < 6; ++i) v[i] = by & 2 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) u[i] = by & 1 ? v[i + 1] : v[i];
+    uint4 all = make_uint4(u[0], u[1], u[2], u[3]);
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t pick = o & 1 ? 0x5432u : 0x3210u;
+      all = make_uint4(__byte_perm(u[0], u[1], pick), __byte_perm(u[1], u[2], pick), __byte_perm(u[2], u[3], pick), __byte_perm(u[3], u[4], pick));
     }
-    return u;
+    Vec<T>{all}.floats(f);
   }
 };
-// N floats of an array of T: in one piece, or two where they are more than 16 bytes
-template <typename T, int N> __device__ __forceinline__ void put_floats(T *p, const float *f)
-{
-  constexpr int M = N * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
+// The same where no piece reaches beyond the row; or, of a thread with a single column, that element (the other words stay 0)
+template <typename T> struct Inside {
+  static constexpr int V = Vec<T>::V;
+  Shifted<T> s;
+  __device__ __forceinline__ void clear()
+  {
+    s.o = 0;
 #pragma unroll
-  for (int i = 0; i < N; i += M) Unit<T, M>::of(f + i).store(p + i);
-}
-// N elements as they lie in memory, in one piece or two
+    for (int i = 0; i < 8; ++i) s.w[i] = 0;
+  }
+  __device__ __forceinline__ void load(const T *p, bool single)
+  {
+    if (single) { s.w[0] = *reinterpret_cast<const typename Shifted<T>::Bits *>(p); return; }
+    s.o = (uint32_t)((uintptr_t)p & 15) / sizeof(T);
+    *reinterpret_cast<uint4 *>(s.w) = *reinterpret_cast<const uint4 *>(p - s.o);
+    if (s.o) *reinterpret_cast<uint4 *>(s.w + 4) = *reinterpret_cast<const uint4 *>(p - s.o + V);
+  }
+  __device__ __forceinline__ void floats(float *f) const { s.shifted(f); }
+};
+// The same of rows that all begin at 16 bytes
+template <typename T> struct Whole {
+  __device__ __forceinline__ void clear() {}
+  __device__ __forceinline__ void load(const T *p, bool) { v = Vec<T>::load(p); }
+  Vec<T> v;
+  __device__ __forceinline__ void load(const T *row, int64_t c, uint32_t) { v = Vec<T>::load(row + c); }
+  __device__ __forceinline__ void floats(float *f) const { v.floats(f); }
+};
+
+// N elements of a row that is written, as they lie in memory
 template <typename T, int N> struct Held {
-  static constexpr int M = N * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : N;
-  Unit<T, M> part[N / M];
+  static constexpr int V = Vec<T>::V, K = N / V ? N / V : 1;
+  Vec<T> part[K];
+  static_assert(N % V == 0, "a table's gradient is of dy's type or a wider one");
   __device__ __forceinline__ void load(const T *p)
   {
 #pragma unroll
-    for (int i = 0; i < N / M; ++i) part[i] = Unit<T, M>::load(p + i * M);
+    for (int i = 0; i < K; ++i) part[i] = Vec<T>::load(p + i * V);
+  }
+  __device__ __forceinline__ void load_each(const T *p, uint32_t n)
+  {
+#pragma unroll
+    for (int i = 0; i < N; ++i) if ((uint32_t)i < n) reinterpret_cast<T *>(part)[i] = p[i];
   }
   __device__ __forceinline__ void floats(float *f) const
   {
 #pragma unroll
-    for (int i = 0; i < N / M; ++i) part[i].floats(f + i * M);
+    for (int i = 0; i < K; ++i) part[i].floats(f + i * V);
+  }
+  __device__ __forceinline__ static void store(T *p, const float *f)
+  {
+#pragma unroll
+    for (int i = 0; i < K; ++i) Vec<T>::of(f + i * V).store(p + i * V);
   }
 };
 
@@ -80,30 +130,38 @@ struct EmbedArgs {
   uint64_t y_stride;
 };
 
-// A team of lanes (a power of two, up to a warp) has a token and M units of E columns per lane; the grid's second dimension has the rest of wide rows
-template <typename T, int E, int M> __global__ void __launch_bounds__(128) embed_kernel(const EmbedArgs a, const uint32_t team)
+// A team of lanes (a power of two, up to a warp) has a token and four slots of 16 bytes of its row per lane; the grid's second dimension has the rest of wide
+// rows.  SHIFT: rows that begin anywhere; slots are those of y's addresses, and a row's first and last may be parts of one.
+template <typename T, bool SHIFT> __global__ void __launch_bounds__(128) embed_kernel(const EmbedArgs a, const uint32_t team)
 {
+  constexpr int V = Vec<T>::V, M = 4;
   const uint64_t i = ((uint64_t)blockIdx.x * 128 + threadIdx.x) / team;
-  const uint32_t lane = threadIdx.x & (team - 1), units = a.cols / E;
+  const uint32_t lane = threadIdx.x & (team - 1);
   pdl_wait();
   pdl_trigger();
   if (i >= a.tokens) return;
   const uint32_t t = token_at(a.token, a.token_bytes, i, a.vocab);
   const T *in = static_cast<const T *>(a.table) + t * a.table_stride;
   T *y = static_cast<T *>(a.y) + i * a.y_stride;
-  for (uint32_t first = blockIdx.y * team * M + lane; first < units; first += gridDim.y * team * M) {
-    Unit<T, E> v[M];
+  const uint32_t ahead = SHIFT ? (uint32_t)((uintptr_t)y & 15) / sizeof(T) : 0, slots = (a.cols + ahead + V - 1) / V;
+  for (uint32_t first = blockIdx.y * team * M + lane; first < slots; first += gridDim.y * team * M) {
+    typename std::conditional<SHIFT, Shifted<T>, Whole<T>>::type v[M];
+    auto column = [&](int k) { return (int64_t)(first + k * team) * V - ahead; };
 #pragma unroll
-    for (int k = 0; k < M; ++k)
-      if (t < a.vocab && first + k * team < units) v[k] = Unit<T, E>::load(in + (uint64_t)(first + k * team) * E);
+    for (int k = 0; k < M; ++k) if (t < a.vocab && first + k * team < slots) v[k].load(in, column(k), a.cols);
 #pragma unroll
     for (int k = 0; k < M; ++k) {
-      if (first + k * team >= units) continue;
-      float f[E];
+      if (first + k * team >= slots) continue;
+      const int64_t c = column(k);
+      float f[V];
       v[k].floats(f);
 #pragma unroll
-      for (int j = 0; j < E; ++j) f[j] = t < a.vocab ? f[j] * a.scale : 0.0f;
-      Unit<T, E>::of(f).store(y + (uint64_t)(first + k * team) * E);
+      for (int j = 0; j < V; ++j) f[j] = t < a.vocab ? f[j] * a.scale : 0.0f;
+      if (!SHIFT || (c >= 0 && c + V <= a.cols)) Vec<T>::of(f).store(y + c);
+      else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) if (c + j >= 0 && c + j < a.cols) y[c + j] = from_float<T>(f[j]);
+      }
     }
   }
 }
@@ -313,101 +371,87 @@ struct SumArgs {
   float *part;                          // [pieces][2][part_cols]: of a long run that begins before the piece, and of one that begins in it
   uint32_t part_cols;
   uint32_t lanes;                       // threads of a piece
+  uint32_t slots, singles;              // of them, those with 16 bytes of columns, and those with a column each
 };
 
 // What a piece adds up: places [from, to), of which the runs of `head` and `tail` are long (else they are ~0)
 struct Piece { uint32_t from, to, head, tail; bool head_before; };
 
-// M units of E columns per thread; a block has kThreads/lanes pieces side by side.  The rows of one step are asked for before those of the step before it are
-// used, whatever runs they belong to, and with them what the table holds where a run ends (ACC).
-template <typename T, typename O, int E, int M, int STEP, bool ACC>
-__global__ void __launch_bounds__(kThreads, ACC && M == 1 ? 2 : 3) embed_sums_kernel(const SumArgs a)
+// A thread has 16 bytes of columns; a block has pieces side by side, each with `lanes` threads.  The rows of one step are asked for before those of the step before it are
+// used, whatever runs they belong to, and with them what the table holds where a run ends (ACC).  SHIFT: rows that begin anywhere, whose first and last columns have
+// a thread each.
+template <typename T, typename O, bool SHIFT, bool ACC>
+__global__ void __launch_bounds__(kThreads, ACC ? 2 : 3) embed_sums_kernel(const SumArgs a)
 {
+  constexpr int E = Vec<T>::V, STEP = SHIFT ? 2 : 4;
   constexpr uint32_t PIECES = kThreads / kLeastLanes;
   __shared__ uint32_t key[PIECES * kMostPiece + 2 * kLong], place[PIECES * kMostPiece + 2 * kLong];
   __shared__ Piece piece[PIECES];
   pdl_wait();
   pdl_trigger();
-  const uint32_t per_block = kThreads / a.lanes, first = blockIdx.x * per_block, lane = threadIdx.x & 31;
+  const uint32_t per_block = blockDim.x / a.lanes, first = blockIdx.x * per_block, lane = threadIdx.x & 31;
   // the places of the block's pieces and kLong on either side; what is no token ends the sorted ones
   const int64_t begin = (int64_t)first * a.piece - kLong;
-  for (uint32_t i = threadIdx.x; i < per_block * a.piece + 2 * kLong; i += kThreads) {
+  for (uint32_t i = threadIdx.x; i < per_block * a.piece + 2 * kLong; i += blockDim.x) {
     const int64_t at = begin + i;
     const bool inside = at >= 0 && at < a.n;
-    key[i] = inside ? a.key[at] : ~0u;
+    const uint32_t k = inside ? a.key[at] : ~0u;
+    key[i] = k < a.vocab ? k : ~0u;
     place[i] = inside ? a.place[at] : 0;
   }
   __syncthreads();
   // a warp looks at a piece: how far the runs of its first and last token go, up to kLong places
-  for (uint32_t p = threadIdx.x >> 5; p < per_block; p += kThreads / 32) {
+  for (uint32_t p = threadIdx.x >> 5; p < per_block; p += blockDim.x / 32) {
     const uint32_t at = kLong + p * a.piece, size = min(a.piece, a.n - min(a.n, (first + p) * a.piece)), last = at + size - 1;
     auto run = [&](uint32_t k, uint32_t from, int step) {        // places from `from` on, in steps, that have token k
       const uint32_t other = ~__ballot_sync(0xffffffffu, key[(int)from + step * (int)lane] == k);
       return other ? (uint32_t)__ffs((int)other) - 1 : 32u;
     };
     Piece q = {at, at, ~0u, ~0u, false};
-    if (size && key[at] < a.vocab) {
+    if (size && key[at] != ~0u) {
       const uint32_t k0 = key[at], before = run(k0, at - 1, -1), after = run(k0, at + 1, 1);
       const bool long0 = before + 1 + after > a.longest;
       const uint32_t k1 = key[last], ahead = run(k1, last - 1, -1), behind = run(k1, last + 1, 1);
-      const bool long1 = k1 < a.vocab && ahead + 1 + behind > a.longest, whole = k0 == k1;
+      const bool long1 = k1 != ~0u && ahead + 1 + behind > a.longest, whole = k0 == k1;
       q.head_before = before > 0;
       if (before && !long0) q.from = at + 1 + after;             // (that run is an earlier piece's)
       if (long0) q.head = k0;
       if (long1) q.tail = k1;
-      q.to = long1 || k1 >= a.vocab ? last + 1 : last + 1 + behind;
+      q.to = long1 || k1 == ~0u ? last + 1 : last + 1 + behind;
       if (q.from > q.to || (whole && before && !long0)) q.to = q.from;
     }
     if (lane == 0) piece[p] = q;
-    if (first + p >= a.pieces || blockIdx.y) continue;
-    // the parts of a long run that begins here: this one, the pieces behind it that it fills, and one that it ends in
-    if (q.tail != ~0u && !(q.tail == q.head && q.head_before)) {
-      uint32_t filled = 32, r = first + p + 1;
-      for (; filled == 32; r += filled) {
-        const uint64_t end = (uint64_t)(r + lane + 1) * a.piece;
-        const uint32_t others = ~__ballot_sync(0xffffffffu, end <= a.n && a.key[end - 1] == q.tail);
-        filled = others ? (uint32_t)__ffs((int)others) - 1 : 32u;
-      }
-      const uint32_t parts = r - (first + p) + (r < a.pieces && a.key[(uint64_t)r * a.piece] == q.tail);
-      if (lane == 0) a.run[atomicAdd(a.runs, 1u)] = make_uint4(first + p, q.tail, parts, 0);
-    }
   }
   __syncthreads();
   const uint32_t mine = threadIdx.x / a.lanes;
   const Piece q = piece[mine];
-  const uint64_t unit = (uint64_t)blockIdx.y * a.lanes * M + (threadIdx.x & (a.lanes - 1));
-  const T *dy = static_cast<const T *>(a.dy) + unit * E;
-  O *out = static_cast<O *>(a.dtable) + unit * E;
-  float *part = a.part + ((uint64_t)(first + mine) * 2 * a.part_cols) + unit * E;
-  bool has[M];
+  // slots from the row's start on, or with a slot left out there; then single columns: those before the slots, and those behind them
+  const uint32_t at = blockIdx.y * a.lanes + (threadIdx.x - mine * a.lanes);
+  const bool single = SHIFT && at >= a.slots, has = at < a.slots + a.singles;
+  const uint32_t ahead = SHIFT && a.slots ? E : 0, width = !has ? 0 : single ? 1 : E;
+  const uint64_t column = !single ? (uint64_t)at * E + ahead : at - a.slots < ahead ? at - a.slots : (uint64_t)a.slots * E + (at - a.slots);
+  const T *dy = static_cast<const T *>(a.dy) + column;
+  O *out = static_cast<O *>(a.dtable) + column;
+  float *part = a.part + ((uint64_t)(first + mine) * 2 * a.part_cols) + column;
+  float sum[E];
 #pragma unroll
-  for (int m = 0; m < M; ++m) has[m] = (unit + (uint64_t)m * a.lanes) * E < a.cols;
-  float sum[M][E];
-#pragma unroll
-  for (int m = 0; m < M; ++m)
-#pragma unroll
-    for (int j = 0; j < E; ++j) sum[m][j] = 0.0f;
+  for (int j = 0; j < E; ++j) sum[j] = 0.0f;
   struct Stage {
     uint32_t k[STEP + 1];               // the places' tokens, and the one behind them; ~0: none
-    Unit<T, E> v[STEP][M];
-    Held<O, E> old[ACC ? STEP : 1][M];
+    typename std::conditional<SHIFT, Inside<T>, Whole<T>>::type v[STEP];
+    Held<O, E> old[ACC ? STEP : 1];
   };
   auto fetch = [&](Stage &g, uint32_t i) {
 #pragma unroll
-    for (int s = 0; s <= STEP; ++s) { g.k[s] = i + s < q.to ? key[i + s] : ~0u; if (g.k[s] >= a.vocab) g.k[s] = ~0u; }
+    for (int s = 0; s <= STEP; ++s) g.k[s] = has && i + s < q.to ? key[i + s] : ~0u;
 #pragma unroll
-    for (int s = 0; s < STEP; ++s) {
-      if (g.k[s] == ~0u) continue;
-      const T *row = dy + place[i + s] * a.dy_stride;
-#pragma unroll
-      for (int m = 0; m < M; ++m) if (has[m]) g.v[s][m] = Unit<T, E>::load(row + (uint64_t)m * a.lanes * E);
-    }
+    for (int s = 0; s < STEP; ++s) if (g.k[s] != ~0u) g.v[s].load(dy + place[i + s] * a.dy_stride, single);
     if constexpr (ACC) {
 #pragma unroll
       for (int s = 0; s < STEP; ++s) {
         if (g.k[s] == g.k[s + 1]) continue;
-#pragma unroll
-        for (int m = 0; m < M; ++m) if (has[m]) g.old[s][m].load(out + g.k[s] * a.stride + (uint64_t)m * a.lanes * E);
+        const O *from = out + g.k[s] * a.stride;
+        if constexpr (SHIFT) g.old[s].load_each(from, width); else g.old[s].load(from);
       }
     }
   };
@@ -415,35 +459,34 @@ __global__ void __launch_bounds__(kThreads, ACC && M == 1 ? 2 : 3) embed_sums_ke
 #pragma unroll
     for (int s = 0; s < STEP; ++s) {
       if (g.k[s] == ~0u) continue;
+      float f[E];
+      g.v[s].floats(f);
 #pragma unroll
-      for (int m = 0; m < M; ++m) {
-        float f[E];
-        g.v[s][m].floats(f);
-#pragma unroll
-        for (int j = 0; j < E; ++j) sum[m][j] += f[j];
-      }
+      for (int j = 0; j < E; ++j) sum[j] += f[j];
       if (g.k[s] == g.k[s + 1]) continue;
       // the run's end, or that of the piece's part of a long one
-      const bool is_long = g.k[s] == q.head || g.k[s] == q.tail;
-      float *to = part + (g.k[s] == q.head && q.head_before ? 0 : a.part_cols);
+      if (g.k[s] == q.head || g.k[s] == q.tail) {
+        float *to = part + (g.k[s] == q.head && q.head_before ? 0 : a.part_cols);
 #pragma unroll
-      for (int m = 0; m < M; ++m) {
-        if (has[m] && is_long) {
+        for (int j = 0; j < E; ++j) if ((uint32_t)j < width) to[j] = sum[j];
+      } else {
+        O *to = out + g.k[s] * a.stride;
+        if constexpr (ACC) g.old[s].floats(f);
 #pragma unroll
-          for (int j = 0; j < E; ++j) to[(uint64_t)m * a.lanes * E + j] = sum[m][j];
-        } else if (has[m]) {
-          float f[E];
-          if constexpr (ACC) g.old[s][m].floats(f);
+        for (int j = 0; j < E; ++j) sum[j] = ACC ? fmaf(sum[j], a.scale, f[j]) : sum[j] * a.scale;
+        if constexpr (!SHIFT) Held<O, E>::store(to, sum);
+        else {
 #pragma unroll
-          for (int j = 0; j < E; ++j) sum[m][j] = ACC ? fmaf(sum[m][j], a.scale, f[j]) : sum[m][j] * a.scale;
-          put_floats<O, E>(out + g.k[s] * a.stride + (uint64_t)m * a.lanes * E, sum[m]);
+          for (int j = 0; j < E; ++j) if ((uint32_t)j < width) to[j] = from_float<O>(sum[j]);
         }
-#pragma unroll
-        for (int j = 0; j < E; ++j) sum[m][j] = 0.0f;
       }
+#pragma unroll
+      for (int j = 0; j < E; ++j) sum[j] = 0.0f;
     }
   };
   Stage one, two;
+#pragma unroll
+  for (int s = 0; s < STEP; ++s) { one.v[s].clear(); two.v[s].clear(); }
   fetch(one, q.from);
   for (uint32_t i = q.from; i < q.to; i += 2 * STEP) {
     fetch(two, i + STEP);
@@ -451,21 +494,33 @@ __global__ void __launch_bounds__(kThreads, ACC && M == 1 ? 2 : 3) embed_sums_ke
     fetch(one, i + 2 * STEP);
     use(two);
   }
+  // the long runs that begin here: this piece, those behind it that the run fills, and one that it ends in
+  for (uint32_t p = threadIdx.x >> 5; p < per_block && blockIdx.y == 0; p += blockDim.x / 32) {
+    const uint32_t k = piece[p].tail;
+    if (k == ~0u || (k == piece[p].head && piece[p].head_before)) continue;
+    uint32_t filled = 32, r = first + p + 1;
+    for (; filled == 32; r += filled) {
+      const uint64_t end = (uint64_t)(r + lane + 1) * a.piece;
+      const uint32_t others = ~__ballot_sync(0xffffffffu, end <= a.n && a.key[end - 1] == k);
+      filled = others ? (uint32_t)__ffs((int)others) - 1 : 32u;
+    }
+    const uint32_t parts = r - (first + p) + (r < a.pieces && a.key[(uint64_t)r * a.piece] == k);
+    if (lane == 0) a.run[atomicAdd(a.runs, 1u)] = make_uint4(first + p, k, parts, 0);
+  }
 }
 
-// The parts of long runs: a block has 128 columns and every gridDim.y-th such run; a warp adds a quarter of the run's parts, in order
-constexpr uint32_t kJoinThreads = 128;
-template <typename O> __global__ void __launch_bounds__(kJoinThreads) embed_join_kernel(const SumArgs a, const int accumulate)
+// The parts of long runs: a block has 32 columns, four to a lane, and every gridDim.y-th such run, whose parts its 32 groups of lanes add in order, each a stretch
+template <typename O> __global__ void __launch_bounds__(kThreads) embed_join_kernel(const SumArgs a, const int accumulate)
 {
-  constexpr uint32_t WARPS = kJoinThreads / 32;
-  __shared__ float sums[WARPS][4][32];
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint64_t c = ((uint64_t)blockIdx.x * 32 + lane) * 4;
+  constexpr uint32_t GROUPS = kThreads / 8;
+  __shared__ float sums[GROUPS][33];
+  const uint32_t group = threadIdx.x / 8, lane = threadIdx.x & 7;
+  const uint64_t c = (uint64_t)blockIdx.x * 32 + lane * 4, column = (uint64_t)blockIdx.x * 32 + threadIdx.x;
   pdl_wait();
   const uint32_t runs = *a.runs;
   for (uint32_t i = blockIdx.y; i < runs; i += gridDim.y) {
     const uint4 run = a.run[i];
-    const uint32_t parts = run.z, each = (parts + WARPS - 1) / WARPS, lo = min(parts, warp * each), hi = min(parts, lo + each);
+    const uint32_t parts = run.z, each = (parts + GROUPS - 1) / GROUPS, lo = min(parts, group * each), hi = min(parts, lo + each);
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (c < a.cols) {
 #pragma unroll 8
@@ -474,18 +529,15 @@ template <typename O> __global__ void __launch_bounds__(kJoinThreads) embed_join
         sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
       }
     }
-    sums[warp][0][lane] = sum.x; sums[warp][1][lane] = sum.y; sums[warp][2][lane] = sum.z; sums[warp][3][lane] = sum.w;
-    // a warp writes 32 columns side by side
-    const uint32_t mine = warp * 32 + lane;
-    const uint64_t column = (uint64_t)blockIdx.x * 128 + mine;
-    O *to = static_cast<O *>(a.dtable) + run.y * a.stride + column;
-    const float old = accumulate && column < a.cols ? to_float(*to) : 0.0f;
+    float *const to = sums[group] + lane * 4;
+    to[0] = sum.x; to[1] = sum.y; to[2] = sum.z; to[3] = sum.w;
     __syncthreads();
-    if (column < a.cols) {
-      float total = 0.0f;
+    if (threadIdx.x < 32 && column < a.cols) {
+      O *out = static_cast<O *>(a.dtable) + run.y * a.stride + column;
+      float total = accumulate ? to_float(*out) : 0.0f, all = 0.0f;
 #pragma unroll
-      for (uint32_t w = 0; w < WARPS; ++w) total += sums[w][mine & 3][mine >> 2];
-      *to = from_float<O>(accumulate ? fmaf(total, a.scale, old) : total * a.scale);
+      for (uint32_t g = 0; g < GROUPS; ++g) all += sums[g][threadIdx.x];
+      *out = from_float<O>(accumulate ? fmaf(all, a.scale, total) : all * a.scale);
     }
     __syncthreads();
   }
@@ -498,17 +550,10 @@ inline int check_tokens(const void *token, int bytes)
   return aligned_to(token, (size_t)bytes) ? ANODE_OK : ANODE_E_ALIGN;
 }
 
-// Columns to a unit that both arrays' rows allow: as many as 16 bytes of the narrower type hold, two, or one
-inline uint32_t unit_of(const void *p, size_t bytes, uint64_t stride, uint64_t rows, const void *q, size_t q_bytes, uint64_t q_stride, uint64_t q_rows, uint32_t cols)
+// Whether rows all begin at 16 bytes and are whole numbers of them
+inline bool whole(const void *p, size_t bytes, uint64_t stride, uint64_t rows, uint32_t cols)
 {
-  auto fits = [&](const void *x, size_t e, uint64_t s, uint64_t n, uint32_t width) {
-    const size_t most = width * e < 16 ? width * e : 16;
-    return aligned_to(x, most) && (n <= 1 || s * e % most == 0);
-  };
-  const size_t least = bytes < q_bytes ? bytes : q_bytes;
-  for (uint32_t width : {(uint32_t)(16 / least), 2u})
-    if (cols % width == 0 && fits(p, bytes, stride, rows, width) && fits(q, q_bytes, q_stride, q_rows, width)) return width;
-  return 1;
+  return aligned_to(p, 16) && cols * bytes % 16 == 0 && (rows <= 1 || stride * bytes % 16 == 0);
 }
 inline uint32_t power_up_to(uint64_t n, uint32_t most)
 {
@@ -517,17 +562,19 @@ inline uint32_t power_up_to(uint64_t n, uint32_t most)
   return v;
 }
 
-// Places of a piece: as many as give each multiprocessor three blocks of a row's width; a run of more is long, or of more than 8
-inline uint32_t piece_of(uint64_t tokens)
+// Places of a piece: as many as give each multiprocessor three blocks, of as many pieces side by side as rows of 16-bit columns leave them; a run of more is long, or
+// of more than 8
+inline uint32_t piece_of(uint64_t tokens, uint32_t cols)
 {
-  const uint64_t each = (tokens + 3 * 148 - 1) / (3 * 148);
+  const uint32_t side_by_side = kThreads / power_up_to(((uint64_t)cols + 7) / 8, kThreads);
+  const uint64_t pieces = 3ull * 148 * side_by_side, each = (tokens + pieces - 1) / pieces;
   return (uint32_t)(each < 4 ? 4 : each < kMostPiece ? each : kMostPiece);
 }
 
 // Where the workspace's arrays begin, in bytes
 struct Layout {
   uint64_t n, piece, longest, pieces, part_cols, runs, run, part, bytes;
-  Layout(uint64_t tokens, uint32_t cols) : n((tokens + 3) / 4 * 4), piece(piece_of(tokens)), longest(piece < 8 ? 8 : piece), pieces((tokens + piece - 1) / piece), part_cols(((uint64_t)cols + 3) / 4 * 4)
+  Layout(uint64_t tokens, uint32_t cols) : n((tokens + 3) / 4 * 4), piece(piece_of(tokens, cols)), longest(piece < 8 ? 8 : piece), pieces((tokens + piece - 1) / piece), part_cols(((uint64_t)cols + 3) / 4 * 4)
   {
     runs = 16 * n;
     run = runs + 16;
@@ -536,26 +583,24 @@ struct Layout {
   }
 };
 
-template <typename T, typename O, int E> int launch_sums(SumArgs a, int accumulate, cudaStream_t stream)
+template <typename T, typename O> int launch_sums(SumArgs a, bool shift, int accumulate, cudaStream_t stream)
 {
-  constexpr int M = E * sizeof(T) == 16 ? 1 : 2;
-  const uint32_t units = a.cols / E;
-  a.lanes = power_up_to((units + M - 1) / M, kThreads);
+  constexpr uint32_t V = Vec<T>::V;
+  a.slots = a.cols / V;
+  // (rows that begin anywhere: two aligned pieces around each slot are to be inside of the row)
+  if (shift) a.slots = a.slots > 2 ? a.slots - 2 : 0;
+  a.singles = a.cols - a.slots * V;
+  const uint32_t all = a.slots + a.singles;
+  a.lanes = all > kThreads ? kThreads : all > 32 ? (all + 31) / 32 * 32 : power_up_to(all, 32);
   if (a.lanes < kLeastLanes) a.lanes = kLeastLanes;
-  const uint32_t per_block = kThreads / a.lanes, wide = (units + a.lanes * M - 1) / (a.lanes * M);
-  const dim3 grid((a.pieces + per_block - 1) / per_block, wide);
-  return accumulate ? launch(embed_sums_kernel<T, O, E, M, 4, true>, grid, kThreads, 0, stream, a)
-                    : launch(embed_sums_kernel<T, O, E, M, 4, false>, grid, kThreads, 0, stream, a);
-}
-template <typename T, typename O> int launch_sums(const SumArgs &a, uint32_t unit, int accumulate, cudaStream_t stream)
-{
-  constexpr int V = 16 / sizeof(T);
-  TRY((unit == (uint32_t)V ? launch_sums<T, O, V>(a, accumulate, stream) : unit == 2 ? launch_sums<T, O, 2>(a, accumulate, stream)
-                                                                                      : launch_sums<T, O, 1>(a, accumulate, stream)));
+  const uint32_t per_block = kThreads / a.lanes;
+  const dim3 grid((a.pieces + per_block - 1) / per_block, (all + a.lanes - 1) / a.lanes);
+  TRY(launch(accumulate ? (shift ? embed_sums_kernel<T, O, true, true> : embed_sums_kernel<T, O, false, true>)
+                        : (shift ? embed_sums_kernel<T, O, true, false> : embed_sums_kernel<T, O, false, false>), grid, per_block * a.lanes, 0, stream, a));
   if (a.n <= a.longest) return ANODE_OK;
   // a run to a block, of the tokens of a training batch: some 50 of 16384 come more than 32 times
-  const uint32_t wide = (uint32_t)(((uint64_t)a.cols + 127) / 128), most = a.n / (a.longest + 1), blocks = (16 * sm_count() + wide - 1) / wide;
-  return launch(embed_join_kernel<O>, dim3(wide, blocks < most ? blocks : most), kJoinThreads, 0, stream, a, accumulate);
+  const uint32_t wide = (uint32_t)(((uint64_t)a.cols + 31) / 32), most = a.n / (a.longest + 1), blocks = (16 * sm_count() + wide - 1) / wide;
+  return launch(embed_join_kernel<O>, dim3(wide, blocks < most ? blocks : most), kThreads, 0, stream, a, accumulate);
 }
 
 }  // namespace rows
@@ -578,15 +623,14 @@ extern "C" int anode_gpu_embed_tokens_fwd(
   TRY(check_rows(y, e, tokens, cols, y_stride, true));
   if (y == table) return ANODE_E_STRIDE;
   const EmbedArgs a = {tokens, vocab, cols, scale, token, token_bytes, table, table_stride, y, y_stride};
-  const uint32_t unit = unit_of(table, e, table_stride, vocab, y, e, y_stride, tokens, cols);
+  const bool shift = !whole(table, e, table_stride, vocab, cols) || !whole(y, e, y_stride, tokens, cols);
   return by_type(type, [&](auto t) {
     using T = decltype(t);
-    constexpr uint32_t V = 16 / sizeof(T);
-    const uint32_t units = cols / unit, each = unit == V ? 4 : 8, team = power_up_to((units + each - 1) / each, 32);
-    const uint64_t wide = ((uint64_t)units + team * each - 1) / (team * each);
+    constexpr uint32_t V = Vec<T>::V;
+    const uint32_t slots = (cols + (shift ? 2 * V - 2 : V - 1)) / V, team = power_up_to((slots + 3) / 4, 32);
+    const uint64_t wide = ((uint64_t)slots + team * 4 - 1) / (team * 4);
     const dim3 grid((uint32_t)((tokens * team + 127) / 128), (uint32_t)(wide < 65535 ? wide : 65535));
-    return unit == V ? launch(embed_kernel<T, (int)V, 4>, grid, 128, 0, stream, a, team)
-         : unit == 2 ? launch(embed_kernel<T, 2, 8>, grid, 128, 0, stream, a, team) : launch(embed_kernel<T, 1, 8>, grid, 128, 0, stream, a, team);
+    return launch(shift ? embed_kernel<T, true> : embed_kernel<T, false>, grid, 128, 0, stream, a, team);
   });
 }
 
@@ -604,7 +648,7 @@ extern "C" int anode_gpu_embed_tokens_bwd(
 {
   (void)cfg;
   if (!known_type(type) || (dtable_type != type && dtable_type != ANODE_TYPE_F32)) return ANODE_E_TYPE;
-  if (!served(0, cols) || !served(0, vocab) || tokens >> 31) return ANODE_E_DIMS;
+  if (!served(0, cols) || !served(0, vocab) || tokens >> 31 || cols >> 25) return ANODE_E_DIMS;      // (a grid's second dimension)
   if (tokens == 0 && accumulate) return ANODE_OK;
   const size_t e = type_bytes(type), oe = type_bytes(dtable_type);
   TRY(check_rows(dtable, oe, vocab, cols, dtable_stride, true));
@@ -641,10 +685,10 @@ extern "C" int anode_gpu_embed_tokens_bwd(
   if (!tokens) return ANODE_OK;
   const SumArgs a = {(uint32_t)tokens, vocab, cols, scale, s.key[0], s.place[0], dy, dy_stride, dtable, dtable_stride, (uint32_t)l.piece, (uint32_t)l.pieces, (uint32_t)l.longest,
                      words + l.runs / 4, reinterpret_cast<uint4 *>(static_cast<char *>(workspace) + l.run), reinterpret_cast<float *>(static_cast<char *>(workspace) + l.part), (uint32_t)l.part_cols, 0};
-  const uint32_t unit = unit_of(dy, e, dy_stride, tokens, dtable, oe, dtable_stride, vocab, cols);
+  const bool shift = !whole(dy, e, dy_stride, tokens, cols) || !whole(dtable, oe, dtable_stride, vocab, cols);
   return by_type(type, [&](auto t) {
     using T = decltype(t);
-    if constexpr (sizeof(T) == 2) { if (dtable_type != ANODE_TYPE_F32) return launch_sums<T, T>(a, unit, accumulate, stream); }
-    return launch_sums<T, float>(a, unit, accumulate, stream);
+    if constexpr (sizeof(T) == 2) { if (dtable_type != ANODE_TYPE_F32) return launch_sums<T, T>(a, shift, accumulate, stream); }
+    return launch_sums<T, float>(a, shift, accumulate, stream);
   });
 }

@@ -609,7 +609,8 @@ int anode_gpu_rotary_positions_bwd(
  * Section 4's conventions hold: element types and strides are arguments, arithmetic is in f32, every output is rounded once, no rows
  * are a call that does nothing, sums are taken in a fixed order, and workspaces hold nothing from call to call.  Tokens are packed signed
  * integers of token_bytes (4 or 8) bytes; one outside of [0, vocab) stands for no token.
- * Sizes: rows and columns as in section 4 (a table's rows and a row's logits count as columns do), fewer than 2^31 tokens of a table.
+ * Sizes: rows and columns as in section 4 (a table's rows and a row's logits count as columns do), fewer than 2^31 tokens of a table, whose gradient has
+ * fewer than 2^25 columns.
  * =================================================================================== */
 
 /* Layer norm with the residual's addition, forward:

@@ -11,8 +11,8 @@ namespace anode_b200 {
 namespace rows {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kMostTop = 128;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kMostThreads = 1024, kMostTop = 128;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFloor = -1e4f;            // below what exp leaves above zero: 0 takes the place of 0 * -infinity
 
 struct ProbsArgs {
@@ -64,17 +64,6 @@ __device__ __forceinline__ float value_of(uint32_t order)
 // the larger value, of equal ones the lower index, is the larger key
 __device__ __forceinline__ uint64_t key_of(float v, uint32_t index) { return (uint64_t)order_of(v) << 32 | (uint32_t)~index; }
 
-__device__ __forceinline__ uint64_t block_max_all(uint64_t v, uint64_t *buf)
-{
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) { const uint64_t w = __shfl_xor_sync(0xffffffffu, v, o); v = w > v ? w : v; }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  for (uint32_t i = 0; i < blockDim.x / 32; ++i) v = buf[i] > v ? buf[i] : v;
-  return v;
-}
-
 __device__ __forceinline__ void put_top(const ProbsArgs &a, uint64_t row, uint32_t k, uint64_t key, float m, float log_sum)
 {
   const float v = value_of((uint32_t)(key >> 32));
@@ -86,47 +75,263 @@ __device__ __forceinline__ void put_top(const ProbsArgs &a, uint64_t row, uint32
   }
 }
 
-// Any rows: a block has a row at a time, element by element: once for the largest, once for the sums, once for each of the likeliest
-template <typename T> __global__ void __launch_bounds__(kThreads) token_log_probs_rows_kernel(const ProbsArgs a)
+// 2^v; v below -126 gives 0
+__device__ __forceinline__ float exp2_of(float v)
 {
-  __shared__ float buf[2][32];
-  __shared__ uint64_t keys[kThreads / 32];
+  float d;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v));
+  return d;
+}
+
+// 16 bytes of logits: the largest of them, and of what is none
+template <typename T> __device__ __forceinline__ float largest_of(const uint4 &v)
+{
+  if constexpr (sizeof(T) == 4) return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+  else {
+    typedef typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type Pair;
+    auto pair = [](uint32_t w) { return *reinterpret_cast<const Pair *>(&w); };
+    const Pair m = __hmax2_nan(__hmax2_nan(pair(v.x), pair(v.y)), __hmax2_nan(pair(v.z), pair(v.w)));
+    return max_nan(to_float(m.x), to_float(m.y));
+  }
+}
+template <typename T> __device__ __forceinline__ uint4 nothing()
+{
+  constexpr uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;      // -infinity
+  return make_uint4(w, w, w, w);
+}
+
+// Of some logits: the largest, the sum of 2^d over them and that of d*2^d, d = (x - largest)*rate in powers of two (log2(e)*scale is `rate`)
+struct Sums {
+  float m, sum, dot;
+  // as if the largest were `to`
+  __device__ __forceinline__ void move(float to, float rate)
+  {
+    const float d = max_nan((m - (to == -INFINITY ? 0.0f : to)) * rate, kFloor), by = exp2_of(d);
+    dot = by * fmaf(d, sum, dot);
+    sum *= by;
+    m = to;
+  }
+};
+
+constexpr uint32_t kBuffer = 1024;         // keys that may be among the likeliest
+
+// A row's logits are shared out to a cluster's blocks, and theirs to the threads by slots of 16 bytes in turn: one pass with a running maximum and sums that
+// follow it.  The likeliest: the k-th largest of the threads' maxima is a bound that k logits reach at least, so that few threads have more of them, whose
+// slots are read again.
+template <typename T, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(kMostThreads) token_log_probs_kernel(const ProbsArgs a, const uint32_t cluster)
+{
+  constexpr int V = Vec<T>::V, U = 4;
+  __shared__ Sums sums[32], block_sums;
+  __shared__ uint64_t buffer[TOP ? kBuffer : 1], best[TOP ? kMostTop : 1], lists[TOP ? 8 * kMostTop : 1];
+  __shared__ uint32_t listed[TOP ? kMostThreads : 1], count, bound_count;
+  const uint32_t threads = blockDim.x, warps = threads / 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t rank = cluster > 1 ? cluster_rank() : 0;
+  const float rate = fminf(a.scale * kLog2e, 3.402823466e38f);
+  auto sync = [&] { if (cluster > 1) cluster_sync(); else __syncthreads(); };
   pdl_wait();
-  for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  pdl_trigger();
+  for (uint64_t row = blockIdx.x / cluster; row < a.rows; row += gridDim.x / cluster) {
     const T *x = static_cast<const T *>(a.logits) + row * a.stride;
-    uint64_t best = 0;
-    for (uint32_t c = threadIdx.x; c < a.vocab; c += kThreads) { const uint64_t k = key_of(to_float(x[c]), c); best = k > best ? k : best; }
-    best = block_max_all(best, keys);
-    const float m = value_of((uint32_t)(best >> 32)), from = m == -INFINITY ? 0.0f : m;
-    float sum = 0.0f, dot = 0.0f;
-    for (uint32_t c = threadIdx.x; c < a.vocab; c += kThreads) {
-      const float z = max_nan(a.scale * (to_float(x[c]) - from), kFloor), e = expf(z);
-      sum += e;
-      dot = fmaf(z, e, dot);
+    // logits before the first whole slot, slots, and logits behind the last; this block's slots [begin, end)
+    const uint32_t head = min(a.vocab, (uint32_t)(-(int)((uintptr_t)x / sizeof(T)) & (V - 1))), slots = (a.vocab - head) / V, tail = a.vocab - head - slots * V;
+    const uint32_t part = (slots + cluster - 1) / cluster, begin = min(slots, rank * part), end = min(slots, begin + part);
+    const uint4 *from = reinterpret_cast<const uint4 *>(x + head);
+    const bool on_edge = rank == 0 && threadIdx.x < head + tail, first = rank == 0 && threadIdx.x == 0;
+    const uint32_t edge = threadIdx.x < head ? threadIdx.x : a.vocab - tail + (threadIdx.x - head);
+    uint32_t token = a.vocab;
+    float picked = 0.0f;
+    if (first && a.logprob) {
+      token = token_at(a.token, a.token_bytes, row, a.vocab);
+      if (token < a.vocab) picked = to_float(x[token]);
     }
-    sum = block_sum_all(sum, buf[0]);
-    dot = block_sum_all(dot, buf[1]);
-    const bool empty = m == -INFINITY;
-    const float log_sum = empty ? 0.0f : logf(sum);
-    if (threadIdx.x == 0) {
-      if (a.logprob) {
-        const uint32_t t = token_at(a.token, a.token_bytes, row, a.vocab);
-        a.logprob[row] = t == a.vocab ? 0.0f : empty ? m : a.scale * (to_float(x[t]) - m) - log_sum;
+    Sums own = {-INFINITY, 0.0f, 0.0f};
+    float2 sum = both(0.0f), dot = both(0.0f);
+    auto absorb = [&](const uint4 *v, int n) {
+      float m = own.m;
+#pragma unroll
+      for (int u = 0; u < n; ++u) m = max_nan(m, largest_of<T>(v[u]));
+      own.sum = sum.x; own.dot = dot.x;
+      Sums other = {own.m, sum.y, dot.y};
+      own.move(m, rate); other.move(m, rate);
+      sum = make_float2(own.sum, other.sum); dot = make_float2(own.dot, other.dot);
+      const float2 minus = both(m == -INFINITY ? 0.0f : -m), times = both(rate);
+#pragma unroll
+      for (int u = 0; u < n; ++u) {
+        float2 f[V / 2];
+        Vec<T>{v[u]}.floats(reinterpret_cast<float *>(f));
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          float2 d = mul2(add2(f[i], minus), times);
+          if (ENTROPY) d = make_float2(max_nan(d.x, kFloor), max_nan(d.y, kFloor));
+          const float2 e = make_float2(exp2_of(d.x), exp2_of(d.y));
+          sum = add2(sum, e);
+          if (ENTROPY) dot = fma2(d, e, dot);
+        }
       }
-      if (a.entropy) a.entropy[row] = empty ? 0.0f : log_sum - dot / sum;
-      if (a.stats) a.stats[row] = make_float2(m, log_sum);
-      if (a.top) put_top(a, row, 0, best, m, log_sum);
+    };
+    uint4 next[U];
+    auto fetch = [&](uint32_t s) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        next[u] = nothing<T>();
+        if (s + u * threads < end) next[u] = from[s + u * threads];
+      }
+    };
+    fetch(begin + threadIdx.x);
+    for (uint32_t s = begin + threadIdx.x; s < end; s += U * threads) {
+      uint4 now[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) now[u] = next[u];
+      fetch(s + U * threads);
+      absorb(now, U);
     }
-    for (uint32_t k = 1; k < a.top; ++k) {
-      uint64_t next = 0;
-      for (uint32_t c = threadIdx.x; c < a.vocab; c += kThreads) { const uint64_t q = key_of(to_float(x[c]), c); if (q < best && q > next) next = q; }
-      best = block_max_all(next, keys);
-      if (threadIdx.x == 0) put_top(a, row, k, best, m, log_sum);
+    if (on_edge) {
+      uint4 v = nothing<T>();
+      *reinterpret_cast<T *>(&v) = x[edge];
+      absorb(&v, 1);
     }
+    own.sum = sum.x + sum.y; own.dot = dot.x + dot.y;
+    const uint32_t order = order_of(own.m);
+    // the block's sums
+    auto warp_join = [&](Sums &v) {
+      float m = v.m;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      v.move(m, rate);
+      v.sum = warp_sum_all(v.sum);
+      if (ENTROPY) v.dot = warp_sum_all(v.dot);
+    };
+    warp_join(own);
+    if (lane == 0) sums[warp] = own;
     __syncthreads();
+    if (warp == 0) {
+      own = lane < warps ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f};
+      if (warps > 1) warp_join(own);
+      if (lane == 0) block_sums = own;
+    }
+    if constexpr (TOP) {
+      // the upper half of the bits of a value that a.top threads' maxima reach
+      uint32_t bound = 0;
+      for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
+        if ((uint32_t)__syncthreads_count(order >= (bound | bit)) >= a.top) bound |= bit;
+      uint64_t least = bound ? (uint64_t)bound << 32 : 1;      // (no logit has the key 0)
+      const uint32_t each = (end - begin + threads - 1) / threads;
+      for (;;) {
+        // the threads whose maxima reach it
+        __syncthreads();
+        if (threadIdx.x == 0) count = bound_count = 0;
+        __syncthreads();
+        if (order >= (uint32_t)(least >> 32)) listed[atomicAdd(&bound_count, 1u)] = threadIdx.x;
+        __syncthreads();
+        const uint32_t found = bound_count;
+        // keys from `least` on: those that find no place in the buffer take one of another, so that it holds some of all
+        auto push = [&](const uint64_t *key, int n) {
+          uint32_t mine = 0;
+#pragma unroll
+          for (int i = 0; i < n; ++i) mine += key[i] >= least;
+          if (!__any_sync(0xffffffffu, mine != 0)) return;
+          uint32_t at = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o *= 2) { const uint32_t w = __shfl_up_sync(0xffffffffu, at, o); if (lane >= o) at += w; }
+          uint32_t start = 0;
+          if (lane == 31) start = atomicAdd(&count, at);
+          at += __shfl_sync(0xffffffffu, start, 31) - mine;
+#pragma unroll
+          for (int i = 0; i < n; ++i)
+            if (key[i] >= least) { buffer[at < kBuffer ? at : (at * 2654435761u) >> 22] = key[i]; ++at; }
+        };
+        for (uint32_t q = warp; q < found; q += warps)
+          for (uint32_t j = 0; j < each; j += 32) {
+            const uint32_t slot = begin + listed[q] + (j + lane) * threads;
+            uint64_t key[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) key[i] = 0;
+            if (j + lane < each && slot < end) {
+              float f[V];
+              Vec<T>{from[slot]}.floats(f);
+#pragma unroll
+              for (int i = 0; i < V; ++i) key[i] = key_of(f[i], head + slot * V + i);
+            }
+            push(key, V);
+          }
+        if (warp == 0) {
+          const uint64_t key = on_edge ? key_of(to_float(x[edge]), edge) : 0;
+          push(&key, 1);
+        }
+        __syncthreads();
+        if (count <= kBuffer) break;
+        // too many: the a.top-th of those in the buffer is a better bound
+        least = 0;
+        for (uint64_t bit = 1ull << 63; bit; bit >>= 1) {
+          uint32_t reach = 0;
+          for (uint32_t i = 0; i < kBuffer; i += threads) reach += __syncthreads_count(i + threadIdx.x < kBuffer && buffer[i + threadIdx.x] >= (least | bit));
+          if (reach >= a.top) least |= bit;
+        }
+      }
+      const uint32_t n = count;
+      for (uint32_t i = threadIdx.x; i < a.top; i += threads) best[i] = 0;
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < n; i += threads) {
+        const uint64_t key = buffer[i];
+        uint32_t before = 0;
+        for (uint32_t j = 0; j < n; ++j) before += buffer[j] > key;
+        if (before < a.top) best[before] = key;
+      }
+    }
+    sync();
+    if (rank == 0) {
+      // the cluster's
+      if (warp == 0) {
+        own = block_sums;
+        if (cluster > 1) {
+          own = Sums{-INFINITY, 0.0f, 0.0f};
+          if (lane < cluster) {
+            uint32_t w[3];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) w[i] = peer_load(reinterpret_cast<const uint32_t *>(&block_sums) + i, lane);
+            own = Sums{__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2])};
+          }
+          warp_join(own);
+        }
+      }
+      const bool empty = own.m == -INFINITY;
+      const float log_sum = empty ? 0.0f : logf(own.sum);
+      if (first) {
+        if (a.logprob) a.logprob[row] = token == a.vocab ? 0.0f : empty ? own.m : a.scale * (picked - own.m) - log_sum;
+        if (ENTROPY && a.entropy) a.entropy[row] = empty ? 0.0f : log_sum - own.dot / own.sum * kLn2;
+        if (a.stats) a.stats[row] = make_float2(own.m, log_sum);
+      }
+      if constexpr (TOP) {
+        if (first) sums[0] = Sums{own.m, log_sum, 0.0f};
+        // a list's keys come in falling order: one's place is its own and that in each other list
+        const uint32_t all = cluster * a.top;
+        for (uint32_t i = threadIdx.x; i < all; i += threads) {
+          const uint32_t r = i / a.top;
+          const uint32_t *p = reinterpret_cast<const uint32_t *>(best + (i - r * a.top));
+          lists[i] = cluster > 1 ? (uint64_t)peer_load(p + 1, r) << 32 | peer_load(p, r) : best[i];
+        }
+        __syncthreads();
+        const float m = sums[0].m, l = sums[0].sum;
+        for (uint32_t i = threadIdx.x; i < all; i += threads) {
+          const uint64_t key = lists[i];
+          const uint32_t mine = i / a.top;
+          uint32_t place = i - mine * a.top;
+          for (uint32_t r = 0; r < cluster; ++r) {
+            if (r == mine) continue;
+            uint32_t low = 0, high = a.top;       // keys of the list that are larger
+            while (low < high) { const uint32_t mid = (low + high) / 2; if (lists[r * a.top + mid] > key) low = mid + 1; else high = mid; }
+            place += low;
+          }
+          if (key && place < a.top) put_top(a, row, place, key, m, l);
+        }
+      }
+    }
+    sync();
   }
 }
 
+// Any rows: a block has a row at a time, element by element
 template <typename T> __global__ void __launch_bounds__(kThreads) token_log_probs_grad_rows_kernel(const ProbsGradArgs a)
 {
   pdl_wait();
@@ -143,6 +348,75 @@ template <typename T> __global__ void __launch_bounds__(kThreads) token_log_prob
       dx[c] = from_float<T>(empty ? 0.0f : a.scale * d);
     }
   }
+}
+
+// The gradient where logits and dlogits begin their rows at the same places of 16 bytes: a block has a stretch of a row, a thread four slots of it, all of which are
+// asked for before the row's numbers are; logits before the first slot and behind the last have a thread each
+constexpr uint32_t kGradSlots = 4;
+template <typename T, bool ENTROPY> __global__ void __launch_bounds__(kThreads) token_log_probs_grad_kernel(const ProbsGradArgs a, const uint32_t cuts)
+{
+  constexpr int V = Vec<T>::V, U = kGradSlots;
+  const uint32_t threads = blockDim.x;
+  const float rate = fminf(a.scale * kLog2e, 3.402823466e38f);
+  pdl_wait();
+  pdl_trigger();
+  for (uint64_t at = blockIdx.x; at < a.rows * cuts; at += gridDim.x) {
+    const uint64_t row = at / cuts;
+    const uint32_t cut = (uint32_t)(at - row * cuts);
+    const T *x = static_cast<const T *>(a.logits) + row * a.stride;
+    T *dx = static_cast<T *>(a.dlogits) + row * a.dstride;
+    const uint32_t head = min(a.vocab, (uint32_t)(-(int)((uintptr_t)x / sizeof(T)) & (V - 1))), slots = (a.vocab - head) / V, tail = a.vocab - head - slots * V;
+    const uint32_t first = cut * U * threads + threadIdx.x;
+    const bool on_edge = cut == 0 && threadIdx.x < head + tail;
+    const uint32_t edge = threadIdx.x < head ? threadIdx.x : a.vocab - tail + (threadIdx.x - head);
+    Vec<T> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) if (first + u * threads < slots) v[u] = Vec<T>::load(x + head + (uint64_t)(first + u * threads) * V);
+    T one = {};
+    if (on_edge) one = x[edge];
+    const float2 stats = a.stats[row];
+    const uint32_t token = a.dlogprob ? token_at(a.token, a.token_bytes, row, a.vocab) : a.vocab;
+    const float dl = token < a.vocab ? a.dlogprob[row] : 0.0f, dh = ENTROPY ? a.dentropy[row] : 0.0f, h = ENTROPY ? a.entropy[row] : 0.0f;
+    // with l = z - L in powers of two, dx = 2^l*(flat + slope*l), and scale*dlogprob more for the token
+    const bool empty = stats.x == -INFINITY;
+    const float log_sum = stats.y * kLog2e, flat = empty ? 0.0f : -a.scale * fmaf(dh, h, dl), slope = empty ? 0.0f : -a.scale * dh * kLn2, more = empty ? 0.0f : a.scale * dl;
+    const float2 minus = both(empty ? 0.0f : -stats.x), times = both(rate), less = both(-log_sum), flat2 = both(flat), slope2 = both(slope);
+    auto gradient = [&](float2 f) {
+      float2 l = mul2(add2(f, minus), times);
+      if (ENTROPY) l = make_float2(max_nan(l.x, kFloor), max_nan(l.y, kFloor));
+      l = add2(l, less);
+      const float2 p = make_float2(exp2_of(l.x), exp2_of(l.y));
+      return mul2(p, ENTROPY ? fma2(slope2, l, flat2) : flat2);
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (first + u * threads >= slots) continue;
+      const uint32_t c = head + (first + u * threads) * V;
+      float2 f[V / 2];
+      v[u].floats(reinterpret_cast<float *>(f));
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) f[i] = gradient(f[i]);
+      if (token - c < V) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (token - c == i) reinterpret_cast<float *>(f)[i] += more;
+      }
+      Vec<T>::of(reinterpret_cast<const float *>(f)).store(dx + c);
+    }
+    if (on_edge) {
+      const float d = gradient(both(to_float(one))).x;
+      dx[edge] = from_float<T>(edge == token ? d + more : d);
+    }
+  }
+}
+
+// Blocks to a row and threads of a block
+void split(uint64_t rows, uint32_t slots, uint32_t &cluster, uint32_t &threads)
+{
+  const uint32_t sms = sm_count();
+  while (cluster < 8 && rows * cluster < 2 * sms && slots / (cluster * 2) >= 256) cluster *= 2;
+  const uint32_t each = (slots / cluster + 127) / 128 * 32;      // (four slots to a thread)
+  const uint32_t most = rows * cluster >= 4 * sms ? 256 : rows * cluster >= 2 * sms ? 512 : kMostThreads;
+  threads = each < 32 ? 32 : each < most ? each : most;
 }
 
 }  // namespace rows
@@ -175,7 +449,17 @@ extern "C" int anode_gpu_token_log_probs_fwd(
       (top && (!aligned_to(top_logprob, 4) || (top_token && !aligned_to(top_token, (size_t)top_token_bytes))))) return ANODE_E_ALIGN;
   const ProbsArgs a = {rows, vocab, scale, logits, logits_stride, token, token_bytes, logprob, entropy, reinterpret_cast<float2 *>(stats), top,
                        top ? top_logprob : nullptr, top ? top_token : nullptr, top_token_bytes};
-  return by_type(type, [&](auto t) { return launch(token_log_probs_rows_kernel<decltype(t)>, dim3(row_blocks(rows)), kThreads, 0, stream, a); });
+  const uint32_t v = (uint32_t)(16 / type_bytes(type)), slots = vocab / v;
+  uint32_t cluster = 1, threads;
+  split(rows, slots, cluster, threads);
+  const uint64_t most = (1u << 30) / cluster;
+  const dim3 grid((uint32_t)(rows < most ? rows : most) * cluster);
+  return by_type(type, [&](auto t) {
+    using T = decltype(t);
+    auto kernel = top ? (entropy ? token_log_probs_kernel<T, true, true> : token_log_probs_kernel<T, false, true>)
+                      : (entropy ? token_log_probs_kernel<T, true, false> : token_log_probs_kernel<T, false, false>);
+    return cluster > 1 ? launch_in_clusters(kernel, grid, cluster, threads, 0, stream, a, cluster) : launch(kernel, grid, threads, 0, stream, a, cluster);
+  });
 }
 
 extern "C" int anode_gpu_token_log_probs_bwd(
@@ -197,5 +481,12 @@ extern "C" int anode_gpu_token_log_probs_bwd(
   if (!apart(dlogits, dlogits_stride, logits, logits_stride, rows)) return ANODE_E_STRIDE;
   const ProbsGradArgs a = {rows, vocab, scale, logits, logits_stride, token, token_bytes, reinterpret_cast<const float2 *>(stats), entropy, dlogprob, dentropy,
                            dlogits, dlogits_stride};
-  return by_type(type, [&](auto t) { return launch(token_log_probs_grad_rows_kernel<decltype(t)>, dim3(row_blocks(rows)), kThreads, 0, stream, a); });
+  const uint32_t v = (uint32_t)(16 / e), slots = vocab / v, each = (slots + 32 * kGradSlots - 1) / (32 * kGradSlots) * 32;
+  const uint32_t threads = each < 32 ? 32 : each < kThreads ? each : kThreads, cuts = slots ? (slots + threads * kGradSlots - 1) / (threads * kGradSlots) : 1;
+  const bool step = in_step(dlogits, e, dlogits_stride, v, logits, e, logits_stride, rows);
+  return by_type(type, [&](auto t) {
+    using T = decltype(t);
+    return step ? launch(dentropy ? token_log_probs_grad_kernel<T, true> : token_log_probs_grad_kernel<T, false>, dim3(row_blocks(rows * cuts)), threads, 0, stream, a, cuts)
+                : launch(token_log_probs_grad_rows_kernel<T>, dim3(row_blocks(rows)), kThreads, 0, stream, a);
+  });
 }

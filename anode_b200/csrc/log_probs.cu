@@ -11,7 +11,7 @@ namespace anode_b200 {
 namespace rows {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kMostThreads = 1024, kMostTop = 128;
+constexpr uint32_t kMostThreads = 512, kMostTop = 128;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFloor = -1e4f;            // below what exp leaves above zero: 0 takes the place of 0 * -infinity
 
@@ -83,17 +83,29 @@ __device__ __forceinline__ float exp2_of(float v)
   return d;
 }
 
-// 16 bytes of logits: the largest of them, and of what is none
-template <typename T> __device__ __forceinline__ float largest_of(const uint4 &v)
-{
-  if constexpr (sizeof(T) == 4) return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
-  else {
-    typedef typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type Pair;
-    auto pair = [](uint32_t w) { return *reinterpret_cast<const Pair *>(&w); };
-    const Pair m = __hmax2_nan(__hmax2_nan(pair(v.x), pair(v.y)), __hmax2_nan(pair(v.z), pair(v.w)));
-    return max_nan(to_float(m.x), to_float(m.y));
+// Slots of 16 bytes of logits: the largest and the smallest (a NaN is the largest), two at a time where they have 16 bits; and a slot of what is none
+template <typename T> struct Extremes {
+  typedef typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type Pair;
+  typedef typename std::conditional<sizeof(T) == 4, float, Pair>::type Value;
+  Value high, low;
+  __device__ __forceinline__ static Value at(const uint4 &v, int i)
+  {
+    const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+    return *reinterpret_cast<const Value *>(&w);
   }
-}
+  __device__ __forceinline__ void start(const uint4 &v) { high = low = at(v, 0); }
+  template <bool LOW> __device__ __forceinline__ void take(const uint4 &v, int from)
+  {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i < from) continue;
+      if constexpr (sizeof(T) == 4) { high = max_nan(high, at(v, i)); if (LOW) low = fminf(low, at(v, i)); }
+      else { high = __hmax2_nan(high, at(v, i)); if (LOW) low = __hmin2(low, at(v, i)); }
+    }
+  }
+  __device__ __forceinline__ float largest() const { if constexpr (sizeof(T) == 4) return high; else return max_nan(to_float(high.x), to_float(high.y)); }
+  __device__ __forceinline__ float smallest() const { if constexpr (sizeof(T) == 4) return low; else return fminf(to_float(low.x), to_float(low.y)); }
+};
 template <typename T> __device__ __forceinline__ uint4 nothing()
 {
   constexpr uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;      // -infinity
@@ -119,10 +131,10 @@ constexpr uint32_t kBuffer = 1024;         // keys that may be among the likelie
 // follow it.  The likeliest: the k-th largest of the threads' maxima is a bound that k logits reach at least, so that few threads have more of them, whose
 // slots are read again.
 template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kMostThreads) token_log_probs_kernel(const ProbsArgs a, const uint32_t cluster)
+__global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const ProbsArgs a, const uint32_t cluster)
 {
   constexpr int V = Vec<T>::V, U = 4;
-  __shared__ Sums sums[32], block_sums;
+  __shared__ Sums sums[kMostThreads / 32], block_sums;
   __shared__ uint64_t buffer[TOP ? kBuffer : 1], best[TOP ? kMostTop : 1], lists[TOP ? 8 * kMostTop : 1];
   __shared__ uint32_t listed[TOP ? kMostThreads : 1], count, bound_count;
   const uint32_t threads = blockDim.x, warps = threads / 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -145,52 +157,73 @@ __global__ void __launch_bounds__(kMostThreads) token_log_probs_kernel(const Pro
       token = token_at(a.token, a.token_bytes, row, a.vocab);
       if (token < a.vocab) picked = to_float(x[token]);
     }
-    Sums own = {-INFINITY, 0.0f, 0.0f};
+    // (sums of every second logit)
+    float m = -INFINITY;
     float2 sum = both(0.0f), dot = both(0.0f);
-    auto absorb = [&](const uint4 *v, int n) {
-      float m = own.m;
+    const float2 times = both(rate);
+    auto absorb = [&](const uint4 *v) {
+      Extremes<T> x;
+      x.start(v[0]);
 #pragma unroll
-      for (int u = 0; u < n; ++u) m = max_nan(m, largest_of<T>(v[u]));
-      own.sum = sum.x; own.dot = dot.x;
-      Sums other = {own.m, sum.y, dot.y};
-      own.move(m, rate); other.move(m, rate);
-      sum = make_float2(own.sum, other.sum); dot = make_float2(own.dot, other.dot);
-      const float2 minus = both(m == -INFINITY ? 0.0f : -m), times = both(rate);
+      for (int u = 0; u < U; ++u) x.template take<ENTROPY>(v[u], u == 0);
+      const float to = max_nan(m, x.largest()), base = to == -INFINITY ? 0.0f : to;
+      const float moved = max_nan((m - base) * rate, kFloor);
+      const float2 by = both(exp2_of(moved));
+      if (ENTROPY) dot = mul2(by, fma2(both(moved), sum, dot));
+      sum = mul2(by, sum);
+      m = to;
+      const float2 minus = both(-base);
+      auto add = [&](auto clamped) {
 #pragma unroll
-      for (int u = 0; u < n; ++u) {
-        float2 f[V / 2];
-        Vec<T>{v[u]}.floats(reinterpret_cast<float *>(f));
+        for (int u = 0; u < U; ++u) {
+          float2 f[V / 2];
+          Vec<T>{v[u]}.floats(reinterpret_cast<float *>(f));
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
-          float2 d = mul2(add2(f[i], minus), times);
-          if (ENTROPY) d = make_float2(max_nan(d.x, kFloor), max_nan(d.y, kFloor));
-          const float2 e = make_float2(exp2_of(d.x), exp2_of(d.y));
-          sum = add2(sum, e);
-          if (ENTROPY) dot = fma2(d, e, dot);
+          for (int i = 0; i < V / 2; ++i) {
+            float2 d = mul2(add2(f[i], minus), times);
+            if (decltype(clamped)::value) d = make_float2(max_nan(d.x, kFloor), max_nan(d.y, kFloor));
+            const float2 e = make_float2(exp2_of(d.x), exp2_of(d.y));
+            sum = add2(sum, e);
+            if (ENTROPY) dot = fma2(d, e, dot);
+          }
         }
-      }
+      };
+      // (0 times -infinity is to be 0: where some logit is that far below)
+      if (!ENTROPY || (x.smallest() - base) * rate >= kFloor) add(std::false_type());
+      else add(std::true_type());
     };
-    uint4 next[U];
-    auto fetch = [&](uint32_t s) {
+    const uint32_t at = begin + threadIdx.x, mine = at < end ? (end - at + threads - 1) / threads : 0;       // this thread's slots
+    const uint4 *p = from + at;
+    auto fetch = [&](uint4 *to) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        next[u] = nothing<T>();
-        if (s + u * threads < end) next[u] = from[s + u * threads];
-      }
+      for (int u = 0; u < U; ++u) to[u] = p[u * threads];
+      p += U * threads;
     };
-    fetch(begin + threadIdx.x);
-    for (uint32_t s = begin + threadIdx.x; s < end; s += U * threads) {
-      uint4 now[U];
+    // two steps in turn, one on its way while the other is used
+    uint4 one[U], two[U];
+    uint32_t steps = mine / U;
+    if (steps) fetch(one);
+    for (; steps >= 2; steps -= 2) {
+      fetch(two);
+      absorb(one);
+      if (steps > 2) fetch(one);
+      absorb(two);
+    }
+    // the last whole step, what is left of one, and a logit beside whole slots
 #pragma unroll
-      for (int u = 0; u < U; ++u) now[u] = next[u];
-      fetch(s + U * threads);
-      absorb(now, U);
+    for (int u = 0; u < U; ++u) {
+      two[u] = nothing<T>();
+      if (u < mine % U) two[u] = p[u * threads];
     }
-    if (on_edge) {
-      uint4 v = nothing<T>();
-      *reinterpret_cast<T *>(&v) = x[edge];
-      absorb(&v, 1);
+    uint4 beside = nothing<T>();
+    if (on_edge) *reinterpret_cast<T *>(&beside) = x[edge];
+#pragma unroll 1
+    for (int k = 0; k < 3; ++k) {
+      if (k == 0 ? steps != 0 : k == 1 ? mine % U != 0 : on_edge) absorb(one);
+#pragma unroll
+      for (int u = 0; u < U; ++u) { one[u] = two[u]; two[u] = u ? nothing<T>() : beside; }
     }
+    Sums own = {m, 0.0f, 0.0f};
     own.sum = sum.x + sum.y; own.dot = dot.x + dot.y;
     const uint32_t order = order_of(own.m);
     // the block's sums
@@ -211,12 +244,28 @@ __global__ void __launch_bounds__(kMostThreads) token_log_probs_kernel(const Pro
       if (lane == 0) block_sums = own;
     }
     if constexpr (TOP) {
-      // the upper half of the bits of a value that a.top threads' maxima reach
-      uint32_t bound = 0;
-      for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
-        if ((uint32_t)__syncthreads_count(order >= (bound | bit)) >= a.top) bound |= bit;
-      uint64_t least = bound ? (uint64_t)bound << 32 : 1;      // (no logit has the key 0)
+      // the a.top-th of the maxima of groups of lanes, as many as leave half as many again: as many logits reach it at least
+      uint32_t group = 32, least_order = 0;
+      while (group > 1 && threads / group < a.top + a.top / 2 + 8) group /= 2;
+      const uint32_t groups = threads / group;
+      uint32_t of_group = order;
+      for (uint32_t o = group / 2; o > 0; o >>= 1) of_group = max(of_group, __shfl_xor_sync(0xffffffffu, of_group, o));
+      if ((threadIdx.x & (group - 1)) == 0) listed[threadIdx.x / group] = of_group;
+      if (threadIdx.x == 0) bound_count = 0;
+      __syncthreads();
+      if (threadIdx.x < groups) {
+        const uint32_t mine = listed[threadIdx.x];
+        uint32_t before = 0;
+        for (uint32_t j = 0; j < groups; ++j) before += listed[j] > mine || (listed[j] == mine && j < threadIdx.x);
+        if (before == a.top - 1) bound_count = mine;
+      }
+      __syncthreads();
+      least_order = bound_count;
+      uint64_t least = least_order ? (uint64_t)least_order << 32 : 1;      // (no logit has the key 0)
+      // lanes that read a thread's slots side by side
       const uint32_t each = (end - begin + threads - 1) / threads;
+      uint32_t lanes = 1;
+      while (lanes < 32 && lanes < each) lanes *= 2;
       for (;;) {
         // the threads whose maxima reach it
         __syncthreads();
@@ -241,13 +290,15 @@ __global__ void __launch_bounds__(kMostThreads) token_log_probs_kernel(const Pro
           for (int i = 0; i < n; ++i)
             if (key[i] >= least) { buffer[at < kBuffer ? at : (at * 2654435761u) >> 22] = key[i]; ++at; }
         };
-        for (uint32_t q = warp; q < found; q += warps)
-          for (uint32_t j = 0; j < each; j += 32) {
-            const uint32_t slot = begin + listed[q] + (j + lane) * threads;
+        for (uint32_t q = warp * (32 / lanes); q < found; q += warps * (32 / lanes)) {
+          const uint32_t which = q + lane / lanes;
+          const uint32_t slot0 = which < found ? begin + listed[which] : end;
+          for (uint32_t j = lane & (lanes - 1); __any_sync(0xffffffffu, j < each); j += lanes) {
+            const uint32_t slot = slot0 + j * threads;
             uint64_t key[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) key[i] = 0;
-            if (j + lane < each && slot < end) {
+            if (j < each && slot < end) {
               float f[V];
               Vec<T>{from[slot]}.floats(f);
 #pragma unroll
@@ -255,6 +306,7 @@ __global__ void __launch_bounds__(kMostThreads) token_log_probs_kernel(const Pro
             }
             push(key, V);
           }
+        }
         if (warp == 0) {
           const uint64_t key = on_edge ? key_of(to_float(x[edge]), edge) : 0;
           push(&key, 1);
@@ -409,14 +461,21 @@ template <typename T, bool ENTROPY> __global__ void __launch_bounds__(kThreads) 
   }
 }
 
-// Blocks to a row and threads of a block
+// Blocks to a row and threads of a block: by what a multiprocessor takes for its blocks, of its share of the bandwidth (44 KB/us) or in steps of four slots to a
+// thread (0.8 us, of 1280 threads at a time), and what a row takes beside that: 3 us, in a cluster half as much again
 void split(uint64_t rows, uint32_t slots, uint32_t &cluster, uint32_t &threads)
 {
-  const uint32_t sms = sm_count();
-  while (cluster < 8 && rows * cluster < 2 * sms && slots / (cluster * 2) >= 256) cluster *= 2;
-  const uint32_t each = (slots / cluster + 127) / 128 * 32;      // (four slots to a thread)
-  const uint32_t most = rows * cluster >= 4 * sms ? 256 : rows * cluster >= 2 * sms ? 512 : kMostThreads;
-  threads = each < 32 ? 32 : each < most ? each : most;
+  const uint64_t sms = sm_count();
+  double least = 0.0;
+  for (uint32_t c = 1; c <= 8 && (c == 1 || slots / c >= 256); c *= 2)
+    for (uint32_t t = 256; t <= kMostThreads; t *= 2) {
+      const uint64_t blocks = (rows * c + sms - 1) / sms, steps = ((uint64_t)slots + c * t * 4ull - 1) / (c * t * 4ull), room = 1280 / t;
+      const double moved = (double)blocks * slots * 16 / c / 44e3, waited = 0.8 * (double)(steps * ((blocks + room - 1) / room));
+      const double cost = (moved > waited ? moved : waited) + (c > 1 ? 4.5 : 3.0);
+      if (least == 0.0 || cost < least) { least = cost; cluster = c; threads = t; }
+    }
+  const uint32_t each = (slots / cluster + 127) / 128 * 32;
+  if (each < threads) threads = each < 32 ? 32 : each;
 }
 
 }  // namespace rows

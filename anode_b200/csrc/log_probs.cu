@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
         if (order >= (uint32_t)(least >> 32)) listed[atomicAdd(&bound_count, 1u)] = threadIdx.x;
         __syncthreads();
         const uint32_t found = bound_count;
-        // keys from `least` on: those that find no place in the buffer take one of another, so that it holds some of all
+        // keys from `least` on: of the n-th, beyond the buffer's size, one in n/size takes another's place, so that the buffer holds some of all alike
         auto push = [&](const uint64_t *key, int n) {
           uint32_t mine = 0;
 #pragma unroll
@@ -288,7 +288,11 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
           at += __shfl_sync(0xffffffffu, start, 31) - mine;
 #pragma unroll
           for (int i = 0; i < n; ++i)
-            if (key[i] >= least) { buffer[at < kBuffer ? at : (at * 2654435761u) >> 22] = key[i]; ++at; }
+            if (key[i] >= least) {
+              const uint32_t place = at < kBuffer ? at : __umulhi(at * 2654435769u, at);
+              if (place < kBuffer) buffer[place] = key[i];
+              ++at;
+            }
         };
         for (uint32_t q = warp * (32 / lanes); q < found; q += warps * (32 / lanes)) {
           const uint32_t which = q + lane / lanes;
@@ -405,7 +409,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) token_log_prob
 // The gradient where logits and dlogits begin their rows at the same places of 16 bytes: a block has a stretch of a row, a thread four slots of it, all of which are
 // asked for before the row's numbers are; logits before the first slot and behind the last have a thread each
 constexpr uint32_t kGradSlots = 4;
-template <typename T, bool ENTROPY> __global__ void __launch_bounds__(kThreads) token_log_probs_grad_kernel(const ProbsGradArgs a, const uint32_t cuts)
+template <typename T, bool ENTROPY> __global__ void __launch_bounds__(kThreads, 6) token_log_probs_grad_kernel(const ProbsGradArgs a, const uint32_t cuts)
 {
   constexpr int V = Vec<T>::V, U = kGradSlots;
   const uint32_t threads = blockDim.x;
@@ -433,29 +437,44 @@ template <typename T, bool ENTROPY> __global__ void __launch_bounds__(kThreads) 
     const bool empty = stats.x == -INFINITY;
     const float log_sum = stats.y * kLog2e, flat = empty ? 0.0f : -a.scale * fmaf(dh, h, dl), slope = empty ? 0.0f : -a.scale * dh * kLn2, more = empty ? 0.0f : a.scale * dl;
     const float2 minus = both(empty ? 0.0f : -stats.x), times = both(rate), less = both(-log_sum), flat2 = both(flat), slope2 = both(slope);
-    auto gradient = [&](float2 f) {
-      float2 l = mul2(add2(f, minus), times);
-      if (ENTROPY) l = make_float2(max_nan(l.x, kFloor), max_nan(l.y, kFloor));
-      l = add2(l, less);
+    // (0 times -infinity is to be 0: CLAMP where some logit is that far below)
+    auto gradient = [&](float2 f, auto clamp) {
+      float2 l = fma2(add2(f, minus), times, less);
+      if (decltype(clamp)::value) l = make_float2(max_nan(l.x, kFloor), max_nan(l.y, kFloor));
       const float2 p = make_float2(exp2_of(l.x), exp2_of(l.y));
       return mul2(p, ENTROPY ? fma2(slope2, l, flat2) : flat2);
     };
+    auto all = [&](auto clamp) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (first + u * threads >= slots) continue;
-      const uint32_t c = head + (first + u * threads) * V;
-      float2 f[V / 2];
-      v[u].floats(reinterpret_cast<float *>(f));
+      for (int u = 0; u < U; ++u) {
+        if (first + u * threads >= slots) continue;
+        const uint32_t c = head + (first + u * threads) * V;
+        float2 f[V / 2];
+        v[u].floats(reinterpret_cast<float *>(f));
 #pragma unroll
-      for (int i = 0; i < V / 2; ++i) f[i] = gradient(f[i]);
-      if (token - c < V) {
+        for (int i = 0; i < V / 2; ++i) f[i] = gradient(f[i], clamp);
+        if (token - c < V) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) if (token - c == i) reinterpret_cast<float *>(f)[i] += more;
+          for (int i = 0; i < V; ++i) if (token - c == i) reinterpret_cast<float *>(f)[i] += more;
+        }
+        Vec<T>::of(reinterpret_cast<const float *>(f)).store(dx + c);
       }
-      Vec<T>::of(reinterpret_cast<const float *>(f)).store(dx + c);
+    };
+    bool far = false;
+    if (ENTROPY) {
+      Extremes<T> low;
+      low.start(nothing<T>());
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (first + u * threads >= slots) continue;
+        if (u == 0) low.start(v[0].bits);
+        low.template take<true>(v[u].bits, u == 0);
+      }
+      far = !(first < slots && fmaf(low.smallest() + minus.x, rate, less.x) >= kFloor);
     }
+    if (far) all(std::true_type()); else all(std::false_type());
     if (on_edge) {
-      const float d = gradient(both(to_float(one))).x;
+      const float d = gradient(both(to_float(one)), std::true_type()).x;
       dx[edge] = from_float<T>(edge == token ? d + more : d);
     }
   }

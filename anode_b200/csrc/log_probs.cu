@@ -161,11 +161,12 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
     float m = -INFINITY;
     float2 sum = both(0.0f), dot = both(0.0f);
     const float2 times = both(rate);
-    auto absorb = [&](const uint4 *v) {
+    auto absorb = [&](const uint4 *v, auto slots_here) {
+      constexpr int N = decltype(slots_here)::value;
       Extremes<T> x;
       x.start(v[0]);
 #pragma unroll
-      for (int u = 0; u < U; ++u) x.template take<ENTROPY>(v[u], u == 0);
+      for (int u = 0; u < N; ++u) x.template take<ENTROPY>(v[u], u == 0);
       const float to = max_nan(m, x.largest()), base = to == -INFINITY ? 0.0f : to;
       const float moved = max_nan((m - base) * rate, kFloor);
       const float2 by = both(exp2_of(moved));
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
       const float2 minus = both(-base);
       auto add = [&](auto clamped) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < N; ++u) {
           float2 f[V / 2];
           Vec<T>{v[u]}.floats(reinterpret_cast<float *>(f));
 #pragma unroll
@@ -199,29 +200,37 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
       for (int u = 0; u < U; ++u) to[u] = p[u * threads];
       p += U * threads;
     };
+    typedef std::integral_constant<int, U> Step;
     // two steps in turn, one on its way while the other is used
     uint4 one[U], two[U];
     uint32_t steps = mine / U;
     if (steps) fetch(one);
     for (; steps >= 2; steps -= 2) {
       fetch(two);
-      absorb(one);
+      absorb(one, Step());
       if (steps > 2) fetch(one);
-      absorb(two);
+      absorb(two, Step());
     }
-    // the last whole step, what is left of one, and a logit beside whole slots
+    // what is left of a step, slot by slot, and a logit beside whole slots
+    uint32_t rest = mine % U;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       two[u] = nothing<T>();
-      if (u < mine % U) two[u] = p[u * threads];
+      if (u < rest) two[u] = p[u * threads];
     }
-    uint4 beside = nothing<T>();
-    if (on_edge) *reinterpret_cast<T *>(&beside) = x[edge];
-#pragma unroll 1
-    for (int k = 0; k < 3; ++k) {
-      if (k == 0 ? steps != 0 : k == 1 ? mine % U != 0 : on_edge) absorb(one);
+    if (on_edge) {
+      uint4 beside = nothing<T>();
+      *reinterpret_cast<T *>(&beside) = x[edge];
 #pragma unroll
-      for (int u = 0; u < U; ++u) { one[u] = two[u]; two[u] = u ? nothing<T>() : beside; }
+      for (int u = 0; u < U; ++u) if (u == rest) two[u] = beside;      // (U - 1 slots at most are left)
+      ++rest;
+    }
+    if (steps) absorb(one, Step());
+#pragma unroll 1
+    for (; rest; --rest) {
+      absorb(two, std::integral_constant<int, 1>());
+#pragma unroll
+      for (int u = 0; u + 1 < U; ++u) two[u] = two[u + 1];
     }
     Sums own = {m, 0.0f, 0.0f};
     own.sum = sum.x + sum.y; own.dot = dot.x + dot.y;
@@ -266,50 +275,86 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
       const uint32_t each = (end - begin + threads - 1) / threads;
       uint32_t lanes = 1;
       while (lanes < 32 && lanes < each) lanes *= 2;
-      for (;;) {
-        // the threads whose maxima reach it
+      // keys from `least` on: of the n-th, beyond the buffer's size, one in n/size takes another's place, so that the buffer holds some of all alike
+      auto push = [&](const uint64_t *key, int n) {
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < n; ++i) mine += key[i] >= least;
+        const uint32_t some = __ballot_sync(0xffffffffu, mine != 0);
+        if (!some) return;
+        uint32_t at = mine;
+        if (__popc(some) <= 4) {         // few: each for itself
+          if (mine) at += atomicAdd(&count, mine);
+        } else {
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) { const uint32_t w = __shfl_up_sync(0xffffffffu, at, o); if (lane >= o) at += w; }
+        uint32_t start = 0;
+        if (lane == 31) start = atomicAdd(&count, at);
+        at += __shfl_sync(0xffffffffu, start, 31);
+        }
+        if (!mine) return;
+        at -= mine;
+#pragma unroll
+        for (int i = 0; i < n; ++i)
+          if (key[i] >= least) {
+            const uint32_t place = at < kBuffer ? at : __umulhi(at * 2654435769u, at);
+            if (place < kBuffer) buffer[place] = key[i];
+            ++at;
+          }
+      };
+      auto push_slot = [&](uint32_t slot, bool there) {
+        uint64_t key[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = 0;
+        if (there) {
+          float f[V];
+          Vec<T>{from[slot]}.floats(f);
+#pragma unroll
+          for (int i = 0; i < V; ++i) key[i] = key_of(f[i], head + slot * V + i);
+        }
+        push(key, V);
+      };
+      auto restart = [&] {
         __syncthreads();
         if (threadIdx.x == 0) count = bound_count = 0;
         __syncthreads();
-        if (order >= (uint32_t)(least >> 32)) listed[atomicAdd(&bound_count, 1u)] = threadIdx.x;
+      };
+      // a better bound: a.top keys of the buffer's n reach it, or a few more (bit by bit; where all have the value of the bound that there is, by their indices alone)
+      auto tighten = [&](uint32_t n) {
+        bool other = false;
+        for (uint32_t i = threadIdx.x; i < n; i += threads) other |= buffer[i] >> 32 != least >> 32;
+        const bool values = __syncthreads_or(other);
+        uint64_t to = values ? 0 : least >> 32 << 32;
+        uint32_t reach = n;
+        for (uint64_t bit = values ? 1ull << 63 : 1ull << 31; bit && reach > a.top + 32; bit >>= 1) {
+          uint32_t now = 0;
+          for (uint32_t i = 0; i < n; i += threads) now += __syncthreads_count(i + threadIdx.x < n && buffer[i + threadIdx.x] >= (to | bit));
+          if (now >= a.top) { to |= bit; reach = now; }
+        }
+        if (to > least) least = to;
+      };
+      for (bool tried = false; ; ) {
+        // the threads whose maxima reach the bound, and whether by more than its value
+        restart();
+        const uint32_t value = (uint32_t)(least >> 32), last = ~(uint32_t)least;
+        if (order >= value) listed[atomicAdd(&bound_count, 1u)] = threadIdx.x | (order > value ? 1u << 31 : 0u);
         __syncthreads();
         const uint32_t found = bound_count;
-        // keys from `least` on: of the n-th, beyond the buffer's size, one in n/size takes another's place, so that the buffer holds some of all alike
-        auto push = [&](const uint64_t *key, int n) {
-          uint32_t mine = 0;
-#pragma unroll
-          for (int i = 0; i < n; ++i) mine += key[i] >= least;
-          if (!__any_sync(0xffffffffu, mine != 0)) return;
-          uint32_t at = mine;
-#pragma unroll
-          for (int o = 1; o < 32; o *= 2) { const uint32_t w = __shfl_up_sync(0xffffffffu, at, o); if (lane >= o) at += w; }
-          uint32_t start = 0;
-          if (lane == 31) start = atomicAdd(&count, at);
-          at += __shfl_sync(0xffffffffu, start, 31) - mine;
-#pragma unroll
-          for (int i = 0; i < n; ++i)
-            if (key[i] >= least) {
-              const uint32_t place = at < kBuffer ? at : __umulhi(at * 2654435769u, at);
-              if (place < kBuffer) buffer[place] = key[i];
-              ++at;
-            }
-        };
+        if (found > 2 * a.top + 64 && !tried) {
+          // many threads with one value: since of equal ones the first count, a bound from the first slots
+          tried = true;
+          restart();
+          push_slot(begin + threadIdx.x, begin + threadIdx.x < end);
+          __syncthreads();
+          const uint32_t had = count;
+          if (had >= a.top) tighten(min(had, kBuffer));
+          continue;
+        }
         for (uint32_t q = warp * (32 / lanes); q < found; q += warps * (32 / lanes)) {
-          const uint32_t which = q + lane / lanes;
-          const uint32_t slot0 = which < found ? begin + listed[which] : end;
-          for (uint32_t j = lane & (lanes - 1); __any_sync(0xffffffffu, j < each); j += lanes) {
-            const uint32_t slot = slot0 + j * threads;
-            uint64_t key[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) key[i] = 0;
-            if (j < each && slot < end) {
-              float f[V];
-              Vec<T>{from[slot]}.floats(f);
-#pragma unroll
-              for (int i = 0; i < V; ++i) key[i] = key_of(f[i], head + slot * V + i);
-            }
-            push(key, V);
-          }
+          const uint32_t which = q + lane / lanes, who = which < found ? listed[which] : 0, slot0 = begin + (who & ~(1u << 31));
+          // (of a thread that has the value only, what lies up to the bound's index)
+          auto there = [&](uint32_t j) { const uint32_t slot = slot0 + j * threads; return which < found && j < each && slot < end && (who >> 31 || head + slot * V <= last); };
+          for (uint32_t j = lane & (lanes - 1); __any_sync(0xffffffffu, there(j)); j += lanes) push_slot(slot0 + j * threads, there(j));
         }
         if (warp == 0) {
           const uint64_t key = on_edge ? key_of(to_float(x[edge]), edge) : 0;
@@ -317,13 +362,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
         }
         __syncthreads();
         if (count <= kBuffer) break;
-        // too many: the a.top-th of those in the buffer is a better bound
-        least = 0;
-        for (uint64_t bit = 1ull << 63; bit; bit >>= 1) {
-          uint32_t reach = 0;
-          for (uint32_t i = 0; i < kBuffer; i += threads) reach += __syncthreads_count(i + threadIdx.x < kBuffer && buffer[i + threadIdx.x] >= (least | bit));
-          if (reach >= a.top) least |= bit;
-        }
+        tighten(kBuffer);               // (too many)
       }
       const uint32_t n = count;
       for (uint32_t i = threadIdx.x; i < a.top; i += threads) best[i] = 0;
@@ -481,16 +520,16 @@ template <typename T, bool ENTROPY> __global__ void __launch_bounds__(kThreads, 
 }
 
 // Blocks to a row and threads of a block: by what a multiprocessor takes for its blocks, of its share of the bandwidth (44 KB/us) or in steps of four slots to a
-// thread (0.8 us, of 1280 threads at a time), and what a row takes beside that: 3 us, in a cluster half as much again
+// thread (0.8 us, of 1024 threads at a time), and what a row takes beside that: 3 us, in a cluster half as much again, and a nanosecond of its threads' joins each
 void split(uint64_t rows, uint32_t slots, uint32_t &cluster, uint32_t &threads)
 {
   const uint64_t sms = sm_count();
   double least = 0.0;
   for (uint32_t c = 1; c <= 8 && (c == 1 || slots / c >= 256); c *= 2)
-    for (uint32_t t = 256; t <= kMostThreads; t *= 2) {
-      const uint64_t blocks = (rows * c + sms - 1) / sms, steps = ((uint64_t)slots + c * t * 4ull - 1) / (c * t * 4ull), room = 1280 / t;
+    for (uint32_t t = 128; t <= kMostThreads; t *= 2) {
+      const uint64_t blocks = (rows * c + sms - 1) / sms, steps = ((uint64_t)slots + c * t * 4ull - 1) / (c * t * 4ull), room = 1024 / t;
       const double moved = (double)blocks * slots * 16 / c / 44e3, waited = 0.8 * (double)(steps * ((blocks + room - 1) / room));
-      const double cost = (moved > waited ? moved : waited) + (c > 1 ? 4.5 : 3.0);
+      const double cost = (moved > waited ? moved : waited) + (c > 1 ? 4.5 : 3.0) + 1e-3 * (double)(blocks * t);
       if (least == 0.0 || cost < least) { least = cost; cluster = c; threads = t; }
     }
   const uint32_t each = (slots / cluster + 127) / 128 * 32;

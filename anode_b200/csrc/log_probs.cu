@@ -275,44 +275,42 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
       const uint32_t each = (end - begin + threads - 1) / threads;
       uint32_t lanes = 1;
       while (lanes < 32 && lanes < each) lanes *= 2;
-      // keys from `least` on: of the n-th, beyond the buffer's size, one in n/size takes another's place, so that the buffer holds some of all alike
-      auto push = [&](const uint64_t *key, int n) {
+      // a key from `least` on, the at-th: beyond the buffer's size, one in `at`/size takes another's place, so that the buffer holds some of all alike
+      auto put = [&](uint64_t key, uint32_t at) {
+        const uint32_t place = at < kBuffer ? at : __umulhi(at * 2654435769u, at);
+        if (place < kBuffer) buffer[place] = key;
+      };
+      // those of a slot (a warp's lanes have one each, or none)
+      auto push_slot = [&](uint32_t slot, bool there) {
+        const uint4 raw = there ? from[slot] : nothing<T>();
+        Extremes<T> of;
+        of.start(raw);
+        of.template take<false>(raw, 1);
+        const bool some = there && order_of(of.largest()) >= (uint32_t)(least >> 32);
+        const uint32_t lanes_with = __ballot_sync(0xffffffffu, some);
+        if (!lanes_with) return;
+        float f[V];
+        Vec<T>{raw}.floats(f);
+        const uint32_t c = head + slot * V;
+        if (__popc(lanes_with) <= 4) {   // few: each for itself
+          if (some) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) { const uint64_t key = key_of(f[i], c + i); if (key >= least) put(key, atomicAdd(&count, 1u)); }
+          }
+          return;
+        }
         uint32_t mine = 0;
 #pragma unroll
-        for (int i = 0; i < n; ++i) mine += key[i] >= least;
-        const uint32_t some = __ballot_sync(0xffffffffu, mine != 0);
-        if (!some) return;
+        for (int i = 0; i < V; ++i) mine += some && key_of(f[i], c + i) >= least;
         uint32_t at = mine;
-        if (__popc(some) <= 4) {         // few: each for itself
-          if (mine) at += atomicAdd(&count, mine);
-        } else {
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) { const uint32_t w = __shfl_up_sync(0xffffffffu, at, o); if (lane >= o) at += w; }
         uint32_t start = 0;
         if (lane == 31) start = atomicAdd(&count, at);
-        at += __shfl_sync(0xffffffffu, start, 31);
-        }
+        at += __shfl_sync(0xffffffffu, start, 31) - mine;
         if (!mine) return;
-        at -= mine;
 #pragma unroll
-        for (int i = 0; i < n; ++i)
-          if (key[i] >= least) {
-            const uint32_t place = at < kBuffer ? at : __umulhi(at * 2654435769u, at);
-            if (place < kBuffer) buffer[place] = key[i];
-            ++at;
-          }
-      };
-      auto push_slot = [&](uint32_t slot, bool there) {
-        uint64_t key[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = 0;
-        if (there) {
-          float f[V];
-          Vec<T>{from[slot]}.floats(f);
-#pragma unroll
-          for (int i = 0; i < V; ++i) key[i] = key_of(f[i], head + slot * V + i);
-        }
-        push(key, V);
+        for (int i = 0; i < V; ++i) { const uint64_t key = key_of(f[i], c + i); if (key >= least) put(key, at++); }
       };
       auto restart = [&] {
         __syncthreads();
@@ -356,9 +354,9 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
           auto there = [&](uint32_t j) { const uint32_t slot = slot0 + j * threads; return which < found && j < each && slot < end && (who >> 31 || head + slot * V <= last); };
           for (uint32_t j = lane & (lanes - 1); __any_sync(0xffffffffu, there(j)); j += lanes) push_slot(slot0 + j * threads, there(j));
         }
-        if (warp == 0) {
-          const uint64_t key = on_edge ? key_of(to_float(x[edge]), edge) : 0;
-          push(&key, 1);
+        if (on_edge) {
+          const uint64_t key = key_of(to_float(x[edge]), edge);
+          if (key >= least) put(key, atomicAdd(&count, 1u));
         }
         __syncthreads();
         if (count <= kBuffer) break;
@@ -520,7 +518,7 @@ template <typename T, bool ENTROPY> __global__ void __launch_bounds__(kThreads, 
 }
 
 // Blocks to a row and threads of a block: by what a multiprocessor takes for its blocks, of its share of the bandwidth (44 KB/us) or in steps of four slots to a
-// thread (0.8 us, of 1024 threads at a time), and what a row takes beside that: 3 us, in a cluster half as much again, and a nanosecond of its threads' joins each
+// thread (0.8 us, of 1024 threads at a time), and what a row takes beside that: 3 us, in a cluster twice that, and the joins of its threads, 1 ns of each
 void split(uint64_t rows, uint32_t slots, uint32_t &cluster, uint32_t &threads)
 {
   const uint64_t sms = sm_count();
@@ -528,8 +526,9 @@ void split(uint64_t rows, uint32_t slots, uint32_t &cluster, uint32_t &threads)
   for (uint32_t c = 1; c <= 8 && (c == 1 || slots / c >= 256); c *= 2)
     for (uint32_t t = 128; t <= kMostThreads; t *= 2) {
       const uint64_t blocks = (rows * c + sms - 1) / sms, steps = ((uint64_t)slots + c * t * 4ull - 1) / (c * t * 4ull), room = 1024 / t;
-      const double moved = (double)blocks * slots * 16 / c / 44e3, waited = 0.8 * (double)(steps * ((blocks + room - 1) / room));
-      const double cost = (moved > waited ? moved : waited) + (c > 1 ? 4.5 : 3.0) + 1e-3 * (double)(blocks * t);
+      // (few threads are slower over long rows: [4096,131072] bf16 170 us with 128, 164 with 256; [4096,50021] 73 and 83)
+      const double moved = (double)blocks * slots * 16 / c / 44e3 * (t == 128 && steps > 16 ? 1.04 : 1.0), waited = 0.8 * (double)(steps * ((blocks + room - 1) / room));
+      const double cost = (moved > waited ? moved : waited) + (c > 1 ? 6.0 : 3.0) + 1e-3 * (double)(blocks * t);
       if (least == 0.0 || cost < least) { least = cost; cluster = c; threads = t; }
     }
   const uint32_t each = (slots / cluster + 127) / 128 * 32;

@@ -1,4 +1,4 @@
-// Normalization over rows and rotary positions on top of anode_ops.hpp (included from there): f32 arrays, sizes fastest-varying first, so
+// Normalization over rows, rotary positions, rows of a table by tokens and log probabilities of tokens on top of anode_ops.hpp (included from there): f32 arrays, sizes fastest-varying first, so
 // rows are [cols, rows...] and heads [dim, heads, tokens].  No counterpart in the reference.
 #pragma once
 
@@ -153,6 +153,103 @@ struct RotaryPositionsOp {
   {
     const uint64_t dim = x.size()[0], n = x.size()[1];
     return AnodeHeads{const_cast<float *>(x.ptr()), 0, dim * n, dim, (uint32_t)n};
+  }
+};
+
+// y = (total - mu)*r*gamma + beta with total = x + residual, mu its mean and r = (mean((total - mu)^2) + epsilon)^-1/2 per row; gamma, beta, residual, total,
+// mean, inv_std may be null
+struct LayerNormalizeAddOp {
+  static void apply(float epsilon, const DeviceArray &x, DeviceArray &y, const DeviceArray *gamma, const DeviceArray *beta, const DeviceArray *residual,
+                    DeviceArray *total, DeviceArray *mean, DeviceArray *inv_std, cudaStream_t s = 0)
+  {
+    const RowDims d = row_dims(x);
+    want_len(y, x.len(), "y"); want_opt(gamma, d.cols, "gamma"); want_opt(beta, d.cols, "beta"); want_opt(residual, x.len(), "residual");
+    want_opt(total, x.len(), "total"); want_opt(mean, d.rows, "mean"); want_opt(inv_std, d.rows, "inv_std");
+    check(anode_gpu_layer_norm_add_fwd(ANODE_TYPE_F32, d.rows, d.cols, epsilon, x.ptr(), d.cols, opt(residual), d.cols, opt(gamma), opt(beta), ANODE_TYPE_F32,
+                                       y.ptr(), d.cols, opt(total), d.cols, opt(mean), opt(inv_std), kernel_config(), raw(s)), "anode_gpu_layer_norm_add_fwd");
+  }
+  static size_t scratch_bytes(const DeviceArray &dy) { const RowDims d = row_dims(dy); return anode_gpu_layer_norm_add_bwd_workspace_bytes(d.rows, d.cols); }
+  // the gradient of x and of the residual; with Accumulate it is added to dx, which then takes the place of dtotal
+  static void adjoint(const DeviceArray &dy, const DeviceArray &total, const DeviceArray &mean, const DeviceArray &inv_std, DeviceArray &dx, const DeviceArray *gamma,
+                      const DeviceArray *dtotal, DeviceArray *dgamma, DeviceArray *dbeta, WriteCap cap, RowScratch *scratch, cudaStream_t s = 0)
+  {
+    const RowDims d = row_dims(dy);
+    const bool adds = cap == WriteCap::Accumulate;
+    if (adds && dtotal && !dtotal->empty()) throw Error(ANODE_E_DIMS, "Accumulate adds into dx, which takes the place of dtotal");
+    want_len(total, dy.len(), "total"); want_len(dx, dy.len(), "dx"); want_len(mean, d.rows, "mean"); want_len(inv_std, d.rows, "inv_std");
+    want_opt(gamma, d.cols, "gamma"); want_opt(dtotal, dy.len(), "dtotal"); want_opt(dgamma, d.cols, "dgamma"); want_opt(dbeta, d.cols, "dbeta");
+    check(anode_gpu_layer_norm_add_bwd(ANODE_TYPE_F32, d.rows, d.cols, dy.ptr(), d.cols, total.ptr(), d.cols, mean.ptr(), inv_std.ptr(), opt(gamma), ANODE_TYPE_F32,
+                                       adds ? dx.ptr() : opt(dtotal), d.cols, dx.ptr(), d.cols, opt(dgamma), opt(dbeta), scratch ? scratch->ptr() : nullptr,
+                                       scratch ? scratch->bytes() : 0, kernel_config(), raw(s)), "anode_gpu_layer_norm_add_bwd");
+  }
+};
+
+// y[i] = scale*table[token[i]]: a table of [cols, vocab], y of [cols, tokens...]; a token outside of the table has a row of zeros and no gradient
+struct EmbedTokensOp {
+  static void apply(const DeviceVector<int64_t> &token, const DeviceArray &table, DeviceArray &y, float scale, cudaStream_t s = 0)
+  {
+    const uint32_t vocab = rows_of(table);
+    want_rows(y, table, token.len(), "y");
+    check(anode_gpu_embed_tokens_fwd(ANODE_TYPE_F32, token.len(), vocab, table.size()[0], scale, token.ptr(), 8, table.ptr(), table.size()[0], y.ptr(),
+                                     table.size()[0], kernel_config(), raw(s)), "anode_gpu_embed_tokens_fwd");
+  }
+  static size_t scratch_bytes(const DeviceVector<int64_t> &token, const DeviceArray &table)
+  {
+    return anode_gpu_embed_tokens_bwd_workspace_bytes(token.len(), rows_of(table), table.size()[0]);
+  }
+  // the whole table's gradient; with Accumulate what the tokens add to it
+  static void adjoint(const DeviceVector<int64_t> &token, const DeviceArray &dy, DeviceArray &dtable, float scale, WriteCap cap, RowScratch *scratch, cudaStream_t s = 0)
+  {
+    const uint32_t vocab = rows_of(dtable);
+    want_rows(dy, dtable, token.len(), "dy");
+    check(anode_gpu_embed_tokens_bwd(ANODE_TYPE_F32, token.len(), vocab, dtable.size()[0], scale, token.ptr(), 8, dy.ptr(), dtable.size()[0], dtable.ptr(),
+                                     dtable.size()[0], ANODE_TYPE_F32, cap == WriteCap::Accumulate, scratch ? scratch->ptr() : nullptr,
+                                     scratch ? scratch->bytes() : 0, kernel_config(), raw(s)), "anode_gpu_embed_tokens_bwd");
+  }
+
+ private:
+  static uint32_t rows_of(const DeviceArray &table)
+  {
+    if (table.size().size() != 2) throw Error(ANODE_E_DIMS, "a table needs [cols, vocab]");
+    return table.size()[1];
+  }
+  static void want_rows(const DeviceArray &rows, const DeviceArray &table, size_t n, const char *what)
+  {
+    want_len(rows, n * table.size()[0], what);
+    if (rows.size().empty() || rows.size()[0] != table.size()[0]) throw Error(ANODE_E_DIMS, std::string(what) + ": expected [cols, tokens...] of the table's columns");
+  }
+};
+
+// Log probabilities of tokens at a temperature of 1/scale: logits of [vocab, rows...], a token, a log probability and an entropy per row, stats of [2, rows...] for
+// the adjoint, the likeliest `top` tokens and their log probabilities of [top, rows...]; what is null is not computed
+struct TokenLogProbsOp {
+  static void apply(const DeviceArray &logits, const DeviceVector<int64_t> *token, DeviceArray *logprob, DeviceArray *entropy, DeviceArray *stats, uint32_t top,
+                    DeviceArray *top_logprob, DeviceVector<int64_t> *top_token, float scale, cudaStream_t s = 0)
+  {
+    const RowDims d = row_dims(logits);
+    want_tokens(token, d.rows);
+    want_opt(logprob, d.rows, "logprob"); want_opt(entropy, d.rows, "entropy"); want_opt(stats, 2 * d.rows, "stats"); want_opt(top_logprob, top * d.rows, "top_logprob");
+    if (top_token && top_token->len() != top * d.rows) throw Error(ANODE_E_DIMS, "top_token: wrong length");
+    check(anode_gpu_token_log_probs_fwd(ANODE_TYPE_F32, d.rows, d.cols, scale, logits.ptr(), d.cols, token ? token->ptr() : nullptr, 8, opt(logprob), opt(entropy),
+                                        opt(stats), top, opt(top_logprob), top_token ? top_token->ptr() : nullptr, 8, kernel_config(), raw(s)),
+          "anode_gpu_token_log_probs_fwd");
+  }
+  // dlogits may be logits
+  static void adjoint(const DeviceArray &logits, const DeviceVector<int64_t> *token, const DeviceArray &stats, const DeviceArray *entropy, const DeviceArray *dlogprob,
+                      const DeviceArray *dentropy, DeviceArray &dlogits, float scale, cudaStream_t s = 0)
+  {
+    const RowDims d = row_dims(logits);
+    want_tokens(token, d.rows);
+    want_len(stats, 2 * d.rows, "stats"); want_len(dlogits, logits.len(), "dlogits");
+    want_opt(entropy, d.rows, "entropy"); want_opt(dlogprob, d.rows, "dlogprob"); want_opt(dentropy, d.rows, "dentropy");
+    check(anode_gpu_token_log_probs_bwd(ANODE_TYPE_F32, d.rows, d.cols, scale, logits.ptr(), d.cols, token ? token->ptr() : nullptr, 8, stats.ptr(), opt(entropy),
+                                        opt(dlogprob), opt(dentropy), dlogits.ptr(), d.cols, kernel_config(), raw(s)), "anode_gpu_token_log_probs_bwd");
+  }
+
+ private:
+  static void want_tokens(const DeviceVector<int64_t> *token, uint64_t rows)
+  {
+    if (token && token->len() != rows) throw Error(ANODE_E_DIMS, "token: one per row");
   }
 };
 

@@ -586,4 +586,129 @@ extern "C" {
     cfg: *const KernelConfig,
     stream: *mut CUstream_st,
   ) -> c_int;
+  // layer norm, rows of a table by tokens, log probabilities of tokens
+  pub fn anode_gpu_layer_norm_add_fwd(
+    type_: c_int,
+    rows: u64,
+    cols: u32,
+    epsilon: f32,
+    x: *const c_void,
+    x_stride: u64,
+    residual: *const c_void,
+    residual_stride: u64,
+    gamma: *const c_void,
+    beta: *const c_void,
+    weight_type: c_int,
+    y: *mut c_void,
+    y_stride: u64,
+    total: *mut c_void,
+    total_stride: u64,
+    mean: *mut f32,
+    inv_std: *mut f32,
+    cfg: *const KernelConfig,
+    stream: *mut CUstream_st,
+  ) -> c_int;
+  pub fn anode_gpu_layer_norm_add_bwd_workspace_bytes(
+    rows: u64,
+    cols: u32,
+  ) -> usize;
+  pub fn anode_gpu_layer_norm_add_bwd(
+    type_: c_int,
+    rows: u64,
+    cols: u32,
+    dy: *const c_void,
+    dy_stride: u64,
+    total: *const c_void,
+    total_stride: u64,
+    mean: *const f32,
+    inv_std: *const f32,
+    gamma: *const c_void,
+    weight_type: c_int,
+    dtotal: *const c_void,
+    dtotal_stride: u64,
+    dx: *mut c_void,
+    dx_stride: u64,
+    dgamma: *mut c_void,
+    dbeta: *mut c_void,
+    workspace: *mut c_void,
+    workspace_bytes: usize,
+    cfg: *const KernelConfig,
+    stream: *mut CUstream_st,
+  ) -> c_int;
+  pub fn anode_gpu_embed_tokens_fwd(
+    type_: c_int,
+    tokens: u64,
+    vocab: u32,
+    cols: u32,
+    scale: f32,
+    token: *const c_void,
+    token_bytes: c_int,
+    table: *const c_void,
+    table_stride: u64,
+    y: *mut c_void,
+    y_stride: u64,
+    cfg: *const KernelConfig,
+    stream: *mut CUstream_st,
+  ) -> c_int;
+  pub fn anode_gpu_embed_tokens_bwd_workspace_bytes(
+    tokens: u64,
+    vocab: u32,
+    cols: u32,
+  ) -> usize;
+  pub fn anode_gpu_embed_tokens_bwd(
+    type_: c_int,
+    tokens: u64,
+    vocab: u32,
+    cols: u32,
+    scale: f32,
+    token: *const c_void,
+    token_bytes: c_int,
+    dy: *const c_void,
+    dy_stride: u64,
+    dtable: *mut c_void,
+    dtable_stride: u64,
+    dtable_type: c_int,
+    accumulate: c_int,
+    workspace: *mut c_void,
+    workspace_bytes: usize,
+    cfg: *const KernelConfig,
+    stream: *mut CUstream_st,
+  ) -> c_int;
+  pub fn anode_gpu_token_log_probs_fwd(
+    type_: c_int,
+    rows: u64,
+    vocab: u32,
+    scale: f32,
+    logits: *const c_void,
+    logits_stride: u64,
+    token: *const c_void,
+    token_bytes: c_int,
+    logprob: *mut f32,
+    entropy: *mut f32,
+    stats: *mut f32,
+    top: u32,
+    top_logprob: *mut f32,
+    top_token: *mut c_void,
+    top_token_bytes: c_int,
+    cfg: *const KernelConfig,
+    stream: *mut CUstream_st,
+  ) -> c_int;
+  pub fn anode_gpu_token_log_probs_bwd(
+    type_: c_int,
+    rows: u64,
+    vocab: u32,
+    scale: f32,
+    logits: *const c_void,
+    logits_stride: u64,
+    token: *const c_void,
+    token_bytes: c_int,
+    stats: *const f32,
+    entropy: *const f32,
+    dlogprob: *const f32,
+    dentropy: *const f32,
+    dlogits: *mut c_void,
+    dlogits_stride: u64,
+    cfg: *const KernelConfig,
+    stream: *mut CUstream_st,
+  ) -> c_int;
 }

@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kGradThreads) layer_norm_grad_kernel(const Lay
   const uint64_t row0 = (uint64_t)blockIdx.x * h.teams + mine;
   const bool works = mine < h.teams && row0 < h.step && row0 < a.rows;
   const uint32_t lanes = h.team < 32 ? ((1u << h.team) - 1) << (lane & ~(h.team - 1)) : 0xffffffffu;      // of this warp in the team
-  const uint32_t nt = blockDim.x;
+  constexpr uint32_t NT = kGradThreads;         // (rings lie as far apart whatever the block's threads)
   uint4 *ring = reinterpret_cast<uint4 *>(shared) + threadIdx.x;
   const T *dy = static_cast<const T *>(a.dy) + row0 * a.dy_stride, *t = static_cast<const T *>(a.total) + row0 * a.total_stride;
   const T *dt = static_cast<const T *>(a.dtotal) + row0 * a.dtotal_stride;
@@ -266,10 +266,10 @@ __global__ void __launch_bounds__(kGradThreads) layer_norm_grad_kernel(const Lay
   float2 dg[CH][H], db[CH][H], gs[GREGS ? CH : 1][H];
   float dg_edge = 0.0f, db_edge = 0.0f, g_edge = on_edge ? a.gamma.at(edge) : 0.0f;
   const bool aligned_gamma = ((uintptr_t)a.gamma.p & 15) == 0;
-  uint4 *gamma_here = ring + h.depth * (CH * 3) * nt;
+  uint4 *gamma_here = ring + h.depth * (CH * 3) * NT;
   auto gamma = [&](int k, float2 *to) {
     float *w = reinterpret_cast<float *>(to);
-    if (G == 1) Vec<T>{gamma_here[k * nt]}.floats(w);
+    if (G == 1) Vec<T>{gamma_here[k * NT]}.floats(w);
     else if (!SHIFT) a.gamma.load<V>(start + k * hop, w);
     else if (aligned_gamma) a.gamma.load_any<V>(start + k * hop, a.cols, w);
     else a.gamma.load_each<V>(start + k * hop, w);
@@ -279,10 +279,10 @@ __global__ void __launch_bounds__(kGradThreads) layer_norm_grad_kernel(const Lay
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       if (!has(k)) continue;
-      if (!SHIFT) gamma_here[k * nt] = Vec<T>::load(from + k * hop).bits;
+      if (!SHIFT) gamma_here[k * NT] = Vec<T>::load(from + k * hop).bits;
       else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) reinterpret_cast<T *>(gamma_here + k * nt)[i] = from[k * hop + i];
+        for (int i = 0; i < V; ++i) reinterpret_cast<T *>(gamma_here + k * NT)[i] = from[k * hop + i];
       }
     }
   }
@@ -317,13 +317,13 @@ __global__ void __launch_bounds__(kGradThreads) layer_norm_grad_kernel(const Lay
   dy += start; t += start; dt += start;
   auto copy = [&] {                     // the next row to be copied
     if (ahead) {
-      uint4 *to = ring + in * (CH * 3) * nt;
+      uint4 *to = ring + in * (CH * 3) * NT;
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
         if (!has(k)) continue;
-        copy_async<16>(to + (3 * k) * nt, dy + k * hop);
-        copy_async<16>(to + (3 * k + 1) * nt, t + k * hop);
-        if (a.dtotal) copy_async<16>(to + (3 * k + 2) * nt, dt + k * hop);
+        copy_async<16>(to + (3 * k) * NT, dy + k * hop);
+        copy_async<16>(to + (3 * k + 1) * NT, t + k * hop);
+        if (a.dtotal) copy_async<16>(to + (3 * k + 2) * NT, dt + k * hop);
       }
       --ahead;
       dy += dy_step; t += t_step; dt += dt_step;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kGradThreads) layer_norm_grad_kernel(const Lay
     copies_commit();
     in = in + 1 == h.depth ? 0 : in + 1;
   };
-  auto row_of = [&](uint32_t place) { return ring + place * (CH * 3) * nt; };
+  auto row_of = [&](uint32_t place) { return ring + place * (CH * 3) * NT; };
   // this thread's part of a row's two sums: of g, and of g*(t - mu)
   auto sums_of = [&](const uint4 *from, const Side &o) {
     const float dy_edge = to_float(o.dy), t_edge = to_float(o.t) - o.mu;
@@ -342,8 +342,8 @@ __global__ void __launch_bounds__(kGradThreads) layer_norm_grad_kernel(const Lay
       if (!has(k)) continue;
       float2 u[H], v[H], w[H];
       if constexpr (!GREGS) gamma(k, w);
-      Vec<T>{from[(3 * k) * nt]}.floats(reinterpret_cast<float *>(u));
-      Vec<T>{from[(3 * k + 1) * nt]}.floats(reinterpret_cast<float *>(v));
+      Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(u));
+      Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(v));
 #pragma unroll
       for (int i = 0; i < H; ++i) {
         const float2 g = mul2(u[i], GREGS ? gs[GREGS ? k : 0][i] : w[i]);
@@ -363,8 +363,8 @@ __global__ void __launch_bounds__(kGradThreads) layer_norm_grad_kernel(const Lay
       if (!has(k)) continue;
       float2 u[H], v[H], w[H], e[H];
       if constexpr (!GREGS) gamma(k, w);
-      Vec<T>{from[(3 * k) * nt]}.floats(reinterpret_cast<float *>(u));
-      Vec<T>{from[(3 * k + 1) * nt]}.floats(reinterpret_cast<float *>(v));
+      Vec<T>{from[(3 * k) * NT]}.floats(reinterpret_cast<float *>(u));
+      Vec<T>{from[(3 * k + 1) * NT]}.floats(reinterpret_cast<float *>(v));
 #pragma unroll
       for (int i = 0; i < H; ++i) {
         const float2 xh = mul2(add2(v[i], away), r);
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kGradThreads) layer_norm_grad_kernel(const Lay
         e[i] = fma2(u[i], GREGS ? gs[GREGS ? k : 0][i] : w[i], fma2(xh, minus, less));
       }
       if (a.dtotal) {
-        Vec<T>{from[(3 * k + 2) * nt]}.floats(reinterpret_cast<float *>(v));
+        Vec<T>{from[(3 * k + 2) * NT]}.floats(reinterpret_cast<float *>(v));
 #pragma unroll
         for (int i = 0; i < H; ++i) e[i] = fma2(e[i], r, v[i]);
       } else {
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kGradThreads) layer_norm_grad_kernel(const Lay
     if (direct) return;
   }
   __syncthreads();
-  for (uint32_t c = threadIdx.x; c < a.cols; c += nt) {
+  for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
     float sum[2] = {0.0f, 0.0f};
     for (uint32_t t = 0; t < parts; ++t)
 #pragma unroll
@@ -574,7 +574,9 @@ bool grad_plan(const LayerGradArgs &a, int type, int weight_type, HeldGrad &h, u
   if (!in_step(a.total, e, a.total_stride, v, a.dy, e, a.dy_stride, a.rows) || !in_step(a.dtotal, e, a.dtotal_stride, v, a.dy, e, a.dy_stride, a.rows) ||
       !in_step(a.dx, e, a.dx_stride, v, a.dy, e, a.dy_stride, a.rows)) return false;
   shift = !aligned_to(a.dy, 16) || a.cols % v || (a.rows > 1 && a.dy_stride % v) || !aligned_to(a.gamma.p, 16);
-  chunks = slots <= 32 ? 1 : slots < 128 ? 2 : slots <= 2048 ? 4 : 8;
+  // four slots to a thread amortize its row's joins ([8192,4096] bf16 51 us, 55 with two), but ragged rows of 16-bit types have no registers for them ([8192,4095] 81
+  // us with four, 61 with two)
+  chunks = slots <= 32 ? 1 : slots < 128 || (shift && v == 8 && slots <= 1024) ? 2 : slots <= 2048 ? 4 : 8;
   if (slots > (v == 8 ? 2048u : 4096u)) return false;
   h.team = (slots + chunks * 32 - 1) / (chunks * 32) * 32;
   if (slots <= 16) {
@@ -591,7 +593,7 @@ bool grad_plan(const LayerGradArgs &a, int type, int weight_type, HeldGrad &h, u
   // a single team of many rows leaves out the threads beyond it, whose rings' place gives it more rows ahead; otherwise they help with the sums
   h.threads = h.teams == 1 && a.rows > 4ull * sms ? h.team : threads;
   // gamma in registers, or its slots beside the ring if they are the rows' and leave it two rows
-  const size_t slot = (size_t)h.threads * chunks * 16;
+  const size_t slot = (size_t)kGradThreads * chunks * 16;
   g = chunks * v <= 16 ? 0 : a.gamma.p && type == weight_type && 7 * slot <= kMostShared ? 1 : 2;
   h.depth = (uint32_t)((kMostShared - (g == 1 ? slot : 0)) / (3 * slot));
   if (h.depth > 4) h.depth = 4;
@@ -607,7 +609,7 @@ template <typename T, int CH, int G> int launch_grad(const LayerGradArgs &a, con
 }
 template <typename T, int CH> int launch_grad(const LayerGradArgs &a, const HeldGrad &h, bool shift, int g, cudaStream_t stream)
 {
-  size_t shared = ((size_t)h.depth * 3 + (g == 1)) * CH * h.threads * 16;
+  size_t shared = ((size_t)h.depth * 3 + (g == 1)) * CH * kGradThreads * 16;
   const size_t sums = (size_t)h.teams * (a.cols + (shift ? a.cols / Vec<T>::V + 1 : 0)) * 8;
   if (shared < sums) shared = sums;
   if constexpr (CH * Vec<T>::V <= 16) return launch_grad<T, CH, 0>(a, h, shift, shared, stream);

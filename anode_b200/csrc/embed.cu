@@ -8,7 +8,7 @@
 //   1. (token, place) are sorted by tokens, and equal ones by places, while other blocks write zeros to the whole table: few by counting for each how many come
 //      before it, more by a radix sort in one cluster;
 //   2. the sorted places are cut into pieces, and a thread per 16 bytes of columns walks down a piece's rows of dy: it writes the sum where a token's run
-//      of places ends.  A run of up to kLong places belongs to the piece where it begins; of a longer one each piece leaves its part in the workspace;
+//      of places ends.  A run of no more places than a piece has belongs to the piece where it begins; of a longer one each piece leaves its part in the workspace;
 //   3. the parts of each long run are joined, in order.
 // All but the sort is bound by memory.
 #include "bn_host.h"
@@ -172,8 +172,8 @@ constexpr uint32_t kCluster = 8, kSortThreads = 512, kSortWarps = kSortThreads /
 constexpr uint32_t kMostBits = 9;                    // of a token to a pass of the sort
 constexpr uint32_t kZeros = 65536;                   // bytes of the table that a block sets to zero
 constexpr uint32_t kCounted = 8192;                  // tokens that are sorted by counting
-constexpr uint32_t kLong = 32;                       // places of a run that one piece adds up, at most
 constexpr uint32_t kMostPiece = 32;                  // places of a piece
+constexpr uint32_t kLong = kMostPiece;               // places on either side that a piece looks at
 constexpr uint32_t kLeastLanes = 4;                  // threads of a piece
 
 struct SortArgs {
@@ -365,7 +365,7 @@ struct SumArgs {
   uint64_t dy_stride;
   void *dtable;
   uint64_t stride;
-  uint32_t piece, pieces, longest;      // places of a piece; a run of more than `longest` (from `piece` to kLong) is long
+  uint32_t piece, pieces;               // places of a piece; a run of more is long
   uint32_t *runs;                       // how many runs are long, in whatever order: each one's first piece, token and count of parts
   uint4 *run;
   float *part;                          // [pieces][2][part_cols]: of a long run that begins before the piece, and of one that begins in it
@@ -383,7 +383,7 @@ struct Piece { uint32_t from, to, head, tail; bool head_before; };
 template <typename T, typename O, bool SHIFT, bool ACC>
 __global__ void __launch_bounds__(kThreads, ACC ? 2 : 3) embed_sums_kernel(const SumArgs a)
 {
-  constexpr int E = Vec<T>::V, STEP = SHIFT ? 2 : 4;
+  constexpr int E = Vec<T>::V, STEP = SHIFT || (ACC && sizeof(O) > sizeof(T)) ? 2 : 4;      // (as there are registers for)
   constexpr uint32_t PIECES = kThreads / kLeastLanes;
   __shared__ uint32_t key[PIECES * kMostPiece + 2 * kLong], place[PIECES * kMostPiece + 2 * kLong];
   __shared__ Piece piece[PIECES];
@@ -410,9 +410,9 @@ __global__ void __launch_bounds__(kThreads, ACC ? 2 : 3) embed_sums_kernel(const
     Piece q = {at, at, ~0u, ~0u, false};
     if (size && key[at] != ~0u) {
       const uint32_t k0 = key[at], before = run(k0, at - 1, -1), after = run(k0, at + 1, 1);
-      const bool long0 = before + 1 + after > a.longest;
+      const bool long0 = before + 1 + after > a.piece;
       const uint32_t k1 = key[last], ahead = run(k1, last - 1, -1), behind = run(k1, last + 1, 1);
-      const bool long1 = k1 != ~0u && ahead + 1 + behind > a.longest, whole = k0 == k1;
+      const bool long1 = k1 != ~0u && ahead + 1 + behind > a.piece, whole = k0 == k1;
       q.head_before = before > 0;
       if (before && !long0) q.from = at + 1 + after;             // (that run is an earlier piece's)
       if (long0) q.head = k0;
@@ -509,18 +509,23 @@ __global__ void __launch_bounds__(kThreads, ACC ? 2 : 3) embed_sums_kernel(const
   }
 }
 
-// The parts of long runs: a block has 32 columns, four to a lane, and every gridDim.y-th such run, whose parts its 32 groups of lanes add in order, each a stretch
+// The parts of long runs: a block has 64 columns, four to a lane, and every gridDim.y-th such run, whose parts its 16 groups of lanes add in order, each a stretch
 template <typename O> __global__ void __launch_bounds__(kThreads) embed_join_kernel(const SumArgs a, const int accumulate)
 {
-  constexpr uint32_t GROUPS = kThreads / 8;
-  __shared__ float sums[GROUPS][33];
-  const uint32_t group = threadIdx.x / 8, lane = threadIdx.x & 7;
-  const uint64_t c = (uint64_t)blockIdx.x * 32 + lane * 4, column = (uint64_t)blockIdx.x * 32 + threadIdx.x;
+  constexpr uint32_t LANES = 16, GROUPS = kThreads / LANES;
+  __shared__ float sums[GROUPS][4 * LANES + 1];
+  const uint32_t group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const uint64_t c = ((uint64_t)blockIdx.x * LANES + lane) * 4, column = (uint64_t)blockIdx.x * 4 * LANES + threadIdx.x;
   pdl_wait();
   const uint32_t runs = *a.runs;
+  uint4 next = a.run[blockIdx.y];        // (what the list does not hold is not used)
   for (uint32_t i = blockIdx.y; i < runs; i += gridDim.y) {
-    const uint4 run = a.run[i];
+    const uint4 run = next;
+    if (i + gridDim.y < runs) next = a.run[i + gridDim.y];
     const uint32_t parts = run.z, each = (parts + GROUPS - 1) / GROUPS, lo = min(parts, group * each), hi = min(parts, lo + each);
+    O *out = static_cast<O *>(a.dtable) + run.y * a.stride + column;
+    const bool writes = threadIdx.x < 4 * LANES && column < a.cols;
+    const float old = accumulate && writes ? to_float(*out) : 0.0f;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (c < a.cols) {
 #pragma unroll 8
@@ -532,12 +537,11 @@ template <typename O> __global__ void __launch_bounds__(kThreads) embed_join_ker
     float *const to = sums[group] + lane * 4;
     to[0] = sum.x; to[1] = sum.y; to[2] = sum.z; to[3] = sum.w;
     __syncthreads();
-    if (threadIdx.x < 32 && column < a.cols) {
-      O *out = static_cast<O *>(a.dtable) + run.y * a.stride + column;
-      float total = accumulate ? to_float(*out) : 0.0f, all = 0.0f;
+    if (writes) {
+      float all = 0.0f;
 #pragma unroll
       for (uint32_t g = 0; g < GROUPS; ++g) all += sums[g][threadIdx.x];
-      *out = from_float<O>(accumulate ? fmaf(all, a.scale, total) : all * a.scale);
+      *out = from_float<O>(accumulate ? fmaf(all, a.scale, old) : all * a.scale);
     }
     __syncthreads();
   }
@@ -562,23 +566,22 @@ inline uint32_t power_up_to(uint64_t n, uint32_t most)
   return v;
 }
 
-// Places of a piece: as many as give each multiprocessor three blocks, of as many pieces side by side as rows of 16-bit columns leave them; a run of more is long, or
-// of more than 8
+// Places of a piece; a run of more is long.  As many as leave the device 2^18 threads, of rows of 16-bit columns that begin anywhere, but 10 at least, where what each piece does
+// beside its rows counts ([4099 tokens, 1001 columns] added to f32: 23.5 us with 10, 26 with 8, 28 with 16; [16384,4096] bf16: 81 us with 32, 86 with 16, 102 with 8)
 inline uint32_t piece_of(uint64_t tokens, uint32_t cols)
 {
-  const uint32_t side_by_side = kThreads / power_up_to(((uint64_t)cols + 7) / 8, kThreads);
-  const uint64_t pieces = 3ull * 148 * side_by_side, each = (tokens + pieces - 1) / pieces;
-  return (uint32_t)(each < 4 ? 4 : each < kMostPiece ? each : kMostPiece);
+  const uint64_t threads = tokens * ((uint64_t)cols / 8 + 16), each = (threads + (1u << 18) - 1) >> 18;
+  return (uint32_t)(each < 10 ? 10 : each < kMostPiece ? each : kMostPiece);
 }
 
 // Where the workspace's arrays begin, in bytes
 struct Layout {
-  uint64_t n, piece, longest, pieces, part_cols, runs, run, part, bytes;
-  Layout(uint64_t tokens, uint32_t cols) : n((tokens + 3) / 4 * 4), piece(piece_of(tokens, cols)), longest(piece < 8 ? 8 : piece), pieces((tokens + piece - 1) / piece), part_cols(((uint64_t)cols + 3) / 4 * 4)
+  uint64_t n, piece, pieces, part_cols, runs, run, part, bytes;
+  Layout(uint64_t tokens, uint32_t cols) : n((tokens + 3) / 4 * 4), piece(piece_of(tokens, cols)), pieces((tokens + piece - 1) / piece), part_cols(((uint64_t)cols + 3) / 4 * 4)
   {
     runs = 16 * n;
     run = runs + 16;
-    part = run + tokens / (longest + 1) * 16;
+    part = run + tokens / (piece + 1) * 16;
     bytes = part + pieces * 2 * part_cols * 4;
   }
 };
@@ -597,9 +600,9 @@ template <typename T, typename O> int launch_sums(SumArgs a, bool shift, int acc
   const dim3 grid((a.pieces + per_block - 1) / per_block, (all + a.lanes - 1) / a.lanes);
   TRY(launch(accumulate ? (shift ? embed_sums_kernel<T, O, true, true> : embed_sums_kernel<T, O, false, true>)
                         : (shift ? embed_sums_kernel<T, O, true, false> : embed_sums_kernel<T, O, false, false>), grid, per_block * a.lanes, 0, stream, a));
-  if (a.n <= a.longest) return ANODE_OK;
+  if (a.n <= a.piece) return ANODE_OK;
   // a run to a block, of the tokens of a training batch: some 50 of 16384 come more than 32 times
-  const uint32_t wide = (uint32_t)(((uint64_t)a.cols + 31) / 32), most = a.n / (a.longest + 1), blocks = (16 * sm_count() + wide - 1) / wide;
+  const uint32_t wide = (uint32_t)(((uint64_t)a.cols + 63) / 64), most = a.n / (a.piece + 1), blocks = (8 * sm_count() + wide - 1) / wide;
   return launch(embed_join_kernel<O>, dim3(wide, blocks < most ? blocks : most), kThreads, 0, stream, a, accumulate);
 }
 
@@ -683,7 +686,7 @@ extern "C" int anode_gpu_embed_tokens_bwd(
                : (oe == 4 ? launch_in_clusters(embed_sort_kernel<uint32_t>, grid, kCluster, kSortThreads, 0, stream, s)
                           : launch_in_clusters(embed_sort_kernel<uint16_t>, grid, kCluster, kSortThreads, 0, stream, s))));
   if (!tokens) return ANODE_OK;
-  const SumArgs a = {(uint32_t)tokens, vocab, cols, scale, s.key[0], s.place[0], dy, dy_stride, dtable, dtable_stride, (uint32_t)l.piece, (uint32_t)l.pieces, (uint32_t)l.longest,
+  const SumArgs a = {(uint32_t)tokens, vocab, cols, scale, s.key[0], s.place[0], dy, dy_stride, dtable, dtable_stride, (uint32_t)l.piece, (uint32_t)l.pieces,
                      words + l.runs / 4, reinterpret_cast<uint4 *>(static_cast<char *>(workspace) + l.run), reinterpret_cast<float *>(static_cast<char *>(workspace) + l.part), (uint32_t)l.part_cols, 0};
   const bool shift = !whole(dy, e, dy_stride, tokens, cols) || !whole(dtable, oe, dtable_stride, vocab, cols);
   return by_type(type, [&](auto t) {

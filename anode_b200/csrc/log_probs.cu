@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
       if (threadIdx.x < groups) {
         const uint32_t mine = listed[threadIdx.x];
         uint32_t before = 0;
+#pragma unroll 8
         for (uint32_t j = 0; j < groups; ++j) before += listed[j] > mine || (listed[j] == mine && j < threadIdx.x);
         if (before == a.top - 1) bound_count = mine;
       }
@@ -368,6 +369,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
       for (uint32_t i = threadIdx.x; i < n; i += threads) {
         const uint64_t key = buffer[i];
         uint32_t before = 0;
+#pragma unroll 8
         for (uint32_t j = 0; j < n; ++j) before += buffer[j] > key;
         if (before < a.top) best[before] = key;
       }
@@ -397,7 +399,6 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
       }
       if constexpr (TOP) {
         if (first) sums[0] = Sums{own.m, log_sum, 0.0f};
-        // a list's keys come in falling order: one's place is its own and that in each other list
         const uint32_t all = cluster * a.top;
         for (uint32_t i = threadIdx.x; i < all; i += threads) {
           const uint32_t r = i / a.top;
@@ -407,15 +408,18 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
         __syncthreads();
         const float m = sums[0].m, l = sums[0].sum;
         for (uint32_t i = threadIdx.x; i < all; i += threads) {
+          // the keys that are larger: all of a few are looked at side by side; of more, a list's come in falling order
           const uint64_t key = lists[i];
-          const uint32_t mine = i / a.top;
-          uint32_t place = i - mine * a.top;
-          for (uint32_t r = 0; r < cluster; ++r) {
-            if (r == mine) continue;
-            uint32_t low = 0, high = a.top;       // keys of the list that are larger
-            while (low < high) { const uint32_t mid = (low + high) / 2; if (lists[r * a.top + mid] > key) low = mid + 1; else high = mid; }
-            place += low;
-          }
+          uint32_t place = 0;
+          if (all <= 256) {
+#pragma unroll 8
+            for (uint32_t j = 0; j < all; ++j) place += lists[j] > key;
+          } else
+            for (uint32_t r = 0; r < cluster; ++r) {
+              uint32_t low = 0, high = a.top;
+              while (low < high) { const uint32_t mid = (low + high) / 2; if (lists[r * a.top + mid] > key) low = mid + 1; else high = mid; }
+              place += low;
+            }
           if (key && place < a.top) put_top(a, row, place, key, m, l);
         }
       }

@@ -125,7 +125,7 @@ struct Sums {
   }
 };
 
-constexpr uint32_t kBuffer = 1024;         // keys that may be among the likeliest
+constexpr uint32_t kBuffer = 512;          // keys that may be among the likeliest
 
 // A row's logits are shared out to a cluster's blocks, and theirs to the threads by slots of 16 bytes in turn: one pass with a running maximum and sums that
 // follow it.  The likeliest: the k-th largest of the threads' maxima is a bound that k logits reach at least, so that few threads have more of them, whose
@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
 {
   constexpr int V = Vec<T>::V, U = 4;
   __shared__ Sums sums[kMostThreads / 32], block_sums;
-  __shared__ uint64_t buffer[TOP ? kBuffer : 1], best[TOP ? kMostTop : 1], lists[TOP ? 8 * kMostTop : 1];
+  __shared__ uint64_t buffer[TOP ? kBuffer : 1], best[TOP ? kMostTop : 1];
+  extern __shared__ uint64_t lists[];        // of a cluster: its blocks' likeliest
   __shared__ uint32_t listed[TOP ? kMostThreads : 1], count, bound_count;
   const uint32_t threads = blockDim.x, warps = threads / 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t rank = cluster > 1 ? cluster_rank() : 0;
@@ -400,14 +401,15 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_log_probs_kernel(const 
       if constexpr (TOP) {
         if (first) sums[0] = Sums{own.m, log_sum, 0.0f};
         const uint32_t all = cluster * a.top;
-        for (uint32_t i = threadIdx.x; i < all; i += threads) {
+        for (uint32_t i = threadIdx.x; cluster > 1 && i < all; i += threads) {
           const uint32_t r = i / a.top;
           const uint32_t *p = reinterpret_cast<const uint32_t *>(best + (i - r * a.top));
-          lists[i] = cluster > 1 ? (uint64_t)peer_load(p + 1, r) << 32 | peer_load(p, r) : best[i];
+          lists[i] = (uint64_t)peer_load(p + 1, r) << 32 | peer_load(p, r);
         }
         __syncthreads();
         const float m = sums[0].m, l = sums[0].sum;
-        for (uint32_t i = threadIdx.x; i < all; i += threads) {
+        if (cluster == 1) { for (uint32_t i = threadIdx.x; i < a.top; i += threads) put_top(a, row, i, best[i], m, l); }      // (a row has that many)
+        else for (uint32_t i = threadIdx.x; i < all; i += threads) {
           // the keys that are larger: all of a few are looked at side by side; of more, a list's come in falling order
           const uint64_t key = lists[i];
           uint32_t place = 0;
@@ -578,7 +580,7 @@ extern "C" int anode_gpu_token_log_probs_fwd(
     using T = decltype(t);
     auto kernel = top ? (entropy ? token_log_probs_kernel<T, true, true> : token_log_probs_kernel<T, false, true>)
                       : (entropy ? token_log_probs_kernel<T, true, false> : token_log_probs_kernel<T, false, false>);
-    return cluster > 1 ? launch_in_clusters(kernel, grid, cluster, threads, 0, stream, a, cluster) : launch(kernel, grid, threads, 0, stream, a, cluster);
+    return cluster > 1 ? launch_in_clusters(kernel, grid, cluster, threads, (size_t)cluster * top * 8, stream, a, cluster) : launch(kernel, grid, threads, 0, stream, a, cluster);
   });
 }
 

@@ -675,11 +675,12 @@ extern "C" int anode_gpu_embed_tokens_bwd(
   if (!accumulate) {
     s.zero_rows = vocab; s.stride = dtable_stride * oe; s.row_bytes = (uint64_t)cols * oe;
     if (dtable_stride == cols) { s.row_bytes *= vocab; s.zero_rows = 1; }      // (one long row)
-    s.cuts = (uint32_t)((s.row_bytes + kZeros - 1) / kZeros);
-    s.rows = s.cuts > 1 ? 1 : (uint32_t)(kZeros / s.row_bytes);
-    blocks = (s.zero_rows + s.rows - 1) / s.rows * s.cuts;
+    const uint64_t cuts = (s.row_bytes + kZeros - 1) / kZeros;
+    s.rows = cuts > 1 ? 1 : (uint32_t)(kZeros / s.row_bytes);
+    blocks = (s.zero_rows + s.rows - 1) / s.rows * cuts;
     if (!counted) blocks = (blocks + kCluster - 1) / kCluster * kCluster;
-    if (blocks >> 30) return ANODE_E_DIMS;
+    if (cuts >> 30 || blocks >> 30) return ANODE_E_DIMS;
+    s.cuts = (uint32_t)cuts;
   }
   const dim3 grid(s.sorting + (uint32_t)blocks);
   TRY((counted ? (oe == 4 ? launch(embed_count_kernel<uint32_t>, grid, kSortThreads, 0, stream, s) : launch(embed_count_kernel<uint16_t>, grid, kSortThreads, 0, stream, s))

@@ -449,10 +449,11 @@ template <typename T> __global__ void __launch_bounds__(kThreads) token_log_prob
   }
 }
 
-// The gradient where logits and dlogits begin their rows at the same places of 16 bytes: a block has a stretch of a row, a thread four slots of it, all of which are
-// asked for before the row's numbers are; logits before the first slot and behind the last have a thread each
-constexpr uint32_t kGradSlots = 4;
-template <typename T, bool ENTROPY> __global__ void __launch_bounds__(kThreads, 6) token_log_probs_grad_kernel(const ProbsGradArgs a, const uint32_t cuts)
+// The gradient where logits and dlogits begin their rows at the same places of 16 bytes: a block has a stretch of a row and walks it in steps of four slots to a thread,
+// the first of which is asked for before the row's numbers are; logits before the first slot and behind the last have a thread each.
+// Stretches of up to four steps: the row's numbers, once for each, are many instructions ([1024,131072] bf16: 55 M warp instructions with one step, 45 M with four).
+constexpr uint32_t kGradSlots = 4, kGradSteps = 4;
+template <typename T, bool ENTROPY> __global__ void __launch_bounds__(kThreads, 6) token_log_probs_grad_kernel(const ProbsGradArgs a, const uint32_t cuts, const uint32_t stretch)
 {
   constexpr int V = Vec<T>::V, U = kGradSlots;
   const uint32_t threads = blockDim.x;
@@ -460,17 +461,22 @@ template <typename T, bool ENTROPY> __global__ void __launch_bounds__(kThreads, 
   pdl_wait();
   pdl_trigger();
   for (uint64_t at = blockIdx.x; at < a.rows * cuts; at += gridDim.x) {
-    const uint64_t row = at / cuts;
+    const uint64_t row = at >> 32 ? at / cuts : (uint32_t)at / cuts;
     const uint32_t cut = (uint32_t)(at - row * cuts);
     const T *x = static_cast<const T *>(a.logits) + row * a.stride;
     T *dx = static_cast<T *>(a.dlogits) + row * a.dstride;
     const uint32_t head = min(a.vocab, (uint32_t)(-(int)((uintptr_t)x / sizeof(T)) & (V - 1))), slots = (a.vocab - head) / V, tail = a.vocab - head - slots * V;
-    const uint32_t first = cut * U * threads + threadIdx.x;
+    const uint32_t end = min(slots, (cut + 1) * stretch);
     const bool on_edge = cut == 0 && threadIdx.x < head + tail;
     const uint32_t edge = threadIdx.x < head ? threadIdx.x : a.vocab - tail + (threadIdx.x - head);
+    uint32_t first = cut * stretch + threadIdx.x;
     Vec<T> v[U];
+    auto fetch = [&] {
+      const T *from = x + head + (uint64_t)first * V;
 #pragma unroll
-    for (int u = 0; u < U; ++u) if (first + u * threads < slots) v[u] = Vec<T>::load(x + head + (uint64_t)(first + u * threads) * V);
+      for (int u = 0; u < U; ++u) if (first + u * threads < end) v[u] = Vec<T>::load(from + u * threads * V);
+    };
+    fetch();
     T one = {};
     if (on_edge) one = x[edge];
     const float2 stats = a.stats[row];
@@ -487,35 +493,34 @@ template <typename T, bool ENTROPY> __global__ void __launch_bounds__(kThreads, 
       const float2 p = make_float2(exp2_of(l.x), exp2_of(l.y));
       return mul2(p, ENTROPY ? fma2(slope2, l, flat2) : flat2);
     };
-    auto all = [&](auto clamp) {
+    auto slot = [&](int u, auto clamp) {
+      const uint32_t c = head + (first + u * threads) * V;
+      float2 f[V / 2];
+      v[u].floats(reinterpret_cast<float *>(f));
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (first + u * threads >= slots) continue;
-        const uint32_t c = head + (first + u * threads) * V;
-        float2 f[V / 2];
-        v[u].floats(reinterpret_cast<float *>(f));
+      for (int i = 0; i < V / 2; ++i) f[i] = gradient(f[i], clamp);
+      if (token - c < V) {
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) f[i] = gradient(f[i], clamp);
-        if (token - c < V) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) if (token - c == i) reinterpret_cast<float *>(f)[i] += more;
-        }
-        Vec<T>::of(reinterpret_cast<const float *>(f)).store(dx + c);
+        for (int i = 0; i < V; ++i) if (token - c == i) reinterpret_cast<float *>(f)[i] += more;
       }
+      Vec<T>::of(reinterpret_cast<const float *>(f)).store(dx + c);
     };
-    bool far = false;
-    if (ENTROPY) {
-      Extremes<T> low;
-      low.start(nothing<T>());
+    while (first < end) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (first + u * threads >= slots) continue;
-        if (u == 0) low.start(v[0].bits);
-        low.template take<true>(v[u].bits, u == 0);
+        if (first + u * threads >= end) continue;
+        bool far = false;
+        if (ENTROPY) {
+          Extremes<T> low;
+          low.start(v[u].bits);
+          low.template take<true>(v[u].bits, 1);
+          far = !(fmaf(low.smallest() + minus.x, rate, less.x) >= kFloor);
+        }
+        if (far) slot(u, std::true_type()); else slot(u, std::false_type());
       }
-      far = !(first < slots && fmaf(low.smallest() + minus.x, rate, less.x) >= kFloor);
+      first += U * threads;
+      fetch();
     }
-    if (far) all(std::true_type()); else all(std::false_type());
     if (on_edge) {
       const float d = gradient(both(to_float(one)), std::true_type()).x;
       dx[edge] = from_float<T>(edge == token ? d + more : d);
@@ -604,11 +609,14 @@ extern "C" int anode_gpu_token_log_probs_bwd(
   const ProbsGradArgs a = {rows, vocab, scale, logits, logits_stride, token, token_bytes, reinterpret_cast<const float2 *>(stats), entropy, dlogprob, dentropy,
                            dlogits, dlogits_stride};
   const uint32_t v = (uint32_t)(16 / e), slots = vocab / v, each = (slots + 32 * kGradSlots - 1) / (32 * kGradSlots) * 32;
-  const uint32_t threads = each < 32 ? 32 : each < kThreads ? each : kThreads, cuts = slots ? (slots + threads * kGradSlots - 1) / (threads * kGradSlots) : 1;
+  const uint32_t threads = each < 32 ? 32 : each < kThreads ? each : kThreads, step_slots = threads * kGradSlots;
+  // more steps to a block where the blocks of one step each would fill the device's places (six of a multiprocessor) four times
+  const uint64_t blocks = rows * (slots / step_slots + 1), steps = blocks / (24ull * anode_b200::sm_count());
+  const uint32_t stretch = step_slots * (uint32_t)(steps < 1 ? 1 : steps < kGradSteps ? steps : kGradSteps), cuts = slots ? (slots + stretch - 1) / stretch : 1;
   const bool step = in_step(dlogits, e, dlogits_stride, v, logits, e, logits_stride, rows);
   return by_type(type, [&](auto t) {
     using T = decltype(t);
-    return step ? launch(dentropy ? token_log_probs_grad_kernel<T, true> : token_log_probs_grad_kernel<T, false>, dim3(row_blocks(rows * cuts)), threads, 0, stream, a, cuts)
+    return step ? launch(dentropy ? token_log_probs_grad_kernel<T, true> : token_log_probs_grad_kernel<T, false>, dim3(row_blocks(rows * cuts)), threads, 0, stream, a, cuts, stretch)
                 : launch(token_log_probs_grad_rows_kernel<T>, dim3(row_blocks(rows)), kThreads, 0, stream, a);
   });
 }

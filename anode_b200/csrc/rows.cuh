@@ -174,13 +174,6 @@ template <typename T> struct Vec {
   static constexpr int V = 16 / sizeof(T);
   uint4 bits;
   __device__ __forceinline__ static Vec load(const T *p) { return Vec{*reinterpret_cast<const uint4 *>(p)}; }
-  // what is read once, and leaves the first-level cache to what is read again
-  __device__ __forceinline__ static Vec pass(const T *p)
-  {
-    Vec v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.bits.x), "=r"(v.bits.y), "=r"(v.bits.z), "=r"(v.bits.w) : "l"(p) : "memory");
-    return v;
-  }
   __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint4 *>(p) = bits; }
   __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? bits.x : i == 1 ? bits.y : i == 2 ? bits.z : bits.w; }
   __device__ __forceinline__ void floats(float *f) const

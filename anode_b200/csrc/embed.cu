@@ -11,9 +11,9 @@
 //      of places ends.  A run of no more places than a piece has belongs to the piece where it begins; of a longer one each piece leaves its part in the workspace;
 //   3. the parts of each long run are joined, in order.
 //
-// Measured on one B200 against its copy bandwidth of 6539 GB/s: rows of 16384 tokens of [32768,8192] bf16 58 us (0.93), of [.,4095] f16 51 us, 32 tokens 1.6 us.  The gradient
+// Measured on one B200 against its copy bandwidth of 6539 GB/s: rows of 16384 tokens of [32768,8192] bf16 59 us (0.93), of [.,4095] f16 51 us, 32 tokens 1.6 us.  The gradient
 // of 16384 tokens of [32768,4096] bf16, whose tokens are common ones mostly, 81 us (0.76): zeros 37 (7.2 TB/s, the sort beside them), sums 35, join 8; rows named twice are
-// written twice.  Added to what is there 69 us, where the sort (15 us, a chain of eight waits of a cluster) is seen; to f32 85.  4099 tokens of [50021,1001] f16 into f32 47 us,
+// written twice.  Added to what is there 69 us, where the sort (17 us, a chain of eight waits of a cluster) is seen; to f32 85.  4099 tokens of [50021,1001] f16 into f32 47 us,
 // added 23.5.  The zeros and the sums are bound by memory, small calls by the chain token -> place -> row -> sum.
 #include "bn_host.h"
 #include "rows.cuh"

@@ -9,12 +9,12 @@
 //
 // Bound by memory where there are many rows, by the chain launch -> load -> sum -> sum -> store where there are few, and in the adjoint by the latency of its
 // instructions (sums of two weights' gradients leave a multiprocessor 16 warps).  Measured on one B200 against its copy bandwidth of 6539 GB/s, with residual:
-//   forward   bf16 [16384,8192] 160 us (1.03 of it), [16384,2048] 43 us (0.95), [1,4096] 2.2 us; f32 [4099,1001] without a residual 11.3 us (a copy of it 11.2)
-//   adjoint   bf16 [8192,4096] 51 us (0.80), [8192,16384] 178 us (0.92), [8192,4095] 67 us (0.61); f32 [4096,8192] 86 us (0.96), [4096,16384] 256 us (0.64: gamma is
+//   forward   bf16 [16384,8192] 157 to 160 us (1.03 of it), [16384,2048] 43 us (0.95), [1,4096] 2.2 us; f32 [4099,1001] without a residual 11.3 to 13.6 us (a copy of it 11.2 to 12.7)
+//   adjoint   bf16 [8192,4096] 51 us (0.80), [8192,16384] 178 us (0.92), [8192,4095] 69 us (0.60); f32 [4096,8192] 86 us (0.96), [4096,16384] 254 us (0.65: gamma is
 //             read anew for every row); f16 [2047,1535] 17 us
 // Three kernels, as the RMS norm has: rows held in registers, the adjoint through rings of asynchronous copies, and plain ones, element by element, for rows that
 // are too wide or do not begin in step.  Tried and dropped: the next row's sums ahead of this row's gradient (65 us in the place of 55 for [8192,4096]); the
-// single row of a ring refilled slot by slot (287 us in the place of 256 for f32 [4096,16384]); joins of a block's warps by loads in the place of shuffles
+// single row of a ring refilled slot by slot (287 us in the place of 254 for f32 [4096,16384]); joins of a block's warps by loads in the place of shuffles
 // ([1,4096] 2.55 us in the place of 2.2).
 #include "bn_host.h"
 #include "rows.cuh"
@@ -585,7 +585,7 @@ bool grad_plan(const LayerGradArgs &a, int type, int weight_type, HeldGrad &h, u
       !in_step(a.dx, e, a.dx_stride, v, a.dy, e, a.dy_stride, a.rows)) return false;
   shift = !aligned_to(a.dy, 16) || a.cols % v || (a.rows > 1 && a.dy_stride % v) || !aligned_to(a.gamma.p, 16);
   // four slots to a thread amortize its row's joins ([8192,4096] bf16 51 us, 55 with two), but ragged rows of 16-bit types have no registers for them ([8192,4095] 81
-  // us with four, 61 with two)
+  // us with four, 67 to 69 with two)
   chunks = slots <= 32 ? 1 : slots < 128 || (shift && v == 8 && slots <= 1024) ? 2 : slots <= 2048 ? 4 : 8;
   if (slots > (v == 8 ? 2048u : 4096u)) return false;
   h.team = (slots + chunks * 32 - 1) / (chunks * 32) * 32;

@@ -6,8 +6,8 @@
 // A row keeps m and L apart, since their sum would lose L's digits beside a large m.
 //
 // Measured on one B200 against its copy bandwidth of 6539 GB/s: bf16 [4096,131072] with entropies 163 us (1.00; 188 in a loop of seconds, near the power cap), [4096,50021]
-// 72 us (0.87), [256,131072] 15 us; f32 [16,131072] with the likeliest twenty 11.4 us, without 6.3.  Gradient bf16 [4096,50021] with entropies 128 us (0.98), without 126.
-// Many long rows are bound by memory (an exponential for each logit keeps its unit busy for two thirds of the time), few by the chain load -> sums -> cluster -> store.
+// 72 to 74 us (0.85 to 0.87), [256,131072] 15 to 16 us; f32 [16,131072] with the likeliest twenty 11.4 to 12.5 us, without 5.7.  Gradient bf16 [4096,50021] with entropies 128 us (0.98), without 123 (1.02).
+// Many long rows are bound by memory (an exponential for each logit keeps its unit busy for 60 % of the time), few by the chain load -> sums -> cluster -> store.
 #include "bn_host.h"
 #include "rows.cuh"
 
@@ -617,8 +617,10 @@ extern "C" int anode_gpu_token_log_probs_bwd(
                            dlogits, dlogits_stride};
   const uint32_t v = (uint32_t)(16 / e), slots = vocab / v, each = (slots + 32 * kGradSlots - 1) / (32 * kGradSlots) * 32;
   const uint32_t threads = each < 32 ? 32 : each < kThreads ? each : kThreads, step_slots = threads * kGradSlots;
-  // more steps to a block where the blocks of one step each would fill the device's places (six of a multiprocessor) four times
-  const uint64_t blocks = rows * (slots / step_slots + 1), steps = blocks / (24ull * anode_b200::sm_count());
+  // more steps to a block where the blocks of one step each would fill the device's places (six of a multiprocessor) four times, and the entropy's gradient is asked for,
+  // whose numbers cost more ([4096,50021] bf16 128 us, 133 with one step).  Without it one step is better: 122.6 us, 126 with four, f32 [2048,65536] 156 and 163; only in
+  // a loop of seconds, near the power cap, is it worse (130 and 127)
+  const uint64_t blocks = rows * (slots / step_slots + 1), steps = !dentropy ? 1 : blocks / (24ull * anode_b200::sm_count());
   const uint32_t stretch = step_slots * (uint32_t)(steps < 1 ? 1 : steps < kGradSteps ? steps : kGradSteps), cuts = slots ? (slots + stretch - 1) / stretch : 1;
   const bool step = in_step(dlogits, e, dlogits_stride, v, logits, e, logits_stride, rows);
   return by_type(type, [&](auto t) {

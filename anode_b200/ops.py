@@ -923,12 +923,16 @@ class LayerNormAdd:
         return y, total
 
     def backward(self, dy, dtotal=None, out=None):
-        """The gradient of x, which is the residual's, too; those of gamma and beta are left in dgamma and dbeta."""
+        """The gradient of x, which is the residual's, too; those of gamma and beta are left in dgamma and dbeta.  In the sum's place
+        (out=total) it is the last one of its forward pass."""
         if self._saved is None:
             raise RuntimeError("backward before forward")
         total, mean, inv_std = self._saved
         dx = out if out is not None else torch.empty_like(dy)
-        return LayerNormalizeAddOp.adjoint(dy, total, mean, inv_std, dx, self.gamma, dtotal, self.dgamma, self.dbeta)
+        LayerNormalizeAddOp.adjoint(dy, total, mean, inv_std, dx, self.gamma, dtotal, self.dgamma, self.dbeta)
+        if out is not None and _share_memory(total, out):
+            self._saved = None
+        return dx
 
 
 class TokenEmbedding:
@@ -985,12 +989,15 @@ class TokenLogProbs:
         return logprob, h
 
     def backward(self, dlogprob, dentropy=None, out=None):
-        """The gradient of the logits, in whose place it may be (out=logits)."""
+        """The gradient of the logits, in whose place it may be (out=logits); it is then the last one of its forward pass."""
         if self._saved is None:
             raise RuntimeError("backward before forward")
         logits, tokens, stats, h = self._saved
         dlogits = out if out is not None else torch.empty_like(logits)
-        return TokenLogProbsOp.adjoint(logits, tokens, stats, dlogprob, dlogits, h if dentropy is not None else None, dentropy, self.scale)
+        TokenLogProbsOp.adjoint(logits, tokens, stats, dlogprob, dlogits, h if dentropy is not None else None, dentropy, self.scale)
+        if out is not None and _share_memory(logits, out):
+            self._saved = None
+        return dlogits
 
 
 class SyncWorkspace(Workspace):

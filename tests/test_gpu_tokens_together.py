@@ -217,3 +217,23 @@ def test_accumulating_grows_from_what_is_there():
         embed.backward(dy, ops.WriteCap.Accumulate if i else ops.WriteCap.Assign)
         want.index_add_(0, tokens, dy.float())
     assert torch.equal(embed.dtable, want)
+
+
+def test_backward_in_the_place_of_what_it_read_is_the_last():
+    """The gradient in the logits' or the sum's place leaves a second backward pass nothing to read; elsewhere, and in the incoming gradient's place, it may be repeated."""
+    logits, tokens = torch.randn(6, 40, device="cuda"), ids(6, 40, 1)
+    probs, w = ops.TokenLogProbs(), torch.ones(6, device="cuda")
+    probs.forward(logits, tokens)
+    first = probs.backward(w, w).clone()
+    assert torch.equal(probs.backward(w, w), first) and torch.equal(probs.backward(w, w, out=logits), first)
+    with pytest.raises(RuntimeError, match="backward before forward"):
+        probs.backward(w, w)
+    probs.forward(torch.randn(6, 40, device="cuda"), tokens)
+    probs.backward(w, w)
+    norm, x, dy = ops.LayerNormAdd(40), torch.randn(6, 40, device="cuda"), torch.randn(6, 40, device="cuda")
+    _, total = norm.forward(x, x)
+    dx = norm.backward(dy, total).clone()
+    assert torch.equal(norm.backward(dy.clone(), total, out=torch.empty_like(dy)), dx)
+    assert torch.equal(norm.backward(dy, total, out=total), dx)
+    with pytest.raises(RuntimeError, match="backward before forward"):
+        norm.backward(dy)

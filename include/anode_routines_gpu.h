@@ -617,7 +617,9 @@ int anode_gpu_rotary_positions_bwd(
  *   total = round(x + residual)                        (x where residual is NULL; stored where total is not NULL)
  *   mu    = sum(total)/cols,  r = (sum((total - mu)^2)/cols + epsilon)^-1/2      per row (stored where mean, inv_std are not NULL)
  *   y     = (total - mu) * r * gamma + beta            (gamma NULL: 1, beta NULL: 0; of one type)
- * As in anode_gpu_rms_norm_add_fwd, the norm reads the sum as it is stored, and total without residual is refused. */
+ * As in anode_gpu_rms_norm_add_fwd, the norm reads the sum as it is stored, and total without residual is refused.  Rows and the squares of
+ * what is left of them are summed in f32: rows whose spread (1/r) reaches 2^64/sqrt(cols) give r = 0 and y = beta, rows whose sum leaves f32's
+ * range, or that hold a NaN or an infinity, give NaN. */
 int anode_gpu_layer_norm_add_fwd(
     int type, uint64_t rows, uint32_t cols, float epsilon,
     const void *x, uint64_t x_stride, const void *residual, uint64_t residual_stride,

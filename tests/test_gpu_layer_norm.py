@@ -290,3 +290,50 @@ def test_more_rows_than_a_launch_has_blocks():
     dx, dg, db = torch.empty_like(x), torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
     ops.LayerNormalizeAddOp.adjoint(y, total, mean, inv, dx, None, res, dg, db)
     check_backward(y, total, mean, inv, None, res, dx, dg, db)
+
+
+# rows, cols, and where in a wider array the rows of dy, total and dx begin
+FORMS = [(5, 64, (0, 0, 0)), (300, 96, (0, 0, 0)), (40, 1024, (0, 0, 0)), (300, 1000, (3, 3, 3)), (7, 77, (1, 1, 1)), (33, 9001, (0, 0, 0)), (5, 100, (0, 1, 2)),
+         (200, 1030, (0, 3, 5)), (3, 20000, (0, 0, 0))]
+
+
+# the rows' spread and the gradients' size: squares of 1e17 pass f32 as the sum of 2e4 columns, and products of a gradient and a row's element stay above 1e-38, the smallest normal number
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("size, small", [(1e8, 1.0), (1e15, 1.0), (1e17, 1.0), (1e13, 1e-9), (1e17, 1e-15), (1e-8, 1.0), (1e-12, 1.0), (1e-15, 1e-6), (1e-17, 1e-12)])
+def test_rows_of_any_size(size, small, dtype):
+    for rows, cols, at in FORMS:
+        def rows_of(seed, first, scale):
+            return (make(rows, cols + 8, torch.float32, seed).double() * scale).to(dtype)[:, first:first + cols]
+        what = "%d rows of %d at %s: " % (rows, cols, at)
+        t, dy, dt = rows_of(1, at[1], size), rows_of(2, at[0], small), rows_of(3, at[2], small / size)
+        gamma, beta = weights(cols, dtype), weights(cols, dtype, 8)
+        y, mean, inv = torch.empty(rows, cols + 8, device="cuda", dtype=dtype)[:, at[2]:at[2] + cols], torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+        ops.LayerNormalizeAddOp.apply(EPS, t, y, gamma, beta, None, None, mean, inv)
+        check_forward(t, None, gamma, beta, y, None, mean, inv, what)
+        var, mean = torch.var_mean(t.double(), -1, correction=0)
+        mean, r = mean.float(), var.rsqrt().float()
+        for weight, extra in ((gamma, None), (None, dt)):
+            dx = torch.empty(rows, cols + 8, device="cuda", dtype=dtype)[:, at[2]:at[2] + cols]
+            dg, db = (torch.empty(cols, device="cuda", dtype=torch.float32 if weight is None else dtype) for _ in range(2))
+            ops.LayerNormalizeAddOp.adjoint(dy, t, mean, r, dx, weight, extra, dg, db)
+            check_backward(dy, t, mean, r, weight, extra, dx, dg, db, what)
+
+
+@pytest.mark.parametrize("cols", [64, 77, 1024, 20000])
+def test_rows_on_either_side_of_the_limits(cols):
+    """Squares that leave f32 as a sum: y = beta; a sum of a row that does: NaN."""
+    sign = torch.where(torch.arange(cols, device="cuda") % 2 == 0, 1.0, -1.0)
+    beta, least = weights(cols, torch.float32, 8), 2.0 ** 64 / cols ** 0.5
+    for first in (0, 1):            # whole and ragged rows
+        x, y = (torch.empty(3, cols + 8, device="cuda")[:, first:first + cols] for _ in range(2))
+        mean, inv = torch.empty(3, device="cuda"), torch.empty(3, device="cuda")
+        x.copy_(sign * (0.99 * least))
+        ops.LayerNormalizeAddOp.apply(EPS, x, y, None, beta, None, None, mean, inv)
+        check_forward(x, None, None, beta, y, None, mean, inv)
+        x.copy_(sign * (1.01 * least))
+        ops.LayerNormalizeAddOp.apply(EPS, x, y, None, beta, None, None, mean, inv)
+        # (the mean of an odd number of columns, 1/cols of their size, takes 1/cols^2 of the squares, 2 in 10^4 of 77)
+        assert (inv == 0).all() and torch.equal(y, beta.expand_as(y))
+        x.fill_(4e38 / cols)
+        ops.LayerNormalizeAddOp.apply(EPS, x, y, None, beta)
+        assert y.isnan().all()

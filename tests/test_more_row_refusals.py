@@ -71,6 +71,7 @@ def probs_grad(**change):
     (embed, dict(vocab=MOST), DIMS), (embed, dict(tokens=MOST), DIMS), (embed, dict(token=None), NULL), (embed, dict(table=None), NULL), (embed, dict(y=None), NULL),
     (embed, dict(token=P + 4), ALIGN), (embed, dict(table=P + 1), ALIGN), (embed, dict(y=P + 1), ALIGN), (embed, dict(y_stride=7), STRIDE), (embed, dict(y=2 * P), STRIDE),
     (embed_grad, dict(type=3), TYPE), (embed_grad, dict(dtable_type=1), TYPE), (embed_grad, dict(token_bytes=1), TYPE), (embed_grad, dict(cols=0), DIMS),
+    (embed_grad, dict(cols=1 << 25, dy_stride=1 << 25, dtable_stride=1 << 25, workspace_bytes=1 << 40), DIMS),
     (embed_grad, dict(vocab=0), DIMS), (embed_grad, dict(tokens=MOST), DIMS), (embed_grad, dict(token=None), NULL), (embed_grad, dict(dy=None), NULL),
     (embed_grad, dict(dtable=None), NULL), (embed_grad, dict(token=P + 2, token_bytes=4), ALIGN), (embed_grad, dict(dtable=P + 2, dtable_type=0), ALIGN),
     (embed_grad, dict(dtable_stride=7), STRIDE), (embed_grad, dict(dtable=2 * P), STRIDE), (embed_grad, dict(workspace=None), WORKSPACE),

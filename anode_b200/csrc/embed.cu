@@ -13,7 +13,7 @@
 //
 // Measured on one B200 against its copy bandwidth of 6539 GB/s: rows of 16384 tokens of [32768,8192] bf16 59 us (0.93), of [.,4095] f16 51 us, 32 tokens 1.6 us.  The gradient
 // of 16384 tokens of [32768,4096] bf16, whose tokens are common ones mostly, 81 us (0.76): zeros 37 (7.2 TB/s, the sort beside them), sums 35, join 8; rows named twice are
-// written twice.  Added to what is there 69 us, where the sort (17 us, a chain of eight waits of a cluster) is seen; to f32 85.  4099 tokens of [50021,1001] f16 into f32 47 us,
+// written twice.  Added to what is there 66 us, where the sort (16 us with caches flushed, a chain of eight waits of a cluster) is seen; to f32 82; 131072 to [32768,1024] 143.  4099 tokens of [50021,1001] f16 into f32 47 us,
 // added 23.5.  The zeros and the sums are bound by memory, small calls by the chain token -> place -> row -> sum.
 #include "bn_host.h"
 #include "rows.cuh"
@@ -172,7 +172,8 @@ template <typename T, bool SHIFT> __global__ void __launch_bounds__(128) embed_k
 
 // ---- the gradient ---------------------------------------------------------------------------------------------------------------
 
-constexpr uint32_t kCluster = 8, kSortThreads = 512, kSortWarps = kSortThreads / 32;
+constexpr uint32_t kCluster = 16, kFewer = 8;         // blocks that sort
+constexpr uint32_t kSortThreads = 512, kSortWarps = kSortThreads / 32;
 constexpr uint32_t kMostBits = 9;                    // of a token to a pass of the sort
 constexpr uint32_t kZeros = 65536;                   // bytes of the table that a block sets to zero
 constexpr uint32_t kCounted = 8192;                  // tokens that are sorted by counting
@@ -197,11 +198,11 @@ struct SortArgs {
 // The first cluster: passes of a radix sort, each over `bits` of the tokens.  A warp has a stretch of the places.  It counts its digits (lanes with the same
 // one find each other, and the first adds for all, so that the order stays); the counts of all warps and blocks before it and of smaller digits
 // are where its own begin.
-__device__ __forceinline__ void sort_tokens(const SortArgs &a, uint32_t (*count)[1u << kMostBits], uint32_t *totals, uint32_t *base)
+template <uint32_t CLUSTER> __device__ __forceinline__ void sort_tokens(const SortArgs &a, uint32_t (*count)[1u << kMostBits], uint32_t *totals, uint32_t *base)
 {
   constexpr uint32_t STEPS = 4;
   const uint32_t rank = cluster_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bins = 1u << a.bits;
-  const uint32_t stretch = (a.n + kCluster * kSortWarps * 32 - 1) / (kCluster * kSortWarps * 32) * 32;
+  const uint32_t stretch = (a.n + CLUSTER * kSortWarps * 32 - 1) / (CLUSTER * kSortWarps * 32) * 32;
   const uint64_t lo = (uint64_t)(rank * kSortWarps + warp) * stretch, hi = min((uint64_t)a.n, lo + stretch);
   uint32_t *mine = count[warp];
   for (uint32_t pass = 0; pass < a.passes; ++pass) {
@@ -249,11 +250,11 @@ __device__ __forceinline__ void sort_tokens(const SortArgs &a, uint32_t (*count)
     cluster_sync();
     uint32_t before = 0, all = 0;
     if (t < bins) {
-      uint32_t c[kCluster];
+      uint32_t c[CLUSTER];
 #pragma unroll
-      for (uint32_t r = 0; r < kCluster; ++r) c[r] = peer_load(totals + t, r);
+      for (uint32_t r = 0; r < CLUSTER; ++r) c[r] = peer_load(totals + t, r);
 #pragma unroll
-      for (uint32_t r = 0; r < kCluster; ++r) { before += r < rank ? c[r] : 0; all += c[r]; }
+      for (uint32_t r = 0; r < CLUSTER; ++r) { before += r < rank ? c[r] : 0; all += c[r]; }
     }
     uint32_t sum = all;
 #pragma unroll
@@ -306,14 +307,14 @@ template <typename W> __device__ __forceinline__ void zero_part(const SortArgs &
   }
 }
 
-template <typename W> __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs a)
+template <typename W, uint32_t CLUSTER> __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const SortArgs a)
 {
   __shared__ uint32_t count[kSortWarps][1u << kMostBits], totals[1u << kMostBits], base[kSortThreads + kSortWarps];
   static_assert(kSortThreads >= 1u << kMostBits, "a thread per digit");
   pdl_wait();
   pdl_trigger();
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.runs = 0;
-  if (blockIdx.x < a.sorting) sort_tokens(a, count, totals, base);
+  if (blockIdx.x < a.sorting) sort_tokens<CLUSTER>(a, count, totals, base);
   else zero_part<W>(a);
 }
 
@@ -590,6 +591,14 @@ struct Layout {
   }
 };
 
+template <typename W> int launch_sort(dim3 grid, cudaStream_t stream, const SortArgs &s)
+{
+  static WideClusters allowed;
+  if (s.sorting == kFewer) return launch_in_clusters(embed_sort_kernel<W, kFewer>, grid, kFewer, kSortThreads, 0, stream, s);
+  if (!allowed.of((const void *)embed_sort_kernel<W, kCluster>)) return ANODE_E_LAUNCH;
+  return launch_in_clusters(embed_sort_kernel<W, kCluster>, grid, kCluster, kSortThreads, 0, stream, s);
+}
+
 template <typename T, typename O> int launch_sums(SumArgs a, bool shift, int accumulate, cudaStream_t stream)
 {
   constexpr uint32_t V = Vec<T>::V;
@@ -674,7 +683,10 @@ extern "C" int anode_gpu_embed_tokens_bwd(
   s.passes = (bits + kMostBits - 1) / kMostBits;
   s.bits = (bits + s.passes - 1) / s.passes;
   const bool counted = tokens <= kCounted;
-  s.sorting = !tokens ? 0 : counted ? (uint32_t)((tokens + 31) / 32) : kCluster;
+  // sixteen blocks to the sort, which sums wait for (16384 tokens added to [32768,4096] bf16 66 us, 69 with eight; 131072 to [32768,1024] 143 and 179), but eight where the zeros take
+  // longer, which clusters of sixteen would write more slowly (16384 tokens of [32768,4096] 81 us, 84 with sixteen; of [32768,1024], 4 KB to a token, 40 and 38)
+  const bool hidden = !accumulate && (uint64_t)vocab * cols * oe > 8192 * tokens;
+  s.sorting = !tokens ? 0 : counted ? (uint32_t)((tokens + 31) / 32) : hidden ? kFewer : kCluster;
   uint64_t blocks = 0;
   if (!accumulate) {
     s.zero_rows = vocab; s.stride = dtable_stride * oe; s.row_bytes = (uint64_t)cols * oe;
@@ -682,14 +694,13 @@ extern "C" int anode_gpu_embed_tokens_bwd(
     const uint64_t cuts = (s.row_bytes + kZeros - 1) / kZeros;
     s.rows = cuts > 1 ? 1 : (uint32_t)(kZeros / s.row_bytes);
     blocks = (s.zero_rows + s.rows - 1) / s.rows * cuts;
-    if (!counted) blocks = (blocks + kCluster - 1) / kCluster * kCluster;
+    if (!counted) blocks = (blocks + s.sorting - 1) / s.sorting * s.sorting;
     if (cuts >> 30 || blocks >> 30) return ANODE_E_DIMS;
     s.cuts = (uint32_t)cuts;
   }
   const dim3 grid(s.sorting + (uint32_t)blocks);
   TRY((counted ? (oe == 4 ? launch(embed_count_kernel<uint32_t>, grid, kSortThreads, 0, stream, s) : launch(embed_count_kernel<uint16_t>, grid, kSortThreads, 0, stream, s))
-               : (oe == 4 ? launch_in_clusters(embed_sort_kernel<uint32_t>, grid, kCluster, kSortThreads, 0, stream, s)
-                          : launch_in_clusters(embed_sort_kernel<uint16_t>, grid, kCluster, kSortThreads, 0, stream, s))));
+               : (oe == 4 ? launch_sort<uint32_t>(grid, stream, s) : launch_sort<uint16_t>(grid, stream, s))));
   if (!tokens) return ANODE_OK;
   const SumArgs a = {(uint32_t)tokens, vocab, cols, scale, s.key[0], s.place[0], dy, dy_stride, dtable, dtable_stride, (uint32_t)l.piece, (uint32_t)l.pieces,
                      words + l.runs / 4, reinterpret_cast<uint4 *>(static_cast<char *>(workspace) + l.run), reinterpret_cast<float *>(static_cast<char *>(workspace) + l.part), (uint32_t)l.part_cols, 0};

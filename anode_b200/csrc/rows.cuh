@@ -287,6 +287,23 @@ class SharedMemory {
   std::atomic<uint64_t> done_{0};
 };
 
+// A kernel's leave to be launched in clusters of more than 8 blocks, asked for once per device
+class WideClusters {
+ public:
+  bool of(const void *kernel)
+  {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (done_.load(std::memory_order_relaxed) >> dev & 1) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) { (void)cudaGetLastError(); return false; }
+    done_.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return true;
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
+
 // A launch that may overlap the tail of the kernel before it on the stream: every kernel here waits for that one's results
 // before it touches memory.
 template <typename... P, typename... A>
@@ -301,7 +318,7 @@ inline int launch(void (*kernel)(P...), dim3 grid, uint32_t threads, size_t shar
   if (cudaLaunchKernelEx(&cfg, kernel, P(args)...) != cudaSuccess) { (void)cudaGetLastError(); return ANODE_E_LAUNCH; }
   return ANODE_OK;
 }
-// The same of a grid of clusters of up to 8 blocks
+// The same of a grid of clusters, of up to 8 blocks or as many as the kernel has leave for
 template <typename... P, typename... A>
 inline int launch_in_clusters(void (*kernel)(P...), dim3 grid, uint32_t cluster, uint32_t threads, size_t shared, cudaStream_t stream, A... args)
 {

@@ -78,7 +78,8 @@ def test_gradient(cols, dtype):
             check_grad(tokens, dy, more, 2.5, before)
 
 
-@pytest.mark.parametrize("n, vocab, cols", [(1, 300000, 16), (5000, 300000, 24), (131072, 32768, 64), (131073, 100, 40), (300001, 70001, 8), (20000, 1 << 20, 20), (65536, 65536, 128)])
+@pytest.mark.parametrize("n, vocab, cols", [(1, 300000, 16), (5000, 300000, 24), (131072, 32768, 64), (131073, 100, 40), (300001, 70001, 8), (20000, 1 << 20, 20), (65536, 65536, 128),
+                                            (8193, 262147, 321), (9001, 1 << 20, 72)])
 @pytest.mark.parametrize("spread", ["zipf", "even", "one"])
 def test_many_tokens_and_large_tables(n, vocab, cols, spread):
     """Whole numbers whose sums are exact, so that no row may be missing or come twice."""
@@ -106,6 +107,22 @@ def test_patterns_of_tokens(pattern, dtype):
     dy, out = make(n, cols, dtype, 1), torch.full((vocab, cols), 7.0, device="cuda", dtype=dtype)
     ops.EmbedTokensOp.adjoint(tokens, dy, out)
     check_grad(tokens, dy, out, 1.0, None, pattern + " ")
+
+
+@pytest.mark.parametrize("pattern", ["runs", "same", "falling", "pairs", "none", "one among none"])
+@pytest.mark.parametrize("n", [8193, 16385, 40001])
+def test_patterns_of_many_tokens(pattern, n):
+    """The same beyond the tokens that are sorted by counting, with whole numbers: both clusters of the sort give the sums exactly, and the same bits again."""
+    vocab, cols = 70001, 136
+    i = torch.arange(n, device="cuda")
+    tokens = {"runs": i // 97, "same": 0 * i + 511, "falling": n - 1 - i, "pairs": (i // 2) % vocab, "none": 0 * i - 1, "one among none": torch.where(i == 1500, 17, -1)}[pattern]
+    dy = torch.randint(-2, 3, (n, cols), generator=torch.Generator(device="cuda").manual_seed(n), device="cuda").to(torch.float16)
+    inside = tokens >= 0
+    want = torch.zeros(vocab, cols, device="cuda").index_add_(0, tokens[inside], dy[inside].float())
+    whole, added = torch.full((vocab, cols), 7.0, device="cuda"), torch.zeros(vocab, cols, device="cuda")
+    ops.EmbedTokensOp.adjoint(tokens, dy, whole)
+    ops.EmbedTokensOp.adjoint(tokens, dy, added, 1.0, ops.WriteCap.Accumulate)
+    assert torch.equal(whole, want) and torch.equal(added, want)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)

@@ -581,6 +581,10 @@ extern "C" int anode_gpu_token_log_probs_fwd(
   if ((logprob && !token) || (top && !top_logprob && !top_token) || !(logprob || entropy || stats || top)) return ANODE_E_NULL;
   if ((logprob && !aligned_to(token, (size_t)token_bytes)) || !aligned_to(logprob, 4) || !aligned_to(entropy, 4) || !aligned_to(stats, 8) ||
       (top && (!aligned_to(top_logprob, 4) || (top_token && !aligned_to(top_token, (size_t)top_token_bytes))))) return ANODE_E_ALIGN;
+  // outputs apart from one another
+  const struct { const void *p; uint64_t bytes; } outs[] = {{logprob, 4 * rows}, {entropy, 4 * rows}, {stats, 8 * rows}, {top ? top_logprob : nullptr, 4 * top * rows},
+                                                            {top ? top_token : nullptr, (uint64_t)top_token_bytes * top * rows}};
+  for (int i = 0; i < 5; ++i) for (int j = 0; j < i; ++j) if (overlap(outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes)) return ANODE_E_STRIDE;
   const ProbsArgs a = {rows, vocab, scale, logits, logits_stride, token, token_bytes, logprob, entropy, reinterpret_cast<float2 *>(stats), top,
                        top ? top_logprob : nullptr, top ? top_token : nullptr, top_token_bytes};
   const uint32_t v = (uint32_t)(16 / type_bytes(type)), slots = vocab / v;

@@ -255,6 +255,9 @@ inline bool apart(const void *out, uint64_t out_stride, const void *in, uint64_t
   return out != in || out_stride == in_stride || rows <= 1;
 }
 
+// Whether n bytes from p on and m bytes from q on have one in common; what is not there has none
+inline bool overlap(const void *p, uint64_t n, const void *q, uint64_t m) { return p && q && (uintptr_t)p < (uintptr_t)q + m && (uintptr_t)q < (uintptr_t)p + n; }
+
 // Whether an array's rows all begin at the same place of a slot of `v` elements as those of the first one
 inline bool in_step(const void *p, size_t bytes, uint64_t stride, uint32_t v, const void *p0, size_t bytes0, uint64_t stride0, uint64_t rows)
 {

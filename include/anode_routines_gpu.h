@@ -665,7 +665,8 @@ int anode_gpu_embed_tokens_bwd(
  *   top_token, top_logprob [rows, top]: the `top` <= min(vocab, 128) likeliest tokens, of top_token_bytes (4 or 8) bytes, and z - L of
  *   them, the largest logit first, of equal ones the lowest index (a NaN counts as larger than all; either may be NULL)
  * A logit of -infinity has probability 0.  A row of nothing else has log probabilities of -infinity, entropy 0 and stats (-infinity, 0); one
- * that holds a NaN or +infinity has NaN for log probabilities and entropy.  At least one output is asked for. */
+ * that holds a NaN or +infinity has NaN for log probabilities and entropy.  At least one output is asked for, and outputs that share memory are refused
+ * (ANODE_E_STRIDE). */
 int anode_gpu_token_log_probs_fwd(
     int type, uint64_t rows, uint32_t vocab, float scale,
     const void *logits, uint64_t logits_stride, const void *token, int token_bytes,

@@ -637,7 +637,7 @@ extern "C" int anode_gpu_embed_tokens_fwd(
   TRY(check_tokens(token, token_bytes));
   TRY(check_rows(table, e, vocab, cols, table_stride, false));
   TRY(check_rows(y, e, tokens, cols, y_stride, true));
-  if (y == table) return ANODE_E_STRIDE;
+  if (rows_meet(y, y_stride * e, tokens, cols * e, table, table_stride * e, vocab, cols * e)) return ANODE_E_STRIDE;
   const EmbedArgs a = {tokens, vocab, cols, scale, token, token_bytes, table, table_stride, y, y_stride};
   const bool shift = !whole(table, e, table_stride, vocab, cols) || !whole(y, e, y_stride, tokens, cols);
   return by_type(type, [&](auto t) {
@@ -671,7 +671,7 @@ extern "C" int anode_gpu_embed_tokens_bwd(
   if (tokens) {
     TRY(check_tokens(token, token_bytes));
     TRY(check_rows(dy, e, tokens, cols, dy_stride, false));
-    if (dy == dtable) return ANODE_E_STRIDE;
+    if (rows_meet(dtable, dtable_stride * oe, vocab, cols * oe, dy, dy_stride * e, tokens, cols * e)) return ANODE_E_STRIDE;
     if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < anode_gpu_embed_tokens_bwd_workspace_bytes(tokens, vocab, cols)) return ANODE_E_WORKSPACE;
   }
   const Layout l(tokens, cols);

@@ -258,6 +258,26 @@ inline bool apart(const void *out, uint64_t out_stride, const void *in, uint64_t
 // Whether n bytes from p on and m bytes from q on have one in common; what is not there has none
 inline bool overlap(const void *p, uint64_t n, const void *q, uint64_t m) { return p && q && (uintptr_t)p < (uintptr_t)q + m && (uintptr_t)q < (uintptr_t)p + n; }
 
+// Whether two arrays of rows, n of p_len bytes p_step apart and m of q_len bytes q_step apart, have a byte in common
+inline bool rows_meet(const void *p, uint64_t p_step, uint64_t n, uint64_t p_len, const void *q, uint64_t q_step, uint64_t m, uint64_t q_len)
+{
+  if (!n || !m || !overlap(p, (n - 1) * p_step + p_len, q, (m - 1) * q_step + q_len)) return false;
+  if (n > m) return rows_meet(q, q_step, m, q_len, p, p_step, n, p_len);
+  const uint64_t a = (uintptr_t)p, b = (uintptr_t)q;
+  // of q's rows the last that begins before p's row ends reaches farthest
+  auto meets = [&](uint64_t i) {
+    const uint64_t first = a + i * p_step, end = first + p_len;
+    if (end <= b) return false;
+    const uint64_t j = q_step ? (end - 1 - b) / q_step : 0;
+    return b + (j < m ? j : m - 1) * q_step + q_len > first;
+  };
+  // at one distance p's rows all lie at the same place among q's, but for those before q's first row or behind its last: the first that ends behind q's first byte
+  // tells (overlapping rows, as those of a broadcast, are looked at one by one, and so are those at two distances)
+  if (p_step == q_step && p_step >= p_len && p_step >= q_len) return meets(a + p_len > b ? 0 : (b - a - p_len) / p_step + 1);
+  for (uint64_t i = 0; i < n; ++i) if (meets(i)) return true;
+  return false;
+}
+
 // Whether an array's rows all begin at the same place of a slot of `v` elements as those of the first one
 inline bool in_step(const void *p, size_t bytes, uint64_t stride, uint32_t v, const void *p0, size_t bytes0, uint64_t stride0, uint64_t rows)
 {

@@ -702,7 +702,7 @@ def layer_norm_workspace_bytes(rows, cols):
 
 class EmbedTokensOp:
     """Rows of a table by tokens: y[i] = scale*table[tokens[i]].  tokens: int32 or int64, packed, of any sizes [*]; table: [vocab, cols], y: [*, cols] of its
-    type, rows at one distance each.  A token outside of [0, vocab) stands for none: its row is zeros, and it has no gradient."""
+    type, rows at one distance each, apart from the table's.  A token outside of [0, vocab) stands for none: its row is zeros, and it has no gradient."""
     @staticmethod
     def apply(tokens, table, y, scale=1.0, cfg=None, stream=None):
         _hint(cfg)

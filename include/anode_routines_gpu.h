@@ -640,7 +640,8 @@ int anode_gpu_layer_norm_add_bwd(
     void *dx, uint64_t dx_stride, void *dgamma, void *dbeta, void *workspace, size_t workspace_bytes,
     const struct KernelConfig *cfg, struct CUstream_st *stream);
 
-/* Rows of a table [vocab, cols]:  y[i] = scale * table[token[i]], zeros where token[i] is none.  y may not meet the table. */
+/* Rows of a table [vocab, cols]:  y[i] = scale * table[token[i]], zeros where token[i] is none.  y may not meet the table (ANODE_E_STRIDE; columns beside
+ * the table's in wider rows are apart from it). */
 int anode_gpu_embed_tokens_fwd(
     int type, uint64_t tokens, uint32_t vocab, uint32_t cols, float scale,
     const void *token, int token_bytes, const void *table, uint64_t table_stride, void *y, uint64_t y_stride,
@@ -649,7 +650,7 @@ int anode_gpu_embed_tokens_fwd(
 /* Its adjoint:  dtable[v] = scale * (sum of dy[i] over token[i] = v), every row of it, zeros where no token names it; with accumulate != 0
  * that is added to what dtable holds, whose other rows are neither read nor written.  dtable's type is dy's or f32.  A row's terms are added in f32,
  * in an order that follows from the tokens alone: the same call gives the same bits.  The workspace
- * (anode_gpu_embed_tokens_bwd_workspace_bytes, 16-byte aligned) is needed wherever there are tokens. */
+ * (anode_gpu_embed_tokens_bwd_workspace_bytes, 16-byte aligned) is needed wherever there are tokens.  dtable may not meet dy (ANODE_E_STRIDE). */
 size_t anode_gpu_embed_tokens_bwd_workspace_bytes(uint64_t tokens, uint32_t vocab, uint32_t cols);
 int anode_gpu_embed_tokens_bwd(
     int type, uint64_t tokens, uint32_t vocab, uint32_t cols, float scale,

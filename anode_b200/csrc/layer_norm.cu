@@ -650,11 +650,11 @@ extern "C" int anode_gpu_layer_norm_add_fwd(
   if (total) {
     if (!residual) return ANODE_E_NULL;
     TRY(check_rows(total, e, rows, cols, total_stride, true));
-    if (total == y || !apart(total, total_stride, x, x_stride, rows) || !apart(total, total_stride, residual, residual_stride, rows)) return ANODE_E_STRIDE;
+    if (rows_meet(total, total_stride * e, rows, cols * e, y, y_stride * e, rows, cols * e) || !apart(total, total_stride, x, x_stride, rows) || !apart(total, total_stride, residual, residual_stride, rows)) return ANODE_E_STRIDE;
   }
   if (!apart(y, y_stride, x, x_stride, rows) || !apart(y, y_stride, residual, residual_stride, rows)) return ANODE_E_STRIDE;
   if (!aligned_to(mean, 4) || !aligned_to(inv_std, 4)) return ANODE_E_ALIGN;
-  if (mean && mean == inv_std) return ANODE_E_STRIDE;
+  if (overlap(mean, 4 * rows, inv_std, 4 * rows)) return ANODE_E_STRIDE;
   const LayerArgs a = {rows, cols, epsilon, 1.0f / (float)cols, x, residual, x_stride, residual_stride, {gamma, weight_type}, {beta, weight_type},
                        y, total, y_stride, total_stride, mean, inv_std};
   Held h = {};
@@ -684,7 +684,9 @@ extern "C" int anode_gpu_layer_norm_add_bwd(
   if (gamma && !aligned_to(gamma, type_bytes(weight_type))) return ANODE_E_ALIGN;
   if (sums) {
     for (void *w : {dgamma, dbeta}) if (w && !aligned_to(w, type_bytes(weight_type))) return ANODE_E_ALIGN;
-    if (dgamma == dbeta || (gamma && dbeta == gamma)) return ANODE_E_STRIDE;
+    // the gradients apart from each other and from gamma, in whose very place dgamma may be
+    const uint64_t bytes = (uint64_t)cols * type_bytes(weight_type);
+    if (overlap(dgamma, bytes, dbeta, bytes) || overlap(dbeta, bytes, gamma, bytes) || (dgamma != gamma && overlap(dgamma, bytes, gamma, bytes))) return ANODE_E_STRIDE;
     if (rows == 0) {
       for (void *w : {dgamma, dbeta})
         if (w && cudaMemsetAsync(w, 0, type_bytes(weight_type) * cols, stream) != cudaSuccess) { (void)cudaGetLastError(); return ANODE_E_LAUNCH; }

@@ -5,7 +5,7 @@ import itertools
 import pytest
 import torch
 
-from tests.test_more_row_refusals import P, STRIDE, embed, embed_grad, probs
+from tests.test_more_row_refusals import P, STRIDE, embed, embed_grad, layer, layer_grad, probs
 
 LAUNCH = -4          # what a call that is taken answers on a machine without a device
 
@@ -74,3 +74,37 @@ def test_many_rows_side_by_side_are_taken_at_once():
     n = 1 << 30
     assert embed(tokens=n, vocab=n, y=P, y_stride=16, table=P + 16, table_stride=16) == LAUNCH
     assert embed(tokens=n, vocab=n, y=P, y_stride=16, table=P + 14, table_stride=16) == STRIDE
+
+
+def test_layer_norm_y_and_the_sum():
+    """4 rows of 8 columns of two bytes each, at distances of their own."""
+    refused = 0
+    for at, s, t in itertools.product(range(-130, 132, 2), (16, 32, 48), (16, 32)):
+        meet = meets(0, s, 4, at, t, 4, 16)
+        refused += meet
+        if meet or not torch.cuda.is_available():
+            assert layer(y=20 * P, y_stride=s // 2, total=20 * P + at, total_stride=t // 2) == (STRIDE if meet else LAUNCH), (at, s, t)
+    assert refused > 100
+
+
+def test_layer_norm_numbers_of_each_row():
+    for at in range(-20, 24, 4):         # 4 rows of four bytes
+        if abs(at) < 16 or not torch.cuda.is_available():
+            assert layer(mean=20 * P, inv_std=20 * P + at) == (STRIDE if abs(at) < 16 else LAUNCH), at
+
+
+def test_layer_norm_gradients_of_the_weights():
+    """8 columns of four bytes: the two gradients apart, dbeta apart from gamma, dgamma in gamma's very place or apart from it."""
+    for at in range(-40, 44, 4):
+        meet = abs(at) < 32
+        if meet or not torch.cuda.is_available():
+            want = STRIDE if meet else LAUNCH
+            assert layer_grad(dgamma=20 * P, dbeta=20 * P + at) == want, at
+            assert layer_grad(gamma=20 * P, dbeta=20 * P + at) == want and layer_grad(gamma=20 * P, dgamma=None, dbeta=20 * P + at) == want, at
+            if at:
+                assert layer_grad(gamma=20 * P, dgamma=20 * P + at) == want and layer_grad(gamma=20 * P, dgamma=20 * P + at, dbeta=None) == want, at
+
+
+@no_device
+def test_layer_norm_gradient_in_the_weight_s_place():
+    assert layer_grad(gamma=20 * P, dgamma=20 * P) == LAUNCH and layer_grad(gamma=None, dgamma=20 * P, dbeta=20 * P + 32) == LAUNCH

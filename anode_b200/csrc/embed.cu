@@ -20,6 +20,7 @@
 
 namespace anode_b200 {
 namespace rows {
+namespace embed {
 
 constexpr uint32_t kThreads = 256;
 
@@ -619,10 +620,12 @@ template <typename T, typename O> int launch_sums(SumArgs a, bool shift, int acc
   return launch(embed_join_kernel<O>, dim3(wide, blocks < most ? blocks : most), kThreads, 0, stream, a, accumulate);
 }
 
+}  // namespace embed
 }  // namespace rows
 }  // namespace anode_b200
 
 using namespace anode_b200::rows;
+using namespace anode_b200::rows::embed;
 
 extern "C" int anode_gpu_embed_tokens_fwd(
     int type, uint64_t tokens, uint32_t vocab, uint32_t cols, float scale,

@@ -21,6 +21,7 @@
 
 namespace anode_b200 {
 namespace rows {
+namespace layer_norm {
 
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMostParts = 148;       // of the sums over rows
@@ -626,10 +627,12 @@ template <typename T, int CH> int launch_grad(const LayerGradArgs &a, const Held
   else return g == 1 ? launch_grad<T, CH, 1>(a, h, shift, shared, stream) : launch_grad<T, CH, 2>(a, h, shift, shared, stream);
 }
 
+}  // namespace layer_norm
 }  // namespace rows
 }  // namespace anode_b200
 
 using namespace anode_b200::rows;
+using namespace anode_b200::rows::layer_norm;
 
 extern "C" int anode_gpu_layer_norm_add_fwd(
     int type, uint64_t rows, uint32_t cols, float epsilon,

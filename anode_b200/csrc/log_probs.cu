@@ -13,6 +13,7 @@
 
 namespace anode_b200 {
 namespace rows {
+namespace log_probs {
 
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMostThreads = 512, kMostTop = 128;
@@ -553,10 +554,12 @@ void split(uint64_t rows, uint32_t slots, uint32_t top, uint32_t &cluster, uint3
   if (each < threads) threads = each < 32 ? 32 : each;
 }
 
+}  // namespace log_probs
 }  // namespace rows
 }  // namespace anode_b200
 
 using namespace anode_b200::rows;
+using namespace anode_b200::rows::log_probs;
 
 static int check_logits(int type, uint64_t rows, uint32_t vocab, float scale)
 {

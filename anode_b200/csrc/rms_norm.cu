@@ -24,6 +24,7 @@
 
 namespace anode_b200 {
 namespace rows {
+namespace rms_norm {
 
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMostParts = 148;       // of dgamma's sums
@@ -734,10 +735,12 @@ int norm_forward(const NormArgs &a, int type, int gamma_type, bool quant, cudaSt
   });
 }
 
+}  // namespace rms_norm
 }  // namespace rows
 }  // namespace anode_b200
 
 using namespace anode_b200::rows;
+using namespace anode_b200::rows::rms_norm;
 
 extern "C" int anode_gpu_rms_norm_add_fwd(
     int type, uint64_t rows, uint32_t cols, float epsilon,

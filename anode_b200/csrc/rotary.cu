@@ -22,6 +22,7 @@
 
 namespace anode_b200 {
 namespace rows {
+namespace rotary_positions {
 
 constexpr uint32_t kThreads = 128, kMostDim = 1024;
 constexpr uint32_t kWarps = kThreads / 32;
@@ -873,10 +874,12 @@ int rotary(RotaryArgs a, const RotaryCall &c, cudaStream_t stream)
                 c.gamma_type);
 }
 
+}  // namespace rotary_positions
 }  // namespace rows
 }  // namespace anode_b200
 
 using namespace anode_b200::rows;
+using namespace anode_b200::rows::rotary_positions;
 
 extern "C" int anode_gpu_rotary_positions_fwd(
     int type, uint32_t batch, uint32_t seq, uint32_t dim, uint32_t rot, int interleaved, float amplitude,

@@ -1,4 +1,5 @@
 // What the row-wise operators (rms_norm.cu, layer_norm.cu, rotary.cu, embed.cu, log_probs.cu) share: element types, checks of strides, the join of column sums.
+// Each has a namespace of its own in this one: their plans and helpers are alike and have the same names, but not the same members and values.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -572,12 +572,36 @@ inline uint32_t power_up_to(uint64_t n, uint32_t most)
   return v;
 }
 
-// Places of a piece; a run of more is long.  As many as leave the device 2^18 threads, of rows of 16-bit columns that begin anywhere, but 10 at least, where what each piece does
-// beside its rows counts ([4099 tokens, 1001 columns] added to f32: 23.5 us with 10, 26 with 8, 28 with 16; [16384,4096] bf16: 81 us with 32, 86 with 16, 102 with 8)
+// How the columns of a piece are shared out: slots of 16 bytes, single columns (SHIFT), threads of a piece, pieces of a block, and blocks side by side
+struct Shares {
+  uint32_t slots, singles, lanes, per_block, wide;
+  Shares(uint32_t cols, uint32_t v, bool shift) : slots(cols / v)
+  {
+    // (rows that begin anywhere: two aligned pieces around each slot are to be inside of the row)
+    if (shift) slots = slots > 2 ? slots - 2 : 0;
+    singles = cols - slots * v;
+    const uint32_t all = slots + singles;
+    lanes = all > kThreads ? kThreads : all > 32 ? (all + 31) / 32 * 32 : power_up_to(all, 32);
+    if (lanes < kLeastLanes) lanes = kLeastLanes;
+    per_block = kThreads / lanes;
+    wide = (all + lanes - 1) / lanes;
+  }
+};
+
+// Places of a piece; a run of more is long.  Short pieces are short chains of rows, long ones have fewer parts to join and fewer borders to look at.  As many as leave
+// the device 2^18 threads of rows of 16-bit columns, and of those where that is few: as many as let all blocks run at once (with 512 threads to a multiprocessor, for which the
+// adding form has registers), if 16 are enough for that, and 8 at least.  Added to what is there, us, tokens of a frequency-ordered vocabulary (8 / 10 / 16 places):
+// [2048,2048] bf16 12.3 / 12.9 / 13.6, [512,1024] 8.2 / 8.9 / 9.2, [1000,768] f32 9.1 / 9.9 / 10.8, [3001,333] f16 18.2 / 20.7 / 26.2, whose blocks all run at once with 8; [4099,1001] f16
+// into f32 26.2 / 23.3 / 27.7 (at once from 10 on), [8192,1024] bf16 28.5 / 28.9 / 25.9 (from 14 on); [16384,4096] 102 with 8, 86 with 16, 81 with 32.
+// The limit of 16: at once from 32 and 28 on, [5000,3001] into f32 65.8 (54.3 with 8) and [32768,300] bf16, assigned, 52.6 (49.6).
+// (from sizes alone, since the workspace's size goes by it)
 inline uint32_t piece_of(uint64_t tokens, uint32_t cols)
 {
+  const Shares s(cols, 8, cols % 8 != 0);
   const uint64_t threads = tokens * ((uint64_t)cols / 8 + 16), each = (threads + (1u << 18) - 1) >> 18;
-  return (uint32_t)(each < 10 ? 10 : each < kMostPiece ? each : kMostPiece);
+  const uint64_t blocks = 148 * (2 * kThreads / (s.per_block * s.lanes)) / s.wide, at_once = (blocks ? blocks : 1) * s.per_block, fits = (tokens + at_once - 1) / at_once;
+  const uint64_t least = fits <= 16 && fits > 8 ? fits : 8, piece = each < least ? least : each;
+  return (uint32_t)(piece < kMostPiece ? piece : kMostPiece);
 }
 
 // Where the workspace's arrays begin, in bytes
@@ -603,17 +627,11 @@ template <typename W> int launch_sort(dim3 grid, cudaStream_t stream, const Sort
 template <typename T, typename O> int launch_sums(SumArgs a, bool shift, int accumulate, cudaStream_t stream)
 {
   constexpr uint32_t V = Vec<T>::V;
-  a.slots = a.cols / V;
-  // (rows that begin anywhere: two aligned pieces around each slot are to be inside of the row)
-  if (shift) a.slots = a.slots > 2 ? a.slots - 2 : 0;
-  a.singles = a.cols - a.slots * V;
-  const uint32_t all = a.slots + a.singles;
-  a.lanes = all > kThreads ? kThreads : all > 32 ? (all + 31) / 32 * 32 : power_up_to(all, 32);
-  if (a.lanes < kLeastLanes) a.lanes = kLeastLanes;
-  const uint32_t per_block = kThreads / a.lanes;
-  const dim3 grid((a.pieces + per_block - 1) / per_block, (all + a.lanes - 1) / a.lanes);
+  const Shares part(a.cols, V, shift);
+  a.slots = part.slots; a.singles = part.singles; a.lanes = part.lanes;
+  const dim3 grid((a.pieces + part.per_block - 1) / part.per_block, part.wide);
   TRY(launch(accumulate ? (shift ? embed_sums_kernel<T, O, true, true> : embed_sums_kernel<T, O, false, true>)
-                        : (shift ? embed_sums_kernel<T, O, true, false> : embed_sums_kernel<T, O, false, false>), grid, per_block * a.lanes, 0, stream, a));
+                        : (shift ? embed_sums_kernel<T, O, true, false> : embed_sums_kernel<T, O, false, false>), grid, part.per_block * a.lanes, 0, stream, a));
   if (a.n <= a.piece) return ANODE_OK;
   // a run to a block, of the tokens of a training batch: some 50 of 16384 come more than 32 times
   const uint32_t wide = (uint32_t)(((uint64_t)a.cols + 63) / 64), most = a.n / (a.piece + 1), blocks = (8 * sm_count() + wide - 1) / wide;

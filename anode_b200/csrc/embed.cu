@@ -11,7 +11,8 @@
 //      of places ends.  A run of no more places than a piece has belongs to the piece where it begins; of a longer one each piece leaves its part in the workspace;
 //   3. the parts of each long run are joined, in order.
 //
-// Measured on one B200 against its copy bandwidth of 6539 GB/s: rows of 16384 tokens of [32768,8192] bf16 59 us (0.93), of [.,4095] f16 51 us, 32 tokens 1.6 us.  The gradient
+// Measured on one B200 against its copy bandwidth of 6539 GB/s: rows of 16384 tokens of [32768,8192] bf16 59 us (0.93), of [.,4096] f16 30, of [.,4095] 51 (two loads
+// to a slot, and a row's first and last elements one by one), 32 tokens 1.6 us.  The gradient
 // of 16384 tokens of [32768,4096] bf16, whose tokens are common ones mostly, 81 us (0.76): zeros 37 (7.2 TB/s, the sort beside them), sums 35, join 8; rows named twice are
 // written twice.  Added to what is there 66 us, where the sort (16 us with caches flushed, a chain of eight waits of a cluster) is seen; to f32 82; 131072 to [32768,1024] 143.  4099 tokens of [50021,1001] f16 into f32 47 us,
 // added 23.5.  The zeros and the sums are bound by memory, small calls by the chain token -> place -> row -> sum.
@@ -705,7 +706,8 @@ extern "C" int anode_gpu_embed_tokens_bwd(
   s.bits = (bits + s.passes - 1) / s.passes;
   const bool counted = tokens <= kCounted;
   // sixteen blocks to the sort, which sums wait for (16384 tokens added to [32768,4096] bf16 66 us, 69 with eight; 131072 to [32768,1024] 143 and 179), but eight where the zeros take
-  // longer, which clusters of sixteen would write more slowly (16384 tokens of [32768,4096] 81 us, 84 with sixteen; of [32768,1024], 4 KB to a token, 40 and 38)
+  // longer, which clusters of sixteen would write more slowly (16384 tokens of [32768,4096] 81 us, 84 with sixteen; of [32768,1024], 4 KB to a token, 40 and 38).  Of 55 sizes, 8200 to
+  // 131072 tokens of bf16 tables of 4096 to 262144 rows of 256 to 8192 columns, the line of 8 KB to a token was wrong by more than 1 % at one (40000 of [262144,1000], 13 KB: 118, 110 with sixteen)
   const bool hidden = !accumulate && (uint64_t)vocab * cols * oe > 8192 * tokens;
   s.sorting = !tokens ? 0 : counted ? (uint32_t)((tokens + 31) / 32) : hidden ? kFewer : kCluster;
   uint64_t blocks = 0;

@@ -8,10 +8,12 @@
 // y, total and dx are rounded once, total before the norm reads it.
 //
 // Bound by memory where there are many rows, by the chain launch -> load -> sum -> sum -> store where there are few, and in the adjoint by the latency of its
-// instructions (sums of two weights' gradients leave a multiprocessor 16 warps).  Measured on one B200 against its copy bandwidth of 6539 GB/s, with residual:
-//   forward   bf16 [16384,8192] 157 to 160 us (1.03 of it), [16384,2048] 43 us (0.95), [1,4096] 2.2 us; f32 [4099,1001] without a residual 11.3 to 13.6 us (a copy of it 11.2 to 12.7)
+// instructions (sums of two weights' gradients leave a multiprocessor 16 warps).  Measured on one B200 against its copy bandwidth of 6539 GB/s, with residual, on the device in runs
+// of some ms (what is above that bandwidth was still in the second-level cache when the clock stopped; in a loop of calls the first takes 170 us, 0.96):
+//   forward   bf16 [16384,8192] 157 to 160 us (1.03 of it), [16384,2048] 43 us (0.95), [1,4096] 2.2 us; f32 [4099,1001] without a residual 11.3 to 13.9 us (a copy of it 11.2 to 12.7)
 //   adjoint   bf16 [8192,4096] 51 us (0.80), [8192,16384] 178 us (0.92), [8192,4095] 69 us (0.60); f32 [4096,8192] 86 us (0.96), [4096,16384] 254 us (0.65: gamma is
-//             read anew for every row); f16 [2047,1535] 17 us
+//             read anew for every row); f16 [2047,1535] 17 us; bf16 rows with f32 weights, whose gamma is read anew, too, [8192,2048] 40 us (30 with bf16 weights),
+//             [8192,4096] 70 (0.59), [8192,8192] 137 (93)
 // Three kernels, as the RMS norm has: rows held in registers, the adjoint through rings of asynchronous copies, and plain ones, element by element, for rows that
 // are too wide or do not begin in step.  Tried and dropped: the next row's sums ahead of this row's gradient (65 us in the place of 55 for [8192,4096]); the
 // single row of a ring refilled slot by slot (287 us in the place of 254 for f32 [4096,16384]); joins of a block's warps by loads in the place of shuffles
@@ -601,7 +603,9 @@ bool grad_plan(const LayerGradArgs &a, int type, int weight_type, HeldGrad &h, u
   // few rows: all in one block, which has nothing to join, or else a row per block first
   if (a.rows <= h.teams) h.teams = (uint32_t)a.rows;
   else if (a.rows < (uint64_t)h.teams * sms) h.teams = (uint32_t)((a.rows + sms - 1) / sms);
-  // a single team of many rows leaves out the threads beyond it, whose rings' place gives it more rows ahead; otherwise they help with the sums
+  // a single team of many rows leaves out the threads beyond it, whose places in the rings stay empty (f32 [4096,4608] 54.5 us, 56.4 with them; [4096,10240] 183 and 186; bf16
+  // [4096,8704] 75 either way); otherwise they help with the sums.  Rings at the block's own distance, which hold more rows of such a team, were slower for what an address then
+  // costs: bf16 [4096,8704] 81 us, [4096,11264] 86 (79), f32 [4096,4224] 56 (52), [4096,8704] 199 (164), though f32 [4096,10240] took 169 so (184) and [4096,12288] 187 (203)
   h.threads = h.teams == 1 && a.rows > 4ull * sms ? h.team : threads;
   // gamma in registers, or its slots beside the ring if they are the rows' and leave it two rows
   const size_t slot = (size_t)kGradThreads * chunks * 16;

@@ -6,7 +6,8 @@
 // A row keeps m and L apart, since their sum would lose L's digits beside a large m.
 //
 // Measured on one B200 against its copy bandwidth of 6539 GB/s: bf16 [4096,131072] with entropies 163 us (1.00; 188 in a loop of seconds, near the power cap), [4096,50021]
-// 72 to 74 us (0.85 to 0.87), [256,131072] 15 to 16 us; f32 [16,131072] with the likeliest twenty 11.4 to 12.5 us, without 5.7.  Gradient bf16 [4096,50021] with entropies 128 us (0.98), without 123 (1.02).
+// 72 to 74 us (0.85 to 0.87), [256,131072] 15 to 16 us; f32 [16,131072] with the likeliest twenty 11.4 to 12.5 us, without 5.7.  Gradient bf16 [4096,50021] with entropies 128 us (0.98), without 123 (1.02: its last writes
+// are still in the second-level cache when the clock stops); where dlogits does not begin its rows at the logits' places of 16 bytes, element by element, 439 us.
 // Many long rows are bound by memory (an exponential for each logit keeps its unit busy for 60 % of the time), few by the chain load -> sums -> cluster -> store.
 #include "bn_host.h"
 #include "rows.cuh"

@@ -732,8 +732,8 @@ class TokenLogProbsOp:
     """Log probabilities over rows of logits [*, vocab], at a temperature of 1/scale, in one launch and one pass: with m = max x, z = scale*(x - m),
     L = log(sum(exp(z))), logprob = z[token] - L of the given tokens (int32 or int64, one per row; one outside of [0, vocab) stands for none and has 0),
     entropy = L - sum(z*exp(z))/sum(exp(z)), and the up to 128 likeliest tokens with their log probabilities, [*, top], the largest logit first, of equal ones
-    the lowest index.  stats: float32, two values per row, (m, L), for the adjoint.  What is None is not computed.
-    A logit of -infinity has probability 0; a row of nothing else has log probabilities of -infinity and entropy 0; one that holds a NaN or +infinity, NaN."""
+    the lowest index.  stats: float32, two values per row, (m, L), for the adjoint.  What is None is not computed;
+    outputs that share memory are refused.  A logit of -infinity has probability 0; a row of nothing else has log probabilities of -infinity and entropy 0; one that holds a NaN or +infinity, NaN."""
     @staticmethod
     def apply(logits, tokens, logprob, entropy=None, stats=None, top_logprob=None, top_token=None, scale=1.0, cfg=None, stream=None):
         _hint(cfg)
@@ -745,7 +745,8 @@ class TokenLogProbsOp:
     @staticmethod
     def adjoint(logits, tokens, stats, dlogprob, dlogits, entropy=None, dentropy=None, scale=1.0, cfg=None, stream=None):
         """dlogits = scale*(dlogprob*([token] - p) - dentropy*p*(z - L + entropy)), p = exp(z - L), from the forward pass's logits, tokens and scale, and the
-        stats and entropies that it stored.  dlogprob or dentropy may be None; a row without a token has no part of dlogprob.  dlogits may be logits."""
+        stats and entropies that it stored.  dlogprob or dentropy may be None; a row without a token has no part of dlogprob.  dlogits may be logits; where its rows begin
+        at other places of 16 bytes than the logits' rows, the call is several times slower."""
         _hint(cfg)
         rc = native().probs_bwd(logits, tokens, stats, dlogprob, dlogits, entropy, dentropy, scale, stream)
         if rc:
@@ -923,8 +924,8 @@ class LayerNormAdd:
         return y, total
 
     def backward(self, dy, dtotal=None, out=None):
-        """The gradient of x, which is the residual's, too; those of gamma and beta are left in dgamma and dbeta.  In the sum's place
-        (out=total) it is the last one of its forward pass."""
+        """The gradient of x, which is the residual's, too; those of gamma and beta are left in dgamma and dbeta, in the place of what was
+        there.  In the sum's place (out=total) it is the last one of its forward pass."""
         if self._saved is None:
             raise RuntimeError("backward before forward")
         total, mean, inv_std = self._saved
@@ -989,7 +990,8 @@ class TokenLogProbs:
         return logprob, h
 
     def backward(self, dlogprob, dentropy=None, out=None):
-        """The gradient of the logits, in whose place it may be (out=logits); it is then the last one of its forward pass."""
+        """The gradient of the logits, in whose place it may be (out=logits); it is then the last one of its forward pass.  For logits that are columns
+        of wider rows (a padded vocabulary) give an `out` whose rows lie at the same distance: into the packed array made here the call is several times slower."""
         if self._saved is None:
             raise RuntimeError("backward before forward")
         logits, tokens, stats, h = self._saved
